@@ -34,7 +34,8 @@ typedef void* ir_stream_t; /* a hipStream_t; NULL is the null stream */
 enum {
   IR_DTYPE_F32 = 0,
   IR_DTYPE_F16 = 1,
-  IR_DTYPE_BF16 = 2
+  IR_DTYPE_BF16 = 2,
+  IR_DTYPE_E4M3 = 3 /* the codes of an 8-bit pool; only where a call says so */
 };
 
 /* return codes */
@@ -245,7 +246,8 @@ int ir_paged_decode_noalloc(const void* q, int64_t q_seq_stride, int64_t q_head_
  *   ir_paged_decode_num_counters(...) int32 of a zero-filled counters buffer,
  *   which the run leaves at zero.
  * ir_paged_decode_plan: writes the plan for (block_tables, context_lens) and a
- *   pool with the given slot/head strides (elements) and dtype. Context
+ *   pool with the given slot/head strides (elements) and dtype (IR_DTYPE_E4M3 for
+ *   an 8-bit pool, strides head_dim and num_blocks * block_size * head_dim). Context
  *   lengths outside [0, max_blocks * block_size] are clamped and flagged
  *   (IR_ERR_CONTEXT_RANGE); block ids outside [0, num_blocks) are flagged
  *   (IR_ERR_BLOCK_RANGE) and their keys masked, as in ir_paged_decode.
@@ -574,6 +576,114 @@ int ir_rope_kv_scatter(const void* q, int64_t q_tok_stride, int64_t q_head_strid
                        const int64_t* slot_mapping, int64_t n_tokens, int num_q_heads,
                        int num_kv_heads, int head_dim, int dtype, int32_t* err_flags,
                        ir_stream_t stream);
+
+/*
+ * Norms of queries and keys for each head, rotary embedding and KV-slot scatter in
+ * one launch: for a model whose attention norms q and k per head before the
+ * rotation. With y = x * rsqrt(mean(x^2) + eps) * weight over a head's head_dim:
+ *   q_out[i, h] = y * cos[i] + rotate_half(y) * sin[i] of q[i, h];
+ *   k_cache[slot_mapping[i], h] = the same of k[i, h];  v_cache[slot_mapping[i], h] = v[i, h],
+ *   in fp32 throughout, rounded to the dtype once (ir_rope_kv_scatter instead rounds
+ *   the tables, the products and the sum, as the reference's tensor operations do).
+ *   q_weight, k_weight: [head_dim] of dtype, 16-byte aligned; eps >= 0.
+ * Everything else as ir_rope_kv_scatter (q_out may alias q); head_dim in {64, 128}.
+ */
+int ir_qk_norm_rope_kv_scatter(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                               int64_t qo_tok_stride, int64_t qo_head_stride, const void* k,
+                               int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                               int64_t v_tok_stride, int64_t v_head_stride, const void* q_weight,
+                               const void* k_weight, float eps, const float* cos, const float* sin,
+                               int64_t cs_tok_stride, void* k_cache, void* v_cache,
+                               int64_t cache_slot_stride, int64_t cache_head_stride, int64_t num_slots,
+                               const int64_t* slot_mapping, int64_t n_tokens, int num_q_heads,
+                               int num_kv_heads, int head_dim, int dtype, int32_t* err_flags,
+                               ir_stream_t stream);
+
+/*
+ * The 8-bit K/V pool. One layer is dense:
+ *   k_cache, v_cache: e4m3 codes (OCP: 448 the largest, no infinities)
+ *                     [num_kv_heads][num_blocks][block_size][head_dim];
+ *   scales:           fp32 [num_kv_heads][num_blocks][2], the scale of the block's K
+ *                     and of its V, powers of two; a value is code * scale.
+ * block_size a multiple of 16, at most 1024; head_dim in {64, 128}; caches 16-byte
+ * and scales 8-byte aligned; num_blocks * block_size < 2^31. dtype is the pool's: the
+ * dtype of the rows written and read and of the queries that attend. Every value the
+ * pool holds is exactly a number of it.
+ *
+ * ir_kv_scatter_q8: ir_kv_scatter into such a layer (slots alike: negative = skip,
+ * past the pool = skip and flag). A block's scale is the least 2^k with
+ * amax <= 448 * 2^k over the magnitudes it has to hold, k in [-100, 119] (f16: [-15, 8]);
+ * codes are rounded to nearest even, magnitudes past 448 * 2^119 (f16: 61440)
+ * saturate, NaN and infinities become NaN and do not count for the scale.
+ *   - A call that writes a block's token 0 starts the block: its scale comes from
+ *     this call's tokens alone, and its tokens that the call does not write become 0.
+ *   - Any other call keeps the block's tokens: its scale is the larger of what it has
+ *     and what the call's tokens need, and if it grows the kept codes are rounded to it.
+ * So a cache filled in order holds what its own sequence wrote, whatever the blocks
+ * held before. Within a call tokens may come in any order and share blocks; of rows
+ * given the same slot the last is written. Calls that write the same block must be
+ * stream-ordered.
+ *
+ * ir_rope_kv_scatter_q8: ir_rope_kv_scatter (weights null), or
+ * ir_qk_norm_rope_kv_scatter (weights given), into such a layer, one launch: the
+ * keys are quantised as they leave the rotation (with norms from fp32, without an
+ * intermediate rounding to dtype).
+ *
+ * ir_gather_slots_q8, ir_paged_gather_q8: ir_gather_slots and ir_paged_gather of such a
+ * layer, values of dtype; outputs 16-byte aligned.
+ */
+int ir_kv_scatter_q8(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, void* k_cache, void* v_cache,
+                     float* scales, int64_t num_blocks, int block_size, const int64_t* slot_mapping,
+                     int64_t n_tokens, int num_kv_heads, int head_dim, int dtype, int32_t* err_flags,
+                     ir_stream_t stream);
+int ir_rope_kv_scatter_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                          int64_t qo_tok_stride, int64_t qo_head_stride, const void* k,
+                          int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_tok_stride, int64_t v_head_stride, const void* q_weight,
+                          const void* k_weight, float eps, const float* cos, const float* sin,
+                          int64_t cs_tok_stride, void* k_cache, void* v_cache, float* scales,
+                          int64_t num_blocks, int block_size, const int64_t* slot_mapping,
+                          int64_t n_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                          int32_t* err_flags, ir_stream_t stream);
+int ir_gather_slots_q8(const void* k_cache, const void* v_cache, const float* scales, int64_t num_blocks,
+                       int block_size, const int64_t* slots, int64_t n, int num_kv_heads, int head_dim,
+                       int dtype, void* out_k, void* out_v, int32_t* err_flags, ir_stream_t stream);
+int ir_paged_gather_q8(const void* k_cache, const void* v_cache, const float* scales, int64_t num_blocks,
+                       int block_size, const int32_t* block_tables, int64_t bt_stride,
+                       int max_blocks_per_seq, const int32_t* context_lens, int num_seqs, int max_ctx,
+                       int num_kv_heads, int head_dim, int dtype, void* out_k, void* out_v,
+                       int32_t* err_flags, ir_stream_t stream);
+
+/*
+ * Attention over the 8-bit pool: ir_paged_decode, ir_paged_decode_planned and
+ * ir_paged_prefill of the values that a layer holds, dtype being that of q and out.
+ * Workspaces, counters and plans are theirs (a decode plan is built with
+ * IR_DTYPE_E4M3 and the layer's strides). The step's new rows are written first
+ * (ir_kv_scatter_q8): their blocks' scales are not known before, so the prefill has no
+ * fused write.
+ */
+int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
+                       const void* v_cache, const float* scales, int64_t num_blocks, int block_size,
+                       const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                       const int32_t* context_lens, void* out, int64_t out_seq_stride,
+                       int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
+                       int head_dim, float scale, int dtype, int partition_tokens, int32_t* counters,
+                       int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                       int32_t* err_flags, ir_stream_t stream);
+int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                               const void* k_cache, const void* v_cache, const float* scales, void* out,
+                               int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
+                               int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
+                               int block_size, float scale, int dtype, int flags, const void* plan,
+                               int32_t* counters, int64_t num_counters, void* workspace,
+                               int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream);
+int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache, const void*
+                        v_cache, const float* scales, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                        int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
+                        int num_seqs, int total_q, int max_q_len, void* out, int64_t out_tok_stride, int64_t
+                        out_head_stride, int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype, void*
+                        plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
 
 /*
  * Read-only HBM streaming roof (a measurement utility; no counterpart in the

@@ -18,6 +18,7 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libinfrared_amd.so")
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+DTYPE_E4M3 = 3  # the codes of an 8-bit pool: decode plans only
 _DTYPE_CODES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
 # err_flags bits (IR_ERR_*)
@@ -134,6 +135,47 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _c_i64, _c_p],
     ),
     "ir_paged_prefill_plan_xcds": (_c_i32, []),
+    "ir_qk_norm_rope_kv_scatter": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
+         _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_p,
+         _c_p],
+    ),
+    "ir_kv_scatter_q8": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32,
+         _c_i32, _c_p, _c_p],
+    ),
+    "ir_rope_kv_scatter_q8": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
+         _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_p,
+         _c_p],
+    ),
+    "ir_gather_slots_q8": (
+        _c_i32,
+        [_c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "ir_paged_gather_q8": (
+        _c_i32,
+        [_c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p,
+         _c_p, _c_p, _c_p],
+    ),
+    "ir_paged_decode_q8": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i64, _c_i64,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "ir_paged_decode_planned_q8": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "ir_paged_prefill_q8": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_i32,
+         _c_i32, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_p, _c_i64, _c_p, _c_p],
+    ),
 }
 
 _lock = threading.Lock()

@@ -66,6 +66,30 @@ void check_tables(const char* name, const Tensor& bt, const Tensor& ctx) {
   require(ctx.is_contiguous(), name, ": context_lens must be contiguous");
 }
 
+// One layer of an 8-bit pool: dense codes [num_slots, num_kv_heads, head_dim] in
+// head-major storage, scales [num_kv_heads, num_blocks, 2].
+void code_layer(const char* name, const Tensor& kc, const Tensor& vc, const Tensor& scales, int64_t block_size) {
+  require_device({&kc, &vc, &scales});
+  cache_layer(name, kc);
+  require(kc.scalar_type() == at::kFloat8_e4m3fn && vc.scalar_type() == at::kFloat8_e4m3fn, name,
+          ": kv_scales go with caches of float8_e4m3fn codes, got ", kc.scalar_type(), " and ", vc.scalar_type());
+  require(vc.sizes() == kc.sizes() && vc.strides() == kc.strides(), name,
+          ": k_cache and v_cache must have the same shape and strides");
+  require(kc.stride(0) == kc.size(2) && (kc.size(1) == 1 || kc.stride(1) == kc.size(0) * kc.size(2)), name,
+          ": a cache of codes must be dense [num_kv_heads, num_slots, head_dim] storage");
+  require(scales.scalar_type() == at::kFloat && scales.dim() == 3 && scales.is_contiguous() &&
+              scales.size(0) == kc.size(1) && scales.size(1) * block_size == kc.size(0) && scales.size(2) == 2,
+          name, ": kv_scales must be contiguous fp32 [num_kv_heads, num_blocks, 2]");
+}
+
+// An output the caller gave for `like`'s shape (strides are the kernel's to check).
+void given_out(const char* name, const Tensor& out, const Tensor& like) {
+  require_device({&like, &out});
+  require(out.sizes() == like.sizes() && out.scalar_type() == like.scalar_type(), name, ": out must be ",
+          like.sizes(), " of ", like.scalar_type());
+  unit_last(name, out);
+}
+
 // A block size the C ABI's int holds (truncated it could divide by zero here).
 void check_block_size(const char* name, int64_t block_size) {
   require(block_size > 0 && block_size <= INT32_MAX, name, "block_size must be positive and fit 32 bits, got ",
@@ -109,17 +133,20 @@ void kv_scatter(const Tensor& kc, const Tensor& vc, const Tensor& k, const Tenso
         "ir_kv_scatter");
 }
 
-Tensor paged_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& bt, const Tensor& ctx,
-                    int64_t block_size, double scale, const OptTensor& out_, int64_t partition,
-                    const OptTensor& workspace, const OptTensor& err, const OptTensor& counters, int64_t stream) {
+// (scales: of an 8-bit pool's layer)
+Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const OptTensor& scales, const Tensor& bt,
+                   const Tensor& ctx, int64_t block_size, double scale, const OptTensor& out_, int64_t partition,
+                   const OptTensor& workspace, const OptTensor& err, const OptTensor& counters, int64_t stream) {
   require_device({&q, &kc, &vc, &bt, &ctx});
   cache_layer("paged_decode", kc);
   check_tables("paged_decode", bt, ctx);
   require(q.dim() == 3, "paged_decode: q must be [B, H_q, D], got ", q.sizes());
   check_block_size("paged_decode: ", block_size);
   const int b = (int)q.size(0), hq = (int)q.size(1), d = (int)q.size(2), h_kv = (int)kc.size(1);
-  require(d == kc.size(2) && q.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes(),
+  require(d == kc.size(2) && (scales || q.scalar_type() == kc.scalar_type()) && vc.sizes() == kc.sizes(),
           "paged_decode: q / pool shape or dtype mismatch");
+  if (scales) code_layer("paged_decode", kc, vc, *scales, block_size);
+  if (scales && out_) given_out("paged_decode", *out_, q);
   require(bt.size(0) == b, "paged_decode: block_tables rows != batch");
   unit_last("paged_decode q", q);
   const Tensor out = out_ ? *out_ : at::empty({b, hq, d}, q.options());
@@ -133,6 +160,16 @@ Tensor paged_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, const T
     n_ctr = ir_paged_decode_num_counters(b, hq, h_kv);
     ctr = counters_for(counters, n_ctr, q);
   }
+  if (scales) {
+    check(ir_paged_decode_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                             (const float*)scales->data_ptr(), kc.size(0) / bs, bs, (const int32_t*)bt.data_ptr(),
+                             bt.stride(0), max_blocks, (const int32_t*)ctx.data_ptr(), out.data_ptr(), out.stride(0),
+                             out.stride(1), b, hq, h_kv, d, (float)scale, dtype_code(q), part,
+                             need > 0 ? (int32_t*)ctr.data_ptr() : nullptr, n_ctr, need > 0 ? ws.data_ptr() : nullptr,
+                             need, (int32_t*)ptr(err), stream_of(stream)),
+          "ir_paged_decode_q8");
+    return out;
+  }
   check(ir_paged_decode(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), kc.stride(0),
                         kc.stride(1), kc.size(0) / bs, bs, (const int32_t*)bt.data_ptr(), bt.stride(0), max_blocks,
                         (const int32_t*)ctx.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), b, hq, h_kv, d,
@@ -142,14 +179,28 @@ Tensor paged_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, const T
   return out;
 }
 
+Tensor paged_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& bt, const Tensor& ctx,
+                    int64_t block_size, double scale, const OptTensor& out, int64_t partition,
+                    const OptTensor& workspace, const OptTensor& err, const OptTensor& counters, int64_t stream) {
+  return decode_call(q, kc, vc, std::nullopt, bt, ctx, block_size, scale, out, partition, workspace, err, counters,
+                     stream);
+}
+
+Tensor paged_decode_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& scales, const Tensor& bt,
+                       const Tensor& ctx, int64_t block_size, double scale, const OptTensor& out, int64_t partition,
+                       const OptTensor& workspace, const OptTensor& err, const OptTensor& counters, int64_t stream) {
+  return decode_call(q, kc, vc, scales, bt, ctx, block_size, scale, out, partition, workspace, err, counters, stream);
+}
+
 // `plan`: the fields of a decode plan in the order of its dataclass, buffer and
 // dtype apart (num_seqs, num_q_heads, num_kv_heads, max_blocks, block_size,
 // num_blocks, slot_stride, head_stride).
-Tensor paged_decode_planned(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& plan_buf,
-                            const std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>& p,
-                            at::ScalarType plan_dtype, int64_t flags, double scale, const OptTensor& out_,
-                            const OptTensor& workspace, const OptTensor& err, const OptTensor& counters,
-                            int64_t stream) {
+using PlanShape = std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>;
+
+Tensor planned_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const OptTensor& scales,
+                    const Tensor& plan_buf, const PlanShape& p, at::ScalarType plan_dtype, int64_t flags, double scale,
+                    const OptTensor& out_, const OptTensor& workspace, const OptTensor& err, const OptTensor& counters,
+                    int64_t stream) {
   require_device({&q, &kc, &vc, &plan_buf});
   cache_layer("paged_decode_planned", kc);
   require(q.dim() == 3, "paged_decode_planned: q must be [B, H_q, D], got ", q.sizes());
@@ -162,13 +213,24 @@ Tensor paged_decode_planned(const Tensor& q, const Tensor& kc, const Tensor& vc,
           "paged_decode_planned: pool layout differs from the plan's");
   require(vc.sizes() == kc.sizes() && vc.strides() == kc.strides(),
           "paged_decode_planned: v_cache must match k_cache's shape and strides");
-  require(d == kc.size(2) && q.scalar_type() == kc.scalar_type(),
+  require(d == kc.size(2) && (scales || q.scalar_type() == kc.scalar_type()),
           "paged_decode_planned: q / pool shape or dtype mismatch");
+  if (scales) code_layer("paged_decode_planned", kc, vc, *scales, bs);
+  if (scales && out_) given_out("paged_decode_planned", *out_, q);
   unit_last("paged_decode_planned q", q);
   const Tensor out = out_ ? *out_ : at::empty({b, hq, d}, q.options());
   const Tensor ws = scratch(workspace, ir_paged_decode_planned_workspace_bytes(b, hq, (int)p_hkv, d), q);
   const int64_t n_ctr = ir_paged_decode_num_counters(b, hq, (int)p_hkv);
   const Tensor ctr = counters_for(counters, n_ctr, q);
+  if (scales) {
+    check(ir_paged_decode_planned_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                                     (const float*)scales->data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), b,
+                                     hq, (int)p_hkv, d, (int)max_blocks, (int)bs, (float)scale, dtype_code(q),
+                                     (int)flags, plan_buf.data_ptr(), (int32_t*)ctr.data_ptr(), n_ctr, ws.data_ptr(),
+                                     ws.numel(), (int32_t*)ptr(err), stream_of(stream)),
+          "ir_paged_decode_planned_q8");
+    return out;
+  }
   check(ir_paged_decode_planned(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), kc.stride(0),
                                 out.data_ptr(), out.stride(0), out.stride(1), b, hq, (int)p_hkv, d, (int)max_blocks,
                                 (int)bs, (float)scale, dtype_code(q), (int)flags, plan_buf.data_ptr(),
@@ -176,6 +238,21 @@ Tensor paged_decode_planned(const Tensor& q, const Tensor& kc, const Tensor& vc,
                                 stream_of(stream)),
         "ir_paged_decode_planned");
   return out;
+}
+
+Tensor paged_decode_planned(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& plan_buf,
+                            const PlanShape& p, at::ScalarType plan_dtype, int64_t flags, double scale,
+                            const OptTensor& out, const OptTensor& workspace, const OptTensor& err,
+                            const OptTensor& counters, int64_t stream) {
+  return planned_call(q, kc, vc, std::nullopt, plan_buf, p, plan_dtype, flags, scale, out, workspace, err, counters,
+                      stream);
+}
+
+Tensor paged_decode_planned_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& scales,
+                               const Tensor& plan_buf, const PlanShape& p, at::ScalarType plan_dtype, int64_t flags,
+                               double scale, const OptTensor& out, const OptTensor& workspace, const OptTensor& err,
+                               const OptTensor& counters, int64_t stream) {
+  return planned_call(q, kc, vc, scales, plan_buf, p, plan_dtype, flags, scale, out, workspace, err, counters, stream);
 }
 
 Tensor paged_attention_masked(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& gs,
@@ -259,6 +336,91 @@ Tensor rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const 
   return qo;
 }
 
+void kv_scatter_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales, const Tensor& k, const Tensor& v,
+                   const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
+  check_block_size("kv_scatter_q8: ", block_size);
+  code_layer("kv_scatter_q8", kc, vc, scales, block_size);
+  require_device({&kc, &k, &v, &slots});
+  require(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == kc.size(1) && k.size(2) == kc.size(2),
+          "kv_scatter_q8: k ", k.sizes(), " / v ", v.sizes(), " do not match pool rows ", kc.sizes().slice(1));
+  require(v.scalar_type() == k.scalar_type(), "kv_scatter_q8: dtype mismatch (", k.scalar_type(), ", ",
+          v.scalar_type(), ")");
+  const int64_t n = k.size(0);
+  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n,
+          "kv_scatter_q8: slots must be int64 [", n, "], got ", slots.scalar_type(), " ", slots.sizes());
+  unit_last("kv_scatter_q8 k", k);
+  unit_last("kv_scatter_q8 v", v);
+  const Tensor s = slots.contiguous();
+  check(ir_kv_scatter_q8(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), kc.data_ptr(),
+                         vc.data_ptr(), (float*)scales.data_ptr(), scales.size(1), (int)block_size,
+                         (const int64_t*)s.data_ptr(), n, (int)k.size(1), (int)k.size(2), dtype_code(k),
+                         (int32_t*)ptr(err), stream_of(stream)),
+        "ir_kv_scatter_q8");
+}
+
+// ir_qk_norm_rope_kv_scatter, and with scales (an 8-bit pool's layer) ir_rope_kv_scatter_q8,
+// whose norms may be absent.
+Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& wq,
+                            const OptTensor& wk, double eps, const Tensor& cos, const Tensor& sin, const Tensor& kc,
+                            const Tensor& vc, const OptTensor& scales, int64_t block_size, const Tensor& slots,
+                            const OptTensor& q_out_, const OptTensor& err, int64_t stream) {
+  const char* name = scales ? "rope_kv_scatter_q8" : "qk_norm_rope_kv_scatter";
+  require_device({&q, &k, &v, &cos, &sin, &kc, &vc, &slots});
+  cache_layer(name, kc);
+  if (scales) {
+    check_block_size("rope_kv_scatter_q8: ", block_size);
+    code_layer(name, kc, vc, *scales, block_size);
+  }
+  require(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes(), name,
+          ": q [N, H_q, D], k and v [N, H_kv, D] expected");
+  const int64_t n = q.size(0), d = q.size(2);
+  require(k.size(0) == n && k.size(2) == d && k.size(1) == kc.size(1) && d == kc.size(2), name,
+          ": k/v rows do not match q or the pool");
+  require(q.scalar_type() == k.scalar_type() && v.scalar_type() == k.scalar_type() &&
+              (scales || kc.scalar_type() == k.scalar_type()),
+          name, ": dtype mismatch");
+  require(vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && vc.scalar_type() == kc.scalar_type(), name,
+          ": k_cache and v_cache must share shape, strides and dtype");
+  require(wq.has_value() == wk.has_value(), name, ": one norm weight without the other");
+  if (wq) {
+    require_device({&q, &*wq, &*wk});
+    for (const auto& [which, t] : {std::pair<const char*, const Tensor*>{"q_norm", &*wq}, {"k_norm", &*wk}})
+      require(t->dim() == 1 && t->size(0) == d && t->is_contiguous() && t->scalar_type() == q.scalar_type(), name, ": ",
+              which, " must be contiguous [", d, "] of ", q.scalar_type());
+  }
+  for (const auto& [which, t] : {std::pair<const char*, const Tensor*>{"cos", &cos}, {"sin", &sin}})
+    require(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == n && t->size(1) == d && t->stride(1) == 1,
+            name, ": ", which, " must be fp32 [N, D] with unit column stride");
+  require(cos.stride(0) == sin.stride(0), name, ": cos and sin must share strides");
+  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name, ": slots must be int64 [N]");
+  unit_last(name, q);
+  unit_last(name, k);
+  unit_last(name, v);
+  if (q_out_) given_out(name, *q_out_, q);
+  const Tensor qo = q_out_ ? *q_out_ : at::empty_like(q);
+  const Tensor s = slots.contiguous();
+  if (scales) {
+    check(ir_rope_kv_scatter_q8(q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+                                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                ptr(wq), ptr(wk), (float)eps, (const float*)cos.data_ptr(),
+                                (const float*)sin.data_ptr(), cos.stride(0), kc.data_ptr(), vc.data_ptr(),
+                                (float*)scales->data_ptr(), scales->size(1), (int)block_size,
+                                (const int64_t*)s.data_ptr(), n, (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q),
+                                (int32_t*)ptr(err), stream_of(stream)),
+          "ir_rope_kv_scatter_q8");
+    return qo;
+  }
+  check(ir_qk_norm_rope_kv_scatter(q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+                                   k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                   ptr(wq), ptr(wk), (float)eps, (const float*)cos.data_ptr(),
+                                   (const float*)sin.data_ptr(), cos.stride(0), kc.data_ptr(), vc.data_ptr(),
+                                   kc.stride(0), kc.stride(1), kc.size(0), (const int64_t*)s.data_ptr(), n,
+                                   (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q), (int32_t*)ptr(err),
+                                   stream_of(stream)),
+        "ir_qk_norm_rope_kv_scatter");
+  return qo;
+}
+
 Tensor paged_prefill(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& bt, const Tensor& cu,
                      const Tensor& q_start, int64_t max_q_len, int64_t block_size, double scale, const OptTensor& out_,
                      const OptTensor& err, const OptTensor& plan_buf, const OptTensor& kn, const OptTensor& vn,
@@ -309,6 +471,36 @@ Tensor paged_prefill(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
   return out;
 }
 
+Tensor paged_prefill_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& scales, const Tensor& bt,
+                        const Tensor& cu, const Tensor& q_start, int64_t max_q_len, int64_t block_size, double scale,
+                        const OptTensor& out_, const OptTensor& err, const OptTensor& plan_buf, int64_t stream) {
+  require_device({&q, &kc, &vc, &bt, &cu, &q_start});
+  require(q.dim() == 3, "paged_prefill: q must be [total_q, H_q, D], got ", q.sizes());
+  check_block_size("paged_prefill: ", block_size);
+  code_layer("paged_prefill", kc, vc, scales, block_size);
+  const int hq = (int)q.size(1), d = (int)q.size(2), h_kv = (int)kc.size(1);
+  require(d == kc.size(2), "paged_prefill: q / pool shape mismatch");
+  require(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.stride(1) == 1,
+          "paged_prefill: block_tables must be int32 [B, max_blocks] with unit column stride");
+  const int64_t b = bt.size(0);
+  for (const auto& [name, t, n] : {std::tuple<const char*, const Tensor*, int64_t>{"cu_seqlens_q", &cu, b + 1},
+                                   {"q_start", &q_start, b}})
+    require(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && t->is_contiguous(),
+            "paged_prefill: ", name, " must be contiguous int32 [", n, "]");
+  unit_last("paged_prefill q", q);
+  if (plan_buf) require_device({&q, &*plan_buf});
+  if (out_) given_out("paged_prefill", *out_, q);
+  const Tensor out = out_ ? *out_ : at::empty(q.sizes(), q.options());
+  check(ir_paged_prefill_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                            (const float*)scales.data_ptr(), scales.size(1), (int)block_size,
+                            (const int32_t*)bt.data_ptr(), bt.stride(0), (int)bt.size(1), (const int32_t*)cu.data_ptr(),
+                            (const int32_t*)q_start.data_ptr(), (int)b, (int)q.size(0), (int)max_q_len, out.data_ptr(),
+                            out.stride(0), out.stride(1), hq, h_kv, d, (float)scale, dtype_code(q), ptr(plan_buf),
+                            plan_buf ? plan_buf->numel() : 0, (int32_t*)ptr(err), stream_of(stream)),
+        "ir_paged_prefill_q8");
+  return out;
+}
+
 // The seam's forms of the calls above: k, v [B, Sq, H_kv, D], q and the result
 // [B, 1, H_q, D].
 void write_step(const Tensor& kc, const Tensor& vc, const Tensor& k, const Tensor& v, const Tensor& slots,
@@ -325,10 +517,9 @@ Tensor decode_step(const Tensor& q, const Tensor& kc, const Tensor& vc, const Te
 }
 
 Tensor decode_step_planned(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& plan_buf,
-                           const std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>& p,
-                           at::ScalarType plan_dtype, int64_t flags, double scale, const OptTensor& out,
-                           const OptTensor& workspace, const OptTensor& err, const OptTensor& counters,
-                           int64_t stream) {
+                           const PlanShape& p, at::ScalarType plan_dtype, int64_t flags, double scale,
+                           const OptTensor& out, const OptTensor& workspace, const OptTensor& err,
+                           const OptTensor& counters, int64_t stream) {
   return paged_decode_planned(q.select(1, 0), kc, vc, plan_buf, p, plan_dtype, flags, scale, out, workspace, err,
                               counters, stream)
       .unsqueeze(1);
@@ -346,6 +537,11 @@ PYBIND11_MODULE(_seam, m) {
   m.def("paged_attention_masked", &paged_attention_masked, nogil());
   m.def("rope_kv_scatter", &rope_kv_scatter, nogil());
   m.def("paged_prefill", &paged_prefill, nogil());
+  m.def("kv_scatter_q8", &kv_scatter_q8, nogil());
+  m.def("norm_rope_kv_scatter", &norm_rope_kv_scatter, nogil());
+  m.def("paged_decode_q8", &paged_decode_q8, nogil());
+  m.def("paged_decode_planned_q8", &paged_decode_planned_q8, nogil());
+  m.def("paged_prefill_q8", &paged_prefill_q8, nogil());
   m.def("write_step", &write_step, nogil());
   m.def("decode_step", &decode_step, nogil());
   m.def("decode_step_planned", &decode_step_planned, nogil());

@@ -44,13 +44,13 @@ __device__ __forceinline__ void merge_partials(const DecodeArgs& a, int seq, int
 // 16-bit dtypes: two wavefronts per SIMD (<= 256 registers each) keep two
 // resident workgroups' worth of loads in flight per CU. fp32 tiles are twice
 // the registers and run one per SIMD.
-template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH>
+template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH, bool Q8 = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 ? 1 : 2)))
 void paged_decode_kernel(DecodeArgs a) {
   typedef TileShape<DT, D> Sh;
-  constexpr int EB = Sh::EB;
+  typedef CacheFormat<DT, D, Q8> F;
   __shared__ MergeSmem<NW, D> sm;
-  __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][KStage<DT, D>::BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][F::STAGE];
   __shared__ int s_last;
 
   const int lane = threadIdx.x & 63;
@@ -77,17 +77,18 @@ void paged_decode_kernel(DecodeArgs a) {
 
   const int h_local = hg * 16 + c;
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
-  const uint8_t* kc = (const uint8_t*)a.kc + (int64_t)kvh * a.c_head * EB;
-  const uint8_t* vc = (const uint8_t*)a.vc + (int64_t)kvh * a.c_head * EB;
-  const LaneOffsets<DT, D> lo = lane_offsets<DT, D>(lane, a.c_slot * EB);
+  const uint8_t* kc = (const uint8_t*)a.kc + (int64_t)kvh * a.c_head * F::EB;
+  const uint8_t* vc = (const uint8_t*)a.vc + (int64_t)kvh * a.c_head * F::EB;
+  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
+  const typename F::Offsets lo = F::offsets(lane, a.c_slot * F::EB);
   uint32_t qr[Sh::KDW];
-  load_query<DT, D>(a, seq, kvh * a.n_rep + h_local, h_local < a.n_rep, g, qr);
+  load_query_for<DT, D, Q8>(a, seq, kvh * a.n_rep + h_local, h_local < a.n_rep, g, qr);
 
   State<D> st;
   state_init(st);
   bool bad = false;
-  attend_tiles<DT, D, BS16, NW, DEPTH>(a, bt_row, kc, vc, lo, qr, tile_lo, tile_hi, t_end, kstage[w], lane, w, st,
-                                       bad);
+  attend_tiles<DT, D, BS16, NW, DEPTH, Q8>(a, bt_row, kc, vc, scales, lo, qr, tile_lo, tile_hi, t_end, kstage[w], lane,
+                                           w, st, bad);
   if (bad) flag_error(a.err, IR_ERR_BLOCK_RANGE);
   st.l = wave_sum_groups(st.l);
 
@@ -243,6 +244,19 @@ int launch_decode(const DecodeArgs& a, bool bs16, bool fused, hipStream_t s) {
   return check_launch("ir_paged_decode");
 }
 
+// An 8-bit cache: 4-wavefront workgroups, whose tiles are half a 16-bit one's bytes.
+template <int DT, int D>
+int launch_decode_q8(const DecodeArgs& a, bool fused, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * a.n_hg), (unsigned)a.max_parts);
+  if (fused || a.max_parts == 1) {
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, true, 2, true>), grid, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, false, 2, true>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_reduce<DT, D>), dim3(grid.x), dim3(256), 0, s, a);
+  }
+  return check_launch("ir_paged_decode_q8");
+}
+
 }  // namespace
 }  // namespace ir
 
@@ -284,44 +298,51 @@ extern "C" int64_t ir_paged_decode_num_counters(int num_seqs, int num_q_heads, i
   return (int64_t)num_seqs * num_kv_heads * ((num_q_heads / num_kv_heads + 15) / 16);
 }
 
-extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
-                               const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
-                               int64_t cache_head_stride, int64_t num_blocks, int block_size,
-                               const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
-                               const int32_t* context_lens, void* out, int64_t out_seq_stride,
-                               int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
-                               int head_dim, float scale, int dtype, int partition_tokens,
-                               int32_t* counters, int64_t num_counters, void* workspace,
-                               int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
+namespace {
+
+// ir_paged_decode, and with `scales` ir_paged_decode_q8 (a dense layer of codes).
+int decode_call(const char* name, const float* scales, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                const void* k_cache, const void* v_cache, int64_t cache_slot_stride, int64_t cache_head_stride,
+                int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                int max_blocks_per_seq, const int32_t* context_lens, void* out, int64_t out_seq_stride,
+                int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                int dtype, int partition_tokens, int32_t* counters, int64_t num_counters, void* workspace,
+                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   const int eb = dtype_bytes(dtype);
-  IR_REQUIRE(eb > 0, "ir_paged_decode: unknown dtype %d", dtype);
+  IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
   IR_REQUIRE(num_seqs >= 0 && num_q_heads > 0 && num_kv_heads > 0 && block_size > 0 &&
                  max_blocks_per_seq >= 0 && num_blocks >= 0,
-             "ir_paged_decode: bad sizes");
-  IR_REQUIRE(num_q_heads % num_kv_heads == 0, "ir_paged_decode: num_q_heads %d not a multiple of num_kv_heads %d",
+             "%s: bad sizes", name);
+  IR_REQUIRE(num_q_heads % num_kv_heads == 0, "%s: num_q_heads %d not a multiple of num_kv_heads %d", name,
              num_q_heads, num_kv_heads);
   if (head_dim != 64 && head_dim != 128)
-    return fail(IR_EUNSUPPORTED, "ir_paged_decode: head_dim %d not supported (64, 128)", head_dim);
+    return fail(IR_EUNSUPPORTED, "%s: head_dim %d not supported (64, 128)", name, head_dim);
   if (num_seqs == 0) return ok();
-  IR_REQUIRE(q && k_cache && v_cache && block_tables && context_lens && out, "ir_paged_decode: null pointer");
+  IR_REQUIRE(q && k_cache && v_cache && block_tables && context_lens && out, "%s: null pointer", name);
   IR_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
-             "ir_paged_decode: q, caches and out must be 16-byte aligned");
+             "%s: q, caches and out must be 16-byte aligned", name);
   IR_REQUIRE((q_seq_stride * eb) % 16 == 0 && (q_head_stride * eb) % 16 == 0 &&
                  (cache_slot_stride * eb) % 16 == 0 && (cache_head_stride * eb) % 16 == 0 &&
                  (out_seq_stride * eb) % 16 == 0 && (out_head_stride * eb) % 16 == 0,
-             "ir_paged_decode: strides must be multiples of 16 bytes");
+             "%s: strides must be multiples of 16 bytes", name);
   if (partition_tokens <= 0)
     partition_tokens = ir_paged_decode_default_partition(num_seqs, num_kv_heads, max_blocks_per_seq, block_size);
   IR_REQUIRE(partition_tokens % 16 == 0 && partition_tokens <= kMaxPartition,
-             "ir_paged_decode: partition_tokens %d must be a multiple of 16 and at most %d", partition_tokens,
+             "%s: partition_tokens %d must be a multiple of 16 and at most %d", name, partition_tokens,
              kMaxPartition);
   IR_REQUIRE((int64_t)max_blocks_per_seq * block_size <= (int64_t)1 << 30,
-             "ir_paged_decode: block tables of %d x %d tokens exceed 2^30 keys", max_blocks_per_seq, block_size);
+             "%s: block tables of %d x %d tokens exceed 2^30 keys", name, max_blocks_per_seq, block_size);
   // A 16-token tile starting at a multiple of 16 stays inside one block when the
   // block size is a multiple of 16: then the block id is wave-uniform.
   const bool bs16 = block_size % 16 == 0;
+  if (scales) {
+    IR_REQUIRE(bs16, "%s: block size %d must be a multiple of 16", name, block_size);
+    IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+  }
 
   DecodeArgs a;
+  a.scales = (const f32x2*)scales;
+  a.block16 = 0;
   a.q = q;
   a.q_seq = q_seq_stride;
   a.q_head = q_head_stride;
@@ -352,16 +373,16 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
   a.err = err_flags;
   a.max_parts = max_parts_for(max_blocks_per_seq, block_size, partition_tokens);
   bool fused = false;
-  IR_REQUIRE(a.max_parts <= 65535, "ir_paged_decode: %d partitions exceed the grid limit", a.max_parts);
+  IR_REQUIRE(a.max_parts <= 65535, "%s: %d partitions exceed the grid limit", name, a.max_parts);
   if (a.max_parts > 1) {
     const int64_t need = ir_paged_decode_workspace_size(num_seqs, num_q_heads, num_kv_heads, head_dim,
                                                         max_blocks_per_seq, block_size, partition_tokens);
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u))
-      return fail(IR_EWORKSPACE, "ir_paged_decode: workspace of %lld bytes (256-byte aligned) required, got %lld",
+      return fail(IR_EWORKSPACE, "%s: workspace of %lld bytes (256-byte aligned) required, got %lld", name,
                   (long long)need, (long long)workspace_bytes);
     const int64_t units = ir_paged_decode_num_counters(num_seqs, num_q_heads, num_kv_heads);
     if (!counters || num_counters < units)
-      return fail(IR_EWORKSPACE, "ir_paged_decode: %lld arrival counters required, got %lld", (long long)units,
+      return fail(IR_EWORKSPACE, "%s: %lld arrival counters required, got %lld", name, (long long)units,
                   (long long)num_counters);
     const WsLayout ly = ws_layout(num_seqs, num_q_heads, head_dim, a.max_parts);
     a.counters = counters;
@@ -370,6 +391,19 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     fused = knobs().fused && ly.acc_bytes < ((int64_t)1 << 31);
   }
   hipStream_t s = (hipStream_t)stream;
+  if (scales) {
+    switch (dtype) {
+      case IR_DTYPE_BF16:
+        return head_dim == 128 ? launch_decode_q8<IR_DTYPE_BF16, 128>(a, fused, s)
+                               : launch_decode_q8<IR_DTYPE_BF16, 64>(a, fused, s);
+      case IR_DTYPE_F16:
+        return head_dim == 128 ? launch_decode_q8<IR_DTYPE_F16, 128>(a, fused, s)
+                               : launch_decode_q8<IR_DTYPE_F16, 64>(a, fused, s);
+      default:
+        return head_dim == 128 ? launch_decode_q8<IR_DTYPE_F32, 128>(a, fused, s)
+                               : launch_decode_q8<IR_DTYPE_F32, 64>(a, fused, s);
+    }
+  }
   switch (dtype) {
     case IR_DTYPE_BF16:
       return head_dim == 128 ? launch_decode<IR_DTYPE_BF16, 128>(a, bs16, fused, s)
@@ -381,4 +415,39 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
       return head_dim == 128 ? launch_decode<IR_DTYPE_F32, 128>(a, bs16, fused, s)
                              : launch_decode<IR_DTYPE_F32, 64>(a, bs16, fused, s);
   }
+}
+
+}  // namespace
+
+extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                               const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
+                               int64_t cache_head_stride, int64_t num_blocks, int block_size,
+                               const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                               const int32_t* context_lens, void* out, int64_t out_seq_stride,
+                               int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
+                               int head_dim, float scale, int dtype, int partition_tokens,
+                               int32_t* counters, int64_t num_counters, void* workspace,
+                               int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
+  return decode_call("ir_paged_decode", nullptr, q, q_seq_stride, q_head_stride, k_cache, v_cache, cache_slot_stride,
+                     cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
+                     context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                     scale, dtype, partition_tokens, counters, num_counters, workspace, workspace_bytes, err_flags,
+                     stream);
+}
+
+extern "C" int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
+                                  const void* v_cache, const float* scales, int64_t num_blocks, int block_size,
+                                  const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                                  const int32_t* context_lens, void* out, int64_t out_seq_stride,
+                                  int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
+                                  int head_dim, float scale, int dtype, int partition_tokens, int32_t* counters,
+                                  int64_t num_counters, void* workspace, int64_t workspace_bytes, int32_t* err_flags,
+                                  ir_stream_t stream) {
+  if (num_seqs == 0) return ok();
+  IR_REQUIRE(scales, "ir_paged_decode_q8: null pointer");
+  return decode_call("ir_paged_decode_q8", scales, q, q_seq_stride, q_head_stride, k_cache, v_cache, head_dim,
+                     num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
+                     max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
+                     num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
+                     workspace_bytes, err_flags, stream);
 }

@@ -26,7 +26,10 @@
 // `softmax(scores.float()).to(q.dtype)` does in the reference.
 #pragma once
 
+#include <type_traits>
+
 #include "attn_tile.hpp"
+#include "e4m3.hpp"
 
 namespace ir {
 
@@ -55,6 +58,9 @@ struct DecodeArgs {
   float* ws_o;        // [seq][q_head][part][D]
   float* ws_ml;       // [seq][q_head][part][2]
   int32_t* err;
+  // 8-bit caches: (K, V) scales [kv_head][block], 16-byte units of a block's codes
+  const f32x2* scales;
+  uint32_t block16;
 };
 
 // Per-lane byte offsets of this lane's K pieces and V rows inside a 16-token
@@ -77,6 +83,66 @@ __device__ __forceinline__ LaneOffsets<DT, D> lane_offsets(int lane, int64_t slo
 #pragma unroll
   for (int r = 0; r < 4; ++r) o.v[r] = (uint32_t)((4 * r + g) * slot_bytes + Sh::TILES * c * Sh::EB);
   return o;
+}
+
+// A tile of an 8-bit cache as it is loaded: 16 dense rows of D codes for K and for
+// V. K: the wavefront's 16-byte pieces in row order; V: head_dim/16 codes of rows
+// 4r+g. Half the bytes of a 16-bit tile, so a wavefront keeps twice as many in
+// flight for the same queue; the codes become numbers in registers (head_dim/4
+// conversions a lane and tile, against some 300 cycles of memory time a tile and CU).
+template <int D>
+struct CodeTile {
+  static constexpr int NI = D / 64;  // K load instructions
+  uint32_t k[4 * NI];
+  uint32_t v[4][NI];
+};
+
+// What a kernel streams: tiles of the dtype itself, or of codes.
+template <int DT, int D, bool Q8>
+struct CacheFormat {
+  typedef Tile<DT, D> Raw;
+  typedef LaneOffsets<DT, D> Offsets;
+  static constexpr int EB = TileShape<DT, D>::EB;          // bytes of an element
+  static constexpr int STAGE = KStage<DT, D>::BYTES;       // LDS bytes of a K tile
+  __device__ __forceinline__ static Offsets offsets(int lane, int64_t slot_bytes) {
+    return lane_offsets<DT, D>(lane, slot_bytes);
+  }
+};
+template <int DT, int D>
+struct CacheFormat<DT, D, true> {
+  typedef CodeTile<D> Raw;
+  struct Offsets {
+    uint32_t k, v;  // of this lane in a tile
+  };
+  static constexpr int EB = 1;
+  static constexpr int STAGE = 16 * D;
+  __device__ __forceinline__ static Offsets offsets(int lane, int64_t) {
+    return Offsets{(uint32_t)lane * 16u, (uint32_t)lane * (D / 16)};
+  }
+};
+
+// Issues a code tile's loads; the tile's first row is at tk / tv.
+template <int DT, int D>
+__device__ __forceinline__ void issue_codes(const uint8_t* tk, const uint8_t* tv,
+                                            const typename CacheFormat<DT, D, true>::Offsets& lo, CodeTile<D>& tl) {
+#pragma unroll
+  for (int i = 0; i < CodeTile<D>::NI; ++i) {
+    const u32x4 x = __builtin_nontemporal_load((const u32x4*)(tk + lo.k + 1024 * i));
+    tl.k[4 * i + 0] = x[0];
+    tl.k[4 * i + 1] = x[1];
+    tl.k[4 * i + 2] = x[2];
+    tl.k[4 * i + 3] = x[3];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if constexpr (D == 128) {
+      const u32x2 x = __builtin_nontemporal_load((const u32x2*)(tv + lo.v + 4 * D * r));
+      tl.v[r][0] = x[0];
+      tl.v[r][1] = x[1];
+    } else {
+      tl.v[r][0] = __builtin_nontemporal_load((const uint32_t*)(tv + lo.v + 4 * D * r));
+    }
+  }
 }
 
 // Issues the loads of the tile starting at key t0 and returns a 4-bit mask of
@@ -172,6 +238,84 @@ __device__ __forceinline__ void compute_tile(const Tile<DT, D>& tl, const uint32
   }
 }
 
+// The same for a tile of codes. The K codes go through LDS as they are and turn into
+// the operand there: lane group g of step j holds elements 64 j + 16 g .. + 15 of its
+// key (load_query_codes: the same of the query), one 16-byte read each. They are used
+// without their scale, which score_scale (times scale * log2 e) holds; the V codes
+// are multiplied by theirs, both exact.
+template <int DT, int D>
+__device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const uint32_t (&qr)[TileShape<DT, D>::KDW],
+                                              uint32_t kmask, float score_scale, float v_scale, uint8_t* kst, int lane,
+                                              State<D>& st, bool col_on = true) {
+  typedef TileShape<DT, D> Sh;
+  constexpr int CPR = D / 16;  // 16-byte chunks per row
+  const int g = lane >> 4, t = staged_token(lane & 15);
+#pragma unroll
+  for (int i = 0; i < CodeTile<D>::NI; ++i) {
+    const int row = (64 * i + lane) / CPR, ch = lane % CPR;
+    *(u32x4*)(kst + row * D + 16 * (ch ^ (row % CPR))) =
+        u32x4{tl.k[4 * i], tl.k[4 * i + 1], tl.k[4 * i + 2], tl.k[4 * i + 3]};
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  uint32_t kop[Sh::KDW];
+#pragma unroll
+  for (int j = 0; j < CodeTile<D>::NI; ++j) {
+    const u32x4 x = *(const u32x4*)(kst + t * D + 16 * ((4 * j + g) ^ (t % CPR)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (Sh::k16) {
+        kop[8 * j + 2 * i] = decode2<DT, false>(x[i], 1.f);
+        kop[8 * j + 2 * i + 1] = decode2<DT, true>(x[i], 1.f);
+      } else {
+        const f32x2 lo = decode2_f32<false>(x[i], 1.f), hi = decode2_f32<true>(x[i], 1.f);
+        kop[16 * j + 4 * i] = __float_as_uint(lo[0]);
+        kop[16 * j + 4 * i + 1] = __float_as_uint(lo[1]);
+        kop[16 * j + 4 * i + 2] = __float_as_uint(hi[0]);
+        kop[16 * j + 4 * i + 3] = __float_as_uint(hi[1]);
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const f32x4 s = qk_tile<DT, D>(kop, qr);
+  uint32_t v[4][Sh::VDW];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < CodeTile<D>::NI; ++i) {
+      if constexpr (Sh::k16) {
+        v[r][2 * i] = decode2<DT, false>(tl.v[r][i], v_scale);
+        v[r][2 * i + 1] = decode2<DT, true>(tl.v[r][i], v_scale);
+      } else {
+        const f32x2 lo = decode2_f32<false>(tl.v[r][i], v_scale), hi = decode2_f32<true>(tl.v[r][i], v_scale);
+        v[r][4 * i] = __float_as_uint(lo[0]);
+        v[r][4 * i + 1] = __float_as_uint(lo[1]);
+        v[r][4 * i + 2] = __float_as_uint(hi[0]);
+        v[r][4 * i + 3] = __float_as_uint(hi[1]);
+      }
+    }
+  float sv[4];
+  bool vok[4];
+  if (__all(kmask == 0xfu)) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vok[r] = true;
+      sv[r] = col_on ? s[r] * score_scale : kNegInf;
+    }
+    softmax_pv<DT, D, true>(sv, v, vok, st);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vok[r] = (kmask >> r) & 1u;
+      sv[r] = vok[r] && col_on ? s[r] * score_scale : kNegInf;
+    }
+    softmax_pv<DT, D, false>(sv, v, vok, st);
+  }
+}
+
 // Context length of `seq`, clamped to what its block table can hold (flagged).
 __device__ __forceinline__ int clamp_ctx(const DecodeArgs& a, int seq, bool report) {
   int ctx = a.ctx[seq];
@@ -187,11 +331,14 @@ __device__ __forceinline__ int clamp_ctx(const DecodeArgs& a, int seq, bool repo
 // (wavefront w takes tiles tile_lo + w, tile_lo + w + NW, ...) into st. Keys
 // at or past t_end are masked. Runs of up to NW * kMaxWaveTiles tiles: each
 // run fetches its block ids once, one per lane.
-template <int DT, int D, bool BS16, int NW, int DEPTH>
+template <int DT, int D, bool BS16, int NW, int DEPTH, bool Q8>
 __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t* bt_row, const uint8_t* kc,
-                                             const uint8_t* vc, const LaneOffsets<DT, D>& lo,
+                                             const uint8_t* vc, const f32x2* scales,
+                                             const typename CacheFormat<DT, D, Q8>::Offsets& lo,
                                              const uint32_t (&qr)[TileShape<DT, D>::KDW], int tile_lo, int tile_hi,
                                              int t_end, uint8_t* kst, int lane, int w, State<D>& st, bool& bad) {
+  static_assert(BS16 || !Q8, "a block of codes holds whole tiles");
+  typedef typename CacheFormat<DT, D, Q8>::Raw Raw;
   constexpr int RUN = NW * kMaxWaveTiles;
   for (int r0 = tile_lo; r0 < tile_hi; r0 += RUN) {
     const int ntiles = min(tile_hi - r0, RUN);
@@ -202,15 +349,39 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     if constexpr (BS16) {
       if (lane < my_tiles) bid_lane = bt_row[(t_begin + 16 * (w + NW * lane)) / a.bs];
     }
-    auto issue = [&](int i, Tile<DT, D>& tl) -> uint32_t {
+    f32x2 sc = {0.f, 0.f};  // scales of this lane's tile
+    if constexpr (Q8) {
+      if (lane < my_tiles && bid_lane >= 0 && (int64_t)bid_lane < a.num_blocks) sc = scales[bid_lane];
+    }
+    auto issue = [&](int i, Raw& tl) -> uint32_t {
       const int32_t bid = BS16 ? __builtin_amdgcn_readlane(bid_lane, i) : 0;
-      return load_tile<DT, D, BS16>(a, bt_row, bid, kc, vc, lo, t_begin + 16 * (w + NW * i), t_end, lane, tl, bad);
+      if constexpr (Q8) {
+        const int g = lane >> 4, t0 = t_begin + 16 * (w + NW * i), blk = t0 / a.bs;
+        const bool ok = bid >= 0 && (int64_t)bid < a.num_blocks;
+        bad |= !ok;
+        const int64_t at = ok ? ((int64_t)bid * a.bs + (t0 - blk * a.bs)) * D : 0;
+        issue_codes<DT, D>(kc + at, vc + at, lo, tl);
+        uint32_t m = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m |= (ok && t0 + 4 * r + g < t_end) ? (1u << r) : 0u;
+        return m;
+      } else
+        return load_tile<DT, D, BS16>(a, bt_row, bid, kc, vc, lo, t_begin + 16 * (w + NW * i), t_end, lane, tl, bad);
     };
     // Register ring of DEPTH tiles: while one tile is in the math, the next
     // DEPTH-1 tiles' loads are in flight.
     const int last = my_tiles - 1;
-    Tile<DT, D> ring[DEPTH];
+    Raw ring[DEPTH];
     uint32_t mk[DEPTH];
+    auto compute = [&](const Raw& tl, int i, uint32_t mask) {
+      if constexpr (Q8) {
+        const int ii = min(i, last);
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[0]), ii));
+        const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[1]), ii));
+        compute_codes<DT, D>(tl, qr, mask, a.scale_log2 * ks, vs, kst, lane, st);
+      } else
+        compute_tile<DT, D>(tl, qr, mask, a.scale_log2, kst, lane, st);
+    };
 #pragma unroll
     for (int r = 0; r < DEPTH; ++r) mk[r] = issue(min(r, last), ring[r]);
     int i = 0;
@@ -220,7 +391,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     for (; i + 2 * DEPTH <= my_tiles; i += DEPTH) {
 #pragma unroll
       for (int r = 0; r < DEPTH; ++r) {
-        compute_tile<DT, D>(ring[r], qr, mk[r], a.scale_log2, kst, lane, st);
+        compute(ring[r], i + r, mk[r]);
         mk[r] = issue(i + r + DEPTH, ring[r]);
       }
     }
@@ -230,7 +401,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     for (; i < my_tiles; i += DEPTH) {
 #pragma unroll
       for (int r = 0; r < DEPTH; ++r) {
-        compute_tile<DT, D>(ring[r], qr, i + r < my_tiles ? mk[r] : 0u, a.scale_log2, kst, lane, st);
+        compute(ring[r], i + r, i + r < my_tiles ? mk[r] : 0u);
         if (i + r + DEPTH <= last) mk[r] = issue(i + r + DEPTH, ring[r]);
       }
     }
@@ -247,6 +418,36 @@ __device__ __forceinline__ void load_query(const DecodeArgs& a, int seq, int qh,
                   qr);
   else
     zero_dwords(qr);
+}
+
+// The query operand that goes with code tiles (compute_codes).
+template <int DT, int D>
+__device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
+                                                 uint32_t (&qr)[TileShape<DT, D>::KDW]) {
+  typedef TileShape<DT, D> Sh;
+  if (!head_ok) {
+    zero_dwords(qr);
+    return;
+  }
+  const uint8_t* row = (const uint8_t*)a.q + ((int64_t)seq * a.q_seq + (int64_t)qh * a.q_head + 16 * g) * Sh::EB;
+  constexpr int DW = 4 * Sh::EB;  // dwords of 16 elements
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+    for (int i = 0; i < DW; i += 4) {
+      const u32x4 x = *(const u32x4*)(row + 64 * j * Sh::EB + 4 * i);
+      qr[DW * j + i + 0] = x[0];
+      qr[DW * j + i + 1] = x[1];
+      qr[DW * j + i + 2] = x[2];
+      qr[DW * j + i + 3] = x[3];
+    }
+}
+
+template <int DT, int D, bool Q8>
+__device__ __forceinline__ void load_query_for(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
+                                               uint32_t (&qr)[TileShape<DT, D>::KDW]) {
+  if constexpr (Q8) load_query_codes<DT, D>(a, seq, qh, head_ok, g, qr);
+  else load_query<DT, D>(a, seq, qh, head_ok, g, qr);
 }
 
 // Writes the workgroup's merged (normalised) result for heads head0..head0+nh.

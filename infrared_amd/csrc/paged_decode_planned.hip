@@ -481,17 +481,21 @@ __device__ __forceinline__ void slot_read(const float* row, int g, f32x4 (&acc)[
 // is built with kernel-argument preloading, which hands the leading scalar
 // arguments over in SGPRs at wave start, so the plan reads do not wait for a
 // kernel-argument load.
-template <int DT, int D, int NW, int DEPTH, bool PAIRS>
+//
+// Q8: the tiles are codes; a run's lanes also fetch the scales of their tiles, whose
+// block the tile's pool offset gives (the layer is dense), ahead of the tiles' own loads.
+template <int DT, int D, int NW, int DEPTH, bool PAIRS, bool Q8 = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 ? 1 : 2)))
 void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32_t o_pair, uint32_t o_whdr,
                                  uint32_t o_first, int B, DecodeArgs a, PlanLayout ly) {
   typedef TileShape<DT, D> Sh;
+  typedef CacheFormat<DT, D, Q8> F;
   constexpr int EB = Sh::EB;
   constexpr int NT = NW * 64;
   constexpr int TILES = D / 16;
   __shared__ WaveSlots<NW, D> sl;
   __shared__ WaveSlots<2, D> stg;  // this slice's cross-workgroup partials: [0] first unit, [1] last unit
-  __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][KStage<DT, D>::BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][F::STAGE];
   __shared__ int s_pre[kPlanMaxSeqs + 1];
   __shared__ int s_pair[PAIRS ? kPlanMaxSeqs : 1];
   __shared__ int s_fl[NW];
@@ -579,11 +583,11 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     const int kvh = a.n_hg == 1 ? j : fdiv(j, a.n_hg);
     if (paired(b)) {  // columns 0..n_rep-1: sequence b, n_rep..2 n_rep-1: b + 1
       const int second = c >= a.n_rep;
-      load_query<DT, D>(a, b + second, kvh * a.n_rep + c - second * a.n_rep, c < 2 * a.n_rep, g, dst);
+      load_query_for<DT, D, Q8>(a, b + second, kvh * a.n_rep + c - second * a.n_rep, c < 2 * a.n_rep, g, dst);
       return;
     }
     const int hl = hg * 16 + c;
-    load_query<DT, D>(a, b, kvh * a.n_rep + hl, hl < a.n_rep, g, dst);
+    load_query_for<DT, D, Q8>(a, b, kvh * a.n_rep + hl, hl < a.n_rep, g, dst);
   };
   uint32_t qr[Sh::KDW], qn[Sh::KDW];
   int q_lbl = -1, qn_lbl = -1;
@@ -599,7 +603,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   // ---- 2. the tile loop
   const uint8_t* kc = (const uint8_t*)a.kc;
   const uint8_t* vc = (const uint8_t*)a.vc;
-  const LaneOffsets<DT, D> lo_off = lane_offsets<DT, D>(lane, a.c_slot * EB);
+  const typename F::Offsets lo_off = F::offsets(lane, a.c_slot * F::EB);
   const int whi = wlo + cnt_w;
   State<D> st;
   state_init(st);
@@ -663,16 +667,23 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     }
     const int cnt = min(kPlanRun, cnt_w - r0);
     const int last = cnt - 1;
+    f32x2 sc = {0.f, 0.f};
+    if constexpr (Q8) {
+      if (lane < cnt) sc = a.scales[info_off / a.block16];
+    }
     // Issues the loads of tile i of the run (`real`: i is known to be a tile of
     // the run). Past the run's end (the ring's last DEPTH issues, never
     // computed) it issues nothing: the end phase reuses the ring's registers,
     // and a load still in flight into them would hold it up (padding loads
     // cost 0.7 us per call this way).
-    auto issue = [&](int i, Tile<DT, D>& tl, int& lb, bool& con, bool real) -> uint32_t {
+    auto issue = [&](int i, typename F::Raw& tl, int& lb, bool& con, bool real) -> uint32_t {
       const int ii = real || i <= last ? i : last;
       const uint32_t off = (uint32_t)__builtin_amdgcn_readlane((int)info_off, ii);
       const uint32_t meta = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, ii);
-      if (real || i <= last) issue_tile<DT, D>(kc, vc, off, lo_off, tl);
+      if (real || i <= last) {
+        if constexpr (Q8) issue_codes<DT, D>(kc + ((uint64_t)off << 4), vc + ((uint64_t)off << 4), lo_off, tl);
+        else issue_tile<DT, D>(kc, vc, off, lo_off, tl);
+      }
       lb = (int)(meta >> 7);
       // this lane's column half sees the tile (column mask bits 5, 6)
       con = !PAIRS || ((meta >> (c >= a.n_rep ? 6 : 5)) & 1u);
@@ -682,12 +693,13 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       for (int r = 0; r < 4; ++r) m |= (4 * r + g < valid) ? (1u << r) : 0u;
       return m;
     };
-    Tile<DT, D> ring[DEPTH];
+    typename F::Raw ring[DEPTH];
     uint32_t mk[DEPTH];
     int lb[DEPTH];
     bool con[DEPTH];
-    // Computes ring slot r, switching units (and queries) at a label change.
-    auto step = [&](int r) {
+    // Computes ring slot r, which holds tile i, switching units (and queries) at a
+    // label change.
+    auto step = [&](int r, int i) {
       if (lb[r] != cur) {
         if (cur >= 0) wave_finish(cur, false);
         cur = lb[r];
@@ -705,7 +717,13 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
           qn_lbl = cur + 1;
         }
       }
-      compute_tile<DT, D>(ring[r], qr, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
+      if constexpr (Q8) {
+        const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
+        const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
+        compute_codes<DT, D>(ring[r], qr, mk[r], a.scale_log2 * ks, vs, kstage[w], lane, st, con[r]);
+      } else {
+        compute_tile<DT, D>(ring[r], qr, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
+      }
     };
 #pragma unroll
     for (int r = 0; r < DEPTH; ++r) mk[r] = issue(r, ring[r], lb[r], con[r], false);
@@ -716,14 +734,14 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     for (; i + 2 * DEPTH <= cnt; i += DEPTH) {
 #pragma unroll
       for (int r = 0; r < DEPTH; ++r) {
-        step(r);
+        step(r, i + r);
         mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], true);
       }
     }
     for (; i < cnt; i += DEPTH) {
 #pragma unroll
       for (int r = 0; r < DEPTH; ++r) {
-        if (i + r < cnt) step(r);
+        if (i + r < cnt) step(r, i + r);
         mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], false);
       }
     }
@@ -839,6 +857,19 @@ void launch_planned_dt_d(const DecodeArgs& a, const uint8_t* plan, const PlanLay
                        0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
 }
 
+template <int DT, int D>
+void launch_planned_q8(const DecodeArgs& a, const uint8_t* plan, const PlanLayout& ly, int grid, bool pairs,
+                       hipStream_t s) {
+  const uint32_t o_sp = (uint32_t)ly.seq_pre, o_pr = (uint32_t)ly.pair, o_wh = (uint32_t)ly.whdr,
+                 o_fi = (uint32_t)ly.first;
+  if (pairs)
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kPlanWaves, 2, true, true>), dim3(grid),
+                       dim3(kPlanWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+  else
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kPlanWaves, 2, false, true>), dim3(grid),
+                       dim3(kPlanWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+}
+
 // Pairs fit one unit's 16 MFMA columns when a KV head has at most 8 query
 // heads (one head group).
 bool pairs_fit(int num_q_heads, int num_kv_heads) { return 2 * (num_q_heads / num_kv_heads) <= 16; }
@@ -887,7 +918,7 @@ extern "C" int ir_paged_decode_plan(const int32_t* block_tables, int64_t bt_stri
                                     int block_size, int64_t num_blocks, int64_t cache_slot_stride,
                                     int64_t cache_head_stride, int dtype, int flags, void* plan, int64_t plan_bytes,
                                     int32_t* err_flags, ir_stream_t stream) {
-  const int eb = dtype_bytes(dtype);
+  const int eb = dtype == IR_DTYPE_E4M3 ? 1 : dtype_bytes(dtype);
   IR_REQUIRE(eb > 0, "ir_paged_decode_plan: unknown dtype %d", dtype);
   IR_REQUIRE((flags & ~IR_PLAN_SHARE_GROUPS) == 0, "ir_paged_decode_plan: unknown flags 0x%x", flags);
   IR_REQUIRE(plannable(num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size),
@@ -930,36 +961,39 @@ extern "C" int ir_paged_decode_plan(const int32_t* block_tables, int64_t bt_stri
   return check_launch("ir_paged_decode_plan");
 }
 
-extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
-                                       const void* v_cache, int64_t cache_slot_stride, void* out,
-                                       int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
-                                       int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
-                                       int block_size, float scale, int dtype, int flags, const void* plan,
-                                       int32_t* counters, int64_t num_counters, void* workspace,
-                                       int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
+namespace {
+
+// ir_paged_decode_planned, and with `scales` ir_paged_decode_planned_q8 (a dense
+// layer of codes).
+int planned_call(const char* name, const float* scales, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                 const void* k_cache, const void* v_cache, int64_t cache_slot_stride, void* out,
+                 int64_t out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
+                 int head_dim, int max_blocks_per_seq, int block_size, float scale, int dtype, int flags,
+                 const void* plan, int32_t* counters, int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                 int32_t* err_flags, ir_stream_t stream) {
   const int eb = dtype_bytes(dtype);
-  IR_REQUIRE(eb > 0, "ir_paged_decode_planned: unknown dtype %d", dtype);
-  IR_REQUIRE((flags & ~IR_PLAN_SHARE_GROUPS) == 0, "ir_paged_decode_planned: unknown flags 0x%x", flags);
+  IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
+  IR_REQUIRE((flags & ~IR_PLAN_SHARE_GROUPS) == 0, "%s: unknown flags 0x%x", name, flags);
   if (head_dim != 64 && head_dim != 128)
-    return fail(IR_EUNSUPPORTED, "ir_paged_decode_planned: head_dim %d not supported (64, 128)", head_dim);
+    return fail(IR_EUNSUPPORTED, "%s: head_dim %d not supported (64, 128)", name, head_dim);
   IR_REQUIRE(plannable(num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size),
-             "ir_paged_decode_planned: shape not plannable");
-  IR_REQUIRE(plan && ((uintptr_t)plan & 255u) == 0, "ir_paged_decode_planned: plan missing or not 256-byte aligned");
-  IR_REQUIRE(q && k_cache && v_cache && out, "ir_paged_decode_planned: null pointer");
+             "%s: shape not plannable", name);
+  IR_REQUIRE(plan && ((uintptr_t)plan & 255u) == 0, "%s: plan missing or not 256-byte aligned", name);
+  IR_REQUIRE(q && k_cache && v_cache && out, "%s: null pointer", name);
   IR_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
-             "ir_paged_decode_planned: q, caches and out must be 16-byte aligned");
+             "%s: q, caches and out must be 16-byte aligned", name);
   IR_REQUIRE((q_seq_stride * eb) % 16 == 0 && (q_head_stride * eb) % 16 == 0 && (cache_slot_stride * eb) % 16 == 0 &&
                  (out_seq_stride * eb) % 16 == 0 && (out_head_stride * eb) % 16 == 0,
-             "ir_paged_decode_planned: strides must be multiples of 16 bytes");
+             "%s: strides must be multiples of 16 bytes", name);
   const int grid = device_cus();
   const int n_hg = n_hg_of(num_q_heads, num_kv_heads);
   const PlannedWs ws = planned_ws((int64_t)num_seqs * num_kv_heads * n_hg, grid, head_dim);
   if (!workspace || workspace_bytes < ws.total() || ((uintptr_t)workspace & 255u))
-    return fail(IR_EWORKSPACE, "ir_paged_decode_planned: workspace of %lld bytes (256-byte aligned) required, got %lld",
+    return fail(IR_EWORKSPACE, "%s: workspace of %lld bytes (256-byte aligned) required, got %lld", name,
                 (long long)ws.total(), (long long)workspace_bytes);
   const int64_t units = (int64_t)num_seqs * num_kv_heads * n_hg;
   if (!counters || num_counters < units)
-    return fail(IR_EWORKSPACE, "ir_paged_decode_planned: %lld arrival counters required, got %lld",
+    return fail(IR_EWORKSPACE, "%s: %lld arrival counters required, got %lld", name,
                 (long long)units, (long long)num_counters);
   DecodeArgs a;
   memset(&a, 0, sizeof(a));
@@ -980,6 +1014,8 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
   a.n_ups = num_kv_heads * n_hg;
   a.scale_log2 = scale * kLog2e;
   a.err = err_flags;
+  a.scales = (const f32x2*)scales;
+  a.block16 = (uint32_t)(block_size * (head_dim / 16));
   a.counters = counters;
   a.ws_o = (float*)workspace;
   a.ws_ml = (float*)((uint8_t*)workspace + ws.acc_bytes);
@@ -988,6 +1024,23 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
   const uint8_t* pl = (const uint8_t*)plan;
   hipStream_t s = (hipStream_t)stream;
   const bool pairs = (flags & IR_PLAN_SHARE_GROUPS) && pairs_fit(num_q_heads, num_kv_heads);
+  if (scales) {
+    IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+    switch (dtype) {
+      case IR_DTYPE_BF16:
+        head_dim == 128 ? launch_planned_q8<IR_DTYPE_BF16, 128>(a, pl, ly, grid, pairs, s)
+                        : launch_planned_q8<IR_DTYPE_BF16, 64>(a, pl, ly, grid, pairs, s);
+        break;
+      case IR_DTYPE_F16:
+        head_dim == 128 ? launch_planned_q8<IR_DTYPE_F16, 128>(a, pl, ly, grid, pairs, s)
+                        : launch_planned_q8<IR_DTYPE_F16, 64>(a, pl, ly, grid, pairs, s);
+        break;
+      default:
+        head_dim == 128 ? launch_planned_q8<IR_DTYPE_F32, 128>(a, pl, ly, grid, pairs, s)
+                        : launch_planned_q8<IR_DTYPE_F32, 64>(a, pl, ly, grid, pairs, s);
+    }
+    return check_launch(name);
+  }
   switch (dtype) {
     case IR_DTYPE_BF16:
       head_dim == 128 ? launch_planned_dt_d<IR_DTYPE_BF16, 128>(a, pl, ly, grid, pairs, s)
@@ -1001,5 +1054,34 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
       head_dim == 128 ? launch_planned_dt_d<IR_DTYPE_F32, 128>(a, pl, ly, grid, pairs, s)
                       : launch_planned_dt_d<IR_DTYPE_F32, 64>(a, pl, ly, grid, pairs, s);
   }
-  return check_launch("ir_paged_decode_planned");
+  return check_launch(name);
+}
+
+}  // namespace
+
+extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
+                                       const void* v_cache, int64_t cache_slot_stride, void* out,
+                                       int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
+                                       int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
+                                       int block_size, float scale, int dtype, int flags, const void* plan,
+                                       int32_t* counters, int64_t num_counters, void* workspace,
+                                       int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
+  return planned_call("ir_paged_decode_planned", nullptr, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                      cache_slot_stride, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                      max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
+                      workspace_bytes, err_flags, stream);
+}
+
+extern "C" int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void*
+                                          k_cache, const void* v_cache, const float* scales, void* out, int64_t
+                                          out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int
+                                          num_kv_heads, int head_dim, int max_blocks_per_seq, int block_size, float
+                                          scale, int dtype, int flags, const void* plan, int32_t* counters, int64_t
+                                          num_counters, void* workspace, int64_t workspace_bytes, int32_t* err_flags,
+                                          ir_stream_t stream) {
+  IR_REQUIRE(scales, "ir_paged_decode_planned_q8: null pointer");
+  return planned_call("ir_paged_decode_planned_q8", scales, q, q_seq_stride, q_head_stride, k_cache, v_cache, head_dim, out,
+                      out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                      max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
+                      workspace_bytes, err_flags, stream);
 }

@@ -69,6 +69,7 @@
 #include <type_traits>
 
 #include "attn_tile.hpp"
+#include "e4m3.hpp"
 #include "status.hpp"
 
 namespace ir {
@@ -122,6 +123,8 @@ struct PrefillArgs {
   const int64_t* write_slots;
   int64_t n_write, src_row0;
   int64_t n_work;  // attending workgroups (the grid less the writers)
+  // 8-bit caches: (K, V) scales [kv head][block] (null: the caches are of the dtype)
+  const f32x2* scales;
 };
 
 // 16-byte pieces a writer lane moves, all loads in flight before any store.
@@ -175,8 +178,6 @@ struct PShape {
   // conflicts only with 32 extra bytes per K row and 16 per V^T row (8 and 16
   // bytes still conflict two ways, measured with SQ_LDS_BANK_CONFLICT)
   static constexpr int KROW = D + 16;  // elements per K row in LDS
-  static constexpr int KCH = BN * D / 8;       // 16-byte K chunks per tile
-  static constexpr int KPT = (KCH + NT - 1) / NT;
   static constexpr int KS = D / 32;   // k-steps of S^T = K . Q^T
   static constexpr int DTL = D / 16;  // d tiles of O^T
 };
@@ -188,7 +189,11 @@ struct PShape {
 // and <= 256 registers, so two 4-wavefront workgroups share a CU).
 constexpr int kLockstep = 0, kRing2 = 2;
 
-template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false>
+// Q8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
+// key's K and of its V with the key's scales, and turns them into the dtype's
+// elements, exactly, where it stores them to LDS; from there on the walk is the
+// same.
+template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
   typedef PShape<D, NW, CTW> S;
@@ -267,8 +272,11 @@ void paged_prefill_kernel(PrefillArgs a) {
     return Col{tq0 + t, kvh * a.n_rep + (j - t * a.n_rep), t < TQ && tq0 + t < q_len};
   };
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
-  const uint16_t* kc = (const uint16_t*)a.kc + (int64_t)kvh * a.c_head;
-  const uint16_t* vc = (const uint16_t*)a.vc + (int64_t)kvh * a.c_head;
+  typedef typename std::conditional<Q8, uint8_t, uint16_t>::type Elt;  // cache element
+  const Elt* kc = (const Elt*)a.kc + (int64_t)kvh * a.c_head;
+  const Elt* vc = (const Elt*)a.vc + (int64_t)kvh * a.c_head;
+  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
+  static_assert(!(FUSED && Q8), "new rows are quantised before they are attended");
 
   // ---- Q^T operands: lane (g, c) holds d = 32 ks + 8 g .. +7 of its column,
   // multiplied by scale * log2(e) and rounded back to the input dtype, so the
@@ -310,7 +318,7 @@ void paged_prefill_kernel(PrefillArgs a) {
   // Slot of absolute key k and whether it may be used: keys at or past kmax are
   // masked out; a bad block id is flagged and its K and V read as zeros. Every
   // load is issued (from slot 0 when unusable) and zeroed afterwards.
-  auto slot_of = [&](int k, bool& use) -> int64_t {
+  auto slot_of = [&](int k, bool& use, int32_t& block) -> int64_t {
     const bool in = k < kmax;
     // an unusable key looks up the cache's first id, inside the staged
     // window (key 0 would index below it once the window has moved)
@@ -320,6 +328,7 @@ void paged_prefill_kernel(PrefillArgs a) {
       const int32_t bid = bt_lds[blk - bt_base];
       use = in && (uint32_t)bid < (uint32_t)a.num_blocks;
       bad |= in && !use;
+      block = use ? bid : 0;
       const int sl = use ? (bid << a.bs_shift) | (kk & (a.bs - 1)) : 0;
       return (int64_t)(uint32_t)__mul24(sl, a.c_slot32);  // element offset
     } else {
@@ -327,6 +336,7 @@ void paged_prefill_kernel(PrefillArgs a) {
       const int32_t bid = bt_lds[blk - bt_base];
       use = in && bid >= 0 && (int64_t)bid < a.num_blocks;
       bad |= in && !use;
+      block = use ? bid : 0;
       return use ? ((int64_t)bid * a.bs + (kk - blk * a.bs)) * a.c_slot : 0;
     }
   };
@@ -336,74 +346,98 @@ void paged_prefill_kernel(PrefillArgs a) {
 
   // K and V of a key share its slot: each thread loads the same 16-byte
   // piece of both
-  u32x4 kreg[S::KPT], vreg[S::KPT];
+  constexpr int PE = Q8 ? 16 : 8;                // elements of a piece
+  constexpr int PIECES = BN * D / PE;            // pieces of a tile
+  constexpr int KPT = (PIECES + NT - 1) / NT;    // of a thread
+  u32x4 kreg[KPT], vreg[KPT];
+  f32x2 screg[KPT];  // Q8: the pieces' scales
   // whether each load in flight reads a usable key: applied when the tile is
   // stored (zero_unless), not when it is loaded, so the loads stay in flight
   // through the next tile's math instead of being waited for at once
-  bool kuse[S::KPT];
+  bool kuse[KPT];
   // Global loads of key tile kb into registers (whole workgroup, uniform call).
   // In a fused call, a tile holding the sequence's new keys reads those keys
   // from the call's new rows (the writers fill their slots concurrently).
   const uint16_t* kn = a.k_new ? (const uint16_t*)a.k_new + (int64_t)kvh * a.kn_head : nullptr;
   const uint16_t* vn = a.v_new ? (const uint16_t*)a.v_new + (int64_t)kvh * a.vn_head : nullptr;
   const int64_t new_row0 = a.src_row0 + q_lo - p0;  // row of new key k: new_row0 + k
-  auto load_into = [&](int kb, u32x4 (&kr)[S::KPT], u32x4 (&vr)[S::KPT], bool (&ku)[S::KPT]) {
+  auto load_into = [&](int kb, u32x4 (&kr)[KPT], u32x4 (&vr)[KPT], f32x2 (&sc)[KPT], bool (&ku)[KPT]) {
     const int k0 = kb * BN;
     const int k_last = min(k0 + BN, kmax) - 1;
     const int last_blk = FAST ? k_last >> a.bs_shift : k_last / a.bs;
     if (last_blk >= bt_base + kBtCache) fill_bt(FAST ? k0 >> a.bs_shift : k0 / a.bs);
-    if (FUSED && k0 + BN > p0) {  // uniform: new keys in this tile
+    int32_t block;
+    if constexpr (FUSED) {
+      if (k0 + BN > p0) {  // uniform: new keys in this tile
 #pragma unroll
-      for (int i = 0; i < S::KPT; ++i) {
-        const int q = tid + NT * i;
-        if (S::KCH % NT == 0 || q < S::KCH) {
-          const int key = q / (D / 8), part = q % (D / 8);
-          const int kk = k0 + key;
-          // a new key is read from the call's rows and needs no block id (the
-          // check after the walk flags a bad one): a tile of new keys only
-          // may be loaded before the block ids are
-          const bool fresh = kk >= p0 && kk < kmax;
-          bool use = fresh;
-          int64_t sl = 0;
-          if (!fresh) sl = slot_of(kk, use);
-          const int64_t row = new_row0 + kk;
-          const uint16_t* kp = fresh ? kn + row * a.kn_tok + part * 8 : kc + sl + part * 8;
-          const uint16_t* vp = fresh ? vn + row * a.vn_tok + part * 8 : vc + sl + part * 8;
-          kr[i] = *(const u32x4*)kp;
-          vr[i] = *(const u32x4*)vp;
-          ku[i] = use;
+        for (int i = 0; i < KPT; ++i) {
+          const int q = tid + NT * i;
+          if (PIECES % NT == 0 || q < PIECES) {
+            const int key = q / (D / PE), part = q % (D / PE);
+            const int kk = k0 + key;
+            // a new key is read from the call's rows and needs no block id (the
+            // check after the walk flags a bad one): a tile of new keys only
+            // may be loaded before the block ids are
+            const bool fresh = kk >= p0 && kk < kmax;
+            bool use = fresh;
+            int64_t sl = 0;
+            if (!fresh) sl = slot_of(kk, use, block);
+            const int64_t row = new_row0 + kk;
+            const uint16_t* kp = fresh ? kn + row * a.kn_tok + part * PE : kc + sl + part * PE;
+            const uint16_t* vp = fresh ? vn + row * a.vn_tok + part * PE : vc + sl + part * PE;
+            kr[i] = *(const u32x4*)kp;
+            vr[i] = *(const u32x4*)vp;
+            ku[i] = use;
+          }
         }
+        return;
       }
-      return;
     }
 #pragma unroll
-    for (int i = 0; i < S::KPT; ++i) {
+    for (int i = 0; i < KPT; ++i) {
       const int q = tid + NT * i;
-      if (S::KCH % NT == 0 || q < S::KCH) {
-        const int key = q / (D / 8), part = q % (D / 8);
+      if (PIECES % NT == 0 || q < PIECES) {
+        const int key = q / (D / PE), part = q % (D / PE);
         bool use;
-        const int64_t sl = slot_of(k0 + key, use);
-        kr[i] = *(const u32x4*)(kc + sl + part * 8);
-        vr[i] = *(const u32x4*)(vc + sl + part * 8);
+        const int64_t sl = slot_of(k0 + key, use, block);
+        kr[i] = *(const u32x4*)(kc + sl + part * PE);
+        vr[i] = *(const u32x4*)(vc + sl + part * PE);
+        if constexpr (Q8) sc[i] = scales[block];
         ku[i] = use;
       }
     }
   };
-  auto load_regs = [&](int kb) { load_into(kb, kreg, vreg, kuse); };
+  auto load_regs = [&](int kb) { load_into(kb, kreg, vreg, screg, kuse); };
   // Registers -> LDS buffer `buf`: K and V tiles both row-major [64 keys][D]
   // (+32 bytes a row).
-  auto store_from = [&](int buf, const u32x4 (&kr)[S::KPT], const u32x4 (&vr)[S::KPT], const bool (&ku)[S::KPT]) {
+  auto store_from = [&](int buf, const u32x4 (&kr)[KPT], const u32x4 (&vr)[KPT], const f32x2 (&sc)[KPT],
+                        const bool (&ku)[KPT]) {
 #pragma unroll
-    for (int i = 0; i < S::KPT; ++i) {
+    for (int i = 0; i < KPT; ++i) {
       const int q = tid + NT * i;
-      if (q < S::KCH) {
-        const int key = q / (D / 8), part = q % (D / 8);
-        *(u32x4*)&ks_lds[buf][key * S::KROW + part * 8] = zero_unless(kr[i], ku[i]);
-        *(u32x4*)&vs_lds[buf][key * S::KROW + part * 8] = zero_unless(vr[i], ku[i]);
+      if (q < PIECES) {
+        const int key = q / (D / PE), part = q % (D / PE);
+        const u32x4 k4 = zero_unless(kr[i], ku[i]), v4 = zero_unless(vr[i], ku[i]);
+        uint16_t* kp = &ks_lds[buf][key * S::KROW + part * PE];
+        uint16_t* vp = &vs_lds[buf][key * S::KROW + part * PE];
+        if constexpr (Q8) {
+          auto wide = [](uint16_t* to, u32x4 x, float scale) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *(u32x4*)(to + 8 * h) =
+                  u32x4{decode2<DT, false>(x[2 * h], scale), decode2<DT, true>(x[2 * h], scale),
+                        decode2<DT, false>(x[2 * h + 1], scale), decode2<DT, true>(x[2 * h + 1], scale)};
+          };
+          wide(kp, k4, sc[i][0]);
+          wide(vp, v4, sc[i][1]);
+        } else {
+          *(u32x4*)kp = k4;
+          *(u32x4*)vp = v4;
+        }
       }
     }
   };
-  auto store_regs = [&](int buf) { store_from(buf, kreg, vreg, kuse); };
+  auto store_regs = [&](int buf) { store_from(buf, kreg, vreg, screg, kuse); };
   // V^T operand of PV step t (d tile t % DTL, 32-key step t / DTL) from the
   // row-major V tile at vb: lane (g, c) needs V[32 st + 4 g + e][16 dt + c]
   // (k-slots 0..3) and V[32 st + 16 + 4 g + e][..] (4..7), e = 0..3: the
@@ -577,20 +611,21 @@ void paged_prefill_kernel(PrefillArgs a) {
     // block ids are, with Q's loads.
     constexpr int R = 4;
     if (t_lo < t_hi) {
-      u32x4 kr[R][S::KPT], vr[R][S::KPT];
-      bool ku[R][S::KPT];
+      u32x4 kr[R][KPT], vr[R][KPT];
+      f32x2 sc8[R][KPT];
+      bool ku[R][KPT];
       const int bt0 = FAST ? (t_lo * BN) >> a.bs_shift : (t_lo * BN) / a.bs;
       if (FUSED && t_lo * BN >= p0) {  // uniform
-        load_into(t_lo, kr[0], vr[0], ku[0]);
+        load_into(t_lo, kr[0], vr[0], sc8[0], ku[0]);
         fill_bt(bt0);
       } else {
         fill_bt(bt0);
-        load_into(t_lo, kr[0], vr[0], ku[0]);
+        load_into(t_lo, kr[0], vr[0], sc8[0], ku[0]);
       }
 #pragma unroll
       for (int j = 1; j < R; ++j)
-        if (t_lo + j < t_hi) load_into(t_lo + j, kr[j], vr[j], ku[j]);
-      store_from(t_lo & 1, kr[0], vr[0], ku[0]);
+        if (t_lo + j < t_hi) load_into(t_lo + j, kr[j], vr[j], sc8[j], ku[j]);
+      store_from(t_lo & 1, kr[0], vr[0], sc8[0], ku[0]);
       __syncthreads();
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -616,8 +651,9 @@ void paged_prefill_kernel(PrefillArgs a) {
 #pragma unroll
         for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
         step(std::false_type{}, kb, sc, sc);
-        if (kb + 1 < t_hi) store_from((kb + 1) & 1, kr[(J + 1) % R], vr[(J + 1) % R], ku[(J + 1) % R]);
-        if (kb + R < t_hi) load_into(kb + R, kr[J], vr[J], ku[J]);
+        if (kb + 1 < t_hi)
+          store_from((kb + 1) & 1, kr[(J + 1) % R], vr[(J + 1) % R], sc8[(J + 1) % R], ku[(J + 1) % R]);
+        if (kb + R < t_hi) load_into(kb + R, kr[J], vr[J], sc8[J], ku[J]);
         __syncthreads();
       };
       for (int kb = t_lo; kb < t_hi; kb += R) {
@@ -831,7 +867,7 @@ void paged_prefill_kernel(PrefillArgs a) {
 constexpr int kF32Threads = 256;
 constexpr int kF32Cols = 64;
 
-template <int D, bool FAST>
+template <int D, bool FAST, bool Q8 = false>
 __global__ __launch_bounds__(kF32Threads) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_prefill_f32_kernel(PrefillArgs a) {
   constexpr int NT = kF32Threads, BN = 64, MT = D / 16, DT4 = D / 4;
@@ -910,8 +946,11 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
   }
 
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
-  const float* kc = (const float*)a.kc + (int64_t)kvh * a.c_head;
-  const float* vc = (const float*)a.vc + (int64_t)kvh * a.c_head;
+  typedef typename std::conditional<Q8, uint8_t, float>::type Elt;  // cache element
+  typedef typename std::conditional<Q8, uint32_t, f32x4>::type Four;
+  const Elt* kc = (const Elt*)a.kc + (int64_t)kvh * a.c_head;
+  const Elt* vc = (const Elt*)a.vc + (int64_t)kvh * a.c_head;
+  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
   const int nblk_needed = (kmax + a.bs - 1) / a.bs;
   int bt_base = 0;
   auto fill_bt = [&](int base) {
@@ -923,7 +962,7 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
   bool bad = false;
   // element offset of key k's row in the pool and whether it may be used
   // (keys past kmax are masked; a bad block id is flagged and reads as zeros)
-  auto slot_of = [&](int k, bool& use) -> int64_t {
+  auto slot_of = [&](int k, bool& use, int32_t& block) -> int64_t {
     const bool in = k < kmax;
     const int kk = in ? k : bt_base * a.bs;
     if constexpr (FAST) {
@@ -931,6 +970,7 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
       const int32_t bid = bt_lds[blk - bt_base];
       use = in && (uint32_t)bid < (uint32_t)a.num_blocks;
       bad |= in && !use;
+      block = use ? bid : 0;
       const int sl = use ? (bid << a.bs_shift) | (kk & (a.bs - 1)) : 0;
       return (int64_t)(uint32_t)__mul24(sl, a.c_slot32);
     } else {
@@ -938,13 +978,23 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
       const int32_t bid = bt_lds[blk - bt_base];
       use = in && bid >= 0 && (int64_t)bid < a.num_blocks;
       bad |= in && !use;
+      block = use ? bid : 0;
       return use ? ((int64_t)bid * a.bs + (kk - blk * a.bs)) * a.c_slot : 0;
     }
   };
   // a tile's 4-key x 4-d blocks: block b = tid + NT i holds keys 4 (b / DT4)
   // .. +3 at d = 4 (b % DT4) .. +3
-  f32x4 kr[BPT][4], vr[BPT][4];
+  Four kr[BPT][4], vr[BPT][4];
+  f32x2 sc[BPT];  // Q8: the scales of the four keys, which share a block
   bool ku[BPT][4];
+  auto widen = [](Four x, float scale) -> f32x4 {
+    if constexpr (Q8) {
+      const f32x2 lo = decode2_f32<false>(x, scale), hi = decode2_f32<true>(x, scale);
+      return f32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      return x;
+    }
+  };
   auto load_tile = [&](int kb) {
     const int k0 = kb * BN;
     const int k_last = min(k0 + BN, kmax) - 1;
@@ -956,10 +1006,12 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         bool use;
-        const int64_t sl = slot_of(k0 + 4 * key4 + e, use);
-        kr[i][e] = *(const f32x4*)(kc + sl + 4 * d4);
-        vr[i][e] = *(const f32x4*)(vc + sl + 4 * d4);
+        int32_t block;
+        const int64_t sl = slot_of(k0 + 4 * key4 + e, use, block);
+        kr[i][e] = *(const Four*)(kc + sl + 4 * d4);
+        vr[i][e] = *(const Four*)(vc + sl + 4 * d4);
         ku[i][e] = use;
+        if (Q8 && e == 0) sc[i] = scales[block];
       }
     }
   };
@@ -968,13 +1020,17 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < BPT; ++i) {
       const int b = tid + NT * i, key4 = b / DT4, d4 = b - key4 * DT4;
+      const float k_scale = Q8 ? sc[i][0] : 1.f, v_scale = Q8 ? sc[i][1] : 1.f;
+      f32x4 v4[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) *(f32x4*)&ks[(4 * key4 + e) * KROW + 4 * d4] = ku[i][e] ? kr[i][e] : zero;
+      for (int e = 0; e < 4; ++e) {
+        *(f32x4*)&ks[(4 * key4 + e) * KROW + 4 * d4] = ku[i][e] ? widen(kr[i][e], k_scale) : zero;
+        v4[e] = widen(vr[i][e], v_scale);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        *(f32x4*)&vt[(4 * d4 + r) * VROW + 4 * key4] =
-            f32x4{ku[i][0] ? vr[i][0][r] : 0.f, ku[i][1] ? vr[i][1][r] : 0.f, ku[i][2] ? vr[i][2][r] : 0.f,
-                  ku[i][3] ? vr[i][3][r] : 0.f};
+        *(f32x4*)&vt[(4 * d4 + r) * VROW + 4 * key4] = f32x4{ku[i][0] ? v4[0][r] : 0.f, ku[i][1] ? v4[1][r] : 0.f,
+                                                             ku[i][2] ? v4[2][r] : 0.f, ku[i][3] ? v4[3][r] : 0.f};
     }
   };
 
@@ -1140,10 +1196,15 @@ int launch_prefill_f32(PrefillArgs a, hipStream_t s) {
   const int64_t slots = a.num_blocks * a.bs;
   const bool fast = a.bs_shift >= 0 && slots < (1 << 23) && a.c_slot < (1 << 23) &&
                     (slots * a.c_slot + a.c_head * a.num_kv_heads) < ((int64_t)1 << 31);
-  if (fast)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true>), dim3((unsigned)grid), dim3(kF32Threads), 0, s, a);
+  const dim3 g((unsigned)grid), block(kF32Threads);
+  if (a.scales && fast)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, true>), g, block, 0, s, a);
+  else if (a.scales)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, true>), g, block, 0, s, a);
+  else if (fast)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true>), g, block, 0, s, a);
   else
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false>), dim3((unsigned)grid), dim3(kF32Threads), 0, s, a);
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false>), g, block, 0, s, a);
   return check_launch("ir_paged_prefill");
 }
 
@@ -1657,6 +1718,32 @@ int launch_prefill(PrefillArgs a, int sched, hipStream_t s) {
   return check_launch("ir_paged_prefill");
 }
 
+// An 8-bit cache: launch_prefill's shapes by the same rules (2-deep rings), the
+// step's rows already written.
+template <int DT, int D>
+int launch_prefill_q8(const PrefillArgs& a, hipStream_t s) {
+  const int64_t grid = a.items ? a.n_items_grid : (int64_t)a.n_qblocks * a.num_kv_heads * a.num_seqs;
+  if (grid <= 0) return ok();
+  if (grid > 0x7fffffff)
+    return fail(IR_EINVAL, "ir_paged_prefill_q8: grid of %lld workgroups too large", (long long)grid);
+  const int64_t slots = a.num_blocks * a.bs;
+  const bool fast = a.bs_shift >= 0 && slots < (1 << 23) &&
+                    (slots * a.c_slot + a.c_head * a.num_kv_heads) < ((int64_t)1 << 31);
+#define IR_PREFILL_Q8(NW_, CT_)                                                                                    \
+  do {                                                                                                            \
+    const dim3 g((unsigned)grid), block(NW_ * 64);                                                                \
+    if (fast)                                                                                                     \
+      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, true, NW_, CT_, kRing2, false, true>), g, block, 0, s, a);  \
+    else                                                                                                          \
+      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, false, NW_, CT_, kRing2, false, true>), g, block, 0, s, a); \
+  } while (0)
+  if (a.nw == 4 && !a.items && grid <= device_cus()) IR_PREFILL_Q8(8, 1);
+  else if (a.nw == 4) IR_PREFILL_Q8(4, 2);
+  else IR_PREFILL_Q8(8, 2);
+#undef IR_PREFILL_Q8
+  return check_launch("ir_paged_prefill_q8");
+}
+
 }  // namespace
 }  // namespace ir
 
@@ -1675,43 +1762,49 @@ extern "C" int64_t ir_paged_prefill_plan_bytes(int num_seqs, int max_q_len, int 
 
 extern "C" int ir_paged_prefill_plan_xcds(void) { return plan_xcds(); }
 
-extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
-                                const void* v_cache, int64_t cache_slot_stride, int64_t cache_head_stride,
-                                int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
-                                int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
-                                int num_seqs, int total_q, int max_q_len, void* out, int64_t out_tok_stride,
-                                int64_t out_head_stride, int num_q_heads, int num_kv_heads, int head_dim, float scale,
-                                int dtype, void* plan, int64_t plan_bytes, const void* k_new,
-                                int64_t k_new_tok_stride, int64_t k_new_head_stride, const void* v_new,
-                                int64_t v_new_tok_stride, int64_t v_new_head_stride, const int64_t* write_slots,
-                                int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
+namespace {
+
+// ir_paged_prefill, and with `scales` ir_paged_prefill_q8 (a dense layer of codes).
+int prefill_call(const char* name, const float* scales, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                 const void* k_cache, const void* v_cache, int64_t cache_slot_stride, int64_t cache_head_stride,
+                 int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride, int
+                 max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q,
+                 int max_q_len, void* out, int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads, int
+                 num_kv_heads, int head_dim, float scale, int dtype, void* plan, int64_t plan_bytes, const void* k_new,
+                 int64_t k_new_tok_stride, int64_t k_new_head_stride, const void* v_new, int64_t v_new_tok_stride,
+                 int64_t v_new_head_stride, const int64_t* write_slots, int64_t n_write, int64_t src_row0, int32_t*
+                 err_flags, ir_stream_t stream) {
   IR_REQUIRE(dtype == IR_DTYPE_BF16 || dtype == IR_DTYPE_F16 || dtype == IR_DTYPE_F32,
-             "ir_paged_prefill: unknown dtype %d", dtype);
+             "%s: unknown dtype %d", name, dtype);
   const bool f32 = dtype == IR_DTYPE_F32;
   const int eb = f32 ? 4 : 2;
   IR_REQUIRE(num_seqs >= 0 && total_q >= 0 && max_q_len >= 0 && num_q_heads > 0 && num_kv_heads > 0 &&
                  block_size > 0 && max_blocks_per_seq >= 0 && num_blocks >= 0,
-             "ir_paged_prefill: bad sizes");
-  IR_REQUIRE(num_q_heads % num_kv_heads == 0, "ir_paged_prefill: num_q_heads %d not a multiple of num_kv_heads %d",
+             "%s: bad sizes", name);
+  IR_REQUIRE(num_q_heads % num_kv_heads == 0, "%s: num_q_heads %d not a multiple of num_kv_heads %d", name,
              num_q_heads, num_kv_heads);
-  IR_REQUIRE(num_q_heads / num_kv_heads <= 256, "ir_paged_prefill: more than 256 query heads per KV head");
+  IR_REQUIRE(num_q_heads / num_kv_heads <= 256, "%s: more than 256 query heads per KV head", name);
   if (f32 && num_q_heads / num_kv_heads > kF32Cols)
-    return fail(IR_EUNSUPPORTED, "ir_paged_prefill: fp32 with more than %d query heads per KV head", kF32Cols);
+    return fail(IR_EUNSUPPORTED, "%s: fp32 with more than %d query heads per KV head", name, kF32Cols);
   if (head_dim != 64 && head_dim != 128)
-    return fail(IR_EUNSUPPORTED, "ir_paged_prefill: head_dim %d not supported (64, 128)", head_dim);
+    return fail(IR_EUNSUPPORTED, "%s: head_dim %d not supported (64, 128)", name, head_dim);
   IR_REQUIRE((int64_t)max_blocks_per_seq * block_size <= (int64_t)1 << 30,
-             "ir_paged_prefill: block tables of %d x %d tokens exceed 2^30 keys", max_blocks_per_seq, block_size);
-  IR_REQUIRE(scale > 0.f, "ir_paged_prefill: scale must be positive");
+             "%s: block tables of %d x %d tokens exceed 2^30 keys", name, max_blocks_per_seq, block_size);
+  IR_REQUIRE(scale > 0.f, "%s: scale must be positive", name);
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
   IR_REQUIRE(q && k_cache && v_cache && block_tables && cu_seqlens_q && q_start && out,
-             "ir_paged_prefill: null pointer");
+             "%s: null pointer", name);
   // each output store is 4 elements: 8 bytes in 16-bit dtypes, 16 in fp32
   IR_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && ((uintptr_t)out % (4 * eb)) == 0,
-             "ir_paged_prefill: q and caches must be 16-byte aligned, out %d-byte aligned", 4 * eb);
+             "%s: q and caches must be 16-byte aligned, out %d-byte aligned", name, 4 * eb);
   IR_REQUIRE((q_tok_stride * eb) % 16 == 0 && (q_head_stride * eb) % 16 == 0 && (cache_slot_stride * eb) % 16 == 0 &&
                  (cache_head_stride * eb) % 16 == 0 && (out_tok_stride * eb) % (4 * eb) == 0 &&
                  (out_head_stride * eb) % (4 * eb) == 0,
-             "ir_paged_prefill: q/cache strides must be multiples of 16 bytes, out strides of %d bytes", 4 * eb);
+             "%s: q/cache strides must be multiples of 16 bytes, out strides of %d bytes", name, 4 * eb);
+  if (scales) {
+    IR_REQUIRE(block_size % 16 == 0, "%s: block size %d must be a multiple of 16", name, block_size);
+    IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+  }
   PrefillArgs a;
   memset(&a, 0, sizeof(a));
   a.q = q;
@@ -1738,13 +1831,13 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
   a.tq = geo.tq;
   a.n_qblocks = geo.n_qblocks;
   const int64_t n_items = (int64_t)num_seqs * a.n_qblocks;
-  IR_REQUIRE(n_items * num_kv_heads <= 0x7fffffff, "ir_paged_prefill: %lld work items x %d KV heads",
+  IR_REQUIRE(n_items * num_kv_heads <= 0x7fffffff, "%s: %lld work items x %d KV heads", name,
              (long long)n_items, num_kv_heads);
   if (plan) {
     const PlanLayout ly = plan_layout(geo, num_seqs, num_kv_heads, head_dim);
     IR_REQUIRE(plan_bytes >= ly.total && ((uintptr_t)plan & 255u) == 0,
-               "ir_paged_prefill: plan of %lld bytes (256-byte aligned) required, got %lld (build it with "
-               "ir_paged_prefill_plan for the same metadata and shapes)",
+               "%s: plan of %lld bytes (256-byte aligned) required, got %lld (build it with "
+               "ir_paged_prefill_plan for the same metadata and shapes)", name,
                (long long)ly.total, (long long)plan_bytes);
     uint8_t* pl = (uint8_t*)plan;
     a.items = (const int2*)pl;
@@ -1754,14 +1847,14 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
     a.n_items_grid = ly.entries;
   }
   if (k_new != nullptr) {
-    IR_REQUIRE(v_new && write_slots, "ir_paged_prefill: k_new given without v_new or write_slots");
+    IR_REQUIRE(v_new && write_slots, "%s: k_new given without v_new or write_slots", name);
     IR_REQUIRE(n_write >= 1 && src_row0 >= 0 && src_row0 + total_q <= n_write,
-               "ir_paged_prefill: the new rows [%lld, %lld) must lie within the %lld rows written",
+               "%s: the new rows [%lld, %lld) must lie within the %lld rows written", name,
                (long long)src_row0, (long long)src_row0 + total_q, (long long)n_write);
     IR_REQUIRE(aligned16(k_new) && aligned16(v_new) && (k_new_tok_stride * eb) % 16 == 0 &&
                    (k_new_head_stride * eb) % 16 == 0 && (v_new_tok_stride * eb) % 16 == 0 &&
                    (v_new_head_stride * eb) % 16 == 0,
-               "ir_paged_prefill: k_new / v_new must be 16-byte aligned with 16-byte strides");
+               "%s: k_new / v_new must be 16-byte aligned with 16-byte strides", name);
     a.k_new = k_new;
     a.v_new = v_new;
     a.kn_tok = k_new_tok_stride;
@@ -1772,6 +1865,7 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
     a.n_write = n_write;
     a.src_row0 = src_row0;
   }
+  a.scales = (const f32x2*)scales;
   a.out = out;
   a.o_tok = out_tok_stride;
   a.o_head = out_head_stride;
@@ -1780,12 +1874,53 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
   a.scale_log2 = scale * kLog2e;
   a.err = err_flags;
   hipStream_t s = (hipStream_t)stream;
+  if (scales && !f32) {
+    if (dtype == IR_DTYPE_BF16)
+      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128>(a, s) : launch_prefill_q8<IR_DTYPE_BF16, 64>(a, s);
+    return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_F16, 128>(a, s) : launch_prefill_q8<IR_DTYPE_F16, 64>(a, s);
+  }
   if (f32) return head_dim == 128 ? launch_prefill_f32<128>(a, s) : launch_prefill_f32<64>(a, s);
   if (dtype == IR_DTYPE_BF16)
     return head_dim == 128 ? launch_prefill<IR_DTYPE_BF16, 128>(a, geo.sched, s)
                            : launch_prefill<IR_DTYPE_BF16, 64>(a, geo.sched, s);
   return head_dim == 128 ? launch_prefill<IR_DTYPE_F16, 128>(a, geo.sched, s)
                          : launch_prefill<IR_DTYPE_F16, 64>(a, geo.sched, s);
+}
+
+}  // namespace
+
+extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
+                                const void* v_cache, int64_t cache_slot_stride, int64_t cache_head_stride,
+                                int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                                int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
+                                int num_seqs, int total_q, int max_q_len, void* out, int64_t out_tok_stride,
+                                int64_t out_head_stride, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                                int dtype, void* plan, int64_t plan_bytes, const void* k_new,
+                                int64_t k_new_tok_stride, int64_t k_new_head_stride, const void* v_new,
+                                int64_t v_new_tok_stride, int64_t v_new_head_stride, const int64_t* write_slots,
+                                int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
+  return prefill_call("ir_paged_prefill", nullptr, q, q_tok_stride, q_head_stride, k_cache, v_cache, cache_slot_stride,
+                      cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
+                      cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride, out_head_stride,
+                      num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, k_new, k_new_tok_stride,
+                      k_new_head_stride, v_new, v_new_tok_stride, v_new_head_stride, write_slots, n_write, src_row0,
+                      err_flags, stream);
+}
+
+extern "C" int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
+                                   const void* v_cache, const float* scales, int64_t num_blocks, int block_size, const
+                                   int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq, const int32_t*
+                                   cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q, int max_q_len,
+                                   void* out, int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads, int
+                                   num_kv_heads, int head_dim, float scale, int dtype, void* plan, int64_t plan_bytes,
+                                   int32_t* err_flags, ir_stream_t stream) {
+  if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
+  IR_REQUIRE(scales, "ir_paged_prefill_q8: null pointer");
+  return prefill_call("ir_paged_prefill_q8", scales, q, q_tok_stride, q_head_stride, k_cache, v_cache, head_dim,
+                      num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
+                      max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
+                      out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, nullptr, 0,
+                      0, nullptr, 0, 0, nullptr, 0, 0, err_flags, stream);
 }
 
 extern "C" int ir_paged_prefill_plan(const int32_t* cu_seqlens_q, const int32_t* q_start, const int32_t* block_tables,

@@ -13,7 +13,9 @@ from dataclasses import dataclass
 
 import torch
 
-from infrared_amd._lib import check, dtype_code, lib, ptr, require_device, seam, stream_of, stream_ptr
+from infrared_amd._lib import DTYPE_E4M3, check, dtype_code, lib, ptr, require_device, seam, stream_of, stream_ptr
+
+CODES = torch.float8_e4m3fn  # dtype of an 8-bit pool's caches
 
 
 def _last_dim_contiguous(name: str, t: torch.Tensor) -> None:
@@ -95,6 +97,90 @@ def paged_gather(
     return out_k, out_v
 
 
+def kv_scatter_q8(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    err_flags: torch.Tensor | None = None,
+) -> None:
+    """:func:`kv_scatter` into one layer of an 8-bit pool (``QuantPagedKVPool.write``
+    semantics): ``k_cache``/``v_cache`` float8_e4m3fn ``[num_slots, H_kv, D]`` in
+    head-major storage, ``kv_scales`` fp32 ``[H_kv, num_blocks, 2]``."""
+    seam().kv_scatter_q8(k_cache, v_cache, kv_scales, k, v, slots, int(block_size), err_flags, stream_of(k_cache))
+
+
+def _code_layer(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: torch.Tensor,
+                block_size: int) -> None:
+    _cache_layer(name, k_cache)
+    slots, h, d = k_cache.shape
+    if k_cache.dtype != CODES or v_cache.dtype != CODES:
+        raise RuntimeError(f"{name}: kv_scales go with caches of {CODES} codes, got {k_cache.dtype}, {v_cache.dtype}")
+    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+        raise RuntimeError(f"{name}: k_cache and v_cache must have the same shape and strides")
+    if k_cache.stride(0) != d or (h > 1 and k_cache.stride(1) != slots * d):
+        raise RuntimeError(f"{name}: a cache of codes must be dense [num_kv_heads, num_slots, head_dim] storage")
+    if (block_size <= 0 or kv_scales.dtype != torch.float32 or not kv_scales.is_contiguous()
+            or slots % block_size or kv_scales.shape != (h, slots // block_size, 2)):
+        raise RuntimeError(f"{name}: kv_scales must be contiguous fp32 [num_kv_heads, num_blocks, 2]")
+
+
+def gather_slots_q8(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    dtype: torch.dtype,
+    err_flags: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`gather_slots` of a layer of an 8-bit pool, as values of ``dtype`` (the
+    pool's, of which each is exactly a number)."""
+    dev = require_device(k_cache, v_cache, kv_scales, slots)
+    _code_layer("gather_slots_q8", k_cache, v_cache, kv_scales, block_size)
+    if slots.dtype != torch.int64:
+        raise RuntimeError("gather_slots_q8: slots must be int64")
+    flat = slots.reshape(-1).contiguous()
+    h, d = k_cache.shape[1:]
+    out = torch.empty(2, flat.numel(), h, d, dtype=dtype, device=dev)
+    rc = lib().ir_gather_slots_q8(
+        ptr(k_cache), ptr(v_cache), ptr(kv_scales), kv_scales.shape[1], block_size, ptr(flat), flat.numel(), h, d,
+        dtype_code(dtype), ptr(out[0]), ptr(out[1]), ptr(err_flags), stream_ptr(dev),
+    )
+    check(rc, "ir_gather_slots_q8")
+    return out[0].reshape(*slots.shape, h, d), out[1].reshape(*slots.shape, h, d)
+
+
+def paged_gather_q8(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    max_ctx: int,
+    dtype: torch.dtype,
+    err_flags: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`paged_gather` of a layer of an 8-bit pool, as values of ``dtype``."""
+    dev = require_device(k_cache, v_cache, kv_scales, block_tables, context_lens)
+    _code_layer("paged_gather_q8", k_cache, v_cache, kv_scales, block_size)
+    _check_tables("paged_gather_q8", block_tables, context_lens)
+    b = block_tables.shape[0]
+    h, d = k_cache.shape[1:]
+    out = torch.empty(2, b, max_ctx, h, d, dtype=dtype, device=dev)
+    rc = lib().ir_paged_gather_q8(
+        ptr(k_cache), ptr(v_cache), ptr(kv_scales), kv_scales.shape[1], block_size, ptr(block_tables),
+        block_tables.stride(0), block_tables.shape[1], ptr(context_lens), b, max_ctx, h, d, dtype_code(dtype),
+        ptr(out[0]), ptr(out[1]), ptr(err_flags), stream_ptr(dev),
+    )
+    check(rc, "ir_paged_gather_q8")
+    return out[0], out[1]
+
+
 def _check_tables(name: str, block_tables: torch.Tensor, context_lens: torch.Tensor) -> None:
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1:
         raise RuntimeError(f"{name}: block_tables must be int32 [B, max_blocks] with contiguous rows")
@@ -135,6 +221,7 @@ def paged_decode(
     workspace: torch.Tensor | None = None,
     err_flags: torch.Tensor | None = None,
     counters: torch.Tensor | None = None,
+    kv_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """GQA paged decode: ``q`` ``[B, H_q, D]`` -> ``[B, H_q, D]``.
 
@@ -142,8 +229,12 @@ def paged_decode(
     ``workspace`` (uint8 scratch, 256-byte aligned) and ``counters`` (int32,
     zero-filled before first use; every call leaves them at zero) are allocated
     when not given and the longest possible context needs more than one
-    partition.
+    partition. ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn)
+    with these scales, ``q`` of the pool's dtype.
     """
+    if kv_scales is not None:
+        return seam().paged_decode_q8(q, k_cache, v_cache, kv_scales, block_tables, context_lens, block_size, scale,
+                                      out, partition_tokens, workspace, err_flags, counters, stream_of(q))
     return seam().paged_decode(q, k_cache, v_cache, block_tables, context_lens, block_size, scale, out,
                                partition_tokens, workspace, err_flags, counters, stream_of(q))
 
@@ -245,7 +336,8 @@ def decode_plan(
     rc = lib().ir_paged_decode_plan(
         ptr(block_tables), block_tables.stride(0), max_blocks, ptr(context_lens), b, num_q_heads, h_kv,
         block_size, k_cache.shape[0] // block_size, k_cache.stride(0), k_cache.stride(1),
-        dtype_code(k_cache.dtype), PLAN_SHARE_GROUPS if share_groups else 0, ptr(buf), buf.numel(), ptr(err_flags),
+        DTYPE_E4M3 if k_cache.dtype == CODES else dtype_code(k_cache.dtype),
+        PLAN_SHARE_GROUPS if share_groups else 0, ptr(buf), buf.numel(), ptr(err_flags),
         stream_ptr(dev),
     )
     check(rc, "ir_paged_decode_plan")
@@ -263,10 +355,15 @@ def paged_decode_planned(
     workspace: torch.Tensor | None = None,
     err_flags: torch.Tensor | None = None,
     counters: torch.Tensor | None = None,
+    kv_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """:func:`paged_decode` over a plan: ``q`` ``[B, H_q, D]`` -> ``[B, H_q, D]``.
     ``workspace`` (uint8 scratch) and ``counters`` (int32 zeros, left at zero)
-    are allocated when not given."""
+    are allocated when not given. ``kv_scales``: as there, the plan built for the
+    float8_e4m3fn layer."""
+    if kv_scales is not None:
+        return seam().paged_decode_planned_q8(q, k_cache, v_cache, kv_scales, *plan.native(), scale, out, workspace,
+                                              err_flags, counters, stream_of(q))
     return seam().paged_decode_planned(q, k_cache, v_cache, *plan.native(), scale, out, workspace, err_flags, counters,
                                        stream_of(q))
 
@@ -313,6 +410,54 @@ def rope_kv_scatter(
     and sequence). ``q_out`` may be ``q`` itself (in place).
     """
     return seam().rope_kv_scatter(q, k, v, cos, sin, k_cache, v_cache, slots, q_out, err_flags, stream_of(q))
+
+
+def qk_norm_rope_kv_scatter(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    q_norm: torch.Tensor,
+    k_norm: torch.Tensor,
+    eps: float,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+    q_out: torch.Tensor | None = None,
+    err_flags: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`rope_kv_scatter` of queries and keys that are normed per head first:
+    ``y = x * rsqrt(mean(x^2) + eps) * weight`` over ``head_dim`` (64 or 128), with
+    ``q_norm``/``k_norm`` ``[D]`` of the activations' dtype, then the rotation of ``y``;
+    fp32 throughout, rounded to the dtype once. One launch."""
+    return seam().norm_rope_kv_scatter(q, k, v, q_norm, k_norm, eps, cos, sin, k_cache, v_cache, None, 0, slots, q_out,
+                                       err_flags, stream_of(q))
+
+
+def rope_kv_scatter_q8(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 0.0,
+    q_out: torch.Tensor | None = None,
+    err_flags: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`rope_kv_scatter`, or given ``q_norm`` and ``k_norm``
+    :func:`qk_norm_rope_kv_scatter`, into one layer of an 8-bit pool: the rotated keys
+    and the values are quantised as :func:`kv_scatter_q8` does, in the same launch
+    (normed keys from fp32, without a rounding to the dtype before)."""
+    return seam().norm_rope_kv_scatter(q, k, v, q_norm, k_norm, eps, cos, sin, k_cache, v_cache, kv_scales,
+                                       int(block_size), slots, q_out, err_flags, stream_of(q))
 
 
 PLAN_SHARE_GROUPS = 1  # IR_PLAN_SHARE_GROUPS
@@ -454,6 +599,7 @@ def paged_prefill(
     plan: PrefillPlan | None = None,
     new_kv: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
     src_row0: int = 0,
+    kv_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Causal paged attention for packed query chunks: ``q`` ``[total_q, H_q, D]``.
 
@@ -469,6 +615,9 @@ def paged_prefill(
     src_row0 + total_q - 1`` are this call's query tokens, whose keys are then
     read from those rows (``ERR_WRITE_SLOT`` is flagged where a token's write
     slot is not its block-table slot).
+    ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn) with these
+    scales, ``q`` of the pool's dtype; its new rows are written before
+    (:func:`kv_scatter_q8`), so there is no ``new_kv``.
     """
     stream = stream_of(q)
     if plan is not None:
@@ -479,6 +628,12 @@ def paged_prefill(
         if plan.f32 != (q.dtype == torch.float32):
             raise RuntimeError("paged_prefill: the plan was built for "
                                + ("fp32" if plan.f32 else "16-bit") + f" calls, q is {q.dtype}")
+    if kv_scales is not None:
+        if new_kv is not None:
+            raise RuntimeError("paged_prefill: new_kv cannot be written to an 8-bit cache by the same launch")
+        return seam().paged_prefill_q8(q, k_cache, v_cache, kv_scales, block_tables, cu_seqlens_q, q_start,
+                                       int(max_q_len), block_size, scale, out, err_flags,
+                                       None if plan is None else plan.buf, stream)
     kn, vn, slots = (None, None, None) if new_kv is None else new_kv
     if new_kv is not None and kn is None:
         raise RuntimeError("paged_prefill: new_kv must be (k, v, slots), each of them a tensor")
@@ -703,8 +858,11 @@ def hbm_read_granule() -> int:
 
 __all__ = [
     "kv_scatter",
+    "kv_scatter_q8",
     "gather_slots",
+    "gather_slots_q8",
     "paged_gather",
+    "paged_gather_q8",
     "paged_decode",
     "paged_attention_masked",
     "paged_prefill",
@@ -713,6 +871,8 @@ __all__ = [
     "prefill_plan_bytes",
     "prefill_plan_pays",
     "rope_kv_scatter",
+    "rope_kv_scatter_q8",
+    "qk_norm_rope_kv_scatter",
     "decode_workspace_bytes",
     "default_partition",
 ]

@@ -29,6 +29,9 @@ decode rows + 4 x 256-token chunks: 187.5 against 177.5 us per layer, with a
 prefill workgroup (~78 KB of LDS) fitting beside each decode workgroup
 (72 KB), so the loss is the branches' cost, not CUs held by the prefill.
 
+Over a ``QuantPagedKVPool`` the write is always its own launch (``fused`` is off):
+the chunks attend what the pool holds.
+
 The per-layer projections around attention are not part of this path; the
 caller supplies each layer's q and new K/V (``MixedInputs``).
 """
@@ -42,7 +45,7 @@ import torch
 
 from infrared_amd import kernels, metadata
 from infrared_amd.hip_graph import capturing
-from infrared_amd.paged_kv_cache import PagedKVPool
+from infrared_amd.paged_kv_cache import PagedKVPool, QuantPagedKVPool
 
 
 @dataclass(frozen=True)
@@ -160,7 +163,8 @@ class MixedStep:
                  overlap: bool = False, fused: bool = True) -> None:
         self.pool, self.batch, self.inputs, self.scale = pool, batch, inputs, scale
         self.overlap = overlap
-        self.fused = fused and not overlap
+        self.quant = isinstance(pool, QuantPagedKVPool)
+        self.fused = fused and not overlap and not self.quant
         dev = pool.device
         self.out_dec = torch.empty_like(inputs.q_dec)
         self.out_pre = torch.empty_like(inputs.q_pre)
@@ -191,17 +195,31 @@ class MixedStep:
         self._side = torch.cuda.Stream(device=dev) if overlap else None
         self._graph: torch.cuda.CUDAGraph | None = None
 
+    def _scales(self, layer: int) -> torch.Tensor | None:
+        return self.pool.kv_scales[layer] if self.quant else None
+
+    def _write(self, layer: int, lo: int = 0, hi: int | None = None) -> None:
+        """Rows ``lo:hi`` of the layer's new K/V into the pool."""
+        pool, rows = self.pool, (self.inputs.k_new[layer, lo:hi], self.inputs.v_new[layer, lo:hi])
+        slots = self.batch.write_slots[lo:hi]
+        if self.quant:
+            kernels.kv_scatter_q8(pool.k[layer], pool.v[layer], pool.kv_scales[layer], *rows, slots, pool.block_size,
+                                  self.err)
+        else:
+            kernels.kv_scatter(pool.k[layer], pool.v[layer], *rows, slots, self.err)
+
     def _decode(self, layer: int) -> None:
         b, inp, pool = self.batch, self.inputs, self.pool
         if self.planned:
             kernels.paged_decode_planned(
                 inp.q_dec[layer], pool.k[layer], pool.v[layer], self.plan, self.scale, out=self.out_dec[layer],
-                workspace=self.workspace, err_flags=self.err, counters=self.counters,
+                workspace=self.workspace, err_flags=self.err, counters=self.counters, kv_scales=self._scales(layer),
             )
             return
         kernels.paged_decode(
             inp.q_dec[layer], pool.k[layer], pool.v[layer], b.dec_tables, b.dec_ctx, pool.block_size, self.scale,
             out=self.out_dec[layer], workspace=self.workspace, err_flags=self.err, counters=self.counters,
+            kv_scales=self._scales(layer),
         )
 
     def _prefill(self, layer: int, fused: bool = False) -> None:
@@ -210,11 +228,10 @@ class MixedStep:
             inp.q_pre[layer], pool.k[layer], pool.v[layer], b.pre_tables, b.cu_seqlens_q, b.q_start, b.max_q_len,
             pool.block_size, self.scale, out=self.out_pre[layer], err_flags=self.err, plan=self.plan_pre,
             new_kv=(inp.k_new[layer], inp.v_new[layer], b.write_slots) if fused else None,
-            src_row0=inp.q_dec.shape[1],
+            src_row0=inp.q_dec.shape[1], kv_scales=self._scales(layer),
         )
 
     def _layer(self, layer: int) -> None:
-        b, inp, pool = self.batch, self.inputs, self.pool
         if self.fused:
             # the prefill launch writes every new row (the decode rows' too)
             # and reads the chunks' own keys from them; the decode follows
@@ -222,21 +239,18 @@ class MixedStep:
             self._decode(layer)
             return
         if self._side is None:
-            kernels.kv_scatter(pool.k[layer], pool.v[layer], inp.k_new[layer], inp.v_new[layer], b.write_slots,
-                               self.err)
+            self._write(layer)
             self._decode(layer)
             self._prefill(layer)
             return
         # the decode rows' new K/V first (the decode reads them), then the
         # chunks' rows and the prefill on the side stream beside the decode
-        nd = inp.q_dec.shape[1]
-        main = torch.cuda.current_stream(pool.device)
-        kernels.kv_scatter(pool.k[layer], pool.v[layer], inp.k_new[layer, :nd], inp.v_new[layer, :nd],
-                           b.write_slots[:nd], self.err)
+        nd = self.inputs.q_dec.shape[1]
+        main = torch.cuda.current_stream(self.pool.device)
+        self._write(layer, 0, nd)
         self._side.wait_stream(main)
         with torch.cuda.stream(self._side):
-            kernels.kv_scatter(pool.k[layer], pool.v[layer], inp.k_new[layer, nd:], inp.v_new[layer, nd:],
-                               b.write_slots[nd:], self.err)
+            self._write(layer, nd)
             self._prefill(layer)
         self._decode(layer)
         main.wait_stream(self._side)  # both are done before the next layer's scatter

@@ -40,6 +40,9 @@ calls once per layer (``infrared/model/layers.py:178-180``):
      exactly as the reference's naive path does
      (``infrared/model/triton_attention.py:110-129``).
 
+Over a ``QuantPagedKVPool`` the write quantises and the first two of these attend
+through the scales; the ones that start from ``gather_slots`` are refused.
+
 ``paged`` may be this package's ``PagedContext`` or any object with the same
 attributes (the reference's own ``PagedContext`` works: it simply lacks the
 block-table fields). There is no CPU path and no Triton: tensors must live on
@@ -52,7 +55,7 @@ import torch
 
 from infrared_amd import kernels
 from infrared_amd._lib import seam, stream_of
-from infrared_amd.paged_kv_cache import PagedKVPool
+from infrared_amd.paged_kv_cache import PagedKVPool, QuantPagedKVPool
 
 _POOL_WRITE = PagedKVPool.write
 
@@ -96,6 +99,10 @@ def rope_paged_attention(
     layer_idx: int,
     scale: float,
     n_rep: int,
+    *,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 1e-6,
 ) -> torch.Tensor:
     """``apply_rotary_pos_emb`` + ``paged_attention`` with the rotation and the K/V
     write fused into one kernel (``ir_rope_kv_scatter``).
@@ -104,6 +111,11 @@ def rope_paged_attention(
     (``infrared/model/layers.py:158-164``) and the step's fp32 ``cos``/``sin``
     ``[B, Sq, D]`` (``RotaryEmbedding`` output); the result is bit-identical to
     rotating with the reference's ops and calling ``paged_attention``.
+
+    ``q_norm``, ``k_norm`` (``[D]``, of the activations' dtype, both or neither):
+    queries and keys are normed per head before the rotation, ``x * rsqrt(mean(x^2) +
+    eps) * weight``, in the same kernel, which then stays in fp32 and rounds once
+    (``ir_qk_norm_rope_kv_scatter``; ``ir_rope_kv_scatter_q8`` for an 8-bit pool).
     """
     pool = paged.pool
     h_kv, d = k.shape[-2], k.shape[-1]
@@ -112,12 +124,35 @@ def rope_paged_attention(
         raise RuntimeError(
             f"rope_paged_attention: q {tuple(q.shape)} inconsistent with k {tuple(k.shape)} and n_rep={n_rep}"
         )
-    q_rot = kernels.rope_kv_scatter(
-        q.reshape(b * sq, hq, d), k.reshape(b * sq, h_kv, d), v.reshape(b * sq, h_kv, d),
-        cos.reshape(b * sq, d), sin.reshape(b * sq, d), pool.k[layer_idx], pool.v[layer_idx],
-        paged.write_slots, err_flags=getattr(pool, "err_flags", None),
-    ).view(b, sq, hq, d)
-    return _attend(q_rot, paged, mask, layer_idx, scale)
+    if (q_norm is None) != (k_norm is None):
+        raise RuntimeError("rope_paged_attention: q_norm and k_norm go together")
+    rows = (q.reshape(b * sq, hq, d), k.reshape(b * sq, h_kv, d), v.reshape(b * sq, h_kv, d))
+    angles = (cos.reshape(b * sq, d), sin.reshape(b * sq, d))
+    caches = (pool.k[layer_idx], pool.v[layer_idx])
+    err = getattr(pool, "err_flags", None)
+    if isinstance(pool, QuantPagedKVPool):
+        _check_quant(pool, q, paged)
+        q_rot = kernels.rope_kv_scatter_q8(*rows, *angles, *caches, pool.kv_scales[layer_idx], paged.write_slots,
+                                           pool.block_size, q_norm, k_norm, eps, err_flags=err)
+    elif q_norm is not None:
+        q_rot = kernels.qk_norm_rope_kv_scatter(*rows, q_norm, k_norm, eps, *angles, *caches, paged.write_slots,
+                                                err_flags=err)
+    else:
+        q_rot = kernels.rope_kv_scatter(*rows, *angles, *caches, paged.write_slots, err_flags=err)
+    return _attend(q_rot.view(b, sq, hq, d), paged, mask, layer_idx, scale)
+
+
+def _check_quant(pool: QuantPagedKVPool, q: torch.Tensor, paged) -> None:
+    """Refuses, before anything is written, what an 8-bit pool has no kernel for."""
+    if q.dtype != pool.dtype:
+        raise RuntimeError(f"paged_attention: q is {q.dtype}, the 8-bit pool's dtype is {pool.dtype}")
+    tables = paged.use_triton and getattr(paged, "block_tables", None) is not None
+    packed = getattr(paged, "cu_seqlens_q", None) is not None and getattr(paged, "q_start", None) is not None
+    if not tables or not (packed or (getattr(paged, "context_lens", None) is not None and q.shape[1] == 1)):
+        raise RuntimeError(
+            "paged_attention: an 8-bit pool is attended through block_tables, with context_lens for a single-token "
+            "decode or cu_seqlens_q and q_start for packed chunks (metadata.decode_context, prefill_context)"
+        )
 
 
 def _attend(q: torch.Tensor, paged, mask: torch.Tensor | None, layer_idx: int, scale: float,
@@ -130,6 +165,8 @@ def _attend(q: torch.Tensor, paged, mask: torch.Tensor | None, layer_idx: int, s
     b, sq = q.shape[:2]
     k_layer, v_layer = pool.k[layer_idx], pool.v[layer_idx]
     err = getattr(pool, "err_flags", None)
+    if isinstance(pool, QuantPagedKVPool):
+        _check_quant(pool, q, paged)
 
     def write():
         if new_kv is None:
@@ -298,6 +335,7 @@ def _prefill(q, pool, layer_idx: int, block_tables, cu_seqlens_q, q_start, max_q
     return kernels.paged_prefill(
         q.reshape(b * sq, hq, d), pool.k[layer_idx], pool.v[layer_idx], block_tables, cu_seqlens_q, q_start, max_q,
         pool.block_size, scale, out=out, err_flags=err, plan=plan, new_kv=new_kv, src_row0=src_row0,
+        kv_scales=_scales(pool, layer_idx),
     ).view(b, sq, hq, d)
 
 
@@ -338,6 +376,10 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
         ctr = pool.decode_counters(kernels.decode_num_counters(b, hq, h_kv))
         if own:
             _hold(holder, ws, ctr)
+        scales = _scales(pool, layer_idx)
+        if scales is not None:
+            return kernels.paged_decode_planned(q[:, 0], k_layer, v_layer, plan, scale, out, ws, err, ctr,
+                                                kv_scales=scales).unsqueeze(1)
         return seam().decode_step_planned(q, k_layer, v_layer, *plan.native(), scale, out, ws, err, ctr, stream_of(q))
     else:
         ws = ctr = None
@@ -348,8 +390,17 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
                 ctr = pool.decode_counters(kernels.decode_num_counters(b, hq, h_kv))
         if ws is not None and getattr(holder, "gate", None) is not None:
             _hold(holder, ws, ctr)
+        scales = _scales(pool, layer_idx)
+        if scales is not None:
+            return kernels.paged_decode(q[:, 0], k_layer, v_layer, block_tables, context_lens, pool.block_size, scale,
+                                        out, 0, ws, err, ctr, kv_scales=scales).unsqueeze(1)
         return seam().decode_step(q, k_layer, v_layer, block_tables, context_lens, pool.block_size, scale, out, ws, err,
                                   ctr, stream_of(q))
+
+
+def _scales(pool, layer_idx: int) -> torch.Tensor | None:
+    """An 8-bit pool's scales of the layer."""
+    return pool.kv_scales[layer_idx] if isinstance(pool, QuantPagedKVPool) else None
 
 
 def _hold(holder, *tensors: torch.Tensor) -> None:

@@ -47,6 +47,7 @@ from infrared_amd._lib import (
     ERR_PLAN,
     ERR_SLOT_RANGE,
     ERR_WRITE_SLOT,
+    dtype_code,
 )
 
 _ERR_NAMES = {
@@ -321,6 +322,93 @@ class PagedKVPool:
             self.err_flags.zero_()
             names = [n for bit, n in _ERR_NAMES.items() if flags & bit]
             raise IndexError("paged kernels flagged: " + ", ".join(names))
+
+
+class QuantPagedKVPool(PagedKVPool):
+    """A K/V pool held in 8 bits: half the memory of a 16-bit one, and half the bytes
+    its attention reads.
+
+    ``dtype`` is the model's (fp32, fp16, bf16): of the rows written, the queries that
+    attend and the values read back. ``k`` / ``v`` ``[num_layers, num_slots,
+    num_kv_heads, head_dim]`` hold float8_e4m3fn codes in head-major storage,
+    ``kv_scales`` ``[num_layers, num_kv_heads, num_blocks, 2]`` the fp32 scale of
+    each block's K and V in a head; a value is code * scale. Scales are powers of two,
+    bounded so that every value is exactly a number of ``dtype``.
+
+    ``write`` quantises (``ir_kv_scatter_q8``). A call that writes a block's first
+    token starts the block: its scale comes from the call's tokens alone and tokens of
+    the block that the call does not write read as zero from then on. Any other
+    call keeps the block's tokens; if its rows need a larger scale, the kept codes are
+    rounded to it. Tokens of a call may come in any order (of equal slots the last is
+    written); calls that write the same block must be stream-ordered. Codes are
+    rounded to nearest even, NaN and infinities become NaN.
+
+    ``gather`` / ``gather_blocks`` return values of ``dtype``. ``paged_attention`` and
+    ``rope_paged_attention`` take the pool with block-table metadata
+    (``metadata.decode_context`` / ``prefill_context``); ``gather_slots`` with a mask
+    alone is refused. ``block_size`` is a multiple of 16 up to 1024, ``head_dim`` 64
+    or 128.
+    """
+
+    def __init__(
+        self,
+        num_layers: int,
+        num_blocks: int,
+        block_size: int,
+        num_kv_heads: int,
+        head_dim: int,
+        dtype: torch.dtype,
+        device: torch.device | str = "cuda",
+        *,
+        strict: bool = False,
+    ) -> None:
+        dtype_code(dtype)
+        if block_size <= 0 or block_size % 16 or block_size > 1024:
+            raise ValueError(f"an 8-bit pool's block size is a multiple of 16, at most 1024; got {block_size}")
+        if head_dim not in (64, 128):
+            raise ValueError(f"an 8-bit pool's head_dim is 64 or 128; got {head_dim}")
+        if num_blocks * block_size >= 2**31:
+            raise ValueError(f"{num_blocks} blocks of {block_size} tokens exceed 2^31 slots")
+        super().__init__(num_layers, num_blocks, block_size, num_kv_heads, head_dim, kernels.CODES, device,
+                         strict=strict)
+        self.dtype = dtype
+        # (empty blocks have the least scale: whatever is written first sets it)
+        self.kv_scales = torch.full((num_layers, num_kv_heads, num_blocks, 2),
+                                    2.0 ** (-15 if dtype == torch.float16 else -100), device=self.device)
+
+    def write(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Quantises this step's K/V (``[N, num_kv_heads, head_dim]`` of ``dtype``) into ``slots``
+        (``[N]`` int64; negative: skipped)."""
+        if k.dtype != self.dtype:
+            raise RuntimeError(f"QuantPagedKVPool.write: k is {k.dtype}, the pool's dtype is {self.dtype}")
+        kernels.kv_scatter_q8(self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], k, v, slots,
+                              self.block_size, self.err_flags)
+        if self.strict:
+            self.check_errors()
+
+    def gather(self, layer_idx: int, gather_slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """``PagedKVPool.gather`` of the values the codes stand for, in ``dtype``."""
+        out = kernels.gather_slots_q8(self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], gather_slots,
+                                      self.block_size, self.dtype, self.err_flags)
+        if self.strict:
+            self.check_errors()
+        return out
+
+    def gather_blocks(
+        self,
+        layer_idx: int,
+        block_tables: torch.Tensor,
+        context_lens: torch.Tensor,
+        max_ctx: int,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """``PagedKVPool.gather_blocks`` of the values the codes stand for, in ``dtype``."""
+        out = kernels.paged_gather_q8(
+            self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], block_tables, context_lens,
+            self.block_size, max_ctx, self.dtype, self.err_flags,
+        )
+        if self.strict:
+            self.check_errors()
+        return out
 
 
 def _metadata_key(gather_slots: torch.Tensor, mask: torch.Tensor) -> tuple:
