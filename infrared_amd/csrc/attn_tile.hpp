@@ -248,13 +248,14 @@ constexpr float kRescaleSlack = 8.f;
 // O^T += V^T . P^T. Unless FULL, `vok[r]` says whether key row 4g+r may be
 // read; rows that may not are zeroed so 0 * V never meets a NaN pattern in
 // stale pool memory. FULL tiles (every key present) skip that masking.
-template <int DT, int D, bool FULL>
+// SWAP: the column's maximum over lane groups by lane swaps instead of LDS.
+template <int DT, int D, bool FULL, bool SWAP = false>
 __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t (&vin)[4][TileShape<DT, D>::VDW],
                                            const bool (&vok)[4], State<D>& st) {
   typedef TileShape<DT, D> Sh;
   constexpr int TILES = Sh::TILES;
   float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-  mx = wave_max_groups(mx);
+  mx = SWAP ? wave_max_groups_swap(mx) : wave_max_groups(mx);
   const bool grow = mx > st.m + kRescaleSlack;
   if (__any(grow)) {
     const float m_new = grow ? mx : st.m;

@@ -305,14 +305,14 @@ __device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const uint3
       vok[r] = true;
       sv[r] = col_on ? s[r] * score_scale : kNegInf;
     }
-    softmax_pv<DT, D, true>(sv, v, vok, st);
+    softmax_pv<DT, D, true, true>(sv, v, vok, st);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       vok[r] = (kmask >> r) & 1u;
       sv[r] = vok[r] && col_on ? s[r] * score_scale : kNegInf;
     }
-    softmax_pv<DT, D, false>(sv, v, vok, st);
+    softmax_pv<DT, D, false, true>(sv, v, vok, st);
   }
 }
 

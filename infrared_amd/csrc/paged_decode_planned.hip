@@ -37,6 +37,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "paged_decode.hpp"
 #include "status.hpp"
 
@@ -45,6 +47,11 @@ namespace {
 
 constexpr int kPlanMaxSeqs = 1024;  // sequences per plan (prefix sums held in LDS)
 constexpr int kPlanWaves = 4;       // streaming wavefronts per workgroup
+// Of a call over an 8-bit cache, whose tiles are half the bytes at as many
+// instructions: two wavefronts per SIMD, each computing while the other waits (64
+// sequences of 512..4096 keys: 45.1 us with four, 33.5 with eight, whatever the number
+// of tiles in flight; twelve are short of registers, 46.5).
+constexpr int kCodeWaves = 8;
 constexpr int kPlanRun = 64;        // tile facts per wavefront and run (one per lane)
 constexpr int kPlanMinTiles = 16;   // smallest slice
 
@@ -63,7 +70,7 @@ struct PlanLayout {
   int64_t hdr, seq_pre, empty, share, pair, whdr, first, facts, total;
 };
 
-PlanLayout plan_layout(int64_t num_seqs, int64_t grid, int64_t t_cap) {
+PlanLayout plan_layout(int64_t num_seqs, int64_t grid, int64_t t_cap, int waves) {
   auto al = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   PlanLayout p;
   p.hdr = 0;
@@ -72,8 +79,8 @@ PlanLayout plan_layout(int64_t num_seqs, int64_t grid, int64_t t_cap) {
   p.share = al(p.empty + num_seqs * 4);
   p.pair = al(p.share + num_seqs * 4);
   p.whdr = al(p.pair + num_seqs * 4);
-  p.first = al(p.whdr + grid * kPlanWaves * 8 * 4);
-  p.facts = al(p.first + grid * kPlanWaves * kPlanRun * 8);
+  p.first = al(p.whdr + grid * waves * 8 * 4);
+  p.facts = al(p.first + grid * waves * kPlanRun * 8);
   p.total = al(p.facts + t_cap * 8);
   return p;
 }
@@ -485,7 +492,7 @@ __device__ __forceinline__ void slot_read(const float* row, int g, f32x4 (&acc)[
 // Q8: the tiles are codes; a run's lanes also fetch the scales of their tiles, whose
 // block the tile's pool offset gives (the layer is dense), ahead of the tiles' own loads.
 template <int DT, int D, int NW, int DEPTH, bool PAIRS, bool Q8 = false>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 ? 1 : 2)))
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 && NW == 4 ? 1 : 2)))
 void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32_t o_pair, uint32_t o_whdr,
                                  uint32_t o_first, int B, DecodeArgs a, PlanLayout ly) {
   typedef TileShape<DT, D> Sh;
@@ -863,11 +870,11 @@ void launch_planned_q8(const DecodeArgs& a, const uint8_t* plan, const PlanLayou
   const uint32_t o_sp = (uint32_t)ly.seq_pre, o_pr = (uint32_t)ly.pair, o_wh = (uint32_t)ly.whdr,
                  o_fi = (uint32_t)ly.first;
   if (pairs)
-    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kPlanWaves, 2, true, true>), dim3(grid),
-                       dim3(kPlanWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, true, true>), dim3(grid),
+                       dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
   else
-    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kPlanWaves, 2, false, true>), dim3(grid),
-                       dim3(kPlanWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, false, true>), dim3(grid),
+                       dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
 }
 
 // Pairs fit one unit's 16 MFMA columns when a KV head has at most 8 query
@@ -903,7 +910,9 @@ extern "C" int64_t ir_paged_decode_plan_bytes(int num_seqs, int num_q_heads, int
                                               int block_size) {
   if (!plannable(num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size)) return 0;
   const int n_ups = num_kv_heads * n_hg_of(num_q_heads, num_kv_heads);
-  return plan_layout(num_seqs, device_cus(), t_cap_of(num_seqs, n_ups, max_blocks_per_seq, block_size)).total;
+  return plan_layout(num_seqs, device_cus(), t_cap_of(num_seqs, n_ups, max_blocks_per_seq, block_size),
+                     std::max(kPlanWaves, kCodeWaves))
+      .total;
 }
 
 extern "C" int64_t ir_paged_decode_planned_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
@@ -952,12 +961,18 @@ extern "C" int ir_paged_decode_plan(const int32_t* block_tables, int64_t bt_stri
   p.pairs = (flags & IR_PLAN_SHARE_GROUPS) && pairs_fit(num_q_heads, num_kv_heads);
   p.plan = (uint8_t*)plan;
   const int grid = device_cus();
-  p.ly = plan_layout(num_seqs, grid, t_cap_of(num_seqs, p.n_ups, max_blocks_per_seq, block_size));
+  const bool codes = dtype == IR_DTYPE_E4M3;
+  p.ly = plan_layout(num_seqs, grid, t_cap_of(num_seqs, p.n_ups, max_blocks_per_seq, block_size),
+                     codes ? kCodeWaves : kPlanWaves);
   p.err = err_flags;
   if (p.pairs)
     hipLaunchKernelGGL(paged_decode_pair_kernel, dim3(num_seqs), dim3(kPairThreads), 0, (hipStream_t)stream, p);
-  hipLaunchKernelGGL((paged_decode_plan_kernel<kPlanWaves>), dim3(grid), dim3(kPlanWaves * 64), 0,
-                     (hipStream_t)stream, p);
+  if (codes)
+    hipLaunchKernelGGL((paged_decode_plan_kernel<kCodeWaves>), dim3(grid), dim3(kCodeWaves * 64), 0,
+                       (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL((paged_decode_plan_kernel<kPlanWaves>), dim3(grid), dim3(kPlanWaves * 64), 0,
+                       (hipStream_t)stream, p);
   return check_launch("ir_paged_decode_plan");
 }
 
@@ -1020,7 +1035,8 @@ int planned_call(const char* name, const float* scales, const void* q, int64_t q
   a.ws_o = (float*)workspace;
   a.ws_ml = (float*)((uint8_t*)workspace + ws.acc_bytes);
   const PlanLayout ly =
-      plan_layout(num_seqs, grid, t_cap_of(num_seqs, a.n_ups, max_blocks_per_seq, block_size));
+      plan_layout(num_seqs, grid, t_cap_of(num_seqs, a.n_ups, max_blocks_per_seq, block_size),
+                  scales ? kCodeWaves : kPlanWaves);
   const uint8_t* pl = (const uint8_t*)plan;
   hipStream_t s = (hipStream_t)stream;
   const bool pairs = (flags & IR_PLAN_SHARE_GROUPS) && pairs_fit(num_q_heads, num_kv_heads);
