@@ -358,6 +358,41 @@ void kv_scatter_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales, con
         "ir_kv_scatter_q8");
 }
 
+// A layer of an 8-bit pool's tensors (the checks are the layer's).
+Tensor layer_of(const Tensor& t, int64_t layer) { return t.select(0, layer); }
+
+void pool_write_q8(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales, int64_t layer, const Tensor& k,
+                   const Tensor& v, const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
+  kv_scatter_q8(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), k, v, slots, block_size, err,
+                stream);
+}
+
+std::tuple<Tensor, Tensor> gather_slots_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales,
+                                           const Tensor& slots, int64_t block_size, at::ScalarType dtype,
+                                           const OptTensor& err, int64_t stream) {
+  check_block_size("gather_slots_q8: ", block_size);
+  code_layer("gather_slots_q8", kc, vc, scales, block_size);
+  require_device({&kc, &slots});
+  require(slots.scalar_type() == at::kLong, "gather_slots_q8: slots must be int64");
+  const Tensor flat = slots.contiguous();
+  const int64_t h = kc.size(1), d = kc.size(2);
+  std::vector<int64_t> shape = slots.sizes().vec();
+  shape.insert(shape.end(), {h, d});
+  const Tensor ok = at::empty(shape, kc.options().dtype(dtype)), ov = at::empty_like(ok);
+  check(ir_gather_slots_q8(kc.data_ptr(), vc.data_ptr(), (const float*)scales.data_ptr(), scales.size(1),
+                           (int)block_size, (const int64_t*)flat.data_ptr(), flat.numel(), (int)h, (int)d,
+                           dtype_code(ok), ok.data_ptr(), ov.data_ptr(), (int32_t*)ptr(err), stream_of(stream)),
+        "ir_gather_slots_q8");
+  return {ok, ov};
+}
+
+std::tuple<Tensor, Tensor> pool_gather_q8(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales,
+                                          int64_t layer, const Tensor& slots, int64_t block_size, at::ScalarType dtype,
+                                          const OptTensor& err, int64_t stream) {
+  return gather_slots_q8(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), slots, block_size,
+                         dtype, err, stream);
+}
+
 // ir_qk_norm_rope_kv_scatter, and with scales (an 8-bit pool's layer) ir_rope_kv_scatter_q8,
 // whose norms may be absent.
 Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& wq,
@@ -538,6 +573,9 @@ PYBIND11_MODULE(_seam, m) {
   m.def("rope_kv_scatter", &rope_kv_scatter, nogil());
   m.def("paged_prefill", &paged_prefill, nogil());
   m.def("kv_scatter_q8", &kv_scatter_q8, nogil());
+  m.def("gather_slots_q8", &gather_slots_q8, nogil());
+  m.def("pool_write_q8", &pool_write_q8, nogil());
+  m.def("pool_gather_q8", &pool_gather_q8, nogil());
   m.def("norm_rope_kv_scatter", &norm_rope_kv_scatter, nogil());
   m.def("paged_decode_q8", &paged_decode_q8, nogil());
   m.def("paged_decode_planned_q8", &paged_decode_planned_q8, nogil());

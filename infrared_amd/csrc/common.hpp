@@ -197,6 +197,35 @@ __device__ __forceinline__ float wave_sum_groups_swap(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// x of the lane that a DPP pattern pairs with this one, within rows of 16 lanes: quad
+// permutations for l ^ 1 and l ^ 2, mirrored half rows and rows. Reductions over
+// 4, 8 or 16 lanes apply them in this order (a mirrored lane holds what its own quad or
+// half row came to, so it may stand for l ^ 4 and l ^ 8).
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
+template <int CTRL>
+__device__ __forceinline__ float dpp_pair(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over the N (4 or 8) lanes that a lane shares a row of data with.
+template <int N>
+__device__ __forceinline__ float row_sum(float x) {
+  static_assert(N == 4 || N == 8, "4 or 8 lanes");
+  x += dpp_pair<kDppXor1>(x);
+  x += dpp_pair<kDppXor2>(x);
+  if constexpr (N == 8) x += dpp_pair<kDppHalfMirror>(x);
+  return x;
+}
+
+// Maximum over the wavefront.
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp_pair<kDppXor1>(x));
+  x = fmaxf(x, dpp_pair<kDppXor2>(x));
+  x = fmaxf(x, dpp_pair<kDppHalfMirror>(x));
+  x = fmaxf(x, dpp_pair<kDppMirror>(x));
+  return wave_max_groups_swap(x);
+}
+
 __device__ __forceinline__ void flag_error(int32_t* err, int32_t bit) {
   if (err) atomicOr(err, bit);
 }

@@ -4,19 +4,26 @@
 // for V and [H_kv][num_blocks][2] scales.
 //
 // The write. A block's scale covers all its tokens, so the tokens of a call that
-// share a block have to be handled together, whatever their order in the call. The
-// workgroup of token i drops out if the token before it is in the same block
-// (which ends most of a prompt's), else it reads every slot of the call once and
-// drops out if an earlier one is in the block; the one that is left owns the block,
-// knows which row each of its tokens takes (the last given), and no other workgroup
-// touches it. That is one launch without a workspace and with a result that does not
-// depend on the order of execution. The slots are 8 bytes a token against about
-// 3 KB of rows at 4 heads of 128, and come from L2, but n / block_size workgroups
-// read them all: 4 us of L2 traffic at 16,384 tokens, growing with the square.
+// share a block have to be handled together, whatever their order in the call. A
+// workgroup looks after one token or a few; a token drops out if the one before it
+// is in the same block (which ends most of a prompt's), else the workgroup reads
+// every slot of the call once and the token drops out if an earlier one is in the
+// block. The one that is left owns the block, its workgroup knows which row each of
+// the block's tokens takes (the last given), and no other workgroup touches it. That is
+// one launch without a workspace, and its result does not depend on the order of
+// execution. The slots are 8 bytes a token against 4 KB of rows at 4 heads of 128, and
+// come from L2, but the workgroups of n / block_size tokens read them all: 128 MB of L2
+// traffic at 16,384 tokens, growing with the square.
+//
+// What bounds it is latency: the slots, the scan, the rows and the codes follow each
+// other (64 tokens 4.3 us a call, 4,096 tokens 9.8 us for 12.6 MB, 28 / 4 heads of 128,
+// of which 2.7 us are the launch of workgroups that find nothing to do).
 //
 // A wavefront then takes K or V of one head: its rows' largest magnitude gives the
 // scale, the rows become codes. A block that is not new keeps its tokens; only when
 // its scale grows are they read, rounded to the wider scale and written back.
+#include <algorithm>
+
 #include "e4m3.hpp"
 #include "norm_rope.hpp"
 #include "status.hpp"
@@ -24,8 +31,14 @@
 namespace ir {
 namespace {
 
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kMaxBlockSize = 1024;
 constexpr int kWriteWaves = 4;
+// Workgroups up to which each looks after one token only: four a CU (2,048 measured
+// 11.8 against 10.3 us on a mixed step of 1,248 tokens, 10.1 against 9.8 on 4,096).
+constexpr int64_t kWriteGroups = 1024;
 
 struct QuantArgs {
   RowArgs r;
@@ -34,7 +47,8 @@ struct QuantArgs {
   float* scales;
   int64_t num_blocks;
   int bs;
-  int kv_groups;   // workgroups per token for its 2 * H_kv (head, K / V) parts
+  int window;      // tokens of the call that a workgroup looks after, at most 16
+  int kv_groups;   // workgroups per window for the 2 * H_kv (head, K / V) parts
   int64_t n_kv;    // workgroups of the write; those after them take query rows
   int32_t* err;
 };
@@ -83,12 +97,263 @@ __device__ __forceinline__ void query_rows(const RowArgs& r, int64_t wave) {
   P::store(r.qo + tok * r.qo_tok + h * r.qo_head, ci, x);
 }
 
+// A lane's part of a new row as it is loaded, with the token's tables for a key that
+// is rotated.
+template <int DT, int D, int MODE>
+struct NewRow {
+  RowPair<DT, D> p;
+  Angles<DT, D, MODE> t;
+  __device__ __forceinline__ void load(const RowArgs& r, int h, int is_v, int64_t j, int ci) {
+    p.load((is_v ? r.v + h * r.v_head + j * r.v_tok : r.k + h * r.k_head + j * r.k_tok), ci);
+    if constexpr (MODE != kRowsPlain) t.load(r.cos + j * r.cs_tok, r.sin + j * r.cs_tok, ci);
+  }
+};
+
+// What the pool holds of a lane's 16 elements before the rounding to codes: rows that
+// are stored as they are stay packed in the 16-bit dtypes, where two elements take one
+// instruction each for the maximum and for the codes (3 a pair instead of some 20).
+template <int DT, int D, int MODE, bool PACKED>
+struct RowValues {
+  float x[16];
+  float most;  // the largest magnitude, infinite if one is no number
+  __device__ __forceinline__ void take(const NewRow<DT, D, MODE>& r, const float (&w)[16], float eps) {
+    r.p.unpack(x);
+    if constexpr (MODE != kRowsPlain) transform_row<DT, D, MODE>(x, w, eps, r.t);
+    most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(x[e]));  // (passes over NaN, whose code is NaN anyway)
+  }
+  __device__ __forceinline__ float finite_most() const {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, finite_abs(x[e]));
+    return m;
+  }
+  __device__ __forceinline__ void careful(uint32_t (&c)[4], float inv) const {
+    float z[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = to_code_range<DT>(x[e], inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = encode4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
+  }
+  __device__ __forceinline__ void quick(uint32_t (&c)[4], float scale) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      i16x2 o = {0, 0};
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, x[4 * i], x[4 * i + 1], scale, false);
+      o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, x[4 * i + 2], x[4 * i + 3], scale, true);
+      c[i] = __builtin_bit_cast(uint32_t, o);
+    }
+  }
+};
+template <int DT, int D, int MODE>
+struct RowValues<DT, D, MODE, true> {
+  uint32_t x[8];
+  float most;
+  __device__ __forceinline__ void take(const NewRow<DT, D, MODE>& r, const float (&)[16], float) {
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = i < 4 ? r.p.a.w[0][i] : r.p.b.w[0][i - 4];
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[i] & 0x7fff7fffu));
+    }
+    constexpr uint32_t inf = DT == IR_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+    const uint32_t u = max((uint32_t)m[0], (uint32_t)m[1]);
+    most = Elem<DT>::to_f32((typename Elem<DT>::storage)min(u, inf));
+  }
+  __device__ __forceinline__ float at(int e) const {
+    return e & 1 ? Elem<DT>::hi(x[e / 2]) : Elem<DT>::lo(x[e / 2]);
+  }
+  __device__ __forceinline__ float finite_most() const {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, finite_abs(at(e)));
+    return m;
+  }
+  __device__ __forceinline__ void careful(uint32_t (&c)[4], float inv) const {
+    float z[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = to_code_range<DT>(at(e), inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = encode4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
+  }
+  __device__ __forceinline__ void quick(uint32_t (&c)[4], float scale) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      i16x2 o = {0, 0};
+      if constexpr (DT == IR_DTYPE_BF16) {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(bf16x2, x[2 * i]), scale, false);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(bf16x2, x[2 * i + 1]), scale, true);
+      } else {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(f16x2, x[2 * i]), scale, false);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(f16x2, x[2 * i + 1]), scale, true);
+      }
+      c[i] = __builtin_bit_cast(uint32_t, o);
+    }
+  }
+};
+
+// Writes K or V of head `h` of a block (block and head `hb`) by this wavefront: s_row
+// gives the row + 1 that each of its tokens takes from the call, `old` its scale.
+template <int DT, int D, int MODE>
+__device__ __forceinline__ void write_part(const QuantArgs& a, int64_t i, int64_t hb, int h, int is_v, float old,
+                                           const int* s_row) {
+  typedef RowPair<DT, D> P;
+  typedef NewRow<DT, D, MODE> Row;
+  typedef RowValues<DT, D, MODE, MODE == kRowsPlain && DT != IR_DTYPE_F32> Values;
+  constexpr int RPP = 64 / P::LPR;  // rows of a wavefront at a time
+  const int lane = threadIdx.x & 63, ci = lane % P::LPR, grp = lane / P::LPR;
+  const bool fresh = s_row[0] != 0;
+  uint8_t* codes = (is_v ? a.vc : a.kc) + hb * a.bs * D;
+  float w[16];
+  if constexpr (MODE == kRowsNorm) {
+    P pw;
+    pw.load(a.r.k_weight, ci);
+    pw.unpack(w);
+  }
+  // the rows of the block's first 16 tokens stay in registers (all their loads in
+  // flight together; a token without a row loads row i, which is there), those of a
+  // larger block are read once for the scale and once for the codes
+  constexpr int KEEP = 16 / RPP;
+  Row row[KEEP];
+  Values x[KEEP];
+  bool has[KEEP];
+#pragma unroll
+  for (int p = 0; p < KEEP; ++p) {
+    const int64_t j = (int64_t)s_row[p * RPP + grp] - 1;  // (a row's lanes go together)
+    has[p] = j >= 0;
+    row[p].load(a.r, h, is_v, has[p] ? j : i, ci);
+  }
+  auto later = [&](int t, Values& y) -> bool {
+    const int64_t j = (int64_t)s_row[t] - 1;
+    if (j < 0) return false;
+    Row r;
+    r.load(a.r, h, is_v, j, ci);
+    y.take(r, w, a.r.eps);
+    return true;
+  };
+  float amax = 0.f;
+#pragma unroll
+  for (int p = 0; p < KEEP; ++p) {
+    x[p].take(row[p], w, a.r.eps);
+    amax = has[p] ? fmaxf(amax, x[p].most) : amax;
+  }
+  for (int t = 16 + grp; t < a.bs; t += RPP) {
+    Values y;
+    if (later(t, y)) amax = fmaxf(amax, y.most);
+  }
+  amax = wave_max(amax);
+  bool careful = false;
+  if (amax > __FLT_MAX__) {  // uniform: there are infinities, or NaN, which do not count
+    careful = true;
+    amax = 0.f;
+#pragma unroll
+    for (int p = 0; p < KEEP; ++p) amax = has[p] ? fmaxf(amax, x[p].finite_most()) : amax;
+    for (int t = 16 + grp; t < a.bs; t += RPP) {
+      Values y;
+      if (later(t, y)) amax = fmaxf(amax, y.finite_most());
+    }
+    amax = wave_max(amax);
+  }
+
+  const int need = scale_exponent<DT>(amax);
+  const int held = max(ScaleBounds<DT>::lo, min(ScaleBounds<DT>::hi, exponent_of(old)));
+  const int k = fresh ? need : max(held, need);
+  const bool grow = !fresh && k > held;
+  careful |= k == ScaleBounds<DT>::hi;  // (magnitudes past the pool's range)
+  // an old code's place under the wider scale: below 2^-100 every code is zero
+  const float shrink = pow2(max(held - k, -100));
+  auto put = [&](int t, bool has_row, const Values& y) {
+    u32x2* p0 = (u32x2*)(codes + (int64_t)t * D + 8 * ci);
+    u32x2* p1 = (u32x2*)(codes + (int64_t)t * D + 8 * ci + D / 2);
+    uint32_t c[4] = {0u, 0u, 0u, 0u};
+    if (has_row) {
+      if (careful) y.careful(c, pow2(-k));
+      else y.quick(c, pow2(k));
+    } else if (grow) {
+      const u32x2 c0 = *p0, c1 = *p1;
+      auto again = [&](uint32_t was) {
+        const f32x2 lo = decode2_f32<false>(was, shrink), hi = decode2_f32<true>(was, shrink);
+        return encode4(lo[0], lo[1], hi[0], hi[1]);
+      };
+      c[0] = again(c0[0]);
+      c[1] = again(c0[1]);
+      c[2] = again(c1[0]);
+      c[3] = again(c1[1]);
+    } else if (!fresh) {
+      return;
+    }
+    *p0 = u32x2{c[0], c[1]};
+    *p1 = u32x2{c[2], c[3]};
+  };
+#pragma unroll
+  for (int p = 0; p < KEEP; ++p) put(p * RPP + grp, has[p], x[p]);
+  for (int t = 16 + grp; t < a.bs; t += RPP) {
+    Values y;
+    const bool has_row = later(t, y);
+    put(t, has_row, y);
+  }
+  if (lane == 0) a.scales[2 * hb + is_v] = pow2(k);
+}
+
+// Writes block `blk`, if token i is the call's first of it: part `part` (K or V of a
+// head) by this wavefront. s_row [kMaxBlockSize], s_earlier: LDS. The whole workgroup
+// calls it alike, parts past the last included.
+template <int DT, int D, int MODE>
+__device__ __forceinline__ void write_block(const QuantArgs& a, int64_t i, int blk, int part, int* s_row,
+                                            int* s_earlier) {
+  constexpr int NT = kWriteWaves * 64;
+  const int tid = threadIdx.x;
+  const int64_t base = (int64_t)blk * a.bs;
+  const bool active = part < 2 * a.r.num_kv_heads;
+  const int h = part >> 1, is_v = part & 1;
+  const int64_t hb = (int64_t)h * a.num_blocks + blk;
+  float old = 0.f;
+  if (active) old = a.scales[2 * hb + is_v];
+  // ---- the block's tokens in this call: row + 1 that each takes, 0: none
+  __syncthreads();  // (the last block's readers are done)
+  for (int t = tid; t < a.bs; t += NT) s_row[t] = 0;
+  if (tid == 0) *s_earlier = 0;
+  __syncthreads();
+  constexpr int SCAN = 8;  // slots of a lane in flight together
+  for (int64_t j0 = tid; j0 < a.r.n_tokens; j0 += SCAN * NT) {
+    int64_t slot[SCAN];
+#pragma unroll
+    for (int u = 0; u < SCAN; ++u) slot[u] = j0 + u * NT < a.r.n_tokens ? a.r.slots[j0 + u * NT] : -1;
+#pragma unroll
+    for (int u = 0; u < SCAN; ++u) {
+      const uint64_t o = (uint64_t)slot[u] - (uint64_t)base;
+      if (o < (uint64_t)a.bs) {
+        atomicMax(&s_row[(int)o], (int)(j0 + u * NT) + 1);
+        if (j0 + u * NT < i) *s_earlier = 1;
+      }
+    }
+  }
+  __syncthreads();
+  if (*s_earlier || !active) return;  // another workgroup's block
+
+  // ---- this wavefront's head, K or V
+  if (MODE == kRowsPlain || is_v)
+    write_part<DT, D, kRowsPlain>(a, i, hb, h, is_v, old, s_row);
+  else
+    write_part<DT, D, MODE>(a, i, hb, h, is_v, old, s_row);
+}
+
+// A workgroup's place among the n of the write. Those of a prompt that own a block come
+// every block_size tokens, and workgroup b runs on XCD b mod 8: in their own order all
+// of them would share one or two XCDs (16.5 us for a mixed step's 1,248 tokens, 13.7
+// spread out). Each run of 8 is rotated by the sum of its index's octal digits, so that places
+// any power of two apart fall on all of them.
+__device__ __forceinline__ uint32_t spread_xcds(uint32_t b, uint32_t n) {
+  const uint32_t k = b >> 3;
+  if (8 * k + 8 > n) return b;  // a last, shorter run
+  const uint32_t turn = k + (k >> 3) + (k >> 6) + (k >> 9) + (k >> 12) + (k >> 15) + (k >> 18);
+  return 8 * k + ((b + turn) & 7u);
+}
+
 template <int DT, int D, int MODE>
 __global__ __launch_bounds__(kWriteWaves * 64) void kv_write_q8_kernel(QuantArgs a) {
-  typedef RowPair<DT, D> P;
-  constexpr int NT = kWriteWaves * 64;
-  constexpr int RPP = 64 / P::LPR;  // rows of a wavefront at a time
-  __shared__ int s_row[kMaxBlockSize];  // row + 1 that each token of the block takes, 0: none
+  __shared__ int s_row[kMaxBlockSize];
   __shared__ int s_earlier;
   if constexpr (MODE != kRowsPlain) {
     if (blockIdx.x >= a.n_kv) {
@@ -97,128 +362,26 @@ __global__ __launch_bounds__(kWriteWaves * 64) void kv_write_q8_kernel(QuantArgs
     }
   }
   const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t i = blockIdx.x / a.kv_groups;
-  const int part0 = (int)(blockIdx.x - i * a.kv_groups) * kWriteWaves;
-  const int64_t slot = a.r.slots[i];
-  if (slot < 0) return;  // padding sentinel
-  if (slot >= a.num_blocks * a.bs) {
-    if (tid == 0 && part0 == 0) flag_error(a.err, IR_ERR_SLOT_RANGE);
-    return;
+  const uint32_t group = spread_xcds(blockIdx.x, (uint32_t)a.n_kv);
+  const int64_t wi = group / (uint32_t)a.kv_groups;
+  const int part = (int)(group - wi * a.kv_groups) * kWriteWaves + (tid >> 6);
+  const int64_t num_slots = a.num_blocks * a.bs;
+  // lane l: token i0 + l of the window; it may own its block unless the token
+  // before it is in the same one
+  const int64_t i0 = wi * a.window;
+  const int wn = (int)min((int64_t)a.window, a.r.n_tokens - i0);
+  const int64_t my_slot = lane < wn ? a.r.slots[i0 + lane] : -1;
+  const int64_t before = lane < wn && i0 + lane > 0 ? a.r.slots[i0 + lane - 1] : -1;
+  const bool valid = my_slot >= 0 && my_slot < num_slots;  // (negative: padding)
+  if (my_slot >= num_slots && part == 0) flag_error(a.err, IR_ERR_SLOT_RANGE);
+  const int my_blk = valid ? (int)((uint32_t)my_slot / (uint32_t)a.bs) : -1;  // (slots fit 31 bits)
+  const int64_t my_base = (int64_t)my_blk * a.bs;
+  uint64_t todo = __ballot(valid && !(before >= my_base && before < my_base + a.bs));
+  while (todo) {  // uniform over the workgroup: every wavefront looks at the same window
+    const int at = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    write_block<DT, D, MODE>(a, i0 + at, __builtin_amdgcn_readlane(my_blk, at), part, s_row, &s_earlier);
   }
-  const int blk = (int)((uint32_t)slot / (uint32_t)a.bs);  // (the pool's slots fit 31 bits)
-  const int64_t base = (int64_t)blk * a.bs;
-  auto inside = [&](int64_t s) { return (uint64_t)s - (uint64_t)base < (uint64_t)a.bs; };
-  if (i > 0 && inside(a.r.slots[i - 1])) return;
-
-  // ---- the block's tokens in this call
-  for (int t = tid; t < a.bs; t += NT) s_row[t] = 0;
-  if (tid == 0) s_earlier = 0;
-  __syncthreads();
-  for (int64_t j = tid; j < a.r.n_tokens; j += NT) {
-    const int64_t s = a.r.slots[j];
-    if (inside(s)) {
-      atomicMax(&s_row[(int)(s - base)], (int)j + 1);
-      if (j < i) s_earlier = 1;
-    }
-  }
-  __syncthreads();
-  if (s_earlier) return;  // uniform
-  const bool fresh = s_row[0] != 0;
-
-  // ---- this wavefront's head, K or V
-  const int part = part0 + (tid >> 6);
-  if (part >= 2 * a.r.num_kv_heads) return;
-  const int h = part >> 1, is_v = part & 1;
-  const int64_t hb = (int64_t)h * a.num_blocks + blk;
-  float* sp = a.scales + 2 * hb + is_v;
-  const float old = *sp;
-  uint8_t* codes = (is_v ? a.vc : a.kc) + hb * a.bs * D;
-  const uint8_t* src = is_v ? a.r.v + h * a.r.v_head : a.r.k + h * a.r.k_head;
-  const int64_t tok_stride = is_v ? a.r.v_tok : a.r.k_tok;
-  const int ci = lane % P::LPR, grp = lane / P::LPR;
-  float w[16];
-  if constexpr (MODE == kRowsNorm) {
-    P pw;
-    pw.load(a.r.k_weight, ci);
-    pw.unpack(w);
-  }
-  // the new row of token t of the block into x; false: none
-  auto row = [&](int t, float (&x)[16]) -> bool {
-    const int64_t j = (int64_t)s_row[t] - 1;
-    if (j < 0) return false;  // (a row's lanes go together)
-    P p;
-    p.load(src + j * tok_stride, ci);
-    p.unpack(x);
-    if constexpr (MODE != kRowsPlain) {
-      if (!is_v) {
-        Angles<DT, D, MODE> t;
-        t.load(a.r.cos + j * a.r.cs_tok, a.r.sin + j * a.r.cs_tok, ci);
-        transform_row<DT, D, MODE>(x, w, a.r.eps, t);
-      }
-    }
-    return true;
-  };
-  // the first passes' rows stay in registers, those of larger blocks are read again
-  constexpr int KEEP = 16 / RPP;
-  float x[KEEP][16];
-  bool has[KEEP];
-  float amax = 0.f;
-#pragma unroll
-  for (int p = 0; p < KEEP; ++p) {
-    has[p] = row(p * RPP + grp, x[p]);
-    if (has[p])
-#pragma unroll
-      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_abs(x[p][e]));
-  }
-  for (int t = 16 + grp; t < a.bs; t += RPP) {
-    float y[16];
-    if (row(t, y))
-#pragma unroll
-      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_abs(y[e]));
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-
-  const int need = scale_exponent<DT>(amax);
-  const int held = max(ScaleBounds<DT>::lo, min(ScaleBounds<DT>::hi, exponent_of(old)));
-  const int k = fresh ? need : max(held, need);
-  const bool grow = !fresh && k > held;
-  const float inv = pow2(-k);
-  // an old code's place under the wider scale: below 2^-100 every code is zero
-  const float shrink = pow2(max(held - k, -100));
-  auto put = [&](int t, bool has_row, const float (&y)[16]) {
-    u32x2* p0 = (u32x2*)(codes + (int64_t)t * D + 8 * ci);
-    u32x2* p1 = (u32x2*)(codes + (int64_t)t * D + 8 * ci + D / 2);
-    u32x2 c0 = {0u, 0u}, c1 = {0u, 0u};
-    if (has_row) {
-      float z[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) z[e] = to_code_range<DT>(y[e], inv);
-      c0 = u32x2{encode4(z[0], z[1], z[2], z[3]), encode4(z[4], z[5], z[6], z[7])};
-      c1 = u32x2{encode4(z[8], z[9], z[10], z[11]), encode4(z[12], z[13], z[14], z[15])};
-    } else if (grow) {
-      c0 = *p0;
-      c1 = *p1;
-      auto again = [&](uint32_t c) {
-        const f32x2 lo = decode2_f32<false>(c, shrink), hi = decode2_f32<true>(c, shrink);
-        return encode4(lo[0], lo[1], hi[0], hi[1]);
-      };
-      c0 = u32x2{again(c0[0]), again(c0[1])};
-      c1 = u32x2{again(c1[0]), again(c1[1])};
-    } else if (!fresh) {
-      return;
-    }
-    *p0 = c0;
-    *p1 = c1;
-  };
-#pragma unroll
-  for (int p = 0; p < KEEP; ++p) put(p * RPP + grp, has[p], x[p]);
-  for (int t = 16 + grp; t < a.bs; t += RPP) {
-    float y[16];
-    const bool has_row = row(t, y);
-    put(t, has_row, y);
-  }
-  if (lane == 0) *sp = pow2(k);
 }
 
 struct ReadArgs {
@@ -308,7 +471,10 @@ int launch_write(const char* name, const QuantArgs& a0, int mode, hipStream_t s)
   QuantArgs a = a0;
   constexpr int G = 64 / (D / 16);
   a.kv_groups = (2 * a.r.num_kv_heads + kWriteWaves - 1) / kWriteWaves;
-  a.n_kv = a.r.n_tokens * a.kv_groups;
+  // one token a workgroup until the workgroups fill the device, then as many as keep
+  // it filled: in a prompt most tokens own no block, in a decode step each does
+  a.window = (int)std::max<int64_t>(1, std::min<int64_t>(16, a.r.n_tokens * a.kv_groups / kWriteGroups));
+  a.n_kv = (a.r.n_tokens + a.window - 1) / a.window * a.kv_groups;
   const int64_t runs = (a.r.num_q_heads + G - 1) / G;
   const int64_t n_q = mode == kRowsPlain ? 0 : (a.r.n_tokens * runs + kWriteWaves - 1) / kWriteWaves;
   IR_REQUIRE(a.r.n_tokens < 0x7fffffff && a.n_kv + n_q <= 0x7fffffff, "%s: too many tokens", name);

@@ -111,9 +111,7 @@ __device__ __forceinline__ void transform_row(float (&x)[16], const float (&w)[1
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
-#pragma unroll
-    for (int o = 1; o < D / 16; o <<= 1) ss += __shfl_xor(ss, o);
-    const float r = rsqrtf(ss * (1.f / D) + eps);
+    const float r = rsqrtf(row_sum<D / 16>(ss) * (1.f / D) + eps);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float a = x[e] * r * w[e], b = x[8 + e] * r * w[8 + e];

@@ -139,19 +139,8 @@ def gather_slots_q8(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """:func:`gather_slots` of a layer of an 8-bit pool, as values of ``dtype`` (the
     pool's, of which each is exactly a number)."""
-    dev = require_device(k_cache, v_cache, kv_scales, slots)
-    _code_layer("gather_slots_q8", k_cache, v_cache, kv_scales, block_size)
-    if slots.dtype != torch.int64:
-        raise RuntimeError("gather_slots_q8: slots must be int64")
-    flat = slots.reshape(-1).contiguous()
-    h, d = k_cache.shape[1:]
-    out = torch.empty(2, flat.numel(), h, d, dtype=dtype, device=dev)
-    rc = lib().ir_gather_slots_q8(
-        ptr(k_cache), ptr(v_cache), ptr(kv_scales), kv_scales.shape[1], block_size, ptr(flat), flat.numel(), h, d,
-        dtype_code(dtype), ptr(out[0]), ptr(out[1]), ptr(err_flags), stream_ptr(dev),
-    )
-    check(rc, "ir_gather_slots_q8")
-    return out[0].reshape(*slots.shape, h, d), out[1].reshape(*slots.shape, h, d)
+    return seam().gather_slots_q8(k_cache, v_cache, kv_scales, slots, int(block_size), dtype, err_flags,
+                                  stream_of(k_cache))
 
 
 def paged_gather_q8(

@@ -48,6 +48,8 @@ from infrared_amd._lib import (
     ERR_SLOT_RANGE,
     ERR_WRITE_SLOT,
     dtype_code,
+    seam,
+    stream_of,
 )
 
 _ERR_NAMES = {
@@ -381,15 +383,15 @@ class QuantPagedKVPool(PagedKVPool):
         (``[N]`` int64; negative: skipped)."""
         if k.dtype != self.dtype:
             raise RuntimeError(f"QuantPagedKVPool.write: k is {k.dtype}, the pool's dtype is {self.dtype}")
-        kernels.kv_scatter_q8(self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], k, v, slots,
-                              self.block_size, self.err_flags)
+        seam().pool_write_q8(self.k, self.v, self.kv_scales, layer_idx, k, v, slots, self.block_size, self.err_flags,
+                             stream_of(self.k))
         if self.strict:
             self.check_errors()
 
     def gather(self, layer_idx: int, gather_slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """``PagedKVPool.gather`` of the values the codes stand for, in ``dtype``."""
-        out = kernels.gather_slots_q8(self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], gather_slots,
-                                      self.block_size, self.dtype, self.err_flags)
+        out = seam().pool_gather_q8(self.k, self.v, self.kv_scales, layer_idx, gather_slots, self.block_size,
+                                    self.dtype, self.err_flags, stream_of(self.k))
         if self.strict:
             self.check_errors()
         return out
