@@ -343,6 +343,7 @@ int decode_call(const char* name, const float* scales, const void* q, int64_t q_
   DecodeArgs a;
   a.scales = (const f32x2*)scales;
   a.block16 = 0;
+  a.merge_later = 0;
   a.q = q;
   a.q_seq = q_seq_stride;
   a.q_head = q_head_stride;

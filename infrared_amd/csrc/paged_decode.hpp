@@ -61,6 +61,7 @@ struct DecodeArgs {
   // 8-bit caches: (K, V) scales [kv_head][block], 16-byte units of a block's codes
   const f32x2* scales;
   uint32_t block16;
+  int merge_later;  // the planned call's partial rows are merged by a launch of their own
 };
 
 // Per-lane byte offsets of this lane's K pieces and V rows inside a 16-token

@@ -793,6 +793,12 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       if (d0 == 0) store_dev2(r_ml, rr * 8, f32x2{stg.m[k][hc], stg.l[k][hc]});
     }
   }
+  if constexpr (Q8) {
+    if (a.merge_later) {
+      if (pend >= 0) write_out(label(pend));
+      return;
+    }
+  }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
@@ -864,6 +870,80 @@ void launch_planned_dt_d(const DecodeArgs& a, const uint8_t* plan, const PlanLay
                        0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
 }
 
+// The merge of the units that several slices share, as a launch of its own: one
+// workgroup per unit and column, D / 4 lanes a row and the rows dealt to its groups
+// of lanes, joined through LDS in group order. The last slice of a unit to arrive
+// merges its rows at one CU's pace, some 4 KB a row: with few units, each over many
+// slices, that pace is the call's (28 / 4 heads of 128: one sequence of 94,208
+// keys, 64 slices a unit, 35.0 us so against 26.4; three of 31,424, 21 slices, 28.8
+// against 26.4). With eight of 11,776, eight slices a unit, it is 25.1 either way, and
+// where the units are many it only adds a launch.
+constexpr int kMergeSlices = 12;  // slices a unit has, on average, from which on
+constexpr int kMergeThreads = 256;
+
+template <int DT, int D>
+__global__ __launch_bounds__(kMergeThreads) void paged_decode_planned_merge(const uint8_t* plan, uint32_t o_seq_pre,
+                                                                            uint32_t o_pair, int pairs, DecodeArgs a) {
+  constexpr int EB = TileShape<DT, D>::EB, LPR = D / 4, G = kMergeThreads / LPR;
+  __shared__ float s_part[G][D + 2];
+  const int32_t* hdr = (const int32_t*)plan;
+  const int32_t* pre = (const int32_t*)(plan + o_seq_pre);
+  const int R = hdr[1];
+  if (hdr[3] != 0 && !pairs) return;  // (flagged by the run)
+  const int u = blockIdx.x, col = blockIdx.y;
+  const int b = u / a.n_ups, j = u - b * a.n_ups;
+  const int ts = pre[b + 1] - pre[b];
+  if (ts == 0) return;
+  const int us = pre[b] * a.n_ups + j * ts, s0 = us / R;
+  const int np = (us + ts - 1) / R - s0 + 1;
+  const bool paired = pairs && ((const int32_t*)(plan + o_pair))[b] > 0;
+  const int hg = j % a.n_hg, kvh = j / a.n_hg;
+  if (np <= 1 || col >= (paired ? 2 * a.n_rep : min(16, a.n_rep - hg * 16))) return;
+  const int grp = threadIdx.x / LPR, d0 = 4 * (threadIdx.x % LPR);
+  float M = kNegInf, L = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int NB = 4;  // rows of a group in flight together
+  for (int p0 = grp; p0 < np; p0 += NB * G) {
+    f32x2 ml[NB];
+    f32x4 x[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int64_t row = (int64_t)(s0 + min(p0 + i * G, np - 1) + u) * 16 + col;
+      ml[i] = *(const f32x2*)(a.ws_ml + row * 2);
+      x[i] = *(const f32x4*)(a.ws_o + row * D + d0);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if (p0 + i * G >= np) continue;
+      // (weight 0 for a row without a key)
+      const float mn = fmaxf(M, ml[i][0]);
+      const float wa = fast_exp2(fmaxf(M - mn, -1e30f)), wb = fast_exp2(fmaxf(ml[i][0] - mn, -1e30f));
+      L = wa * L + wb * ml[i][1];
+      o = wa * o + wb * x[i];
+      M = mn;
+    }
+  }
+  *(f32x4*)&s_part[grp][d0] = o;
+  if (d0 == 0) {
+    s_part[grp][D] = L;
+    s_part[grp][D + 1] = M;
+  }
+  __syncthreads();
+  if (grp != 0) return;
+  for (int q = 1; q < min(G, np); ++q) {
+    const float mq = s_part[q][D + 1], mn = fmaxf(M, mq);
+    const float wa = fast_exp2(fmaxf(M - mn, -1e30f)), wb = fast_exp2(fmaxf(mq - mn, -1e30f));
+    L = wa * L + wb * s_part[q][D];
+    o = wa * o + wb * *(const f32x4*)&s_part[q][d0];
+    M = mn;
+  }
+  const int second = paired && col >= a.n_rep;
+  const int h = kvh * a.n_rep + hg * 16 + col - second * a.n_rep;
+  const float acc[4] = {o[0], o[1], o[2], o[3]};
+  store4<DT>((uint8_t*)a.out + ((int64_t)(b + second) * a.o_seq + (int64_t)h * a.o_head + d0) * EB, acc,
+             L > 0.f ? 1.f / L : 0.f);
+}
+
 template <int DT, int D>
 void launch_planned_q8(const DecodeArgs& a, const uint8_t* plan, const PlanLayout& ly, int grid, bool pairs,
                        hipStream_t s) {
@@ -875,6 +955,9 @@ void launch_planned_q8(const DecodeArgs& a, const uint8_t* plan, const PlanLayou
   else
     hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, false, true>), dim3(grid),
                        dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+  if (a.merge_later)
+    hipLaunchKernelGGL((paged_decode_planned_merge<DT, D>), dim3(a.num_seqs * a.n_ups, std::min(16, 2 * a.n_rep)),
+                       dim3(kMergeThreads), 0, s, plan, o_sp, o_pr, pairs ? 1 : 0, a);
 }
 
 // Pairs fit one unit's 16 MFMA columns when a KV head has at most 8 query
@@ -1031,6 +1114,7 @@ int planned_call(const char* name, const float* scales, const void* q, int64_t q
   a.err = err_flags;
   a.scales = (const f32x2*)scales;
   a.block16 = (uint32_t)(block_size * (head_dim / 16));
+  a.merge_later = scales && units * kMergeSlices <= grid;
   a.counters = counters;
   a.ws_o = (float*)workspace;
   a.ws_ml = (float*)((uint8_t*)workspace + ws.acc_bytes);

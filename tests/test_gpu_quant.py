@@ -343,6 +343,37 @@ def test_decode_of_long_contexts_and_shared_prefixes(planned):
     assert torch.equal(out, run_decode(pool, q, bt, ctx, planned))  # nothing of a call is left for the next
 
 
+@pytest.mark.parametrize("dtype, hq, h, d, lens", [
+    (torch.bfloat16, 28, 4, 128, [20011]), (torch.float16, 14, 2, 64, [9000, 0, 17]), (torch.float32, 6, 2, 128, [5000]),
+    (torch.bfloat16, 40, 2, 64, [8191, 4000]), (torch.bfloat16, 8, 1, 128, [300, 1, 0]),
+])
+def test_decode_of_few_sequences_over_many_slices(dtype, hq, h, d, lens):
+    """Few units, whose partial rows a launch of their own merges: groups of more than 16
+    query heads, an empty sequence, and the same with a sequence that shares a prefix."""
+    bs = 16
+    pool, tables, values = filled(23, dtype, lens, h, d, bs)
+    if lens[0] > 1000:
+        tables.append(tables[0][:200])
+        lens = lens + [200 * bs - 3]
+        tables, lens = [tables[0], tables[-1], *tables[1:-1]], [lens[0], lens[-1], *lens[1:-1]]
+    assert len(lens) * h * -(-hq // h // 16) * 12 <= 256
+    q = torch.randn(len(lens), hq, d, generator=gen(10), device=DEV).to(dtype)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    bt = device_tables(tables)
+    out = run_decode(pool, q, bt, ctx, True)
+    pool.check_errors()
+    for i, n in enumerate(lens):
+        if n == 0:
+            assert not out[i].any()
+            continue
+        o, a, reach = quant.attend(q[i : i + 1], values, tables[i], bs, n - 1, d**-0.5)
+        tol = fp32_tolerance(o, a, reach, d) if dtype == torch.float32 else (
+            decode_tolerance(o, a, dtype) + 4 * (d + 8) * 2.0**-24 * reach[..., None] * a)
+        err = (out[i : i + 1].double().cpu() - o).abs()
+        assert (err <= tol).all(), (i, n, (err / tol).max())
+    assert torch.equal(out, run_decode(pool, q, bt, ctx, True))
+
+
 @pytest.mark.parametrize("planned", [False, True])
 def test_decode_masks_bad_blocks_and_lengths(planned):
     bs, hq, h, d = 16, 8, 2, 64
