@@ -200,8 +200,12 @@ void paged_prefill_kernel(PrefillArgs a) {
   constexpr int EB = 2;
   constexpr int CT = S::CT, BN = S::BN, NT = S::NT;
   constexpr int RING = SCHED == kRing2 ? 2 : 3;
-  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][BN * S::KROW];
+  // QC: the keys stay codes and the queries become two pieces of codes each (bf16)
+  constexpr bool QC = Q8 && DT == IR_DTYPE_BF16;
+  constexpr int CROW = D + 16;  // bytes per key row of codes in LDS (16 rows apart without bank conflicts)
+  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][QC ? BN * CROW / 2 : BN * S::KROW];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[RING][BN * S::KROW];
+  __shared__ int ke_lds[QC ? RING : 1][4];  // QC: exponents of the scales of a tile's 16-key runs
   __shared__ int32_t bt_lds[kBtCache];
 
   const int tid = threadIdx.x;
@@ -285,7 +289,53 @@ void paged_prefill_kernel(PrefillArgs a) {
   // and scales it once its first key tile is staged, so Q's round trip
   // overlaps the block ids' and the first tile's instead of preceding them.
   constexpr bool EARLY = NW == 8 && CT == 1 && SCHED == kRing2;
+  // QC: a query times scale * log2 e, q = hi 2^e + lo 2^(e - 4) with e4m3 codes hi and lo
+  // (the first four and the last four bits of its significand: off by at most 2^-9 of
+  // q's power of two, half of what rounding to bf16 would be). At head_dim 64 one product
+  // of 128 k-slots holds both pieces, the codes of K twice; at 128 two follow each other.
   u32x4 qreg[CT][S::KS];
+  i32x8 qc[CT][D / 64];
+  int qe[CT][D / 64];
+  auto split_query = [&](int ct, const u32x4 (&x)[S::KS]) {
+    float v[S::KS * 8], most = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[8 * ks + 2 * i] = Elem<DT>::lo(x[ks][i]) * a.scale_log2;
+        v[8 * ks + 2 * i + 1] = Elem<DT>::hi(x[ks][i]) * a.scale_log2;
+        most = fmaxf(most, fmaxf(fabsf(v[8 * ks + 2 * i]), fabsf(v[8 * ks + 2 * i + 1])));
+      }
+    most = wave_max_groups_swap(most);
+    const int e = scale_exponent<IR_DTYPE_BF16>(most);
+    const float s_hi = pow2(e), s_lo = pow2(e - 4);
+    // (an infinite query becomes NaN, not a large number; NaN does by itself)
+    const int bad = __float_as_uint(most) >= 0x7f800000u ? 0x7f7f7f7f : 0;
+    typedef short i16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < S::KS * 2; ++i) {  // four elements
+      i16x2 h = {0, 0}, l = {0, 0};
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[4 * i], v[4 * i + 1], s_hi, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[4 * i + 2], v[4 * i + 3], s_hi, true);
+      const uint32_t hw = __builtin_bit_cast(uint32_t, h);
+      const f32x2 r0 = decode2_f32<false>(hw, s_hi), r1 = decode2_f32<true>(hw, s_hi);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, v[4 * i] - r0[0], v[4 * i + 1] - r0[1], s_lo, false);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, v[4 * i + 2] - r1[0], v[4 * i + 3] - r1[1], s_lo, true);
+      const int lw = __builtin_bit_cast(int, l);
+      qc[ct][0][i] = (int)hw | bad;
+      if constexpr (D == 128) qc[ct][1][i] = lw;
+      else qc[ct][0][4 + i] = lw;
+    }
+    if constexpr (D == 128) {
+      qe[ct][0] = e + 127;
+      qe[ct][1] = e - 4 + 127;
+    } else {
+      qe[ct][0] = (g < 2 ? e : e - 4) + 127;
+    }
+  };
+  // the lane's elements of a query row, ks-th eight: with codes, the k-slots of lane
+  // group g are the 16-code chunks g and g + 4 of the row
+  auto q_at = [&](int ks) { return QC ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : ks * 32 + 8 * g; };
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const Col col = column(ct);
@@ -293,8 +343,8 @@ void paged_prefill_kernel(PrefillArgs a) {
                            (int64_t)(col.ok ? col.head : 0) * a.q_head;
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
-      if constexpr (EARLY) {
-        const u32x4 x = *(const u32x4*)(qrow + ks * 32 + 8 * g);  // (a valid row when !col.ok)
+      if constexpr (EARLY || QC) {
+        const u32x4 x = *(const u32x4*)(qrow + q_at(ks));  // (a valid row when !col.ok)
         qreg[ct][ks] = col.ok ? x : u32x4{0u, 0u, 0u, 0u};
       } else {
         const u32x4 x = col.ok ? *(const u32x4*)(qrow + ks * 32 + 8 * g) : u32x4{0u, 0u, 0u, 0u};
@@ -303,6 +353,7 @@ void paged_prefill_kernel(PrefillArgs a) {
           qreg[ct][ks][e] = Elem<DT>::pack2(Elem<DT>::lo(x[e]) * a.scale_log2, Elem<DT>::hi(x[e]) * a.scale_log2);
       }
     }
+    if constexpr (QC && !EARLY) split_query(ct, qreg[ct]);
   }
 
   // ---- block-id cache: ids [bt_base, bt_base + kBtCache) of this sequence
@@ -402,7 +453,7 @@ void paged_prefill_kernel(PrefillArgs a) {
         const int64_t sl = slot_of(k0 + key, use, block);
         kr[i] = *(const u32x4*)(kc + sl + part * PE);
         vr[i] = *(const u32x4*)(vc + sl + part * PE);
-        if constexpr (Q8) sc[i] = scales[block];
+        if constexpr (Q8) sc[i] = scales[block];  // (block 0's for an unusable key, whose codes become 0)
         ku[i] = use;
       }
     }
@@ -428,7 +479,13 @@ void paged_prefill_kernel(PrefillArgs a) {
                   u32x4{decode2<DT, false>(x[2 * h], scale), decode2<DT, true>(x[2 * h], scale),
                         decode2<DT, false>(x[2 * h + 1], scale), decode2<DT, true>(x[2 * h + 1], scale)};
           };
-          wide(kp, k4, sc[i][0]);
+          if constexpr (QC) {
+            *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
+            if (part == 0 && (key & 15) == 0)
+              ke_lds[buf][key >> 4] = ku[i] ? (int)(__float_as_uint(sc[i][0]) >> 23) : 127;
+          } else {
+            wide(kp, k4, sc[i][0]);
+          }
           wide(vp, v4, sc[i][1]);
         } else {
           *(u32x4*)kp = k4;
@@ -478,6 +535,18 @@ void paged_prefill_kernel(PrefillArgs a) {
     const u32x4 ka = *(const u32x4*)&kb_lds[(kt * 16 + c) * S::KROW + ks * 32 + 8 * g];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) x[ct][kt] = mfma_k32<DT>(ka, qreg[ct][ks], x[ct][kt]);
+  };
+  // QC: all of key tile kt's scores from the codes staged in buffer buf.
+  auto qk_codes = [&](int buf, int kt, f32x4 (&x)[CT][4]) {
+    const uint8_t* row = (const uint8_t*)ks_lds[buf] + (kt * 16 + c) * CROW + 16 * g;
+    const u32x4 k0 = *(const u32x4*)row;
+    const u32x4 k1 = D == 128 ? *(const u32x4*)(row + 64) : k0;
+    const i32x8 ka = {(int)k0[0], (int)k0[1], (int)k0[2], (int)k0[3], (int)k1[0], (int)k1[1], (int)k1[2], (int)k1[3]};
+    const int ke = ke_lds[buf][kt];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) x[ct][kt] = mfma_codes_k128(ka, ke, qc[ct][i], qe[ct][i], x[ct][kt]);
   };
   auto zero_s = [](f32x4 (&x)[CT][4]) {
 #pragma unroll
@@ -628,7 +697,11 @@ void paged_prefill_kernel(PrefillArgs a) {
       store_from(t_lo & 1, kr[0], vr[0], sc8[0], ku[0]);
       __syncthreads();
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < CT; ++ct) {
+        if constexpr (QC) {
+          split_query(ct, qreg[ct]);
+          continue;
+        }
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
           const u32x4 x = qreg[ct][ks];
@@ -638,6 +711,7 @@ void paged_prefill_kernel(PrefillArgs a) {
             y[e] = Elem<DT>::pack2(Elem<DT>::lo(x[e]) * a.scale_log2, Elem<DT>::hi(x[e]) * a.scale_log2);
           qreg[ct][ks] = y;
         }
+      }
       f32x4 sc[CT][4];
       // tile kb (slot J): its scores, softmax and PV product from LDS buffer
       // kb % 2; tile kb + 1 staged from slot J + 1; tile kb + R's loads into slot J
@@ -648,8 +722,13 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
+        if constexpr (QC) {
 #pragma unroll
-        for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
+          for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
+        }
         step(std::false_type{}, kb, sc, sc);
         if (kb + 1 < t_hi)
           store_from((kb + 1) & 1, kr[(J + 1) % R], vr[(J + 1) % R], sc8[(J + 1) % R], ku[(J + 1) % R]);
@@ -680,8 +759,13 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
+        if constexpr (QC) {
 #pragma unroll
-        for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
+          for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
+        }
         step(std::false_type{}, kb, sc, sc);
         if (kb + 1 < t_hi) store_regs((kb + 1) & 1);
         if (kb + 2 < t_hi) load_regs(kb + 2);

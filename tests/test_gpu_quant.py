@@ -424,6 +424,37 @@ def test_prefill(plan, dtype, hq, h, d, bs):
         row += n
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_of_queries_of_any_size(dtype, d):
+    """Queries of zeros, of the type's small numbers, with one element that dwarfs the
+    others; infinite and NaN ones spoil their own rows alone."""
+    bs, hq, h, n = 16, 4, 2, 40
+    pool, tables, values = filled(33, dtype, [60], h, d, bs)
+    q = torch.randn(n, hq, d, generator=gen(14), device=DEV)
+    q[1] = 0.0
+    q[2] *= 1e-4
+    q[3, :, 5] *= 3e3
+    q[4, :, 5] *= 300.0
+    q[5] *= 60.0
+    q = q.to(dtype)
+    spoiled = torch.zeros(n, hq, dtype=torch.bool)
+    for i, x in ((7, float("inf")), (9, float("-inf")), (11, float("nan"))):
+        q[i, 1, 3] = x
+        spoiled[i, 1] = True
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    start = torch.tensor([20], dtype=torch.int32, device=DEV)
+    out = kernels.paged_prefill(q, pool.k[0], pool.v[0], device_tables(tables), cu, start, n, bs, d**-0.5,
+                                err_flags=pool.err_flags, kv_scales=pool.kv_scales[0])
+    o, a, reach = quant.attend(q.nan_to_num(0.0, 0.0, 0.0), values, tables[0], bs, 20, d**-0.5)
+    tol = fp32_tolerance(o, a, reach, d)
+    if dtype != torch.float32:
+        tol = tol + prefill_tolerance(o, a, reach, dtype)
+    out = out.double().cpu()
+    assert ((out - o).abs() <= tol)[~spoiled].all()
+    assert out[spoiled].isnan().any(-1).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_prefill_over_many_workgroups_and_wide_groups(dtype):
     """More workgroups than the device holds, cut items; 8-wavefront workgroups (more than
