@@ -469,6 +469,7 @@ void paged_prefill_kernel(PrefillArgs a) {
       if (q < PIECES) {
         const int key = q / (D / PE), part = q % (D / PE);
         const u32x4 k4 = zero_unless(kr[i], ku[i]), v4 = zero_unless(vr[i], ku[i]);
+        const f32x2 s2 = Q8 && ku[i] ? sc[i] : f32x2{1.f, 1.f};
         uint16_t* kp = &ks_lds[buf][key * S::KROW + part * PE];
         uint16_t* vp = &vs_lds[buf][key * S::KROW + part * PE];
         if constexpr (Q8) {
@@ -482,11 +483,11 @@ void paged_prefill_kernel(PrefillArgs a) {
           if constexpr (QC) {
             *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
             if (part == 0 && (key & 15) == 0)
-              ke_lds[buf][key >> 4] = ku[i] ? (int)(__float_as_uint(sc[i][0]) >> 23) : 127;
+              ke_lds[buf][key >> 4] = (int)(__float_as_uint(s2[0]) >> 23);
           } else {
-            wide(kp, k4, sc[i][0]);
+            wide(kp, k4, s2[0]);
           }
-          wide(vp, v4, sc[i][1]);
+          wide(vp, v4, s2[1]);
         } else {
           *(u32x4*)kp = k4;
           *(u32x4*)vp = v4;
@@ -610,6 +611,11 @@ void paged_prefill_kernel(PrefillArgs a) {
     // Program order is kept step by step (sched_barrier): each step's K operand
     // was read one step earlier, its MFMAs go to the matrix pipe and the
     // exponentials of SPS scores fill the VALU meanwhile.
+    // Q8: the wavefront in its exponentials goes first. Two workgroups share a CU, and
+    // the one in its products has the matrix pipe to itself either way, while the other
+    // would be held up by the operand reads between them (8 chunks of 512 tokens: 303 us
+    // without, 267 so; priority for the products instead 272..283).
+    if constexpr (Q8) __builtin_amdgcn_s_setprio(1);
     constexpr int NQK = 4 * S::KS, SPS = CT * 16 / NQK;
     auto k_operand = [&](int t) {
       return *(const u32x4*)&kn[((t % 4) * 16 + c) * S::KROW + (t / 4) * 32 + 8 * g];
@@ -656,6 +662,7 @@ void paged_prefill_kernel(PrefillArgs a) {
     auto v_operand = [&](int t) {
       return v_operand_tr(vb_lds, t);
     };
+    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
     u32x4 vring[kOperandAhead];
 #pragma unroll
     for (int t = 0; t < kOperandAhead; ++t) vring[t] = v_operand(t);
