@@ -659,7 +659,8 @@ int ir_paged_gather_q8(const void* k_cache, const void* v_cache, const float* sc
  * Attention over the 8-bit pool: ir_paged_decode, ir_paged_decode_planned and
  * ir_paged_prefill of the values that a layer holds, dtype being that of q and out.
  * Workspaces, counters and plans are theirs (a decode plan is built with
- * IR_DTYPE_E4M3 and the layer's strides). The step's new rows are written first
+ * IR_DTYPE_E4M3 and the layer's strides; partition_tokens 0 is
+ * ir_paged_decode_default_partition, at least 128). The step's new rows are written first
  * (ir_kv_scatter_q8): their blocks' scales are not known before, so the prefill has no
  * fused write.
  */

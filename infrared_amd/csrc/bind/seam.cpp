@@ -164,9 +164,9 @@ Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const Op
     check(ir_paged_decode_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                              (const float*)scales->data_ptr(), kc.size(0) / bs, bs, (const int32_t*)bt.data_ptr(),
                              bt.stride(0), max_blocks, (const int32_t*)ctx.data_ptr(), out.data_ptr(), out.stride(0),
-                             out.stride(1), b, hq, h_kv, d, (float)scale, dtype_code(q), part,
-                             need > 0 ? (int32_t*)ctr.data_ptr() : nullptr, n_ctr, need > 0 ? ws.data_ptr() : nullptr,
-                             need, (int32_t*)ptr(err), stream_of(stream)),
+                             out.stride(1), b, hq, h_kv, d, (float)scale, dtype_code(q),
+                             partition > 0 ? part : 0, need > 0 ? (int32_t*)ctr.data_ptr() : nullptr, n_ctr,
+                             need > 0 ? ws.data_ptr() : nullptr, need, (int32_t*)ptr(err), stream_of(stream)),
           "ir_paged_decode_q8");
     return out;
   }

@@ -11,6 +11,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "paged_decode.hpp"
 #include "status.hpp"
 
@@ -244,7 +246,13 @@ int launch_decode(const DecodeArgs& a, bool bs16, bool fused, hipStream_t s) {
   return check_launch("ir_paged_decode");
 }
 
-// An 8-bit cache: 4-wavefront workgroups, whose tiles are half a 16-bit one's bytes.
+// An 8-bit cache: 4-wavefront workgroups with two tiles in flight each. A partition has
+// two tiles a wavefront at least: a tile is half a 16-bit one's bytes, and merging more
+// partitions costs more than the shorter walk saves (8 sequences of <= 512 keys, 14 / 2
+// heads of 64: 6.6 us a call in partitions of 64 tokens, 6.0 of 128; one of 2048, 28 / 4
+// heads of 128: 11.9 and 9.1). A workspace sized for the default partition is enough.
+constexpr int kCodePartition = 128;
+
 template <int DT, int D>
 int launch_decode_q8(const DecodeArgs& a, bool fused, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * a.n_hg), (unsigned)a.max_parts);
@@ -325,8 +333,10 @@ int decode_call(const char* name, const float* scales, const void* q, int64_t q_
                  (cache_slot_stride * eb) % 16 == 0 && (cache_head_stride * eb) % 16 == 0 &&
                  (out_seq_stride * eb) % 16 == 0 && (out_head_stride * eb) % 16 == 0,
              "%s: strides must be multiples of 16 bytes", name);
-  if (partition_tokens <= 0)
+  if (partition_tokens <= 0) {
     partition_tokens = ir_paged_decode_default_partition(num_seqs, num_kv_heads, max_blocks_per_seq, block_size);
+    if (scales) partition_tokens = std::max(partition_tokens, kCodePartition);
+  }
   IR_REQUIRE(partition_tokens % 16 == 0 && partition_tokens <= kMaxPartition,
              "%s: partition_tokens %d must be a multiple of 16 and at most %d", name, partition_tokens,
              kMaxPartition);
