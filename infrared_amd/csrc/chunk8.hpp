@@ -37,6 +37,18 @@ struct Chunk8 {
       *(u32x4*)p = u32x4{E::pack2(x[0], x[1]), E::pack2(x[2], x[3]), E::pack2(x[4], x[5]), E::pack2(x[6], x[7])};
     }
   }
+  // non-temporal: for rows that the next kernel reads, on any XCD, and so not from the
+  // L2 that they would stay in
+  __device__ __forceinline__ static void store_nt(uint8_t* p, const float (&x)[8]) {
+    if constexpr (DT == IR_DTYPE_F32) {
+      __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, (f32x4*)p);
+      __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, (f32x4*)(p + 16));
+    } else {
+      using E = Elem<DT>;
+      __builtin_nontemporal_store(
+          u32x4{E::pack2(x[0], x[1]), E::pack2(x[2], x[3]), E::pack2(x[4], x[5]), E::pack2(x[6], x[7])}, (u32x4*)p);
+    }
+  }
   struct Raw {
     u32x4 w[EB / 2];
   };
@@ -47,6 +59,10 @@ struct Chunk8 {
   __device__ __forceinline__ static void raw_store(uint8_t* p, const Raw& r) {
 #pragma unroll
     for (int i = 0; i < EB / 2; ++i) *(u32x4*)(p + 16 * i) = r.w[i];
+  }
+  __device__ __forceinline__ static void raw_store_nt(uint8_t* p, const Raw& r) {
+#pragma unroll
+    for (int i = 0; i < EB / 2; ++i) __builtin_nontemporal_store(r.w[i], (u32x4*)(p + 16 * i));
   }
   __device__ __forceinline__ static void unpack(const Raw& r, float (&x)[8]) {
     if constexpr (DT == IR_DTYPE_F32) {

@@ -446,8 +446,8 @@ __global__ __launch_bounds__(256) void kv_read_q8_kernel(ReadArgs a) {
       v8[4 * i] = v0[0], v8[4 * i + 1] = v0[1], v8[4 * i + 2] = v1[0], v8[4 * i + 3] = v1[1];
     }
   }
-  C::store(a.ok + idx * 8 * C::EB, k8);
-  C::store(a.ov + idx * 8 * C::EB, v8);
+  C::store_nt(a.ok + idx * 8 * C::EB, k8);
+  C::store_nt(a.ov + idx * 8 * C::EB, v8);
 }
 
 // What every call on the pool checks.

@@ -57,8 +57,8 @@ struct RowPair {
     C::raw_load(p + ci * 8 * C::EB + HALF, b);
   }
   __device__ __forceinline__ void store_raw(uint8_t* p, int ci) const {
-    C::raw_store(p + ci * 8 * C::EB, a);
-    C::raw_store(p + ci * 8 * C::EB + HALF, b);
+    C::raw_store_nt(p + ci * 8 * C::EB, a);
+    C::raw_store_nt(p + ci * 8 * C::EB + HALF, b);
   }
   __device__ __forceinline__ void unpack(float (&x)[16]) const {
     float lo[8], hi[8];
@@ -77,8 +77,8 @@ struct RowPair {
       lo[e] = x[e];
       hi[e] = x[8 + e];
     }
-    C::store(p + ci * 8 * C::EB, lo);
-    C::store(p + ci * 8 * C::EB + HALF, hi);
+    C::store_nt(p + ci * 8 * C::EB, lo);
+    C::store_nt(p + ci * 8 * C::EB + HALF, hi);
   }
 };
 

