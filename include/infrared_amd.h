@@ -627,7 +627,9 @@ int ir_qk_norm_rope_kv_scatter(const void* q, int64_t q_tok_stride, int64_t q_he
  * ir_rope_kv_scatter_q8: ir_rope_kv_scatter (weights null), or
  * ir_qk_norm_rope_kv_scatter (weights given), into such a layer, one launch: the
  * keys are quantised as they leave the rotation (with norms from fp32, without an
- * intermediate rounding to dtype).
+ * intermediate rounding to dtype). q_out_dtype: dtype, or IR_DTYPE_F32 for queries as they
+ * leave the rotation (q_out and its strides are fp32's then), which the attention
+ * below takes.
  *
  * ir_gather_slots_q8, ir_paged_gather_q8: ir_gather_slots and ir_paged_gather of such a
  * layer, values of dtype; outputs 16-byte aligned.
@@ -645,7 +647,7 @@ int ir_rope_kv_scatter_q8(const void* q, int64_t q_tok_stride, int64_t q_head_st
                           int64_t cs_tok_stride, void* k_cache, void* v_cache, float* scales,
                           int64_t num_blocks, int block_size, const int64_t* slot_mapping,
                           int64_t n_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
-                          int32_t* err_flags, ir_stream_t stream);
+                          int q_out_dtype, int32_t* err_flags, ir_stream_t stream);
 int ir_gather_slots_q8(const void* k_cache, const void* v_cache, const float* scales, int64_t num_blocks,
                        int block_size, const int64_t* slots, int64_t n, int num_kv_heads, int head_dim,
                        int dtype, void* out_k, void* out_v, int32_t* err_flags, ir_stream_t stream);
@@ -657,7 +659,9 @@ int ir_paged_gather_q8(const void* k_cache, const void* v_cache, const float* sc
 
 /*
  * Attention over the 8-bit pool: ir_paged_decode, ir_paged_decode_planned and
- * ir_paged_prefill of the values that a layer holds, dtype being that of q and out.
+ * ir_paged_prefill of the values that a layer holds, dtype being that of the pool and out.
+ * q_dtype: dtype, or IR_DTYPE_F32 with a 16-bit dtype for queries that were not rounded to
+ * it; they are used to 14 bits at least.
  * Workspaces, counters and plans are theirs (a decode plan is built with
  * IR_DTYPE_E4M3 and the layer's strides; partition_tokens 0 is
  * ir_paged_decode_default_partition, at least 128). The step's new rows are written first
@@ -669,22 +673,22 @@ int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q_head_strid
                        const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
                        const int32_t* context_lens, void* out, int64_t out_seq_stride,
                        int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
-                       int head_dim, float scale, int dtype, int partition_tokens, int32_t* counters,
+                       int head_dim, float scale, int dtype, int q_dtype, int partition_tokens, int32_t* counters,
                        int64_t num_counters, void* workspace, int64_t workspace_bytes,
                        int32_t* err_flags, ir_stream_t stream);
 int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
                                const void* k_cache, const void* v_cache, const float* scales, void* out,
                                int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
                                int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
-                               int block_size, float scale, int dtype, int flags, const void* plan,
+                               int block_size, float scale, int dtype, int q_dtype, int flags, const void* plan,
                                int32_t* counters, int64_t num_counters, void* workspace,
                                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream);
 int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache, const void*
                         v_cache, const float* scales, int64_t num_blocks, int block_size, const int32_t* block_tables,
                         int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
                         int num_seqs, int total_q, int max_q_len, void* out, int64_t out_tok_stride, int64_t
-                        out_head_stride, int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype, void*
-                        plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
+                        out_head_stride, int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype,
+                        int q_dtype, void* plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
 
 /*
  * Read-only HBM streaming roof (a measurement utility; no counterpart in the

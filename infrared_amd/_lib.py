@@ -149,8 +149,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ir_rope_kv_scatter_q8": (
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
-         _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_p,
-         _c_p],
+         _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_p, _c_p],
     ),
     "ir_gather_slots_q8": (
         _c_i32,
@@ -164,17 +164,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ir_paged_decode_q8": (
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i64, _c_i64,
-         _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
     ),
     "ir_paged_decode_planned_q8": (
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
-         _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+         _c_i32, _c_f32, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
     ),
     "ir_paged_prefill_q8": (
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_i32,
-         _c_i32, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_p, _c_i64, _c_p, _c_p],
+         _c_i32, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_p],
     ),
 }
 

@@ -82,11 +82,14 @@ void code_layer(const char* name, const Tensor& kc, const Tensor& vc, const Tens
           name, ": kv_scales must be contiguous fp32 [num_kv_heads, num_blocks, 2]");
 }
 
-// An output the caller gave for `like`'s shape (strides are the kernel's to check).
-void given_out(const char* name, const Tensor& out, const Tensor& like) {
+// An output the caller gave for `like`'s shape (strides are the kernel's to check). One of
+// them may be fp32 beside the other's 16 bits, the one that `wide` names.
+enum class Wide { kOut, kLike };
+void given_out(const char* name, const Tensor& out, const Tensor& like, Wide wide) {
   require_device({&like, &out});
-  require(out.sizes() == like.sizes() && out.scalar_type() == like.scalar_type(), name, ": out must be ",
-          like.sizes(), " of ", like.scalar_type());
+  const Tensor& w = wide == Wide::kOut ? out : like;
+  require(out.sizes() == like.sizes() && (out.scalar_type() == like.scalar_type() || w.scalar_type() == at::kFloat),
+          name, ": out must be ", like.sizes(), " of ", like.scalar_type());
   unit_last(name, out);
 }
 
@@ -146,7 +149,7 @@ Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const Op
   require(d == kc.size(2) && (scales || q.scalar_type() == kc.scalar_type()) && vc.sizes() == kc.sizes(),
           "paged_decode: q / pool shape or dtype mismatch");
   if (scales) code_layer("paged_decode", kc, vc, *scales, block_size);
-  if (scales && out_) given_out("paged_decode", *out_, q);
+  if (scales && out_) given_out("paged_decode", *out_, q, Wide::kLike);
   require(bt.size(0) == b, "paged_decode: block_tables rows != batch");
   unit_last("paged_decode q", q);
   const Tensor out = out_ ? *out_ : at::empty({b, hq, d}, q.options());
@@ -164,7 +167,7 @@ Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const Op
     check(ir_paged_decode_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                              (const float*)scales->data_ptr(), kc.size(0) / bs, bs, (const int32_t*)bt.data_ptr(),
                              bt.stride(0), max_blocks, (const int32_t*)ctx.data_ptr(), out.data_ptr(), out.stride(0),
-                             out.stride(1), b, hq, h_kv, d, (float)scale, dtype_code(q),
+                             out.stride(1), b, hq, h_kv, d, (float)scale, dtype_code(out), dtype_code(q),
                              partition > 0 ? part : 0, need > 0 ? (int32_t*)ctr.data_ptr() : nullptr, n_ctr,
                              need > 0 ? ws.data_ptr() : nullptr, need, (int32_t*)ptr(err), stream_of(stream)),
           "ir_paged_decode_q8");
@@ -216,7 +219,7 @@ Tensor planned_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const O
   require(d == kc.size(2) && (scales || q.scalar_type() == kc.scalar_type()),
           "paged_decode_planned: q / pool shape or dtype mismatch");
   if (scales) code_layer("paged_decode_planned", kc, vc, *scales, bs);
-  if (scales && out_) given_out("paged_decode_planned", *out_, q);
+  if (scales && out_) given_out("paged_decode_planned", *out_, q, Wide::kLike);
   unit_last("paged_decode_planned q", q);
   const Tensor out = out_ ? *out_ : at::empty({b, hq, d}, q.options());
   const Tensor ws = scratch(workspace, ir_paged_decode_planned_workspace_bytes(b, hq, (int)p_hkv, d), q);
@@ -225,9 +228,9 @@ Tensor planned_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const O
   if (scales) {
     check(ir_paged_decode_planned_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                                      (const float*)scales->data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), b,
-                                     hq, (int)p_hkv, d, (int)max_blocks, (int)bs, (float)scale, dtype_code(q),
-                                     (int)flags, plan_buf.data_ptr(), (int32_t*)ctr.data_ptr(), n_ctr, ws.data_ptr(),
-                                     ws.numel(), (int32_t*)ptr(err), stream_of(stream)),
+                                     hq, (int)p_hkv, d, (int)max_blocks, (int)bs, (float)scale, dtype_code(out),
+                                     dtype_code(q), (int)flags, plan_buf.data_ptr(), (int32_t*)ctr.data_ptr(), n_ctr,
+                                     ws.data_ptr(), ws.numel(), (int32_t*)ptr(err), stream_of(stream)),
           "ir_paged_decode_planned_q8");
     return out;
   }
@@ -431,7 +434,10 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
   unit_last(name, q);
   unit_last(name, k);
   unit_last(name, v);
-  if (q_out_) given_out(name, *q_out_, q);
+  if (q_out_) {
+    given_out(name, *q_out_, q, Wide::kOut);
+    require(scales || q_out_->scalar_type() == q.scalar_type(), name, ": q_out must be of ", q.scalar_type());
+  }
   const Tensor qo = q_out_ ? *q_out_ : at::empty_like(q);
   const Tensor s = slots.contiguous();
   if (scales) {
@@ -441,7 +447,7 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
                                 (const float*)sin.data_ptr(), cos.stride(0), kc.data_ptr(), vc.data_ptr(),
                                 (float*)scales->data_ptr(), scales->size(1), (int)block_size,
                                 (const int64_t*)s.data_ptr(), n, (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q),
-                                (int32_t*)ptr(err), stream_of(stream)),
+                                dtype_code(qo), (int32_t*)ptr(err), stream_of(stream)),
           "ir_rope_kv_scatter_q8");
     return qo;
   }
@@ -524,14 +530,14 @@ Tensor paged_prefill_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, con
             "paged_prefill: ", name, " must be contiguous int32 [", n, "]");
   unit_last("paged_prefill q", q);
   if (plan_buf) require_device({&q, &*plan_buf});
-  if (out_) given_out("paged_prefill", *out_, q);
+  if (out_) given_out("paged_prefill", *out_, q, Wide::kLike);
   const Tensor out = out_ ? *out_ : at::empty(q.sizes(), q.options());
   check(ir_paged_prefill_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                             (const float*)scales.data_ptr(), scales.size(1), (int)block_size,
                             (const int32_t*)bt.data_ptr(), bt.stride(0), (int)bt.size(1), (const int32_t*)cu.data_ptr(),
                             (const int32_t*)q_start.data_ptr(), (int)b, (int)q.size(0), (int)max_q_len, out.data_ptr(),
-                            out.stride(0), out.stride(1), hq, h_kv, d, (float)scale, dtype_code(q), ptr(plan_buf),
-                            plan_buf ? plan_buf->numel() : 0, (int32_t*)ptr(err), stream_of(stream)),
+                            out.stride(0), out.stride(1), hq, h_kv, d, (float)scale, dtype_code(out), dtype_code(q),
+                            ptr(plan_buf), plan_buf ? plan_buf->numel() : 0, (int32_t*)ptr(err), stream_of(stream)),
         "ir_paged_prefill_q8");
   return out;
 }

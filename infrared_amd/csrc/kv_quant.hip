@@ -94,7 +94,9 @@ __device__ __forceinline__ void query_rows(const RowArgs& r, int64_t wave) {
   }
   p.unpack(x);
   transform_row<DT, D, MODE>(x, w, r.eps, t);
-  P::store(r.qo + tok * r.qo_tok + h * r.qo_head, ci, x);
+  uint8_t* to = r.qo + tok * r.qo_tok + h * r.qo_head;
+  if (r.qo_wide) RowPair<IR_DTYPE_F32, D>::store(to, ci, x);
+  else P::store(to, ci, x);
 }
 
 // A lane's part of a new row as it is loaded, with the token's tables for a key that
@@ -568,10 +570,13 @@ extern "C" int ir_rope_kv_scatter_q8(const void* q, int64_t q_tok_stride, int64_
                                      const float* cos, const float* sin, int64_t cs_tok_stride, void* k_cache,
                                      void* v_cache, float* scales, int64_t num_blocks, int block_size,
                                      const int64_t* slot_mapping, int64_t n_tokens, int num_q_heads, int num_kv_heads,
-                                     int head_dim, int dtype, int32_t* err_flags, ir_stream_t stream) {
+                                     int head_dim, int dtype, int q_out_dtype, int32_t* err_flags,
+                                     ir_stream_t stream) {
   const char* name = "ir_rope_kv_scatter_q8";
   const int eb = dtype_bytes(dtype);
   IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
+  IR_REQUIRE(q_out_dtype == dtype || q_out_dtype == IR_DTYPE_F32, "%s: unknown q_out_dtype %d for dtype %d", name,
+             q_out_dtype, dtype);
   IR_REQUIRE(n_tokens >= 0 && num_q_heads >= 0, "%s: bad sizes", name);
   if (n_tokens == 0) return ok();
   int rc = check_pool(name, k_cache, v_cache, scales, num_blocks, block_size, num_kv_heads, head_dim);
@@ -579,7 +584,7 @@ extern "C" int ir_rope_kv_scatter_q8(const void* q, int64_t q_tok_stride, int64_
   QuantArgs a = {};
   rc = fill_row_args(name, a.r, q, q_tok_stride, q_head_stride, q_out, qo_tok_stride, qo_head_stride, k, k_tok_stride,
                      k_head_stride, v, v_tok_stride, v_head_stride, q_weight, k_weight, eps, cos, sin, cs_tok_stride,
-                     slot_mapping, n_tokens, num_q_heads, num_kv_heads, eb);
+                     slot_mapping, n_tokens, num_q_heads, num_kv_heads, eb, dtype_bytes(q_out_dtype));
   if (rc != IR_OK) return rc;
   a.kc = (uint8_t*)k_cache;
   a.vc = (uint8_t*)v_cache;

@@ -21,6 +21,7 @@ struct RowArgs {
   const uint8_t* q;
   int64_t q_tok, q_head;  // bytes, as every stride here
   uint8_t* qo;
+  int qo_wide;  // the rotated queries are stored as fp32, whatever the dtype
   int64_t qo_tok, qo_head;
   const uint8_t* k;
   int64_t k_tok, k_head;
@@ -37,13 +38,13 @@ struct RowArgs {
   int num_q_heads, num_kv_heads;
 };
 
-// Checks a C call's row arguments (strides in elements of eb bytes; the norm
+// Checks a C call's row arguments (strides in elements of eb bytes, q_out's of qo_eb; the norm
 // weights both given or both null) and fills r; an IR_E* code on refusal.
 int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, int64_t q_head, void* q_out,
                   int64_t qo_tok, int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v,
                   int64_t v_tok, int64_t v_head, const void* q_weight, const void* k_weight, float eps,
                   const float* cos, const float* sin, int64_t cs_tok, const int64_t* slots, int64_t n_tokens,
-                  int num_q_heads, int num_kv_heads, int eb);
+                  int num_q_heads, int num_kv_heads, int eb, int qo_eb);
 
 // Lane `ci` of a row: its 16 elements of the row at `p`, [8 ci, +8) of either half.
 template <int DT, int D>

@@ -46,7 +46,7 @@ __device__ __forceinline__ void merge_partials(const DecodeArgs& a, int seq, int
 // 16-bit dtypes: two wavefronts per SIMD (<= 256 registers each) keep two
 // resident workgroups' worth of loads in flight per CU. fp32 tiles are twice
 // the registers and run one per SIMD.
-template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH, bool Q8 = false>
+template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH, bool Q8 = false, bool QF = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 ? 1 : 2)))
 void paged_decode_kernel(DecodeArgs a) {
   typedef TileShape<DT, D> Sh;
@@ -83,14 +83,15 @@ void paged_decode_kernel(DecodeArgs a) {
   const uint8_t* vc = (const uint8_t*)a.vc + (int64_t)kvh * a.c_head * F::EB;
   const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
   const typename F::Offsets lo = F::offsets(lane, a.c_slot * F::EB);
-  uint32_t qr[Sh::KDW];
+  QueryRegs<DT, D, QF> qr;
   load_query_for<DT, D, Q8>(a, seq, kvh * a.n_rep + h_local, h_local < a.n_rep, g, qr);
+  qr.split();
 
   State<D> st;
   state_init(st);
   bool bad = false;
-  attend_tiles<DT, D, BS16, NW, DEPTH, Q8>(a, bt_row, kc, vc, scales, lo, qr, tile_lo, tile_hi, t_end, kstage[w], lane,
-                                           w, st, bad);
+  attend_tiles<DT, D, BS16, NW, DEPTH, Q8, QF>(a, bt_row, kc, vc, scales, lo, qr, tile_lo, tile_hi, t_end, kstage[w],
+                                               lane, w, st, bad);
   if (bad) flag_error(a.err, IR_ERR_BLOCK_RANGE);
   st.l = wave_sum_groups(st.l);
 
@@ -253,13 +254,13 @@ int launch_decode(const DecodeArgs& a, bool bs16, bool fused, hipStream_t s) {
 // heads of 128: 11.9 and 9.1). A workspace sized for the default partition is enough.
 constexpr int kCodePartition = 128;
 
-template <int DT, int D>
+template <int DT, int D, bool QF>
 int launch_decode_q8(const DecodeArgs& a, bool fused, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * a.n_hg), (unsigned)a.max_parts);
   if (fused || a.max_parts == 1) {
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, true, 2, true>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, true, 2, true, QF>), grid, dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, false, 2, true>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, false, 2, true, QF>), grid, dim3(256), 0, s, a);
     hipLaunchKernelGGL((paged_decode_reduce<DT, D>), dim3(grid.x), dim3(256), 0, s, a);
   }
   return check_launch("ir_paged_decode_q8");
@@ -309,8 +310,9 @@ extern "C" int64_t ir_paged_decode_num_counters(int num_seqs, int num_q_heads, i
 namespace {
 
 // ir_paged_decode, and with `scales` ir_paged_decode_q8 (a dense layer of codes).
-int decode_call(const char* name, const float* scales, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
-                const void* k_cache, const void* v_cache, int64_t cache_slot_stride, int64_t cache_head_stride,
+int decode_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_seq_stride,
+                int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
+                int64_t cache_head_stride,
                 int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                 int max_blocks_per_seq, const int32_t* context_lens, void* out, int64_t out_seq_stride,
                 int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, float scale,
@@ -318,6 +320,9 @@ int decode_call(const char* name, const float* scales, const void* q, int64_t q_
                 int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   const int eb = dtype_bytes(dtype);
   IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
+  IR_REQUIRE(q_dtype == dtype || (scales && q_dtype == IR_DTYPE_F32), "%s: unknown q_dtype %d for dtype %d", name,
+             q_dtype, dtype);
+  const int q_eb = dtype_bytes(q_dtype);
   IR_REQUIRE(num_seqs >= 0 && num_q_heads > 0 && num_kv_heads > 0 && block_size > 0 &&
                  max_blocks_per_seq >= 0 && num_blocks >= 0,
              "%s: bad sizes", name);
@@ -329,7 +334,7 @@ int decode_call(const char* name, const float* scales, const void* q, int64_t q_
   IR_REQUIRE(q && k_cache && v_cache && block_tables && context_lens && out, "%s: null pointer", name);
   IR_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
              "%s: q, caches and out must be 16-byte aligned", name);
-  IR_REQUIRE((q_seq_stride * eb) % 16 == 0 && (q_head_stride * eb) % 16 == 0 &&
+  IR_REQUIRE((q_seq_stride * q_eb) % 16 == 0 && (q_head_stride * q_eb) % 16 == 0 &&
                  (cache_slot_stride * eb) % 16 == 0 && (cache_head_stride * eb) % 16 == 0 &&
                  (out_seq_stride * eb) % 16 == 0 && (out_head_stride * eb) % 16 == 0,
              "%s: strides must be multiples of 16 bytes", name);
@@ -403,17 +408,18 @@ int decode_call(const char* name, const float* scales, const void* q, int64_t q_
   }
   hipStream_t s = (hipStream_t)stream;
   if (scales) {
+    const bool qf = q_dtype != dtype;
+#define IR_DECODE_Q8(DT_, QF_) \
+  (head_dim == 128 ? launch_decode_q8<DT_, 128, QF_>(a, fused, s) : launch_decode_q8<DT_, 64, QF_>(a, fused, s))
     switch (dtype) {
       case IR_DTYPE_BF16:
-        return head_dim == 128 ? launch_decode_q8<IR_DTYPE_BF16, 128>(a, fused, s)
-                               : launch_decode_q8<IR_DTYPE_BF16, 64>(a, fused, s);
+        return qf ? IR_DECODE_Q8(IR_DTYPE_BF16, true) : IR_DECODE_Q8(IR_DTYPE_BF16, false);
       case IR_DTYPE_F16:
-        return head_dim == 128 ? launch_decode_q8<IR_DTYPE_F16, 128>(a, fused, s)
-                               : launch_decode_q8<IR_DTYPE_F16, 64>(a, fused, s);
+        return qf ? IR_DECODE_Q8(IR_DTYPE_F16, true) : IR_DECODE_Q8(IR_DTYPE_F16, false);
       default:
-        return head_dim == 128 ? launch_decode_q8<IR_DTYPE_F32, 128>(a, fused, s)
-                               : launch_decode_q8<IR_DTYPE_F32, 64>(a, fused, s);
+        return IR_DECODE_Q8(IR_DTYPE_F32, false);
     }
+#undef IR_DECODE_Q8
   }
   switch (dtype) {
     case IR_DTYPE_BF16:
@@ -439,8 +445,8 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
                                int head_dim, float scale, int dtype, int partition_tokens,
                                int32_t* counters, int64_t num_counters, void* workspace,
                                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
-  return decode_call("ir_paged_decode", nullptr, q, q_seq_stride, q_head_stride, k_cache, v_cache, cache_slot_stride,
-                     cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
+  return decode_call("ir_paged_decode", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                     cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
                      context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
                      scale, dtype, partition_tokens, counters, num_counters, workspace, workspace_bytes, err_flags,
                      stream);
@@ -451,12 +457,12 @@ extern "C" int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q
                                   const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
                                   const int32_t* context_lens, void* out, int64_t out_seq_stride,
                                   int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
-                                  int head_dim, float scale, int dtype, int partition_tokens, int32_t* counters,
-                                  int64_t num_counters, void* workspace, int64_t workspace_bytes, int32_t* err_flags,
-                                  ir_stream_t stream) {
+                                  int head_dim, float scale, int dtype, int q_dtype, int partition_tokens,
+                                  int32_t* counters, int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                                  int32_t* err_flags, ir_stream_t stream) {
   if (num_seqs == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_decode_q8: null pointer");
-  return decode_call("ir_paged_decode_q8", scales, q, q_seq_stride, q_head_stride, k_cache, v_cache, head_dim,
+  return decode_call("ir_paged_decode_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache, head_dim,
                      num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
                      max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
                      num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,

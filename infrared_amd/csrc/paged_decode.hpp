@@ -122,6 +122,34 @@ struct CacheFormat<DT, D, true> {
   }
 };
 
+// A query operand in registers; with QF (an fp32 query of a 16-bit pool) first the 16
+// elements of a step as they are loaded, x then rest, and after split() two pieces.
+template <int DT, int D, bool QF>
+struct QueryRegs {
+  uint32_t x[TileShape<DT, D>::KDW];
+  __device__ __forceinline__ void split() {}
+};
+template <int DT, int D>
+struct QueryRegs<DT, D, true> {
+  static constexpr int N = TileShape<DT, D>::KDW;
+  uint32_t x[N], rest[N];
+  __device__ __forceinline__ void split() {
+    uint32_t hi[N], lo[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {  // elements 2i, 2i + 1 of the lane's
+      const float a = __uint_as_float(2 * i < N ? x[2 * i] : rest[2 * i - N]);
+      const float b = __uint_as_float(2 * i < N ? x[2 * i + 1] : rest[2 * i + 1 - N]);
+      hi[i] = Elem<DT>::pack2(a, b);
+      lo[i] = Elem<DT>::pack2(a - Elem<DT>::lo(hi[i]), b - Elem<DT>::hi(hi[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x[i] = hi[i];
+      rest[i] = lo[i];
+    }
+  }
+};
+
 // Issues a code tile's loads; the tile's first row is at tk / tv.
 template <int DT, int D>
 __device__ __forceinline__ void issue_codes(const uint8_t* tk, const uint8_t* tv,
@@ -244,10 +272,13 @@ __device__ __forceinline__ void compute_tile(const Tile<DT, D>& tl, const uint32
 // key (load_query_codes: the same of the query), one 16-byte read each. They are used
 // without their scale, which score_scale (times scale * log2 e) holds; the V codes
 // are multiplied by theirs, both exact.
-template <int DT, int D>
-__device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const uint32_t (&qr)[TileShape<DT, D>::KDW],
-                                              uint32_t kmask, float score_scale, float v_scale, uint8_t* kst, int lane,
-                                              State<D>& st, bool col_on = true) {
+//
+// QF: a 16-bit pool's query is fp32 and held in two pieces of the dtype, its rounded
+// value and what that leaves, off by 2^-16 of it (f16: 2^-22) instead of 2^-8 (2^-11).
+template <int DT, int D, bool QF>
+__device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const QueryRegs<DT, D, QF>& q, uint32_t kmask,
+                                              float score_scale, float v_scale, uint8_t* kst, int lane, State<D>& st,
+                                              bool col_on = true) {
   typedef TileShape<DT, D> Sh;
   constexpr int CPR = D / 16;  // 16-byte chunks per row
   const int g = lane >> 4, t = staged_token(lane & 15);
@@ -281,7 +312,8 @@ __device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const uint3
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  const f32x4 s = qk_tile<DT, D>(kop, qr);
+  f32x4 s = qk_tile<DT, D>(kop, q.x);
+  if constexpr (QF) s += qk_tile<DT, D>(kop, q.rest);
   uint32_t v[4][Sh::VDW];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -332,12 +364,12 @@ __device__ __forceinline__ int clamp_ctx(const DecodeArgs& a, int seq, bool repo
 // (wavefront w takes tiles tile_lo + w, tile_lo + w + NW, ...) into st. Keys
 // at or past t_end are masked. Runs of up to NW * kMaxWaveTiles tiles: each
 // run fetches its block ids once, one per lane.
-template <int DT, int D, bool BS16, int NW, int DEPTH, bool Q8>
+template <int DT, int D, bool BS16, int NW, int DEPTH, bool Q8, bool QF>
 __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t* bt_row, const uint8_t* kc,
                                              const uint8_t* vc, const f32x2* scales,
                                              const typename CacheFormat<DT, D, Q8>::Offsets& lo,
-                                             const uint32_t (&qr)[TileShape<DT, D>::KDW], int tile_lo, int tile_hi,
-                                             int t_end, uint8_t* kst, int lane, int w, State<D>& st, bool& bad) {
+                                             const QueryRegs<DT, D, QF>& qr, int tile_lo, int tile_hi, int t_end,
+                                             uint8_t* kst, int lane, int w, State<D>& st, bool& bad) {
   static_assert(BS16 || !Q8, "a block of codes holds whole tiles");
   typedef typename CacheFormat<DT, D, Q8>::Raw Raw;
   constexpr int RUN = NW * kMaxWaveTiles;
@@ -379,9 +411,9 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
         const int ii = min(i, last);
         const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[0]), ii));
         const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[1]), ii));
-        compute_codes<DT, D>(tl, qr, mask, a.scale_log2 * ks, vs, kst, lane, st);
+        compute_codes<DT, D, QF>(tl, qr, mask, a.scale_log2 * ks, vs, kst, lane, st);
       } else
-        compute_tile<DT, D>(tl, qr, mask, a.scale_log2, kst, lane, st);
+        compute_tile<DT, D>(tl, qr.x, mask, a.scale_log2, kst, lane, st);
     };
 #pragma unroll
     for (int r = 0; r < DEPTH; ++r) mk[r] = issue(min(r, last), ring[r]);
@@ -421,34 +453,38 @@ __device__ __forceinline__ void load_query(const DecodeArgs& a, int seq, int qh,
     zero_dwords(qr);
 }
 
-// The query operand that goes with code tiles (compute_codes).
-template <int DT, int D>
+// The query operand that goes with code tiles (compute_codes), before its split().
+template <int DT, int D, bool QF>
 __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
-                                                 uint32_t (&qr)[TileShape<DT, D>::KDW]) {
+                                                 QueryRegs<DT, D, QF>& q) {
   typedef TileShape<DT, D> Sh;
-  if (!head_ok) {
-    zero_dwords(qr);
-    return;
-  }
-  const uint8_t* row = (const uint8_t*)a.q + ((int64_t)seq * a.q_seq + (int64_t)qh * a.q_head + 16 * g) * Sh::EB;
-  constexpr int DW = 4 * Sh::EB;  // dwords of 16 elements
+  constexpr int EB = QF ? 4 : Sh::EB;
+  constexpr int DW = 4 * EB;  // dwords of 16 elements
+  const uint8_t* row = (const uint8_t*)a.q + ((int64_t)seq * a.q_seq + (int64_t)qh * a.q_head + 16 * g) * EB;
 #pragma unroll
   for (int j = 0; j < D / 64; ++j)
 #pragma unroll
     for (int i = 0; i < DW; i += 4) {
-      const u32x4 x = *(const u32x4*)(row + 64 * j * Sh::EB + 4 * i);
-      qr[DW * j + i + 0] = x[0];
-      qr[DW * j + i + 1] = x[1];
-      qr[DW * j + i + 2] = x[2];
-      qr[DW * j + i + 3] = x[3];
+      const u32x4 x = head_ok ? *(const u32x4*)(row + 64 * j * EB + 4 * i) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = DW * j + i + e;
+        if constexpr (QF) {
+          if (at >= Sh::KDW) q.rest[at - Sh::KDW] = x[e];
+          else q.x[at] = x[e];
+        } else {
+          q.x[at] = x[e];
+        }
+      }
     }
 }
 
-template <int DT, int D, bool Q8>
+template <int DT, int D, bool Q8, bool QF>
 __device__ __forceinline__ void load_query_for(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
-                                               uint32_t (&qr)[TileShape<DT, D>::KDW]) {
-  if constexpr (Q8) load_query_codes<DT, D>(a, seq, qh, head_ok, g, qr);
-  else load_query<DT, D>(a, seq, qh, head_ok, g, qr);
+                                               QueryRegs<DT, D, QF>& q) {
+  static_assert(Q8 || !QF, "16-bit caches take queries of their dtype");
+  if constexpr (Q8) load_query_codes<DT, D>(a, seq, qh, head_ok, g, q);
+  else load_query<DT, D>(a, seq, qh, head_ok, g, q.x);
 }
 
 // Writes the workgroup's merged (normalised) result for heads head0..head0+nh.

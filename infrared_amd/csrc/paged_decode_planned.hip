@@ -491,7 +491,7 @@ __device__ __forceinline__ void slot_read(const float* row, int g, f32x4 (&acc)[
 //
 // Q8: the tiles are codes; a run's lanes also fetch the scales of their tiles, whose
 // block the tile's pool offset gives (the layer is dense), ahead of the tiles' own loads.
-template <int DT, int D, int NW, int DEPTH, bool PAIRS, bool Q8 = false>
+template <int DT, int D, int NW, int DEPTH, bool PAIRS, bool Q8 = false, bool QF = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 && NW == 4 ? 1 : 2)))
 void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32_t o_pair, uint32_t o_whdr,
                                  uint32_t o_first, int B, DecodeArgs a, PlanLayout ly) {
@@ -583,7 +583,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     return x;
   };
   auto paired = [&](int b) { return PAIRS && s_pair[b] > 0; };
-  auto q_of = [&](int u, uint32_t (&dst)[Sh::KDW]) {
+  auto q_of = [&](int u, QueryRegs<DT, D, QF>& dst) {
     const int b = fdiv(u, n_ups);
     const int j = u - b * n_ups;
     const int hg = a.n_hg == 1 ? 0 : j - fdiv(j, a.n_hg) * a.n_hg;
@@ -596,9 +596,12 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     const int hl = hg * 16 + c;
     load_query_for<DT, D, Q8>(a, b, kvh * a.n_rep + hl, hl < a.n_rep, g, dst);
   };
-  uint32_t qr[Sh::KDW], qn[Sh::KDW];
+  QueryRegs<DT, D, QF> qr, qn;
   int q_lbl = -1, qn_lbl = -1;
-  if (cnt_w > 0) {
+  if (QF) {  // (split when it is needed, not as soon as it is here)
+    if (cnt_w > 0) q_of(fl, qn);
+    qn_lbl = fl;
+  } else if (cnt_w > 0) {
     q_of(fl, qr);
     q_lbl = fl;
     if (fl < ll) {
@@ -711,12 +714,9 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
         if (cur >= 0) wave_finish(cur, false);
         cur = lb[r];
         if (q_lbl != cur) {
-          if (qn_lbl == cur) {
-#pragma unroll
-            for (int k = 0; k < Sh::KDW; ++k) qr[k] = qn[k];
-          } else {
-            q_of(cur, qr);
-          }
+          if (qn_lbl == cur) qr = qn;
+          else q_of(cur, qr);
+          qr.split();
           q_lbl = cur;
         }
         if (cur + 1 <= ll && qn_lbl != cur + 1) {
@@ -727,9 +727,9 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       if constexpr (Q8) {
         const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
         const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
-        compute_codes<DT, D>(ring[r], qr, mk[r], a.scale_log2 * ks, vs, kstage[w], lane, st, con[r]);
+        compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2 * ks, vs, kstage[w], lane, st, con[r]);
       } else {
-        compute_tile<DT, D>(ring[r], qr, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
+        compute_tile<DT, D>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
       }
     };
 #pragma unroll
@@ -944,16 +944,16 @@ __global__ __launch_bounds__(kMergeThreads) void paged_decode_planned_merge(cons
              L > 0.f ? 1.f / L : 0.f);
 }
 
-template <int DT, int D>
+template <int DT, int D, bool QF>
 void launch_planned_q8(const DecodeArgs& a, const uint8_t* plan, const PlanLayout& ly, int grid, bool pairs,
                        hipStream_t s) {
   const uint32_t o_sp = (uint32_t)ly.seq_pre, o_pr = (uint32_t)ly.pair, o_wh = (uint32_t)ly.whdr,
                  o_fi = (uint32_t)ly.first;
   if (pairs)
-    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, true, true>), dim3(grid),
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, true, true, QF>), dim3(grid),
                        dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
   else
-    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, false, true>), dim3(grid),
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, false, true, QF>), dim3(grid),
                        dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
   if (a.merge_later)
     hipLaunchKernelGGL((paged_decode_planned_merge<DT, D>), dim3(a.num_seqs * a.n_ups, std::min(16, 2 * a.n_rep)),
@@ -1063,7 +1063,8 @@ namespace {
 
 // ir_paged_decode_planned, and with `scales` ir_paged_decode_planned_q8 (a dense
 // layer of codes).
-int planned_call(const char* name, const float* scales, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+int planned_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_seq_stride,
+                 int64_t q_head_stride,
                  const void* k_cache, const void* v_cache, int64_t cache_slot_stride, void* out,
                  int64_t out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
                  int head_dim, int max_blocks_per_seq, int block_size, float scale, int dtype, int flags,
@@ -1071,6 +1072,9 @@ int planned_call(const char* name, const float* scales, const void* q, int64_t q
                  int32_t* err_flags, ir_stream_t stream) {
   const int eb = dtype_bytes(dtype);
   IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
+  IR_REQUIRE(q_dtype == dtype || (scales && q_dtype == IR_DTYPE_F32), "%s: unknown q_dtype %d for dtype %d", name,
+             q_dtype, dtype);
+  const int q_eb = dtype_bytes(q_dtype);
   IR_REQUIRE((flags & ~IR_PLAN_SHARE_GROUPS) == 0, "%s: unknown flags 0x%x", name, flags);
   if (head_dim != 64 && head_dim != 128)
     return fail(IR_EUNSUPPORTED, "%s: head_dim %d not supported (64, 128)", name, head_dim);
@@ -1080,7 +1084,8 @@ int planned_call(const char* name, const float* scales, const void* q, int64_t q
   IR_REQUIRE(q && k_cache && v_cache && out, "%s: null pointer", name);
   IR_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
              "%s: q, caches and out must be 16-byte aligned", name);
-  IR_REQUIRE((q_seq_stride * eb) % 16 == 0 && (q_head_stride * eb) % 16 == 0 && (cache_slot_stride * eb) % 16 == 0 &&
+  IR_REQUIRE((q_seq_stride * q_eb) % 16 == 0 && (q_head_stride * q_eb) % 16 == 0 &&
+                 (cache_slot_stride * eb) % 16 == 0 &&
                  (out_seq_stride * eb) % 16 == 0 && (out_head_stride * eb) % 16 == 0,
              "%s: strides must be multiples of 16 bytes", name);
   const int grid = device_cus();
@@ -1126,19 +1131,21 @@ int planned_call(const char* name, const float* scales, const void* q, int64_t q
   const bool pairs = (flags & IR_PLAN_SHARE_GROUPS) && pairs_fit(num_q_heads, num_kv_heads);
   if (scales) {
     IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+    const bool qf = q_dtype != dtype;
+#define IR_PLANNED_Q8(DT_, QF_)                                                   \
+  (head_dim == 128 ? launch_planned_q8<DT_, 128, QF_>(a, pl, ly, grid, pairs, s) \
+                   : launch_planned_q8<DT_, 64, QF_>(a, pl, ly, grid, pairs, s))
     switch (dtype) {
       case IR_DTYPE_BF16:
-        head_dim == 128 ? launch_planned_q8<IR_DTYPE_BF16, 128>(a, pl, ly, grid, pairs, s)
-                        : launch_planned_q8<IR_DTYPE_BF16, 64>(a, pl, ly, grid, pairs, s);
+        qf ? IR_PLANNED_Q8(IR_DTYPE_BF16, true) : IR_PLANNED_Q8(IR_DTYPE_BF16, false);
         break;
       case IR_DTYPE_F16:
-        head_dim == 128 ? launch_planned_q8<IR_DTYPE_F16, 128>(a, pl, ly, grid, pairs, s)
-                        : launch_planned_q8<IR_DTYPE_F16, 64>(a, pl, ly, grid, pairs, s);
+        qf ? IR_PLANNED_Q8(IR_DTYPE_F16, true) : IR_PLANNED_Q8(IR_DTYPE_F16, false);
         break;
       default:
-        head_dim == 128 ? launch_planned_q8<IR_DTYPE_F32, 128>(a, pl, ly, grid, pairs, s)
-                        : launch_planned_q8<IR_DTYPE_F32, 64>(a, pl, ly, grid, pairs, s);
+        IR_PLANNED_Q8(IR_DTYPE_F32, false);
     }
+#undef IR_PLANNED_Q8
     return check_launch(name);
   }
   switch (dtype) {
@@ -1166,9 +1173,9 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
                                        int block_size, float scale, int dtype, int flags, const void* plan,
                                        int32_t* counters, int64_t num_counters, void* workspace,
                                        int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
-  return planned_call("ir_paged_decode_planned", nullptr, q, q_seq_stride, q_head_stride, k_cache, v_cache,
-                      cache_slot_stride, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
-                      max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
+  return planned_call("ir_paged_decode_planned", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                      cache_slot_stride, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads,
+                      head_dim, max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
                       workspace_bytes, err_flags, stream);
 }
 
@@ -1176,12 +1183,12 @@ extern "C" int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, i
                                           k_cache, const void* v_cache, const float* scales, void* out, int64_t
                                           out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int
                                           num_kv_heads, int head_dim, int max_blocks_per_seq, int block_size, float
-                                          scale, int dtype, int flags, const void* plan, int32_t* counters, int64_t
-                                          num_counters, void* workspace, int64_t workspace_bytes, int32_t* err_flags,
+                                          scale, int dtype, int q_dtype, int flags, const void* plan, int32_t*
+                                          counters, int64_t num_counters, void* workspace, int64_t workspace_bytes, int32_t* err_flags,
                                           ir_stream_t stream) {
   IR_REQUIRE(scales, "ir_paged_decode_planned_q8: null pointer");
-  return planned_call("ir_paged_decode_planned_q8", scales, q, q_seq_stride, q_head_stride, k_cache, v_cache, head_dim, out,
-                      out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
+  return planned_call("ir_paged_decode_planned_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                      head_dim, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
                       max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
                       workspace_bytes, err_flags, stream);
 }

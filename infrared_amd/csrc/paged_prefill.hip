@@ -125,6 +125,7 @@ struct PrefillArgs {
   int64_t n_work;  // attending workgroups (the grid less the writers)
   // 8-bit caches: (K, V) scales [kv head][block] (null: the caches are of the dtype)
   const f32x2* scales;
+  int q_f32;  // 8-bit caches: q is fp32, whatever the dtype
 };
 
 // 16-byte pieces a writer lane moves, all loads in flight before any store.
@@ -190,22 +191,21 @@ struct PShape {
 constexpr int kLockstep = 0, kRing2 = 2;
 
 // Q8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
-// key's K and of its V with the key's scales, and turns them into the dtype's
-// elements, exactly, where it stores them to LDS; from there on the walk is the
-// same.
-template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false>
+// key's K and of its V with the key's scales. V turns into the dtype's elements,
+// exactly, where it is stored to LDS; K stays codes, and its products with the queries
+// are code products, the queries being QP pieces of codes each. From the scores on the
+// walk is the same.
+template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false, int QP = 2>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
   typedef PShape<D, NW, CTW> S;
   constexpr int EB = 2;
   constexpr int CT = S::CT, BN = S::BN, NT = S::NT;
   constexpr int RING = SCHED == kRing2 ? 2 : 3;
-  // QC: the keys stay codes and the queries become two pieces of codes each (bf16)
-  constexpr bool QC = Q8 && DT == IR_DTYPE_BF16;
   constexpr int CROW = D + 16;  // bytes per key row of codes in LDS (16 rows apart without bank conflicts)
-  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][QC ? BN * CROW / 2 : BN * S::KROW];
+  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][Q8 ? BN * CROW / 2 : BN * S::KROW];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[RING][BN * S::KROW];
-  __shared__ int ke_lds[QC ? RING : 1][4];  // QC: exponents of the scales of a tile's 16-key runs
+  __shared__ int ke_lds[Q8 ? RING : 1][4];  // Q8: exponents of the scales of a tile's 16-key runs
   __shared__ int32_t bt_lds[kBtCache];
 
   const int tid = threadIdx.x;
@@ -289,61 +289,93 @@ void paged_prefill_kernel(PrefillArgs a) {
   // and scales it once its first key tile is staged, so Q's round trip
   // overlaps the block ids' and the first tile's instead of preceding them.
   constexpr bool EARLY = NW == 8 && CT == 1 && SCHED == kRing2;
-  // QC: a query times scale * log2 e, q = hi 2^e + lo 2^(e - 4) with e4m3 codes hi and lo
-  // (the first four and the last four bits of its significand: off by at most 2^-9 of
-  // q's power of two, half of what rounding to bf16 would be). At head_dim 64 one product
-  // of 128 k-slots holds both pieces, the codes of K twice; at 128 two follow each other.
+  // Q8: a query times scale * log2 e is the sum of QP pieces of e4m3 codes, piece p times
+  // 2^(e - 4 p): each takes four bits of what the ones before leave. Two are off by at most
+  // 2^-9 of an element's power of two, half of what rounding to bf16 would be, three by
+  // 2^-14, which fp16 queries and fp32 ones (normed rows as they left the rotation) take:
+  // an error of a query is one of all its scores (four 256-token chunks, 32 / 4 heads of
+  // 128: 39.6 us in two pieces from bf16, 42.8 in three from fp32; the outputs' error in a
+  // step that norms its queries 0.0033 -> 0.0022 of their size, 0.0017 being the rounding
+  // of the outputs alone). At head_dim 64 one product of 128
+  // k-slots holds two pieces, the codes of K twice; at 128 it holds one.
+  constexpr int NP = D == 128 ? QP : (QP + 1) / 2;  // products of a score
   u32x4 qreg[CT][S::KS];
-  i32x8 qc[CT][D / 64];
-  int qe[CT][D / 64];
-  auto split_query = [&](int ct, const u32x4 (&x)[S::KS]) {
-    float v[S::KS * 8], most = 0.f;
+  i32x8 qc[CT][NP];
+  int qe[CT][NP];
+  auto split_query = [&](int ct, float (&v)[S::KS * 8]) {
+    float most = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < S::KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[8 * ks + 2 * i] = Elem<DT>::lo(x[ks][i]) * a.scale_log2;
-        v[8 * ks + 2 * i + 1] = Elem<DT>::hi(x[ks][i]) * a.scale_log2;
-        most = fmaxf(most, fmaxf(fabsf(v[8 * ks + 2 * i]), fabsf(v[8 * ks + 2 * i + 1])));
-      }
+    for (int i = 0; i < S::KS * 8; ++i) {
+      v[i] *= a.scale_log2;
+      most = fmaxf(most, fabsf(v[i]));
+    }
     most = wave_max_groups_swap(most);
     const int e = scale_exponent<IR_DTYPE_BF16>(most);
-    const float s_hi = pow2(e), s_lo = pow2(e - 4);
     // (an infinite query becomes NaN, not a large number; NaN does by itself)
     const int bad = __float_as_uint(most) >= 0x7f800000u ? 0x7f7f7f7f : 0;
     typedef short i16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int i = 0; i < S::KS * 2; ++i) {  // four elements
-      i16x2 h = {0, 0}, l = {0, 0};
-      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[4 * i], v[4 * i + 1], s_hi, false);
-      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[4 * i + 2], v[4 * i + 3], s_hi, true);
-      const uint32_t hw = __builtin_bit_cast(uint32_t, h);
-      const f32x2 r0 = decode2_f32<false>(hw, s_hi), r1 = decode2_f32<true>(hw, s_hi);
-      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, v[4 * i] - r0[0], v[4 * i + 1] - r0[1], s_lo, false);
-      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, v[4 * i + 2] - r1[0], v[4 * i + 3] - r1[1], s_lo, true);
-      const int lw = __builtin_bit_cast(int, l);
-      qc[ct][0][i] = (int)hw | bad;
-      if constexpr (D == 128) qc[ct][1][i] = lw;
-      else qc[ct][0][4 + i] = lw;
+      float x[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+#pragma unroll
+      for (int p = 0; p < (D == 128 ? QP : 2 * NP); ++p) {
+        i16x2 h = {0, 0};
+        if (p < QP) {
+          const float s = pow2(e - 4 * p);
+          h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[0], x[1], s, false);
+          h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[2], x[3], s, true);
+          const uint32_t hw = __builtin_bit_cast(uint32_t, h);
+          const f32x2 r0 = decode2_f32<false>(hw, s), r1 = decode2_f32<true>(hw, s);
+          x[0] -= r0[0];
+          x[1] -= r0[1];
+          x[2] -= r1[0];
+          x[3] -= r1[1];
+        }
+        const int word = __builtin_bit_cast(int, h) | (p == 0 ? bad : 0);
+        if constexpr (D == 128) qc[ct][p][i] = word;
+        else qc[ct][p / 2][4 * (p & 1) + i] = word;
+      }
     }
-    if constexpr (D == 128) {
-      qe[ct][0] = e + 127;
-      qe[ct][1] = e - 4 + 127;
-    } else {
-      qe[ct][0] = (g < 2 ? e : e - 4) + 127;
-    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j) qe[ct][j] = 127 + (D == 128 ? e - 4 * j : e - 8 * j - (g < 2 ? 0 : 4));
+  };
+  auto split_raw = [&](int ct) {
+    float v[S::KS * 8];
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[8 * ks + 2 * i] = Elem<DT>::lo(qreg[ct][ks][i]);
+        v[8 * ks + 2 * i + 1] = Elem<DT>::hi(qreg[ct][ks][i]);
+      }
+    split_query(ct, v);
   };
   // the lane's elements of a query row, ks-th eight: with codes, the k-slots of lane
   // group g are the 16-code chunks g and g + 4 of the row
-  auto q_at = [&](int ks) { return QC ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : ks * 32 + 8 * g; };
+  auto q_at = [&](int ks) { return Q8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : ks * 32 + 8 * g; };
+  const bool wide_q = QP == 3 && a.q_f32;  // (uniform)
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const Col col = column(ct);
-    const uint16_t* qrow = (const uint16_t*)a.q + (int64_t)(q_lo + (col.ok ? col.tok : 0)) * a.q_tok +
-                           (int64_t)(col.ok ? col.head : 0) * a.q_head;
+    const int64_t q_off =
+        (int64_t)(q_lo + (col.ok ? col.tok : 0)) * a.q_tok + (int64_t)(col.ok ? col.head : 0) * a.q_head;
+    if constexpr (QP == 3) {
+      if (wide_q) {
+        float v[S::KS * 8];
+#pragma unroll
+        for (int i = 0; i < S::KS * 2; ++i) {
+          const f32x4 x = *(const f32x4*)((const float*)a.q + q_off + q_at(i >> 1) + 4 * (i & 1));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * i + j] = col.ok ? x[j] : 0.f;
+        }
+        split_query(ct, v);
+        continue;
+      }
+    }
+    const uint16_t* qrow = (const uint16_t*)a.q + q_off;
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
-      if constexpr (EARLY || QC) {
+      if constexpr (EARLY || Q8) {
         const u32x4 x = *(const u32x4*)(qrow + q_at(ks));  // (a valid row when !col.ok)
         qreg[ct][ks] = col.ok ? x : u32x4{0u, 0u, 0u, 0u};
       } else {
@@ -353,7 +385,7 @@ void paged_prefill_kernel(PrefillArgs a) {
           qreg[ct][ks][e] = Elem<DT>::pack2(Elem<DT>::lo(x[e]) * a.scale_log2, Elem<DT>::hi(x[e]) * a.scale_log2);
       }
     }
-    if constexpr (QC && !EARLY) split_query(ct, qreg[ct]);
+    if constexpr (Q8 && !EARLY) split_raw(ct);
   }
 
   // ---- block-id cache: ids [bt_base, bt_base + kBtCache) of this sequence
@@ -470,26 +502,17 @@ void paged_prefill_kernel(PrefillArgs a) {
         const int key = q / (D / PE), part = q % (D / PE);
         const u32x4 k4 = zero_unless(kr[i], ku[i]), v4 = zero_unless(vr[i], ku[i]);
         const f32x2 s2 = Q8 && ku[i] ? sc[i] : f32x2{1.f, 1.f};
-        uint16_t* kp = &ks_lds[buf][key * S::KROW + part * PE];
         uint16_t* vp = &vs_lds[buf][key * S::KROW + part * PE];
         if constexpr (Q8) {
-          auto wide = [](uint16_t* to, u32x4 x, float scale) {
+          *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
+          if (part == 0 && (key & 15) == 0) ke_lds[buf][key >> 4] = (int)(__float_as_uint(s2[0]) >> 23);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              *(u32x4*)(to + 8 * h) =
-                  u32x4{decode2<DT, false>(x[2 * h], scale), decode2<DT, true>(x[2 * h], scale),
-                        decode2<DT, false>(x[2 * h + 1], scale), decode2<DT, true>(x[2 * h + 1], scale)};
-          };
-          if constexpr (QC) {
-            *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
-            if (part == 0 && (key & 15) == 0)
-              ke_lds[buf][key >> 4] = (int)(__float_as_uint(s2[0]) >> 23);
-          } else {
-            wide(kp, k4, s2[0]);
-          }
-          wide(vp, v4, s2[1]);
+          for (int h = 0; h < 2; ++h)
+            *(u32x4*)(vp + 8 * h) =
+                u32x4{decode2<DT, false>(v4[2 * h], s2[1]), decode2<DT, true>(v4[2 * h], s2[1]),
+                      decode2<DT, false>(v4[2 * h + 1], s2[1]), decode2<DT, true>(v4[2 * h + 1], s2[1])};
         } else {
-          *(u32x4*)kp = k4;
+          *(u32x4*)&ks_lds[buf][key * S::KROW + part * PE] = k4;
           *(u32x4*)vp = v4;
         }
       }
@@ -537,7 +560,7 @@ void paged_prefill_kernel(PrefillArgs a) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) x[ct][kt] = mfma_k32<DT>(ka, qreg[ct][ks], x[ct][kt]);
   };
-  // QC: all of key tile kt's scores from the codes staged in buffer buf.
+  // Q8: all of key tile kt's scores from the codes staged in buffer buf.
   auto qk_codes = [&](int buf, int kt, f32x4 (&x)[CT][4]) {
     const uint8_t* row = (const uint8_t*)ks_lds[buf] + (kt * 16 + c) * CROW + 16 * g;
     const u32x4 k0 = *(const u32x4*)row;
@@ -547,7 +570,7 @@ void paged_prefill_kernel(PrefillArgs a) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) x[ct][kt] = mfma_codes_k128(ka, ke, qc[ct][i], qe[ct][i], x[ct][kt]);
+      for (int i = 0; i < NP; ++i) x[ct][kt] = mfma_codes_k128(ka, ke, qc[ct][i], qe[ct][i], x[ct][kt]);
   };
   auto zero_s = [](f32x4 (&x)[CT][4]) {
 #pragma unroll
@@ -705,8 +728,8 @@ void paged_prefill_kernel(PrefillArgs a) {
       __syncthreads();
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        if constexpr (QC) {
-          split_query(ct, qreg[ct]);
+        if constexpr (Q8) {
+          if (!wide_q) split_raw(ct);
           continue;
         }
 #pragma unroll
@@ -729,7 +752,7 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
-        if constexpr (QC) {
+        if constexpr (Q8) {
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
         } else {
@@ -766,7 +789,7 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
-        if constexpr (QC) {
+        if constexpr (Q8) {
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
         } else {
@@ -1811,7 +1834,7 @@ int launch_prefill(PrefillArgs a, int sched, hipStream_t s) {
 
 // An 8-bit cache: launch_prefill's shapes by the same rules (2-deep rings), the
 // step's rows already written.
-template <int DT, int D>
+template <int DT, int D, int QP>
 int launch_prefill_q8(const PrefillArgs& a, hipStream_t s) {
   const int64_t grid = a.items ? a.n_items_grid : (int64_t)a.n_qblocks * a.num_kv_heads * a.num_seqs;
   if (grid <= 0) return ok();
@@ -1824,9 +1847,9 @@ int launch_prefill_q8(const PrefillArgs& a, hipStream_t s) {
   do {                                                                                                            \
     const dim3 g((unsigned)grid), block(NW_ * 64);                                                                \
     if (fast)                                                                                                     \
-      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, true, NW_, CT_, kRing2, false, true>), g, block, 0, s, a);  \
+      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, true, NW_, CT_, kRing2, false, true, QP>), g, block, 0, s, a);  \
     else                                                                                                          \
-      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, false, NW_, CT_, kRing2, false, true>), g, block, 0, s, a); \
+      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, false, NW_, CT_, kRing2, false, true, QP>), g, block, 0, s, a); \
   } while (0)
   if (a.nw == 4 && !a.items && grid <= device_cus()) IR_PREFILL_Q8(8, 1);
   else if (a.nw == 4) IR_PREFILL_Q8(4, 2);
@@ -1856,8 +1879,9 @@ extern "C" int ir_paged_prefill_plan_xcds(void) { return plan_xcds(); }
 namespace {
 
 // ir_paged_prefill, and with `scales` ir_paged_prefill_q8 (a dense layer of codes).
-int prefill_call(const char* name, const float* scales, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
-                 const void* k_cache, const void* v_cache, int64_t cache_slot_stride, int64_t cache_head_stride,
+int prefill_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_tok_stride,
+                 int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
+                 int64_t cache_head_stride,
                  int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride, int
                  max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q,
                  int max_q_len, void* out, int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads, int
@@ -1869,6 +1893,9 @@ int prefill_call(const char* name, const float* scales, const void* q, int64_t q
              "%s: unknown dtype %d", name, dtype);
   const bool f32 = dtype == IR_DTYPE_F32;
   const int eb = f32 ? 4 : 2;
+  IR_REQUIRE(q_dtype == dtype || (scales && q_dtype == IR_DTYPE_F32), "%s: unknown q_dtype %d for dtype %d", name,
+             q_dtype, dtype);
+  const int q_eb = q_dtype == IR_DTYPE_F32 ? 4 : 2;
   IR_REQUIRE(num_seqs >= 0 && total_q >= 0 && max_q_len >= 0 && num_q_heads > 0 && num_kv_heads > 0 &&
                  block_size > 0 && max_blocks_per_seq >= 0 && num_blocks >= 0,
              "%s: bad sizes", name);
@@ -1888,9 +1915,9 @@ int prefill_call(const char* name, const float* scales, const void* q, int64_t q
   // each output store is 4 elements: 8 bytes in 16-bit dtypes, 16 in fp32
   IR_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && ((uintptr_t)out % (4 * eb)) == 0,
              "%s: q and caches must be 16-byte aligned, out %d-byte aligned", name, 4 * eb);
-  IR_REQUIRE((q_tok_stride * eb) % 16 == 0 && (q_head_stride * eb) % 16 == 0 && (cache_slot_stride * eb) % 16 == 0 &&
-                 (cache_head_stride * eb) % 16 == 0 && (out_tok_stride * eb) % (4 * eb) == 0 &&
-                 (out_head_stride * eb) % (4 * eb) == 0,
+  IR_REQUIRE((q_tok_stride * q_eb) % 16 == 0 && (q_head_stride * q_eb) % 16 == 0 &&
+                 (cache_slot_stride * eb) % 16 == 0 && (cache_head_stride * eb) % 16 == 0 &&
+                 (out_tok_stride * eb) % (4 * eb) == 0 && (out_head_stride * eb) % (4 * eb) == 0,
              "%s: q/cache strides must be multiples of 16 bytes, out strides of %d bytes", name, 4 * eb);
   if (scales) {
     IR_REQUIRE(block_size % 16 == 0, "%s: block size %d must be a multiple of 16", name, block_size);
@@ -1957,6 +1984,7 @@ int prefill_call(const char* name, const float* scales, const void* q, int64_t q
     a.src_row0 = src_row0;
   }
   a.scales = (const f32x2*)scales;
+  a.q_f32 = q_dtype == IR_DTYPE_F32;
   a.out = out;
   a.o_tok = out_tok_stride;
   a.o_head = out_head_stride;
@@ -1966,9 +1994,14 @@ int prefill_call(const char* name, const float* scales, const void* q, int64_t q
   a.err = err_flags;
   hipStream_t s = (hipStream_t)stream;
   if (scales && !f32) {
-    if (dtype == IR_DTYPE_BF16)
-      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128>(a, s) : launch_prefill_q8<IR_DTYPE_BF16, 64>(a, s);
-    return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_F16, 128>(a, s) : launch_prefill_q8<IR_DTYPE_F16, 64>(a, s);
+    if (dtype == IR_DTYPE_F16)
+      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_F16, 128, 3>(a, s)
+                             : launch_prefill_q8<IR_DTYPE_F16, 64, 3>(a, s);
+    if (a.q_f32)
+      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128, 3>(a, s)
+                             : launch_prefill_q8<IR_DTYPE_BF16, 64, 3>(a, s);
+    return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128, 2>(a, s)
+                           : launch_prefill_q8<IR_DTYPE_BF16, 64, 2>(a, s);
   }
   if (f32) return head_dim == 128 ? launch_prefill_f32<128>(a, s) : launch_prefill_f32<64>(a, s);
   if (dtype == IR_DTYPE_BF16)
@@ -1990,8 +2023,8 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
                                 int64_t k_new_tok_stride, int64_t k_new_head_stride, const void* v_new,
                                 int64_t v_new_tok_stride, int64_t v_new_head_stride, const int64_t* write_slots,
                                 int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
-  return prefill_call("ir_paged_prefill", nullptr, q, q_tok_stride, q_head_stride, k_cache, v_cache, cache_slot_stride,
-                      cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
+  return prefill_call("ir_paged_prefill", nullptr, dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
+                      cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
                       cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride, out_head_stride,
                       num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, k_new, k_new_tok_stride,
                       k_new_head_stride, v_new, v_new_tok_stride, v_new_head_stride, write_slots, n_write, src_row0,
@@ -2003,12 +2036,12 @@ extern "C" int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t 
                                    int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq, const int32_t*
                                    cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q, int max_q_len,
                                    void* out, int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads, int
-                                   num_kv_heads, int head_dim, float scale, int dtype, void* plan, int64_t plan_bytes,
-                                   int32_t* err_flags, ir_stream_t stream) {
+                                   num_kv_heads, int head_dim, float scale, int dtype, int q_dtype, void* plan,
+                                   int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream) {
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_prefill_q8: null pointer");
-  return prefill_call("ir_paged_prefill_q8", scales, q, q_tok_stride, q_head_stride, k_cache, v_cache, head_dim,
-                      num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
+  return prefill_call("ir_paged_prefill_q8", scales, q_dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
+                      head_dim, num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
                       max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
                       out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, nullptr, 0,
                       0, nullptr, 0, 0, nullptr, 0, 0, err_flags, stream);

@@ -91,7 +91,7 @@ int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, in
                   int64_t qo_tok, int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v,
                   int64_t v_tok, int64_t v_head, const void* q_weight, const void* k_weight, float eps,
                   const float* cos, const float* sin, int64_t cs_tok, const int64_t* slots, int64_t n_tokens,
-                  int num_q_heads, int num_kv_heads, int eb) {
+                  int num_q_heads, int num_kv_heads, int eb, int qo_eb) {
   IR_REQUIRE(k && v && cos && sin && slots && (num_q_heads == 0 || (q && q_out)), "%s: null pointer", name);
   IR_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cos) && aligned16(sin) &&
                  (num_q_heads == 0 || (aligned16(q) && aligned16(q_out))),
@@ -100,14 +100,17 @@ int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, in
   IR_REQUIRE(aligned16(q_weight) && aligned16(k_weight), "%s: norm weights must be 16-byte aligned", name);
   IR_REQUIRE(!q_weight || eps >= 0.f, "%s: eps must not be negative", name);
   IR_REQUIRE(cs_tok % 4 == 0, "%s: cos/sin row stride must be a multiple of 4 elements", name);
-  for (int64_t st : {q_tok, q_head, qo_tok, qo_head, k_tok, k_head, v_tok, v_head})
+  for (int64_t st : {qo_tok, qo_head})
+    IR_REQUIRE((st * qo_eb) % 16 == 0, "%s: strides must be multiples of 16 bytes", name);
+  for (int64_t st : {q_tok, q_head, k_tok, k_head, v_tok, v_head})
     IR_REQUIRE((st * eb) % 16 == 0, "%s: strides must be multiples of 16 bytes", name);
   r.q = (const uint8_t*)q;
   r.q_tok = q_tok * eb;
   r.q_head = q_head * eb;
   r.qo = (uint8_t*)q_out;
-  r.qo_tok = qo_tok * eb;
-  r.qo_head = qo_head * eb;
+  r.qo_wide = qo_eb != eb;
+  r.qo_tok = qo_tok * qo_eb;
+  r.qo_head = qo_head * qo_eb;
   r.k = (const uint8_t*)k;
   r.k_tok = k_tok * eb;
   r.k_head = k_head * eb;
@@ -149,7 +152,7 @@ extern "C" int ir_qk_norm_rope_kv_scatter(
   NormRopeArgs a;
   const int rc = fill_row_args(name, a.r, q, q_tok_stride, q_head_stride, q_out, qo_tok_stride, qo_head_stride, k,
                                k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride, q_weight, k_weight, eps,
-                               cos, sin, cs_tok_stride, slot_mapping, n_tokens, num_q_heads, num_kv_heads, eb);
+                               cos, sin, cs_tok_stride, slot_mapping, n_tokens, num_q_heads, num_kv_heads, eb, eb);
   if (rc != IR_OK) return rc;
   IR_REQUIRE(q_weight && k_cache && v_cache, "%s: null pointer", name);
   IR_REQUIRE(aligned16(k_cache) && aligned16(v_cache) && (cache_slot_stride * eb) % 16 == 0 &&

@@ -219,7 +219,8 @@ def paged_decode(
     zero-filled before first use; every call leaves them at zero) are allocated
     when not given and the longest possible context needs more than one
     partition. ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn)
-    with these scales, ``q`` of the pool's dtype.
+    with these scales; ``q`` is of the pool's dtype, or fp32 (queries that were not
+    rounded to it) with ``out`` of it.
     """
     if kv_scales is not None:
         return seam().paged_decode_q8(q, k_cache, v_cache, kv_scales, block_tables, context_lens, block_size, scale,
@@ -348,8 +349,8 @@ def paged_decode_planned(
 ) -> torch.Tensor:
     """:func:`paged_decode` over a plan: ``q`` ``[B, H_q, D]`` -> ``[B, H_q, D]``.
     ``workspace`` (uint8 scratch) and ``counters`` (int32 zeros, left at zero)
-    are allocated when not given. ``kv_scales``: as there, the plan built for the
-    float8_e4m3fn layer."""
+    are allocated when not given. ``kv_scales``, and ``q``'s dtype with them: as there,
+    the plan built for the float8_e4m3fn layer."""
     if kv_scales is not None:
         return seam().paged_decode_planned_q8(q, k_cache, v_cache, kv_scales, *plan.native(), scale, out, workspace,
                                               err_flags, counters, stream_of(q))
@@ -444,7 +445,9 @@ def rope_kv_scatter_q8(
     """:func:`rope_kv_scatter`, or given ``q_norm`` and ``k_norm``
     :func:`qk_norm_rope_kv_scatter`, into one layer of an 8-bit pool: the rotated keys
     and the values are quantised as :func:`kv_scatter_q8` does, in the same launch
-    (normed keys from fp32, without a rounding to the dtype before)."""
+    (normed keys from fp32, without a rounding to the dtype before). A ``q_out`` of fp32
+    takes the queries as they leave the rotation, for an attention that is given them
+    so."""
     return seam().norm_rope_kv_scatter(q, k, v, q_norm, k_norm, eps, cos, sin, k_cache, v_cache, kv_scales,
                                        int(block_size), slots, q_out, err_flags, stream_of(q))
 
@@ -605,8 +608,9 @@ def paged_prefill(
     read from those rows (``ERR_WRITE_SLOT`` is flagged where a token's write
     slot is not its block-table slot).
     ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn) with these
-    scales, ``q`` of the pool's dtype; its new rows are written before
-    (:func:`kv_scatter_q8`), so there is no ``new_kv``.
+    scales; ``q`` is of the pool's dtype, or fp32 (queries that were not rounded to it)
+    with ``out`` of it. Its new rows are written before (:func:`kv_scatter_q8`), so
+    there is no ``new_kv``.
     """
     stream = stream_of(q)
     if plan is not None:
@@ -614,7 +618,8 @@ def paged_prefill(
         if (plan.num_seqs, plan.max_q_len, plan.num_q_heads, plan.num_kv_heads, plan.head_dim) != (
                 block_tables.shape[0], int(max_q_len), hq, k_cache.shape[1], d):
             raise RuntimeError("paged_prefill: the plan was built for other shapes")
-        if plan.f32 != (q.dtype == torch.float32):
+        dtype = q.dtype if kv_scales is None or out is None else out.dtype
+        if plan.f32 != (dtype == torch.float32):
             raise RuntimeError("paged_prefill: the plan was built for "
                                + ("fp32" if plan.f32 else "16-bit") + f" calls, q is {q.dtype}")
     if kv_scales is not None:

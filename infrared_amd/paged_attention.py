@@ -115,7 +115,8 @@ def rope_paged_attention(
     ``q_norm``, ``k_norm`` (``[D]``, of the activations' dtype, both or neither):
     queries and keys are normed per head before the rotation, ``x * rsqrt(mean(x^2) +
     eps) * weight``, in the same kernel, which then stays in fp32 and rounds once
-    (``ir_qk_norm_rope_kv_scatter``; ``ir_rope_kv_scatter_q8`` for an 8-bit pool).
+    (``ir_qk_norm_rope_kv_scatter``; ``ir_rope_kv_scatter_q8`` for an 8-bit pool, whose
+    attention takes the queries unrounded).
     """
     pool = paged.pool
     h_kv, d = k.shape[-2], k.shape[-1]
@@ -132,8 +133,11 @@ def rope_paged_attention(
     err = getattr(pool, "err_flags", None)
     if isinstance(pool, QuantPagedKVPool):
         _check_quant(pool, q, paged)
+        # normed queries stay fp32 up to the scores, as normed keys do up to their codes: a
+        # rounding of theirs would be as large an error of the outputs as all others
+        q_out = None if q_norm is None else torch.empty(b * sq, hq, d, dtype=torch.float32, device=q.device)
         q_rot = kernels.rope_kv_scatter_q8(*rows, *angles, *caches, pool.kv_scales[layer_idx], paged.write_slots,
-                                           pool.block_size, q_norm, k_norm, eps, err_flags=err)
+                                           pool.block_size, q_norm, k_norm, eps, q_out, err_flags=err)
     elif q_norm is not None:
         q_rot = kernels.qk_norm_rope_kv_scatter(*rows, q_norm, k_norm, eps, *angles, *caches, paged.write_slots,
                                                 err_flags=err)
@@ -165,7 +169,7 @@ def _attend(q: torch.Tensor, paged, mask: torch.Tensor | None, layer_idx: int, s
     b, sq = q.shape[:2]
     k_layer, v_layer = pool.k[layer_idx], pool.v[layer_idx]
     err = getattr(pool, "err_flags", None)
-    if isinstance(pool, QuantPagedKVPool):
+    if isinstance(pool, QuantPagedKVPool) and new_kv is not None:
         _check_quant(pool, q, paged)
 
     def write():
@@ -279,7 +283,9 @@ def _split_step(q, pool, layer_idx: int, split, scale: float, err, new_kv: tuple
     Returns ``q``'s shape."""
     b, sq, hq, d = q.shape
     qf = q.reshape(b * sq, hq, d)
-    out = torch.empty_like(qf)
+    out = _out_for(qf, pool)
+    if out is None:
+        out = torch.empty_like(qf)
     (d0, d1), (p0, p1) = split.dec_range, split.pre_range
     if new_kv is not None and p1 <= p0:
         pool.write(layer_idx, *new_kv)
@@ -320,13 +326,16 @@ def _prefill(q, pool, layer_idx: int, block_tables, cu_seqlens_q, q_start, max_q
     b, sq, hq, d = q.shape
     h_kv = pool.k.shape[-2]
     nseq = q_start.shape[0]
+    if out is None:
+        out = _out_for(q.reshape(b * sq, hq, d), pool)
+    dtype = q.dtype if out is None else out.dtype
     plan = getattr(holder, "prefill_plan", None)
-    if plan is not None and plan.f32 != (q.dtype == torch.float32):
+    if plan is not None and plan.f32 != (dtype == torch.float32):
         plan = None  # (a plan of the other kind: rebuilt below and kept)
     if plan is None and kernels.prefill_plan_pays(
-            nseq, max_q, hq, h_kv, q.device, max_keys=block_tables.shape[1] * pool.block_size, dtype=q.dtype):
+            nseq, max_q, hq, h_kv, q.device, max_keys=block_tables.shape[1] * pool.block_size, dtype=dtype):
         plan = kernels.prefill_plan(
-            cu_seqlens_q, q_start, block_tables, b * sq, max_q, pool.block_size, hq, h_kv, d, dtype=q.dtype
+            cu_seqlens_q, q_start, block_tables, b * sq, max_q, pool.block_size, hq, h_kv, d, dtype=dtype
         )
         try:
             holder.prefill_plan = plan
@@ -345,6 +354,8 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
     the device (cached on ``holder.decode_plan`` for the step's other layers),
     else the fixed split-KV partitions. Returns ``[B, 1, H_q, D]``."""
     b, _, hq, d = q.shape
+    if out is None:
+        out = _out_for(q[:, 0], pool)
     h_kv = pool.k.shape[-2]
     k_layer, v_layer = pool.k[layer_idx], pool.v[layer_idx]
     max_blocks = block_tables.shape[1]
@@ -396,6 +407,14 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
                                         out, 0, ws, err, ctr, kv_scales=scales).unsqueeze(1)
         return seam().decode_step(q, k_layer, v_layer, block_tables, context_lens, pool.block_size, scale, out, ws, err,
                                   ctr, stream_of(q))
+
+
+def _out_for(q: torch.Tensor, pool) -> torch.Tensor | None:
+    """The output for rows ``q`` ``[N, H_q, D]`` of fp32 that attend an 8-bit pool of
+    another dtype; None where it is of ``q``'s."""
+    if not isinstance(pool, QuantPagedKVPool) or q.dtype == pool.dtype:
+        return None
+    return torch.empty(q.shape, dtype=pool.dtype, device=q.device)
 
 
 def _scales(pool, layer_idx: int) -> torch.Tensor | None:

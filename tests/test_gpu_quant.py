@@ -487,6 +487,108 @@ def test_prefill_over_many_workgroups_and_wide_groups(dtype):
                 row += n
 
 
+# fp32 queries of a 16-bit pool: the decode holds a query to 2^-16 of each element at least,
+# the prefill to 2^-14, and the code products lose at most as much again where they align
+# eight products. So scores move by at most 2^-13 reach. Rounding the queries to the dtype
+# moves them by u * reach; at scale 1 that is far more than what the outputs' own
+# roundings (u a + u |o|) leave, and shows that it is not done.
+# (At scale 1 many probabilities are below fp16's smallest normal number, 2^-14 of the
+# largest, where a rounding is off by up to 2^-25 and not by u of the probability: for
+# the sums, whose divisor is at least the largest probability, 1, by 2^-25 sum |v|.)
+
+
+@pytest.mark.parametrize("path", ["decode", "planned", "prefill", "prefill_plan"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq, h, d, bs", [(28, 4, 128, 16), (14, 2, 64, 32), (130, 1, 64, 16)])
+def test_fp32_queries_of_a_16_bit_pool(path, dtype, hq, h, d, bs):
+    lens = [1, 16, 33, 300, 700, 64]
+    pool, tables, values = filled(41 + hq, dtype, lens, h, d, bs)
+    q = torch.randn(len(lens), 2 * hq, d, generator=gen(42), device=DEV)[:, :hq]
+    bt, out = device_tables(tables), torch.empty(len(lens), hq, d, dtype=dtype, device=DEV)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    common = {"err_flags": pool.err_flags, "kv_scales": pool.kv_scales[0], "out": out}
+    if path == "decode":
+        kernels.paged_decode(q, pool.k[0], pool.v[0], bt, ctx, bs, 1.0, **common)
+    elif path == "planned":
+        plan = kernels.decode_plan(bt, ctx, hq, pool.k[0], bs)
+        kernels.paged_decode_planned(q, pool.k[0], pool.v[0], plan, 1.0, **common)
+    else:
+        cu = torch.arange(len(lens) + 1, dtype=torch.int32, device=DEV)
+        plan = None
+        if path == "prefill_plan":
+            plan = kernels.prefill_plan(cu, ctx - 1, bt, len(lens), 1, bs, hq, h, d, dtype=dtype)
+        kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, ctx - 1, 1, bs, 1.0, plan=plan, **common)
+    pool.check_errors()
+    off = rounded = 0.0
+    for i, n in enumerate(lens):
+        o, a, reach = quant.attend(q[i : i + 1], values, tables[i], bs, n - 1, 1.0)
+        tol = fp32_tolerance(o, a, reach, d) + decode_tolerance(o, a, dtype) + 4 * 2.0**-13 * reach[..., None] * a
+        if dtype == torch.float16:
+            t = torch.arange(n)
+            v = values[1, torch.tensor(tables[i])[t // bs] * bs + t % bs]
+            tol = tol + 2.0**-25 * v.abs().sum(0).repeat_interleave(hq // h, 0)
+        err = (out[i : i + 1].double().cpu() - o).abs()
+        assert (err <= tol).all(), (i, n, (err / tol).max())
+        off += err.square().sum().item()
+        r, _, _ = quant.attend(q[i : i + 1].to(dtype), values, tables[i], bs, n - 1, 1.0)
+        rounded += (r - o).square().sum().item()
+    assert off < 0.25 * rounded, (off, rounded)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq, h, d, bs", [(28, 4, 128, 16), (5, 5, 64, 32)])
+def test_rotated_queries_in_fp32(dtype, hq, h, d, bs):
+    """What the dtype's own output is the rounding of; without norms the same numbers."""
+    g, n = gen(43), 37
+    q, k, v = rows(g, n, hq + 2 * h, d, dtype).split([hq, h, h], 1)
+    wq, wk = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+    cos, sin = rotation(g, n, d)
+    slots = torch.arange(n, device=DEV)
+    for norms in ((wq, wk, 1e-6), ()):
+        got = []
+        for t in (dtype, torch.float32):
+            pool = QuantPagedKVPool(1, 4, bs, h, d, dtype)
+            q_out = torch.empty(n, hq + 1, d, dtype=t, device=DEV)[:, 1:]
+            kernels.rope_kv_scatter_q8(q, k, v, cos, sin, pool.k[0], pool.v[0], pool.kv_scales[0], slots, bs, *norms,
+                                       q_out=q_out)
+            got.append((q_out, pool.k.view(torch.uint8).clone(), pool.kv_scales.clone()))
+        assert torch.equal(got[0][0], got[1][0].to(dtype))
+        assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][2], got[1][2])
+        if norms:
+            o = quant.norm_rope(q, wq, 1e-6, cos, sin)
+            tol = norm_tolerance(q, wq, 1e-6, cos, sin, o, dtype, stored=False)
+            assert ((got[1][0].double().cpu() - o).abs() <= tol).all()
+        else:
+            assert torch.equal(got[1][0].to(dtype).float(), got[1][0])
+
+
+def test_refusals_of_fp32_queries():
+    pool = QuantPagedKVPool(1, 4, 16, 2, 64, torch.bfloat16)
+    q = torch.zeros(1, 4, 64, device=DEV)
+    tables, ctx = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    caches, scales = (pool.k[0], pool.v[0]), pool.kv_scales[0]
+    half, bf16 = q.half(), q.bfloat16()
+    with pytest.raises(RuntimeError, match="out must be"):
+        kernels.paged_decode(half, *caches, tables, ctx, 16, 0.1, out=bf16, kv_scales=scales)
+    with pytest.raises(RuntimeError, match="out must be"):
+        kernels.paged_prefill(half, *caches, tables, cu, ctx - 1, 1, 16, 0.1, out=q, kv_scales=scales)
+    plan = kernels.prefill_plan(cu, ctx - 1, tables, 1, 1, 16, 4, 2, 64, dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="plan was built"):
+        kernels.paged_prefill(q, *caches, tables, cu, ctx - 1, 1, 16, 0.1, out=bf16, plan=plan, kv_scales=scales)
+    plain = PagedKVPool(1, 4, 16, 2, 64, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="mismatch"):
+        kernels.paged_decode(q, plain.k[0], plain.v[0], tables, ctx, 16, 0.1, out=bf16)
+    rows3, cs, w = (bf16, bf16[:, :2], bf16[:, :2]), torch.zeros(1, 64, device=DEV), torch.ones(64, device=DEV)
+    slots = torch.zeros(1, dtype=torch.long, device=DEV)
+    with pytest.raises(RuntimeError, match="out must be"):
+        kernels.rope_kv_scatter_q8(*rows3, cs, cs, *caches, scales, slots, 16, q_out=half)
+    with pytest.raises(RuntimeError, match="q_out must be"):
+        kernels.qk_norm_rope_kv_scatter(*rows3, w.bfloat16(), w.bfloat16(), 1e-6, cs, cs, plain.k[0], plain.v[0],
+                                        slots, q_out=q)
+    assert not pool.k.view(torch.uint8).any() and not plain.k.any()
+
+
 # ---- norms and rotation
 #
 # In fp32 the sum of squares of d numbers is off by at most d / 2 + 8 steps of 2^-24, the

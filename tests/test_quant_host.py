@@ -79,6 +79,8 @@ def _rope(fn, q8, **kw):
              eps=1e-6, cos=P, sin=P, cs=128, kc=P, vc=P)
     a.update(dict(sc=P, nb=4, bs=16) if q8 else dict(cst=128, csh=8192, ns=64))
     a.update(slots=P, n=3, hq=4, h=2, d=128, dt=2)
+    if q8:
+        a.update(qdt=2)
     a.update(kw)
     return getattr(_lib.lib(), fn)(*a.values(), None, None)
 
@@ -102,6 +104,13 @@ def test_norm_rope_needs_weights_where_it_norms():
     assert _rope("ir_rope_kv_scatter_q8", True, n=0) == 0
 
 
+def test_queries_leave_the_rotation_in_the_dtype_or_fp32():
+    assert _rope("ir_rope_kv_scatter_q8", True, qdt=1) == -1
+    assert b"q_out_dtype" in _lib.lib().ir_last_error()
+    assert _rope("ir_rope_kv_scatter_q8", True, qdt=0, qot=514) == -1  # (fp32's strides)
+    assert b"strides" in _lib.lib().ir_last_error()
+
+
 def test_read_refusals():
     lib = _lib.lib()
     ok = (P, P, P, 4, 16, P, 3, 2, 128, 2, P, P, None, None)
@@ -116,15 +125,19 @@ def test_read_refusals():
 def test_attention_refusals():
     lib = _lib.lib()
     # scales missing, a block size that is no multiple of 16, scales off their alignment
-    dec = [P, 512, 128, P, P, P, 4, 16, P, 4, 4, P, P, 512, 128, 2, 4, 2, 128, 1.0, 2, 0, P, 64, P, 1 << 30, None, None]
-    for at, x, text in ((5, None, b"null"), (7, 24, b"block size"), (5, P + 4, b"aligned"), (20, 3, b"dtype")):
+    dec = [P, 512, 128, P, P, P, 4, 16, P, 4, 4, P, P, 512, 128, 2, 4, 2, 128, 1.0, 2, 2, 0, P, 64, P, 1 << 30, None,
+           None]
+    for at, x, text in ((5, None, b"null"), (7, 24, b"block size"), (5, P + 4, b"aligned"), (20, 3, b"dtype"),
+                        (21, 1, b"q_dtype"), (0, P + 8, b"aligned")):
         a = dec[:at] + [x] + dec[at + 1 :]
         assert lib.ir_paged_decode_q8(*a) == -1 and text in lib.ir_last_error(), at
-    pre = [P, 512, 128, P, P, P, 4, 16, P, 4, 4, P, P, 2, 8, 8, P, 512, 128, 4, 2, 128, 1.0, 2, None, 0, None, None]
-    for at, x, text in ((5, None, b"null"), (7, 24, b"block size"), (5, P + 4, b"aligned"), (23, 3, b"dtype")):
+    pre = [P, 512, 128, P, P, P, 4, 16, P, 4, 4, P, P, 2, 8, 8, P, 512, 128, 4, 2, 128, 1.0, 2, 2, None, 0, None, None]
+    for at, x, text in ((5, None, b"null"), (7, 24, b"block size"), (5, P + 4, b"aligned"), (23, 3, b"dtype"),
+                        (24, 1, b"q_dtype"), (1, 514, b"strides")):
         a = pre[:at] + [x] + pre[at + 1 :]
         assert lib.ir_paged_prefill_q8(*a) == -1 and text in lib.ir_last_error(), at
-    plan = [P, 512, 128, P, P, P, P, 512, 128, 2, 4, 2, 128, 4, 16, 1.0, 2, 0, P, P, 64, P, 1 << 30, None, None]
-    for at, x, text in ((5, None, b"null"), (5, P + 4, b"aligned"), (16, 3, b"dtype"), (14, 24, b"plannable")):
+    plan = [P, 512, 128, P, P, P, P, 512, 128, 2, 4, 2, 128, 4, 16, 1.0, 2, 2, 0, P, P, 64, P, 1 << 30, None, None]
+    for at, x, text in ((5, None, b"null"), (5, P + 4, b"aligned"), (16, 3, b"dtype"), (14, 24, b"plannable"),
+                        (17, 1, b"q_dtype")):
         a = plan[:at] + [x] + plan[at + 1 :]
         assert lib.ir_paged_decode_planned_q8(*a) == -1 and text in lib.ir_last_error(), at
