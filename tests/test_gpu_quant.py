@@ -854,6 +854,174 @@ def test_mixed_step_over_the_8_bit_pool(overlap):
     assert ((eager[1][1, 40:80].double().cpu() - o).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("layout", ["head_major", "slot_major"])
+def test_normed_seam_over_the_16_bit_pool(layout):
+    """Norms through ``rope_paged_attention``: the normed rotation, then the attention alone."""
+    hq, h, d, bs, dtype = 6, 2, 64, 16, torch.bfloat16
+    g = gen(51)
+    wq, wk = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+    pools = [PagedKVPool(1, 12, bs, h, d, dtype, layout=layout) for _ in range(2)]
+    for cached, new in (([0, 0], [20, 33]), ([20, 33], [1, 1])):
+        for pool, whole in zip(pools, (True, False)):
+            if max(new) > 1:
+                paged, mask = metadata.prefill_context(pool, [[3, 1, 5], [0, 2, 4]], cached, new)
+                b, n = 1, sum(new)
+            else:
+                paged, mask = metadata.decode_context(pool, [[3, 1, 5], [0, 2, 4]], cached)
+                b, n = 2, 1
+            if whole:
+                x = step_inputs(g, b, n, hq, h, d, dtype)
+            q, k, v, cos, sin = x
+            if whole:
+                want = rope_paged_attention(q, k, v, cos, sin, paged, mask, 0, d**-0.5, 3, q_norm=wq, k_norm=wk)
+                continue
+            spare = PagedKVPool(1, 12, bs, h, d, dtype)
+            args = (q.reshape(-1, hq, d), k.reshape(-1, h, d), v.reshape(-1, h, d))
+            qr = kernels.qk_norm_rope_kv_scatter(*args, wq, wk, 1e-6, cos.view(-1, d), sin.view(-1, d), spare.k[0],
+                                                 spare.v[0], paged.write_slots)
+            kr, vr = (t[0, paged.write_slots].view(b, n, h, d) for t in (spare.k, spare.v))
+            got = paged_attention(qr.view(b, n, hq, d), kr, vr, paged, mask, 0, d**-0.5, 3)
+            assert torch.equal(got, want)
+    assert torch.equal(pools[0].k, pools[1].k) and torch.equal(pools[0].v, pools[1].v)
+
+
+def test_one_graph_of_every_call():
+    """Writes, normed rotations into both kinds of pool, reading back and attention in one
+    graph, replayed on other inputs with eager work and synchronizations between."""
+    hq, h, d, bs, n, dtype = 8, 2, 64, 16, 50, torch.bfloat16
+    g = gen(52)
+    w = (1 + 0.3 * torch.randn(d, generator=g, device=DEV)).to(dtype)
+    slots = torch.arange(n, device=DEV) + 16
+    tables = torch.tensor([[1, 2, 3, 4]], dtype=torch.int32, device=DEV)
+    ctx = torch.tensor([n], dtype=torch.int32, device=DEV)
+    cu, start = torch.tensor([0, n], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    x = rows(g, n, hq + 2 * h, d, dtype)
+    cos, sin = rotation(g, n, d)
+
+    def pools():
+        return QuantPagedKVPool(2, 6, bs, h, d, dtype), PagedKVPool(1, 6, bs, h, d, dtype)
+
+    def step(x, quantised, plain):
+        q, k, v = x.split([hq, h, h], 1)
+        quantised.write(0, k, v, slots)
+        q_out = torch.empty(n, hq, d, device=DEV)
+        kernels.rope_kv_scatter_q8(q, k, v, cos, sin, quantised.k[1], quantised.v[1], quantised.kv_scales[1], slots, bs,
+                                   w, w, 1e-6, q_out)
+        q16 = kernels.qk_norm_rope_kv_scatter(q, k, v, w, w, 1e-6, cos, sin, plain.k[0], plain.v[0], slots)
+        out = torch.empty(n, hq, d, dtype=dtype, device=DEV)
+        plan = kernels.prefill_plan(cu, start, tables, n, n, bs, hq, h, d, dtype=dtype)
+        kernels.paged_prefill(q_out, quantised.k[1], quantised.v[1], tables, cu, start, n, bs, d**-0.5, out=out,
+                              plan=plan, kv_scales=quantised.kv_scales[1])
+        decode = kernels.decode_plan(tables, ctx, hq, quantised.k[0], bs)
+        one = kernels.paged_decode_planned(q16[:1], quantised.k[0], quantised.v[0], decode, d**-0.5,
+                                           kv_scales=quantised.kv_scales[0])
+        return (q_out, q16, out, one, *quantised.gather(0, slots), *quantised.gather_blocks(1, tables, ctx, n),
+                plain.k, plain.v)
+
+    static, mine, other = x.clone(), pools(), pools()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static, *mine)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(static, *mine)
+    for i in range(4):
+        static.copy_(rows(g, n, hq + 2 * h, d, dtype) * 2.0 ** (3 * i - 4))
+        want = [t.clone() for t in step(static, *other)]
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i
+
+
+def test_layers_on_two_streams():
+    """Two layers of a pool written and attended on streams of their own at the same time."""
+    hq, h, d, bs, n, dtype = 28, 4, 128, 16, 700, torch.bfloat16
+    g = gen(53)
+    pools = [QuantPagedKVPool(2, 50, bs, h, d, dtype) for _ in range(2)]
+    data = [rows(g, n, hq + 2 * h, d, dtype).split([hq, h, h], 1) for _ in range(2)]
+    slots = torch.randperm(n, generator=g, device=DEV)
+    tables = torch.arange(44, dtype=torch.int32, device=DEV)[None]
+    cu, start = torch.tensor([0, n], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    ctx = torch.tensor([n], dtype=torch.int32, device=DEV)
+
+    def run(pool, layer):
+        q, k, v = data[layer]
+        pool.write(layer, k, v, slots)
+        s = pool.kv_scales[layer]
+        a = kernels.paged_prefill(q, pool.k[layer], pool.v[layer], tables, cu, start, n, bs, d**-0.5, kv_scales=s)
+        b = kernels.paged_decode(q[:1].contiguous(), pool.k[layer], pool.v[layer], tables, ctx, bs, d**-0.5, kv_scales=s)
+        return a, b, *pool.gather(layer, slots)
+
+    want = [run(pools[0], layer) for layer in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for layer, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[layer] = run(pools[1], layer)
+    torch.cuda.synchronize()
+    for layer in range(2):
+        for a, b in zip(got[layer], want[layer]):
+            assert torch.equal(a, b)
+
+
+def test_write_of_very_many_tokens_in_any_order():
+    """One call of 70,000 shuffled tokens against calls that each take some whole blocks."""
+    h, d, bs, dtype = 2, 64, 48, torch.bfloat16
+    g = gen(54)
+    blocks = 1459
+    n = blocks * bs
+    k, v = rows(g, n, h, d, dtype), rows(g, n, h, d, dtype)
+    slots = torch.randperm(n, generator=g, device=DEV)
+    one, many = (QuantPagedKVPool(1, blocks, bs, h, d, dtype) for _ in range(2))
+    one.write(0, k, v, slots)
+    order = slots.argsort()
+    for lo in range(0, n, 200 * bs):
+        i = order[lo : lo + 200 * bs]
+        many.write(0, k[i], v[i], slots[i])
+    assert torch.equal(one.kv_scales, many.kv_scales)
+    for a, b in ((one.k, many.k), (one.v, many.v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_rows_far_apart():
+    """Queries, keys and values whose rows are more than 2^31 elements apart."""
+    hq, h, d, bs, dtype = 4, 2, 64, 16, torch.bfloat16
+    far = torch.empty(3, (1 << 30) + 64, dtype=dtype, device=DEV)
+    g = gen(55)
+    x = rows(g, 3, hq + 2 * h, d, dtype)
+    far[:, : (hq + 2 * h) * d] = x.flatten(1)
+    wide = far[:, : (hq + 2 * h) * d].unflatten(1, (hq + 2 * h, d))
+    assert wide.stride(0) * 2 > 1 << 31
+    w = torch.ones(d, dtype=dtype, device=DEV)
+    cos, sin = rotation(g, 3, d)
+    slots = torch.arange(3, device=DEV)
+    outs = []
+    for t in (x, wide):
+        q, k, v = t.split([hq, h, h], 1)
+        quantised, plain = QuantPagedKVPool(2, 1, bs, h, d, dtype), PagedKVPool(1, 1, bs, h, d, dtype)
+        quantised.write(0, k, v, slots)
+        tables = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+        cu = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+        args = (quantised.k[0], quantised.v[0])
+        outs.append([
+            kernels.qk_norm_rope_kv_scatter(q, k, v, w, w, 1e-6, cos, sin, plain.k[0], plain.v[0], slots).contiguous(),
+            kernels.rope_kv_scatter_q8(q, k, v, cos, sin, quantised.k[1], quantised.v[1], quantised.kv_scales[1], slots,
+                                       bs, w, w, 1e-6).contiguous(),
+            kernels.paged_prefill(q, *args, tables, cu, cu[:1], 3, bs, 0.125, kv_scales=quantised.kv_scales[0]),
+            kernels.paged_decode(q, *args, tables.expand(3, 1).contiguous(), cu[1:].expand(3).contiguous(), bs, 0.125,
+                                 kv_scales=quantised.kv_scales[0]),
+            quantised.k.view(torch.uint8), quantised.v.view(torch.uint8), quantised.kv_scales, plain.k, plain.v])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
 def test_refusals():
     h, d, bs = 2, 64, 16
     pool = QuantPagedKVPool(1, 8, bs, h, d, torch.bfloat16)
