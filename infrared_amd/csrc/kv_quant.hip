@@ -12,10 +12,14 @@
 // the block's tokens takes (the last given), and no other workgroup touches it. That is
 // one launch without a workspace, and its result does not depend on the order of
 // execution. The slots are 8 bytes a token against 4 KB of rows at 4 heads of 128, and
-// come from L2, but the workgroups of n / block_size tokens read them all: 128 MB of L2
-// traffic at 16,384 tokens, growing with the square.
+// come from L2, but every workgroup with a block to own reads them all. So those of a long
+// call look after up to 256 tokens and read them once for 16 blocks (write_blocks):
+// 131,072 tokens of 4 heads of 128 in order 216 us (944 with one reading a block), shuffled
+// 2.6 ms (14.3); 16,384 in order 28 us (30), shuffled 89 (295). Below that a reading a block is
+// as fast or faster (written and read back, 64 single tokens 7.0 us against 7.5 and 4,096
+// in order 14.5 against 15.3).
 //
-// What bounds it is latency: the slots, the scan, the rows and the codes follow each
+// What bounds a call of usual size is latency: the slots, the scan, the rows and the codes follow each
 // other (64 tokens 4.3 us a call, 4,096 tokens 9.8 us for 12.6 MB, 28 / 4 heads of 128,
 // of which 2.7 us are the launch of workgroups that find nothing to do).
 //
@@ -23,6 +27,7 @@
 // scale, the rows become codes. A block that is not new keeps its tokens; only when
 // its scale grows are they read, rounded to the wider scale and written back.
 #include <algorithm>
+#include <type_traits>
 
 #include "e4m3.hpp"
 #include "norm_rope.hpp"
@@ -36,6 +41,10 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kMaxBlockSize = 1024;
 constexpr int kWriteWaves = 4;
+constexpr int kMaxWindow = 256;
+constexpr int kWanted = 16;        // blocks found in one reading of the slots
+constexpr int kWantedRows = 4096;  // their tokens
+constexpr int kKeys = 256;
 // Workgroups up to which each looks after one token only: four a CU (2,048 measured
 // 11.8 against 10.3 us on a mixed step of 1,248 tokens, 10.1 against 9.8 on 4,096).
 constexpr int64_t kWriteGroups = 1024;
@@ -47,7 +56,7 @@ struct QuantArgs {
   float* scales;
   int64_t num_blocks;
   int bs;
-  int window;      // tokens of the call that a workgroup looks after, at most 16
+  int window;      // tokens of the call that a workgroup looks after, at most kMaxWindow
   int kv_groups;   // workgroups per window for the 2 * H_kv (head, K / V) parts
   int64_t n_kv;    // workgroups of the write; those after them take query rows
   int32_t* err;
@@ -341,6 +350,86 @@ __device__ __forceinline__ void write_block(const QuantArgs& a, int64_t i, int b
     write_part<DT, D, MODE>(a, i, hb, h, is_v, old, s_row);
 }
 
+struct OneBlock {
+  int row[kMaxBlockSize], earlier;
+};
+
+// Blocks a workgroup is after at a time, with the rows that their tokens take.
+struct Wanted {
+  int blk[kWanted], earlier[kWanted];
+  int64_t tok[kWanted];
+  int row[kWantedRows];  // [wanted][block_size]: row + 1, 0: none
+  int key[kKeys], of[kKeys];  // open addressing: block (-1: none), the first wanted that names it
+};
+
+// Where block `blk` is in the table, or would be: an entry of it or an empty one.
+__device__ __forceinline__ int find_key(const Wanted& s, int blk) {
+  int p = blk & (kKeys - 1);
+  for (int key = s.key[p]; key != blk && key != -1; key = s.key[p]) p = (p + 1) & (kKeys - 1);
+  return p;
+}
+
+// Writes those of the `count` wanted blocks whose token is the call's first of the block:
+// part `part` (K or V of a head) by this wavefront. The whole workgroup calls it alike,
+// parts past the last included; blk and tok are set, with no barrier behind them yet.
+template <int DT, int D, int MODE>
+__device__ __forceinline__ void write_blocks(const QuantArgs& a, int count, int part, Wanted& s) {
+  constexpr int NT = kWriteWaves * 64;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const bool active = part < 2 * a.r.num_kv_heads;
+  const int h = part >> 1, is_v = part & 1;
+  const int64_t h0 = (int64_t)h * a.num_blocks;
+  for (int t = tid; t < count * a.bs; t += NT) s.row[t] = 0;
+  if (tid < kWanted) s.earlier[tid] = 0;
+  for (int t = tid; t < kKeys; t += NT) {
+    s.key[t] = -1;
+    s.of[t] = kWanted;
+  }
+  __syncthreads();
+  float old = 0.f;  // lane c: the scale of wanted block c
+  if (active && lane < count) old = a.scales[2 * (h0 + s.blk[lane]) + is_v];
+  if (tid < count) {
+    int p = s.blk[tid] & (kKeys - 1);
+    for (;;) {  // (at most 16 of 256 entries are taken)
+      const int was = atomicCAS(&s.key[p], -1, s.blk[tid]);
+      if (was == -1 || was == s.blk[tid]) break;
+      p = (p + 1) & (kKeys - 1);
+    }
+    atomicMin(&s.of[p], tid);
+  }
+  __syncthreads();
+  // ---- the blocks' tokens in this call
+  const int64_t num_slots = a.num_blocks * a.bs;
+  constexpr int SCAN = 8;  // slots of a lane in flight together
+  for (int64_t j0 = tid; j0 < a.r.n_tokens; j0 += SCAN * NT) {
+    int64_t slot[SCAN];
+#pragma unroll
+    for (int u = 0; u < SCAN; ++u) slot[u] = j0 + u * NT < a.r.n_tokens ? a.r.slots[j0 + u * NT] : -1;
+#pragma unroll
+    for (int u = 0; u < SCAN; ++u) {
+      if ((uint64_t)slot[u] >= (uint64_t)num_slots) continue;  // (slots fit 31 bits)
+      const int blk = (int)((uint32_t)slot[u] / (uint32_t)a.bs);
+      const int p = find_key(s, blk);
+      if (s.key[p] == -1) continue;
+      const int c = s.of[p];
+      atomicMax(&s.row[c * a.bs + ((int)slot[u] - blk * a.bs)], (int)(j0 + u * NT) + 1);
+      if (j0 + u * NT < s.tok[c]) s.earlier[c] = 1;
+    }
+  }
+  __syncthreads();
+
+  // ---- this wavefront's head, K or V
+  for (int c = 0; c < count; ++c) {
+    const int blk = s.blk[c];
+    if (s.earlier[c] || !active || s.of[find_key(s, blk)] != c) continue;  // another's block
+    const float was = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(old), c));
+    if (MODE == kRowsPlain || is_v)
+      write_part<DT, D, kRowsPlain>(a, s.tok[c], h0 + blk, h, is_v, was, s.row + c * a.bs);
+    else
+      write_part<DT, D, MODE>(a, s.tok[c], h0 + blk, h, is_v, was, s.row + c * a.bs);
+  }
+}
+
 // A workgroup's place among the n of the write. Those of a prompt that own a block come
 // every block_size tokens, and workgroup b runs on XCD b mod 8: in their own order all
 // of them would share one or two XCDs (16.5 us for a mixed step's 1,248 tokens, 13.7
@@ -353,10 +442,10 @@ __device__ __forceinline__ uint32_t spread_xcds(uint32_t b, uint32_t n) {
   return 8 * k + ((b + turn) & 7u);
 }
 
-template <int DT, int D, int MODE>
+// MANY: windows of more than 16 tokens.
+template <int DT, int D, int MODE, bool MANY>
 __global__ __launch_bounds__(kWriteWaves * 64) void kv_write_q8_kernel(QuantArgs a) {
-  __shared__ int s_row[kMaxBlockSize];
-  __shared__ int s_earlier;
+  __shared__ std::conditional_t<MANY, Wanted, OneBlock> s;
   if constexpr (MODE != kRowsPlain) {
     if (blockIdx.x >= a.n_kv) {
       query_rows<DT, D, MODE>(a.r, (blockIdx.x - a.n_kv) * kWriteWaves + (threadIdx.x >> 6));
@@ -368,21 +457,43 @@ __global__ __launch_bounds__(kWriteWaves * 64) void kv_write_q8_kernel(QuantArgs
   const int64_t wi = group / (uint32_t)a.kv_groups;
   const int part = (int)(group - wi * a.kv_groups) * kWriteWaves + (tid >> 6);
   const int64_t num_slots = a.num_blocks * a.bs;
-  // lane l: token i0 + l of the window; it may own its block unless the token
-  // before it is in the same one
   const int64_t i0 = wi * a.window;
   const int wn = (int)min((int64_t)a.window, a.r.n_tokens - i0);
-  const int64_t my_slot = lane < wn ? a.r.slots[i0 + lane] : -1;
-  const int64_t before = lane < wn && i0 + lane > 0 ? a.r.slots[i0 + lane - 1] : -1;
-  const bool valid = my_slot >= 0 && my_slot < num_slots;  // (negative: padding)
-  if (my_slot >= num_slots && part == 0) flag_error(a.err, IR_ERR_SLOT_RANGE);
-  const int my_blk = valid ? (int)((uint32_t)my_slot / (uint32_t)a.bs) : -1;  // (slots fit 31 bits)
-  const int64_t my_base = (int64_t)my_blk * a.bs;
-  uint64_t todo = __ballot(valid && !(before >= my_base && before < my_base + a.bs));
-  while (todo) {  // uniform over the workgroup: every wavefront looks at the same window
-    const int at = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    write_block<DT, D, MODE>(a, i0 + at, __builtin_amdgcn_readlane(my_blk, at), part, s_row, &s_earlier);
+  // lane l: token first + l of the window; it may own its block unless the token before it
+  // is in the same one. What follows is uniform over the workgroup: every wavefront looks at
+  // the same window.
+  int my_blk = -1;
+  auto owners = [&](int64_t first) -> uint64_t {
+    const bool in = first + lane < i0 + wn;
+    const int64_t my_slot = in ? a.r.slots[first + lane] : -1;
+    const int64_t before = in && first + lane > 0 ? a.r.slots[first + lane - 1] : -1;
+    const bool valid = my_slot >= 0 && my_slot < num_slots;  // (negative: padding)
+    if (my_slot >= num_slots && part == 0) flag_error(a.err, IR_ERR_SLOT_RANGE);
+    my_blk = valid ? (int)((uint32_t)my_slot / (uint32_t)a.bs) : -1;  // (slots fit 31 bits)
+    const int64_t my_base = (int64_t)my_blk * a.bs;
+    return __ballot(valid && !(before >= my_base && before < my_base + a.bs));
+  };
+  if constexpr (!MANY) {
+    for (uint64_t todo = owners(i0); todo; todo &= todo - 1) {
+      const int at = __builtin_ctzll(todo);
+      write_block<DT, D, MODE>(a, i0 + at, __builtin_amdgcn_readlane(my_blk, at), part, s.row, &s.earlier);
+    }
+  } else {
+    const int most = min(kWanted, kWantedRows / a.bs);
+    int count = 0;
+    for (int64_t first = i0; first < i0 + wn; first += 64)
+      for (uint64_t todo = owners(first); todo; todo &= todo - 1) {
+        const int at = __builtin_ctzll(todo), blk = __builtin_amdgcn_readlane(my_blk, at);
+        if (tid == 0) {
+          s.blk[count] = blk;
+          s.tok[count] = first + at;
+        }
+        if (++count < most) continue;
+        write_blocks<DT, D, MODE>(a, count, part, s);
+        __syncthreads();  // (its readers are done before the next are set)
+        count = 0;
+      }
+    if (count) write_blocks<DT, D, MODE>(a, count, part, s);
   }
 }
 
@@ -474,19 +585,26 @@ int launch_write(const char* name, const QuantArgs& a0, int mode, hipStream_t s)
   constexpr int G = 64 / (D / 16);
   a.kv_groups = (2 * a.r.num_kv_heads + kWriteWaves - 1) / kWriteWaves;
   // one token a workgroup until the workgroups fill the device, then as many as keep
-  // it filled: in a prompt most tokens own no block, in a decode step each does
-  a.window = (int)std::max<int64_t>(1, std::min<int64_t>(16, a.r.n_tokens * a.kv_groups / kWriteGroups));
+  // it filled: in a prompt most tokens own no block, in a decode step each does; past 16
+  // they share the reading of the slots
+  a.window = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxWindow, a.r.n_tokens * a.kv_groups / kWriteGroups));
   a.n_kv = (a.r.n_tokens + a.window - 1) / a.window * a.kv_groups;
   const int64_t runs = (a.r.num_q_heads + G - 1) / G;
   const int64_t n_q = mode == kRowsPlain ? 0 : (a.r.n_tokens * runs + kWriteWaves - 1) / kWriteWaves;
   IR_REQUIRE(a.r.n_tokens < 0x7fffffff && a.n_kv + n_q <= 0x7fffffff, "%s: too many tokens", name);
   const dim3 grid((unsigned)(a.n_kv + n_q)), block(kWriteWaves * 64);
-  if (mode == kRowsPlain)
-    hipLaunchKernelGGL((kv_write_q8_kernel<DT, D, kRowsPlain>), grid, block, 0, s, a);
-  else if (mode == kRowsNorm)
-    hipLaunchKernelGGL((kv_write_q8_kernel<DT, D, kRowsNorm>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((kv_write_q8_kernel<DT, D, kRowsRotate>), grid, block, 0, s, a);
+  const bool many = a.window > 16;
+#define IR_WRITE(MODE_)                                                                         \
+  do {                                                                                          \
+    if (many)                                                                                   \
+      hipLaunchKernelGGL((kv_write_q8_kernel<DT, D, MODE_, true>), grid, block, 0, s, a);       \
+    else                                                                                        \
+      hipLaunchKernelGGL((kv_write_q8_kernel<DT, D, MODE_, false>), grid, block, 0, s, a);      \
+  } while (0)
+  if (mode == kRowsPlain) IR_WRITE(kRowsPlain);
+  else if (mode == kRowsNorm) IR_WRITE(kRowsNorm);
+  else IR_WRITE(kRowsRotate);
+#undef IR_WRITE
   return check_launch(name);
 }
 

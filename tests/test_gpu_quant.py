@@ -145,6 +145,30 @@ def test_write_takes_tokens_in_any_order(dtype):
             pool.check_errors()
 
 
+@pytest.mark.parametrize("d, h, bs, n", [(64, 64, 16, 700), (128, 64, 48, 900), (64, 65, 1024, 1300)])
+def test_write_of_long_calls(d, h, bs, n):
+    """Calls whose workgroups share the reading of the slots (many heads make a call long):
+    shuffled tokens, slots given twice, skipped and past the pool; then in order, over
+    blocks that hold tokens already."""
+    g, blocks, dtype = gen(d + bs), max(4, 1000 // bs), torch.bfloat16
+    pool, want = QuantPagedKVPool(1, blocks, bs, h, d, dtype), quant.QuantCache(blocks, bs, h, d, dtype)
+    slots = torch.randint(0, pool.num_slots, (n,), generator=g, device=DEV)
+    slots[::17] = -1
+    slots[5] = pool.num_slots
+    k, v = rows(g, n, h, d, dtype), rows(g, n, h, d, dtype)
+    pool.write(0, k, v, slots)
+    with pytest.raises(IndexError, match="slot"):
+        pool.check_errors()
+    want.write(k, v, slots)
+    check_cache(pool, want)
+    m = min(n, pool.num_slots - 7)
+    k, v = rows(g, m, h, d, dtype) * 4, rows(g, m, h, d, dtype) * 4
+    pool.write(0, k, v, torch.arange(7, 7 + m, device=DEV))
+    want.write(k, v, torch.arange(7, 7 + m))
+    pool.check_errors()
+    check_cache(pool, want)
+
+
 def test_a_fresh_block_owes_nothing_to_what_it_held():
     pool = QuantPagedKVPool(1, 2, 16, 2, 64, torch.bfloat16)
     g = gen(4)
@@ -344,7 +368,8 @@ def test_decode_of_long_contexts_and_shared_prefixes(planned):
 
 
 @pytest.mark.parametrize("dtype, hq, h, d, lens", [
-    (torch.bfloat16, 28, 4, 128, [20011]), (torch.float16, 14, 2, 64, [9000, 0, 17]), (torch.float32, 6, 2, 128, [5000]),
+    (torch.bfloat16, 28, 4, 128, [20011]), (torch.float16, 14, 2, 64, [9000, 0, 17]),
+    (torch.float32, 6, 2, 128, [5000]),
     (torch.bfloat16, 40, 2, 64, [8191, 4000]), (torch.bfloat16, 8, 1, 128, [300, 1, 0]),
 ])
 def test_decode_of_few_sequences_over_many_slices(dtype, hq, h, d, lens):
@@ -712,6 +737,28 @@ def test_normed_rotation_into_the_8_bit_pool(dtype, hq, h, d, bs):
     assert (got[0, slots.cpu()] != want.values[0, slots.cpu()]).double().mean() < 1e-3
 
 
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rotation_of_a_long_call_is_that_of_its_blocks(dtype, normed):
+    """A call whose workgroups share the reading of the slots against calls of some blocks."""
+    g, hq, h, d, bs, n = gen(17), 3, 64, 64, 16, 720
+    q, k, v = rows(g, n, hq + 2 * h, d, dtype).split([hq, h, h], 1)
+    w = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+    norms = (*w, 1e-6) if normed else ()
+    cos, sin = rotation(g, n, d)
+    slots = (torch.randperm(n // bs, generator=g, device=DEV)[:, None] * bs + torch.arange(bs, device=DEV)).flatten()
+    one, many = (QuantPagedKVPool(1, n // bs, bs, h, d, dtype) for _ in range(2))
+    a = kernels.rope_kv_scatter_q8(q, k, v, cos, sin, one.k[0], one.v[0], one.kv_scales[0], slots, bs, *norms)
+    for i in range(0, n, 5 * bs):
+        t = slice(i, i + 5 * bs)
+        b = kernels.rope_kv_scatter_q8(q[t], k[t], v[t], cos[t], sin[t], many.k[0], many.v[0], many.kv_scales[0],
+                                       slots[t], bs, *norms)
+        assert torch.equal(a[t], b)
+    assert torch.equal(one.kv_scales, many.kv_scales)
+    for x, y in ((one.k, many.k), (one.v, many.v)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 # ---- together
 
 
@@ -954,7 +1001,8 @@ def test_layers_on_two_streams():
         pool.write(layer, k, v, slots)
         s = pool.kv_scales[layer]
         a = kernels.paged_prefill(q, pool.k[layer], pool.v[layer], tables, cu, start, n, bs, d**-0.5, kv_scales=s)
-        b = kernels.paged_decode(q[:1].contiguous(), pool.k[layer], pool.v[layer], tables, ctx, bs, d**-0.5, kv_scales=s)
+        one = q[:1].contiguous()
+        b = kernels.paged_decode(one, pool.k[layer], pool.v[layer], tables, ctx, bs, d**-0.5, kv_scales=s)
         return a, b, *pool.gather(layer, slots)
 
     want = [run(pools[0], layer) for layer in range(2)]
