@@ -129,14 +129,15 @@ def rope_paged_attention(
         raise RuntimeError("rope_paged_attention: q_norm and k_norm go together")
     rows = (q.reshape(b * sq, hq, d), k.reshape(b * sq, h_kv, d), v.reshape(b * sq, h_kv, d))
     angles = (cos.reshape(b * sq, d), sin.reshape(b * sq, d))
-    caches = (pool.k[layer_idx], pool.v[layer_idx])
+    k_layer, v_layer, scales = _layer(pool, layer_idx)
+    caches = (k_layer, v_layer)
     err = getattr(pool, "err_flags", None)
-    if isinstance(pool, QuantPagedKVPool):
+    if scales is not None:
         _check_quant(pool, q, paged)
         # normed queries stay fp32 up to the scores, as normed keys do up to their codes: a
         # rounding of theirs would be as large an error of the outputs as all others
         q_out = None if q_norm is None else torch.empty(b * sq, hq, d, dtype=torch.float32, device=q.device)
-        q_rot = kernels.rope_kv_scatter_q8(*rows, *angles, *caches, pool.kv_scales[layer_idx], paged.write_slots,
+        q_rot = kernels.rope_kv_scatter_q8(*rows, *angles, *caches, scales, paged.write_slots,
                                            pool.block_size, q_norm, k_norm, eps, q_out, err_flags=err)
     elif q_norm is not None:
         q_rot = kernels.qk_norm_rope_kv_scatter(*rows, q_norm, k_norm, eps, *angles, *caches, paged.write_slots,
@@ -167,7 +168,7 @@ def _attend(q: torch.Tensor, paged, mask: torch.Tensor | None, layer_idx: int, s
     ``pool.write``)."""
     pool = paged.pool
     b, sq = q.shape[:2]
-    k_layer, v_layer = pool.k[layer_idx], pool.v[layer_idx]
+    k_layer, v_layer, _ = _layer(pool, layer_idx)
     err = getattr(pool, "err_flags", None)
     if isinstance(pool, QuantPagedKVPool) and new_kv is not None:
         _check_quant(pool, q, paged)
@@ -341,10 +342,11 @@ def _prefill(q, pool, layer_idx: int, block_tables, cu_seqlens_q, q_start, max_q
             holder.prefill_plan = plan
         except AttributeError:  # a context object without the field keeps none
             pass
+    k_layer, v_layer, scales = _layer(pool, layer_idx)
     return kernels.paged_prefill(
-        q.reshape(b * sq, hq, d), pool.k[layer_idx], pool.v[layer_idx], block_tables, cu_seqlens_q, q_start, max_q,
+        q.reshape(b * sq, hq, d), k_layer, v_layer, block_tables, cu_seqlens_q, q_start, max_q,
         pool.block_size, scale, out=out, err_flags=err, plan=plan, new_kv=new_kv, src_row0=src_row0,
-        kv_scales=_scales(pool, layer_idx),
+        kv_scales=scales,
     ).view(b, sq, hq, d)
 
 
@@ -357,7 +359,7 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
     if out is None:
         out = _out_for(q[:, 0], pool)
     h_kv = pool.k.shape[-2]
-    k_layer, v_layer = pool.k[layer_idx], pool.v[layer_idx]
+    k_layer, v_layer, scales = _layer(pool, layer_idx)
     max_blocks = block_tables.shape[1]
     if hasattr(pool, "plan_buffer") and kernels.decode_plan_pays(b, hq, h_kv, max_blocks, pool.block_size, q.device):
         # balanced schedule: built by the step's first layer, reused by the
@@ -387,7 +389,6 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
         ctr = pool.decode_counters(kernels.decode_num_counters(b, hq, h_kv))
         if own:
             _hold(holder, ws, ctr)
-        scales = _scales(pool, layer_idx)
         if scales is not None:
             return kernels.paged_decode_planned(q[:, 0], k_layer, v_layer, plan, scale, out, ws, err, ctr,
                                                 kv_scales=scales).unsqueeze(1)
@@ -401,7 +402,6 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
                 ctr = pool.decode_counters(kernels.decode_num_counters(b, hq, h_kv))
         if ws is not None and getattr(holder, "gate", None) is not None:
             _hold(holder, ws, ctr)
-        scales = _scales(pool, layer_idx)
         if scales is not None:
             return kernels.paged_decode(q[:, 0], k_layer, v_layer, block_tables, context_lens, pool.block_size, scale,
                                         out, 0, ws, err, ctr, kv_scales=scales).unsqueeze(1)
@@ -417,9 +417,11 @@ def _out_for(q: torch.Tensor, pool) -> torch.Tensor | None:
     return torch.empty(q.shape, dtype=pool.dtype, device=q.device)
 
 
-def _scales(pool, layer_idx: int) -> torch.Tensor | None:
-    """An 8-bit pool's scales of the layer."""
-    return pool.kv_scales[layer_idx] if isinstance(pool, QuantPagedKVPool) else None
+def _layer(pool, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """The layer's K, V and, of an 8-bit pool, scales."""
+    if isinstance(pool, QuantPagedKVPool):
+        return pool.layer(layer_idx)
+    return pool.k[layer_idx], pool.v[layer_idx], None
 
 
 def _hold(holder, *tensors: torch.Tensor) -> None:

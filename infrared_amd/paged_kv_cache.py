@@ -374,9 +374,17 @@ class QuantPagedKVPool(PagedKVPool):
         super().__init__(num_layers, num_blocks, block_size, num_kv_heads, head_dim, kernels.CODES, device,
                          strict=strict)
         self.dtype = dtype
+        self._layers: tuple | None = None
         # (empty blocks have the least scale: whatever is written first sets it)
         self.kv_scales = torch.full((num_layers, num_kv_heads, num_blocks, 2),
                                     2.0 ** (-15 if dtype == torch.float16 else -100), device=self.device)
+
+    def layer(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One layer's ``(k, v, kv_scales)`` (views, made once for the tensors the pool has)."""
+        held = self._layers
+        if held is None or held[0] is not self.k or held[1] is not self.v or held[2] is not self.kv_scales:
+            held = self._layers = (self.k, self.v, self.kv_scales, list(zip(self.k, self.v, self.kv_scales)))
+        return held[3][layer_idx]
 
     def write(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantises this step's K/V (``[N, num_kv_heads, head_dim]`` of ``dtype``) into ``slots``

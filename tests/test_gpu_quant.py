@@ -1127,3 +1127,14 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="kv_scales"):
         kernels.gather_slots_q8(pool.k[0], pool.v[0], scales, paged.write_slots, 32, torch.bfloat16)
     torch.cuda.synchronize()
+
+
+def test_layers_are_those_of_the_tensors_the_pool_has_now():
+    pool = QuantPagedKVPool(2, 2, 16, 2, 64, torch.bfloat16)
+    assert all(a.data_ptr() == b[1].data_ptr() for a, b in zip(pool.layer(1), (pool.k, pool.v, pool.kv_scales)))
+    first = pool.layer(0)
+    assert pool.layer(0)[0] is first[0] and pool.layer(-1)[2] is pool.layer(1)[2]
+    pool.kv_scales = pool.kv_scales.clone()
+    assert pool.layer(1)[2].data_ptr() == pool.kv_scales[1].data_ptr()
+    with pytest.raises(IndexError):
+        pool.layer(2)
