@@ -192,9 +192,11 @@ constexpr int kLockstep = 0, kRing2 = 2;
 
 // Q8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
 // key's K and of its V with the key's scales. V turns into the dtype's elements,
-// exactly, where it is stored to LDS; K stays codes, and its products with the queries
-// are code products, the queries being QP pieces of codes each. From the scores on the
-// walk is the same.
+// exactly, where it is stored to LDS. In bf16 K stays codes, and its products with the
+// queries are code products, the queries being QP pieces of codes each. In fp16 K turns
+// into fp16 too, the queries being two pieces of fp16: a code product keeps some 17 bits
+// of the largest number in a sum, which shows in a score of a hundred (rows of such
+// scores 0.0012 off in fp16, whose rounding is 0.0002). From the scores on the walk is the same.
 template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false, int QP = 2>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
@@ -202,10 +204,12 @@ void paged_prefill_kernel(PrefillArgs a) {
   constexpr int EB = 2;
   constexpr int CT = S::CT, BN = S::BN, NT = S::NT;
   constexpr int RING = SCHED == kRing2 ? 2 : 3;
+  constexpr bool QC = Q8 && DT == IR_DTYPE_BF16;  // keys stay codes
+  constexpr bool Q2 = Q8 && !QC;                  // queries in two pieces of the dtype
   constexpr int CROW = D + 16;  // bytes per key row of codes in LDS (16 rows apart without bank conflicts)
-  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][Q8 ? BN * CROW / 2 : BN * S::KROW];
+  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][QC ? BN * CROW / 2 : BN * S::KROW];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[RING][BN * S::KROW];
-  __shared__ int ke_lds[Q8 ? RING : 1][4];  // Q8: exponents of the scales of a tile's 16-key runs
+  __shared__ int ke_lds[QC ? RING : 1][4];  // QC: exponents of the scales of a tile's 16-key runs
   __shared__ int32_t bt_lds[kBtCache];
 
   const int tid = threadIdx.x;
@@ -289,20 +293,32 @@ void paged_prefill_kernel(PrefillArgs a) {
   // and scales it once its first key tile is staged, so Q's round trip
   // overlaps the block ids' and the first tile's instead of preceding them.
   constexpr bool EARLY = NW == 8 && CT == 1 && SCHED == kRing2;
-  // Q8: a query times scale * log2 e is the sum of QP pieces of e4m3 codes, piece p times
+  // QC: a query times scale * log2 e is the sum of QP pieces of e4m3 codes, piece p times
   // 2^(e - 4 p): each takes four bits of what the ones before leave. Two are off by at most
   // 2^-9 of an element's power of two, half of what rounding to bf16 would be, three by
-  // 2^-14, which fp16 queries and fp32 ones (normed rows as they left the rotation) take:
-  // an error of a query is one of all its scores (four 256-token chunks, 32 / 4 heads of
-  // 128: 39.6 us in two pieces from bf16, 42.8 in three from fp32; the outputs' error in a
-  // step that norms its queries 0.0033 -> 0.0022 of their size, 0.0017 being the rounding
-  // of the outputs alone). At head_dim 64 one product of 128
-  // k-slots holds two pieces, the codes of K twice; at 128 it holds one.
+  // 2^-14, which fp32 queries (normed rows as they left the rotation) take: an error of a
+  // query is one of all its scores (four 256-token chunks, 32 / 4 heads of 128: 39.6 us in
+  // two pieces from bf16, 42.8 in three from fp32; the outputs' error in a step that norms
+  // its queries 0.0033 -> 0.0022 of their size, 0.0017 being the rounding of the outputs
+  // alone). At head_dim 64 one product of 128 k-slots holds two pieces, the codes of K
+  // twice; at 128 it holds one.
   constexpr int NP = D == 128 ? QP : (QP + 1) / 2;  // products of a score
-  u32x4 qreg[CT][S::KS];
+  u32x4 qreg[CT][S::KS], qrest[Q2 ? CT : 1][S::KS];
   i32x8 qc[CT][NP];
   int qe[CT][NP];
   auto split_query = [&](int ct, float (&v)[S::KS * 8]) {
+    if constexpr (Q2) {  // off by 2^-22 of an element
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = v[8 * ks + 2 * i] * a.scale_log2, y = v[8 * ks + 2 * i + 1] * a.scale_log2;
+          const uint32_t hi = Elem<DT>::pack2(x, y);
+          qreg[ct][ks][i] = hi;
+          qrest[ct][ks][i] = Elem<DT>::pack2(x - Elem<DT>::lo(hi), y - Elem<DT>::hi(hi));
+        }
+      return;
+    }
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < S::KS * 8; ++i) {
@@ -350,16 +366,17 @@ void paged_prefill_kernel(PrefillArgs a) {
       }
     split_query(ct, v);
   };
-  // the lane's elements of a query row, ks-th eight: with codes, the k-slots of lane
+  // the lane's elements of a query row, ks-th eight: with QC, the k-slots of lane
   // group g are the 16-code chunks g and g + 4 of the row
-  auto q_at = [&](int ks) { return Q8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : ks * 32 + 8 * g; };
-  const bool wide_q = QP == 3 && a.q_f32;  // (uniform)
+  auto q_at = [&](int ks) { return QC ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : ks * 32 + 8 * g; };
+  constexpr bool WIDE = Q2 || QP == 3;  // takes fp32 queries
+  const bool wide_q = WIDE && a.q_f32;   // (uniform)
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const Col col = column(ct);
     const int64_t q_off =
         (int64_t)(q_lo + (col.ok ? col.tok : 0)) * a.q_tok + (int64_t)(col.ok ? col.head : 0) * a.q_head;
-    if constexpr (QP == 3) {
+    if constexpr (WIDE) {
       if (wide_q) {
         float v[S::KS * 8];
 #pragma unroll
@@ -504,13 +521,20 @@ void paged_prefill_kernel(PrefillArgs a) {
         const f32x2 s2 = Q8 && ku[i] ? sc[i] : f32x2{1.f, 1.f};
         uint16_t* vp = &vs_lds[buf][key * S::KROW + part * PE];
         if constexpr (Q8) {
-          *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
-          if (part == 0 && (key & 15) == 0) ke_lds[buf][key >> 4] = (int)(__float_as_uint(s2[0]) >> 23);
+          auto wide = [](uint16_t* to, u32x4 x, float scale) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            *(u32x4*)(vp + 8 * h) =
-                u32x4{decode2<DT, false>(v4[2 * h], s2[1]), decode2<DT, true>(v4[2 * h], s2[1]),
-                      decode2<DT, false>(v4[2 * h + 1], s2[1]), decode2<DT, true>(v4[2 * h + 1], s2[1])};
+            for (int h = 0; h < 2; ++h)
+              *(u32x4*)(to + 8 * h) =
+                  u32x4{decode2<DT, false>(x[2 * h], scale), decode2<DT, true>(x[2 * h], scale),
+                        decode2<DT, false>(x[2 * h + 1], scale), decode2<DT, true>(x[2 * h + 1], scale)};
+          };
+          if constexpr (QC) {
+            *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
+            if (part == 0 && (key & 15) == 0) ke_lds[buf][key >> 4] = (int)(__float_as_uint(s2[0]) >> 23);
+          } else {
+            wide(&ks_lds[buf][key * S::KROW + part * PE], k4, s2[0]);
+          }
+          wide(vp, v4, s2[1]);
         } else {
           *(u32x4*)&ks_lds[buf][key * S::KROW + part * PE] = k4;
           *(u32x4*)vp = v4;
@@ -558,9 +582,12 @@ void paged_prefill_kernel(PrefillArgs a) {
   auto qk_step = [&](const uint16_t* kb_lds, int kt, int ks, f32x4 (&x)[CT][4]) {
     const u32x4 ka = *(const u32x4*)&kb_lds[(kt * 16 + c) * S::KROW + ks * 32 + 8 * g];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) x[ct][kt] = mfma_k32<DT>(ka, qreg[ct][ks], x[ct][kt]);
+    for (int ct = 0; ct < CT; ++ct) {
+      x[ct][kt] = mfma_k32<DT>(ka, qreg[ct][ks], x[ct][kt]);
+      if constexpr (Q2) x[ct][kt] = mfma_k32<DT>(ka, qrest[ct][ks], x[ct][kt]);
+    }
   };
-  // Q8: all of key tile kt's scores from the codes staged in buffer buf.
+  // QC: all of key tile kt's scores from the codes staged in buffer buf.
   auto qk_codes = [&](int buf, int kt, f32x4 (&x)[CT][4]) {
     const uint8_t* row = (const uint8_t*)ks_lds[buf] + (kt * 16 + c) * CROW + 16 * g;
     const u32x4 k0 = *(const u32x4*)row;
@@ -752,7 +779,7 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
-        if constexpr (Q8) {
+        if constexpr (QC) {
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
         } else {
@@ -789,7 +816,7 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
-        if constexpr (Q8) {
+        if constexpr (QC) {
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
         } else {
@@ -1995,8 +2022,8 @@ int prefill_call(const char* name, const float* scales, int q_dtype, const void*
   hipStream_t s = (hipStream_t)stream;
   if (scales && !f32) {
     if (dtype == IR_DTYPE_F16)
-      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_F16, 128, 3>(a, s)
-                             : launch_prefill_q8<IR_DTYPE_F16, 64, 3>(a, s);
+      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_F16, 128, 2>(a, s)
+                             : launch_prefill_q8<IR_DTYPE_F16, 64, 2>(a, s);
     if (a.q_f32)
       return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128, 3>(a, s)
                              : launch_prefill_q8<IR_DTYPE_BF16, 64, 3>(a, s);
