@@ -480,6 +480,27 @@ def test_prefill_of_queries_of_any_size(dtype, d):
     assert out[spoiled].isnan().any(-1).all()
 
 
+# Scores of some hundred: what is lost of them is lost of every probability. In the mean over
+# many outputs a rounding to nearest is off by at most u / sqrt(3) of a number, and the
+# probabilities and the output are rounded once each: sqrt(2 / 3) u, and 10% for the fp32
+# sums and for rows where the values cancel.
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_of_large_scores_in_fp16(d):
+    bs, hq, h, n, cached = 16, 6, 2, 90, 1500
+    pool, tables, values = filled(35, torch.float16, [cached + n], h, d, bs)
+    q = (12.0 * torch.randn(n, hq, d, generator=gen(15), device=DEV)).half()
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    start = torch.tensor([cached], dtype=torch.int32, device=DEV)
+    bt = device_tables(tables)
+    o, _, reach = quant.attend(q, values, tables[0], bs, cached, d**-0.5)
+    assert reach.max() > 200
+    for plan in (None, kernels.prefill_plan(cu, start, bt, n, n, bs, hq, h, d, dtype=torch.float16)):
+        out = kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, start, n, bs, d**-0.5, plan=plan,
+                                    kv_scales=pool.kv_scales[0])
+        off = (out.double().cpu() - o).norm() / o.norm()
+        assert off <= 1.1 * (2 / 3) ** 0.5 * 2.0**-11, off
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_prefill_over_many_workgroups_and_wide_groups(dtype):
     """More workgroups than the device holds, cut items; 8-wavefront workgroups (more than
