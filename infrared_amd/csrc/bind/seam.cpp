@@ -430,7 +430,8 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
     require(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == n && t->size(1) == d && t->stride(1) == 1,
             name, ": ", which, " must be fp32 [N, D] with unit column stride");
   require(cos.stride(0) == sin.stride(0), name, ": cos and sin must share strides");
-  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name, ": slots must be int64 [N]");
+  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name,
+          ": slots must be int64 [N]");
   unit_last(name, q);
   unit_last(name, k);
   unit_last(name, v);

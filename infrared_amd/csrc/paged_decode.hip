@@ -446,7 +446,8 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
                                int32_t* counters, int64_t num_counters, void* workspace,
                                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   return decode_call("ir_paged_decode", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
-                     cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
+                     cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride,
+                     max_blocks_per_seq,
                      context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
                      scale, dtype, partition_tokens, counters, num_counters, workspace, workspace_bytes, err_flags,
                      stream);

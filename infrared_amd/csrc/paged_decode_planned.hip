@@ -1175,7 +1175,8 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
                                        int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   return planned_call("ir_paged_decode_planned", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                       cache_slot_stride, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads,
-                      head_dim, max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
+                      head_dim, max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters,
+                      workspace,
                       workspace_bytes, err_flags, stream);
 }
 
@@ -1184,7 +1185,8 @@ extern "C" int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, i
                                           out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int
                                           num_kv_heads, int head_dim, int max_blocks_per_seq, int block_size, float
                                           scale, int dtype, int q_dtype, int flags, const void* plan, int32_t*
-                                          counters, int64_t num_counters, void* workspace, int64_t workspace_bytes, int32_t* err_flags,
+                                          counters, int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                                          int32_t* err_flags,
                                           ir_stream_t stream) {
   IR_REQUIRE(scales, "ir_paged_decode_planned_q8: null pointer");
   return planned_call("ir_paged_decode_planned_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,

@@ -2051,7 +2051,8 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
                                 int64_t v_new_tok_stride, int64_t v_new_head_stride, const int64_t* write_slots,
                                 int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
   return prefill_call("ir_paged_prefill", nullptr, dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
-                      cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride, max_blocks_per_seq,
+                      cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride,
+                      max_blocks_per_seq,
                       cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride, out_head_stride,
                       num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, k_new, k_new_tok_stride,
                       k_new_head_stride, v_new, v_new_tok_stride, v_new_head_stride, write_slots, n_write, src_row0,
