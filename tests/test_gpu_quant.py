@@ -582,6 +582,26 @@ def test_fp32_queries_of_a_16_bit_pool(path, dtype, hq, h, d, bs):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq, h, d, bs", [(28, 4, 128, 16), (14, 2, 64, 32)])
+def test_fp32_queries_of_sequences_that_share_blocks(dtype, hq, h, d, bs):
+    """The planned decode's pairs, whose units hold the queries of two sequences."""
+    pool, tables, values = filled(44, dtype, [700, 40, 530], h, d, bs)
+    use, lens = [0, 0, 1, 2, 2, 0], [700, 655, 33, 1, 530, 90]
+    q = torch.randn(len(lens), hq, d, generator=gen(45), device=DEV)
+    bt = device_tables([tables[i] for i in use])
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    plan = kernels.decode_plan(bt, ctx, hq, pool.k[0], bs, share_groups=True)
+    out = kernels.paged_decode_planned(q, pool.k[0], pool.v[0], plan, d**-0.5, err_flags=pool.err_flags,
+                                       out=torch.empty_like(q, dtype=dtype), kv_scales=pool.kv_scales[0])
+    pool.check_errors()
+    for i, n in enumerate(lens):
+        o, a, reach = quant.attend(q[i : i + 1], values, tables[use[i]], bs, n - 1, d**-0.5)
+        tol = fp32_tolerance(o, a, reach, d) + decode_tolerance(o, a, dtype) + 4 * 2.0**-13 * reach[..., None] * a
+        err = (out[i : i + 1].double().cpu() - o).abs()
+        assert (err <= tol).all(), (i, n, (err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("hq, h, d, bs", [(28, 4, 128, 16), (5, 5, 64, 32)])
 def test_rotated_queries_in_fp32(dtype, hq, h, d, bs):
     """What the dtype's own output is the rounding of; without norms the same numbers."""
