@@ -52,15 +52,18 @@ __device__ __forceinline__ f32x2 decode2_f32(uint32_t w, float scale) {
   return __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, HI));
 }
 
-// D += A . B of 128 e4m3 codes a row and column (16 rows, 16 columns): 32 codes of A and
-// of B per lane, of scales 2^(ea - 127) and 2^(eb - 127). The k-slots of lane group g
-// are [16 g, +16) in the first four registers and [64 + 16 g, +16) in the last four, and
-// the scale of k-slots [32 b, +32) is the one that lane group b gives (both measured).
-// The instruction sums eight products at a time aligned to the largest of them, some 17
-// bits below which are lost (measured: 1 next to 448^2), and these sums in fp32.
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ f32x4 mfma_codes_k128(i32x8 a, int ea, i32x8 b, int eb, f32x4 c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, ea, 0, eb);
+// The power of two that brings a row's largest magnitude to [2^14, 2^15), where fp16 has
+// the most room below it (k in [-113, 126], so that 2^k and 2^-k are normal numbers).
+__device__ __forceinline__ int row_shift(float most) { return max(-113, min(126, 14 - exponent_of(most))); }
+
+// a and b, fp32, in two pieces of dtype DT each: hi their rounding, lo that of what it leaves.
+struct Pieces {
+  uint32_t hi, lo;
+};
+template <int DT>
+__device__ __forceinline__ Pieces split2(float a, float b) {
+  const uint32_t hi = Elem<DT>::pack2(a, b);
+  return {hi, Elem<DT>::pack2(a - Elem<DT>::lo(hi), b - Elem<DT>::hi(hi))};
 }
 
 }  // namespace ir

@@ -125,7 +125,6 @@ struct PrefillArgs {
   int64_t n_work;  // attending workgroups (the grid less the writers)
   // 8-bit caches: (K, V) scales [kv head][block] (null: the caches are of the dtype)
   const f32x2* scales;
-  int q_f32;  // 8-bit caches: q is fp32, whatever the dtype
 };
 
 // 16-byte pieces a writer lane moves, all loads in flight before any store.
@@ -191,25 +190,22 @@ struct PShape {
 constexpr int kLockstep = 0, kRing2 = 2;
 
 // Q8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
-// key's K and of its V with the key's scales. V turns into the dtype's elements,
-// exactly, where it is stored to LDS. In bf16 K stays codes, and its products with the
-// queries are code products, the queries being QP pieces of codes each. In fp16 K turns
-// into fp16 too, the queries being two pieces of fp16: a code product keeps some 17 bits
-// of the largest number in a sum, which shows in a score of a hundred (rows of such
-// scores 0.0012 off in fp16, whose rounding is 0.0002). From the scores on the walk is the same.
-template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false, int QP = 2>
+// key's K and of its V with the key's scales, which turn into the dtype's elements,
+// exactly, where they are stored to LDS. The queries are used as they are given, in QP
+// pieces of the dtype: one for queries of it, so that a score is the sum of exact products in
+// fp32, two for fp32 queries (below). scale * log2 e is multiplied with a score less the
+// running maximum, in fp32, where its exponential is taken.
+template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false, int QP = 1>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
   typedef PShape<D, NW, CTW> S;
   constexpr int EB = 2;
   constexpr int CT = S::CT, BN = S::BN, NT = S::NT;
   constexpr int RING = SCHED == kRing2 ? 2 : 3;
-  constexpr bool QC = Q8 && DT == IR_DTYPE_BF16;  // keys stay codes
-  constexpr bool Q2 = Q8 && !QC;                  // queries in two pieces of the dtype
-  constexpr int CROW = D + 16;  // bytes per key row of codes in LDS (16 rows apart without bank conflicts)
-  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][QC ? BN * CROW / 2 : BN * S::KROW];
+  constexpr bool WIDE = QP == 2;  // fp32 queries of a 16-bit pool
+  static_assert(Q8 || !WIDE, "16-bit caches take queries of their dtype");
+  __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][BN * S::KROW];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[RING][BN * S::KROW];
-  __shared__ int ke_lds[QC ? RING : 1][4];  // QC: exponents of the scales of a tile's 16-key runs
   __shared__ int32_t bt_lds[kBtCache];
 
   const int tid = threadIdx.x;
@@ -293,107 +289,46 @@ void paged_prefill_kernel(PrefillArgs a) {
   // and scales it once its first key tile is staged, so Q's round trip
   // overlaps the block ids' and the first tile's instead of preceding them.
   constexpr bool EARLY = NW == 8 && CT == 1 && SCHED == kRing2;
-  // QC: a query times scale * log2 e is the sum of QP pieces of e4m3 codes, piece p times
-  // 2^(e - 4 p): each takes four bits of what the ones before leave. Two are off by at most
-  // 2^-9 of an element's power of two, half of what rounding to bf16 would be, three by
-  // 2^-14, which fp32 queries (normed rows as they left the rotation) take: an error of a
-  // query is one of all its scores (four 256-token chunks, 32 / 4 heads of 128: 39.6 us in
-  // two pieces from bf16, 42.8 in three from fp32; the outputs' error in a step that norms
-  // its queries 0.0033 -> 0.0022 of their size, 0.0017 being the rounding of the outputs
-  // alone). At head_dim 64 one product of 128 k-slots holds two pieces, the codes of K
-  // twice; at 128 it holds one.
-  constexpr int NP = D == 128 ? QP : (QP + 1) / 2;  // products of a score
-  u32x4 qreg[CT][S::KS], qrest[Q2 ? CT : 1][S::KS];
-  i32x8 qc[CT][NP];
-  int qe[CT][NP];
-  auto split_query = [&](int ct, float (&v)[S::KS * 8]) {
-    if constexpr (Q2) {  // off by 2^-22 of an element
-#pragma unroll
-      for (int ks = 0; ks < S::KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = v[8 * ks + 2 * i] * a.scale_log2, y = v[8 * ks + 2 * i + 1] * a.scale_log2;
-          const uint32_t hi = Elem<DT>::pack2(x, y);
-          qreg[ct][ks][i] = hi;
-          qrest[ct][ks][i] = Elem<DT>::pack2(x - Elem<DT>::lo(hi), y - Elem<DT>::hi(hi));
-        }
-      return;
-    }
-    float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < S::KS * 8; ++i) {
-      v[i] *= a.scale_log2;
-      most = fmaxf(most, fabsf(v[i]));
-    }
-    most = wave_max_groups_swap(most);
-    const int e = scale_exponent<IR_DTYPE_BF16>(most);
-    // (an infinite query becomes NaN, not a large number; NaN does by itself)
-    const int bad = __float_as_uint(most) >= 0x7f800000u ? 0x7f7f7f7f : 0;
-    typedef short i16x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < S::KS * 2; ++i) {  // four elements
-      float x[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-#pragma unroll
-      for (int p = 0; p < (D == 128 ? QP : 2 * NP); ++p) {
-        i16x2 h = {0, 0};
-        if (p < QP) {
-          const float s = pow2(e - 4 * p);
-          h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[0], x[1], s, false);
-          h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[2], x[3], s, true);
-          const uint32_t hw = __builtin_bit_cast(uint32_t, h);
-          const f32x2 r0 = decode2_f32<false>(hw, s), r1 = decode2_f32<true>(hw, s);
-          x[0] -= r0[0];
-          x[1] -= r0[1];
-          x[2] -= r1[0];
-          x[3] -= r1[1];
-        }
-        const int word = __builtin_bit_cast(int, h) | (p == 0 ? bad : 0);
-        if constexpr (D == 128) qc[ct][p][i] = word;
-        else qc[ct][p / 2][4 * (p & 1) + i] = word;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NP; ++j) qe[ct][j] = 127 + (D == 128 ? e - 4 * j : e - 8 * j - (g < 2 ? 0 : 4));
-  };
-  auto split_raw = [&](int ct) {
-    float v[S::KS * 8];
-#pragma unroll
-    for (int ks = 0; ks < S::KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[8 * ks + 2 * i] = Elem<DT>::lo(qreg[ct][ks][i]);
-        v[8 * ks + 2 * i + 1] = Elem<DT>::hi(qreg[ct][ks][i]);
-      }
-    split_query(ct, v);
-  };
-  // the lane's elements of a query row, ks-th eight: with QC, the k-slots of lane
-  // group g are the 16-code chunks g and g + 4 of the row
-  auto q_at = [&](int ks) { return QC ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : ks * 32 + 8 * g; };
-  constexpr bool WIDE = Q2 || QP == 3;  // takes fp32 queries
-  const bool wide_q = WIDE && a.q_f32;   // (uniform)
+  // WIDE: a row of fp32 queries is multiplied by the power of two that brings its largest
+  // magnitude to [2^14, 2^15), and held in two pieces of the dtype, its rounded value and what
+  // that leaves: off by 2^-18 of an element in bf16; in fp16 by 2^-24 of it or, where the pieces
+  // are subnormal, 2^-39 of the row's largest. unit takes the power back.
+  u32x4 qreg[CT][S::KS], qrest[WIDE ? CT : 1][S::KS];
+  float unit[CT];  // Q8: factor of a column's scores to base-2 exponents
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const Col col = column(ct);
     const int64_t q_off =
         (int64_t)(q_lo + (col.ok ? col.tok : 0)) * a.q_tok + (int64_t)(col.ok ? col.head : 0) * a.q_head;
+    unit[ct] = a.scale_log2;
     if constexpr (WIDE) {
-      if (wide_q) {
-        float v[S::KS * 8];
+      float v[S::KS * 8], most = 0.f;
 #pragma unroll
-        for (int i = 0; i < S::KS * 2; ++i) {
-          const f32x4 x = *(const f32x4*)((const float*)a.q + q_off + q_at(i >> 1) + 4 * (i & 1));
+      for (int i = 0; i < S::KS * 2; ++i) {
+        const f32x4 x = *(const f32x4*)((const float*)a.q + q_off + 32 * (i >> 1) + 8 * g + 4 * (i & 1));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[4 * i + j] = col.ok ? x[j] : 0.f;
+        for (int j = 0; j < 4; ++j) {
+          v[4 * i + j] = col.ok ? x[j] : 0.f;
+          most = fmaxf(most, fabsf(v[4 * i + j]));
         }
-        split_query(ct, v);
-        continue;
       }
+      const int up = row_shift(wave_max_groups_swap(most));
+      unit[ct] = fmaxf(unit[ct] * pow2(-up), __FLT_MIN__);  // (not 0: a masked score is infinite)
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Pieces p = split2<DT>(v[8 * ks + 2 * i] * pow2(up), v[8 * ks + 2 * i + 1] * pow2(up));
+          qreg[ct][ks][i] = p.hi;
+          qrest[ct][ks][i] = p.lo;
+        }
+      continue;
     }
     const uint16_t* qrow = (const uint16_t*)a.q + q_off;
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
       if constexpr (EARLY || Q8) {
-        const u32x4 x = *(const u32x4*)(qrow + q_at(ks));  // (a valid row when !col.ok)
+        const u32x4 x = *(const u32x4*)(qrow + ks * 32 + 8 * g);  // (a valid row when !col.ok)
         qreg[ct][ks] = col.ok ? x : u32x4{0u, 0u, 0u, 0u};
       } else {
         const u32x4 x = col.ok ? *(const u32x4*)(qrow + ks * 32 + 8 * g) : u32x4{0u, 0u, 0u, 0u};
@@ -402,7 +337,6 @@ void paged_prefill_kernel(PrefillArgs a) {
           qreg[ct][ks][e] = Elem<DT>::pack2(Elem<DT>::lo(x[e]) * a.scale_log2, Elem<DT>::hi(x[e]) * a.scale_log2);
       }
     }
-    if constexpr (Q8 && !EARLY) split_raw(ct);
   }
 
   // ---- block-id cache: ids [bt_base, bt_base + kBtCache) of this sequence
@@ -519,6 +453,7 @@ void paged_prefill_kernel(PrefillArgs a) {
         const int key = q / (D / PE), part = q % (D / PE);
         const u32x4 k4 = zero_unless(kr[i], ku[i]), v4 = zero_unless(vr[i], ku[i]);
         const f32x2 s2 = Q8 && ku[i] ? sc[i] : f32x2{1.f, 1.f};
+        uint16_t* kp = &ks_lds[buf][key * S::KROW + part * PE];
         uint16_t* vp = &vs_lds[buf][key * S::KROW + part * PE];
         if constexpr (Q8) {
           auto wide = [](uint16_t* to, u32x4 x, float scale) {
@@ -528,15 +463,10 @@ void paged_prefill_kernel(PrefillArgs a) {
                   u32x4{decode2<DT, false>(x[2 * h], scale), decode2<DT, true>(x[2 * h], scale),
                         decode2<DT, false>(x[2 * h + 1], scale), decode2<DT, true>(x[2 * h + 1], scale)};
           };
-          if constexpr (QC) {
-            *(u32x4*)((uint8_t*)ks_lds[buf] + key * CROW + part * PE) = k4;
-            if (part == 0 && (key & 15) == 0) ke_lds[buf][key >> 4] = (int)(__float_as_uint(s2[0]) >> 23);
-          } else {
-            wide(&ks_lds[buf][key * S::KROW + part * PE], k4, s2[0]);
-          }
+          wide(kp, k4, s2[0]);
           wide(vp, v4, s2[1]);
         } else {
-          *(u32x4*)&ks_lds[buf][key * S::KROW + part * PE] = k4;
+          *(u32x4*)kp = k4;
           *(u32x4*)vp = v4;
         }
       }
@@ -560,7 +490,7 @@ void paged_prefill_kernel(PrefillArgs a) {
   };
 
   // ---- online softmax state, per column tile: lane owns column c of it.
-  // negm[ct] holds -m (the running base-2 max, 0 before the first tile) in
+  // negm[ct] holds -m (the running base-2 max, in Q8 that of the products; 0 before the first tile) in
   // all four slots: it is the accumulator a tile's score MFMAs start from, so
   // the scores arrive as s - m and need only the exponential.
   f32x4 acc[CT][S::DTL], negm[CT];
@@ -584,20 +514,8 @@ void paged_prefill_kernel(PrefillArgs a) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       x[ct][kt] = mfma_k32<DT>(ka, qreg[ct][ks], x[ct][kt]);
-      if constexpr (Q2) x[ct][kt] = mfma_k32<DT>(ka, qrest[ct][ks], x[ct][kt]);
+      if constexpr (WIDE) x[ct][kt] = mfma_k32<DT>(ka, qrest[ct][ks], x[ct][kt]);
     }
-  };
-  // QC: all of key tile kt's scores from the codes staged in buffer buf.
-  auto qk_codes = [&](int buf, int kt, f32x4 (&x)[CT][4]) {
-    const uint8_t* row = (const uint8_t*)ks_lds[buf] + (kt * 16 + c) * CROW + 16 * g;
-    const u32x4 k0 = *(const u32x4*)row;
-    const u32x4 k1 = D == 128 ? *(const u32x4*)(row + 64) : k0;
-    const i32x8 ka = {(int)k0[0], (int)k0[1], (int)k0[2], (int)k0[3], (int)k1[0], (int)k1[1], (int)k1[2], (int)k1[3]};
-    const int ke = ke_lds[buf][kt];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int i = 0; i < NP; ++i) x[ct][kt] = mfma_codes_k128(ka, ke, qc[ct][i], qe[ct][i], x[ct][kt]);
   };
   auto zero_s = [](f32x4 (&x)[CT][4]) {
 #pragma unroll
@@ -635,11 +553,11 @@ void paged_prefill_kernel(PrefillArgs a) {
       for (int kt = 0; kt < 4; ++kt)
         mx = fmaxf(mx, fmaxf(fmaxf(cur[ct][kt][0], cur[ct][kt][1]), fmaxf(cur[ct][kt][2], cur[ct][kt][3])));
       mx = wave_max_groups_swap(mx);  // relative to m; finite on the first tile (key 0 is always visible)
-      const bool grow = first || mx > kRescaleSlack;
+      const bool grow = first || (Q8 ? mx * unit[ct] : mx) > kRescaleSlack;
       if (__any(grow)) {
         const float d = grow ? mx : 0.f;  // the max moves up by d
         if (!first) {
-          const float alpha = fast_exp2(-d);
+          const float alpha = fast_exp2(Q8 ? -d * unit[ct] : -d);
           l[ct] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < S::DTL; ++dt) acc[ct][dt] *= alpha;
@@ -661,11 +579,11 @@ void paged_prefill_kernel(PrefillArgs a) {
     // Program order is kept step by step (sched_barrier): each step's K operand
     // was read one step earlier, its MFMAs go to the matrix pipe and the
     // exponentials of SPS scores fill the VALU meanwhile.
-    // Q8: the wavefront in its exponentials goes first. Two workgroups share a CU, and
-    // the one in its products has the matrix pipe to itself either way, while the other
-    // would be held up by the operand reads between them (8 chunks of 512 tokens: 303 us
-    // without, 267 so; priority for the products instead 272..283).
-    if constexpr (Q8) __builtin_amdgcn_s_setprio(1);
+    // Q8: a wavefront in its products, or on the way to them, goes before one in its
+    // exponentials. Two workgroups share a CU, and the matrix pipe runs on while the VALU is the
+    // other's (8 chunks of 512 tokens, 28 / 4 heads of 128: 338 us without, 333 the other way
+    // round, 305 so; 325 with the stores of the next tile to LDS at low priority too).
+    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
     constexpr int NQK = 4 * S::KS, SPS = CT * 16 / NQK;
     auto k_operand = [&](int t) {
       return *(const u32x4*)&kn[((t % 4) * 16 + c) * S::KROW + (t / 4) * 32 + 8 * g];
@@ -685,7 +603,7 @@ void paged_prefill_kernel(PrefillArgs a) {
       for (int j = 0; j < SPS; ++j) {
         const int i = t * SPS + j;
         const int ct = i / 16, kt = (i % 16) / 4, r = i % 4;
-        cur[ct][kt][r] = fast_exp2(cur[ct][kt][r]);
+        cur[ct][kt][r] = fast_exp2(Q8 ? cur[ct][kt][r] * unit[ct] : cur[ct][kt][r]);
       }
       // (no scheduling barrier)
     }
@@ -712,7 +630,7 @@ void paged_prefill_kernel(PrefillArgs a) {
     auto v_operand = [&](int t) {
       return v_operand_tr(vb_lds, t);
     };
-    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
+    if constexpr (Q8) __builtin_amdgcn_s_setprio(1);
     u32x4 vring[kOperandAhead];
 #pragma unroll
     for (int t = 0; t < kOperandAhead; ++t) vring[t] = v_operand(t);
@@ -755,10 +673,7 @@ void paged_prefill_kernel(PrefillArgs a) {
       __syncthreads();
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        if constexpr (Q8) {
-          if (!wide_q) split_raw(ct);
-          continue;
-        }
+        if constexpr (Q8) continue;
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
           const u32x4 x = qreg[ct][ks];
@@ -779,13 +694,8 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
-        if constexpr (QC) {
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
-        }
+        for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
         step(std::false_type{}, kb, sc, sc);
         if (kb + 1 < t_hi)
           store_from((kb + 1) & 1, kr[(J + 1) % R], vr[(J + 1) % R], sc8[(J + 1) % R], ku[(J + 1) % R]);
@@ -816,13 +726,8 @@ void paged_prefill_kernel(PrefillArgs a) {
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt) sc[ct][kt] = negm[ct];
-        if constexpr (QC) {
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt) qk_codes(kb & 1, kt, sc);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
-        }
+        for (int t = 0; t < 4 * S::KS; ++t) qk_step(ks_lds[kb & 1], t % 4, t / 4, sc);
         step(std::false_type{}, kb, sc, sc);
         if (kb + 1 < t_hi) store_regs((kb + 1) & 1);
         if (kb + 2 < t_hi) load_regs(kb + 2);
@@ -912,13 +817,14 @@ void paged_prefill_kernel(PrefillArgs a) {
   const int row_step = a.num_kv_heads * COLS;  // rows between parts of one item
   const int row_base = (pbase * a.num_kv_heads + kvh) * COLS;  // part 0, column 0
   float lsum[CT];
+  auto top = [&](int qt) { return Q8 ? -negm[qt][0] * unit[qt] : -negm[qt][0]; };  // in base 2
 #pragma unroll
   for (int qt = 0; qt < CT; ++qt) {
     lsum[qt] = wave_sum_groups_swap(l[qt]);
     const int row = row_base + part * row_step + w * (CT * 16) + qt * 16 + c;
 #pragma unroll
     for (int dt = 0; dt < S::DTL; ++dt) store_dev4(r_o, (row * D + dt * 16 + 4 * g) * 4, acc[qt][dt]);
-    if (g == 0) store_dev2(r_ml, row * 8, f32x2{-negm[qt][0], lsum[qt]});
+    if (g == 0) store_dev2(r_ml, row * 8, f32x2{top(qt), lsum[qt]});
   }
   __shared__ int s_last;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -946,7 +852,7 @@ void paged_prefill_kernel(PrefillArgs a) {
     if (p == part) {
 #pragma unroll
       for (int qt = 0; qt < CT; ++qt) {
-        mp[qt] = -negm[qt][0];
+        mp[qt] = top(qt);
         lp[qt] = lsum[qt];
 #pragma unroll
         for (int dt = 0; dt < S::DTL; ++dt) op[qt][dt] = acc[qt][dt];
@@ -2011,7 +1917,6 @@ int prefill_call(const char* name, const float* scales, int q_dtype, const void*
     a.src_row0 = src_row0;
   }
   a.scales = (const f32x2*)scales;
-  a.q_f32 = q_dtype == IR_DTYPE_F32;
   a.out = out;
   a.o_tok = out_tok_stride;
   a.o_head = out_head_stride;
@@ -2021,14 +1926,12 @@ int prefill_call(const char* name, const float* scales, int q_dtype, const void*
   a.err = err_flags;
   hipStream_t s = (hipStream_t)stream;
   if (scales && !f32) {
-    if (dtype == IR_DTYPE_F16)
-      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_F16, 128, 2>(a, s)
-                             : launch_prefill_q8<IR_DTYPE_F16, 64, 2>(a, s);
-    if (a.q_f32)
-      return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128, 3>(a, s)
-                             : launch_prefill_q8<IR_DTYPE_BF16, 64, 3>(a, s);
-    return head_dim == 128 ? launch_prefill_q8<IR_DTYPE_BF16, 128, 2>(a, s)
-                           : launch_prefill_q8<IR_DTYPE_BF16, 64, 2>(a, s);
+    const bool wide = q_dtype == IR_DTYPE_F32;
+#define IR_PREFILL_Q8(DT_, QP_) \
+  (head_dim == 128 ? launch_prefill_q8<DT_, 128, QP_>(a, s) : launch_prefill_q8<DT_, 64, QP_>(a, s))
+    if (dtype == IR_DTYPE_F16) return wide ? IR_PREFILL_Q8(IR_DTYPE_F16, 2) : IR_PREFILL_Q8(IR_DTYPE_F16, 1);
+    return wide ? IR_PREFILL_Q8(IR_DTYPE_BF16, 2) : IR_PREFILL_Q8(IR_DTYPE_BF16, 1);
+#undef IR_PREFILL_Q8
   }
   if (f32) return head_dim == 128 ? launch_prefill_f32<128>(a, s) : launch_prefill_f32<64>(a, s);
   if (dtype == IR_DTYPE_BF16)

@@ -70,10 +70,8 @@ class QuantCache:
                     self.exps[h, b, kv] = exp
 
 
-def attend(q: torch.Tensor, values: torch.Tensor, table, block_size: int, start: int, scale: float):
-    """Queries ``[n, H_q, D]`` at positions ``start ..`` over ``values`` ``[2, slots, H_kv, D]``
-    through a block table. Returns the output and, per (query, head), what bounds a
-    kernel's error: the attention over ``|V|`` and the largest ``scale * sum |q k|``."""
+def _scores(q: torch.Tensor, values: torch.Tensor, table, block_size: int, start: int, scale: float):
+    """Scores ``[H_q, n, T]`` (-inf where unseen), their ``scale * sum |q k|`` (0 there) and V ``[H_q, T, D]``."""
     n, hq, d = q.shape
     h_kv = values.shape[2]
     t = torch.arange(start + n)
@@ -82,9 +80,43 @@ def attend(q: torch.Tensor, values: torch.Tensor, table, block_size: int, start:
     x = q.cpu().double().transpose(0, 1)
     seen = t[None, :] <= torch.arange(start, start + n)[:, None]
     s = torch.where(seen, x @ k.transpose(1, 2) * scale, -torch.inf)
+    return s, torch.where(seen, x.abs() @ k.abs().transpose(1, 2) * scale, torch.zeros(())), v
+
+
+def attend(q: torch.Tensor, values: torch.Tensor, table, block_size: int, start: int, scale: float):
+    """Queries ``[n, H_q, D]`` at positions ``start ..`` over ``values`` ``[2, slots, H_kv, D]``
+    through a block table. Returns the output and, per (query, head), what bounds a
+    kernel's error: the attention over ``|V|`` and the largest ``scale * sum |q k|``."""
+    s, reach, v = _scores(q, values, table, block_size, start, scale)
     p = torch.softmax(s, -1)
-    reach = torch.where(seen, x.abs() @ k.abs().transpose(1, 2) * scale, torch.zeros(())).amax(-1)
-    return (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1), reach.transpose(0, 1)
+    return (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1), reach.amax(-1).transpose(0, 1)
+
+
+def attend_spread(q: torch.Tensor, values: torch.Tensor, table, block_size: int, start: int, scale: float):
+    """The output of ``attend`` and what errors of the keys' probabilities, each on its own
+    and relative to it, come to in an output: ``sqrt(sum p^2 v^2)``; with the largest
+    ``scale * sum |q k|``."""
+    s, reach, v = _scores(q, values, table, block_size, start, scale)
+    p = torch.softmax(s, -1)
+    return ((p @ v).transpose(0, 1), (p.square() @ v.square()).sqrt().transpose(0, 1),
+            reach.amax(-1).transpose(0, 1))
+
+
+def error_bound(o: torch.Tensor, spread: torch.Tensor, reach: torch.Tensor, dtype: torch.dtype,
+                round_p: float = 0.0) -> float:
+    """Bound of ``|out - o|`` in the norm over all elements, for outputs ``o`` of ``attend_spread``
+    rounded to ``dtype`` once, 5% above what the roundings come to:
+
+    - the output's own: that of ``o``;
+    - with ``round_p``, each probability's to ``dtype``, half a step u at most: uniform
+      within it, u / sqrt(3) in the mean square, times ``round_p``;
+    - fp32 sums: a score's partial sums are some reach / sqrt(d), d of them, so it is off by a step
+      or two of 2^-24 of ``reach``; the exponential and the sums over keys by a few dozen."""
+    u = torch.finfo(dtype).eps / 2
+    own = (o.to(dtype).double() - o).norm()
+    p = round_p * u / 3**0.5 * spread.norm()
+    fp32 = 2.0**-24 * (((32 + 2 * reach[..., None]) * spread).norm() + 32 * o.norm())
+    return float(1.05 * torch.sqrt(own**2 + p**2 + fp32**2))
 
 
 def norm_rope(x: torch.Tensor, w: torch.Tensor, eps: float, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:

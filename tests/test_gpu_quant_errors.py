@@ -1,0 +1,179 @@
+"""Errors of the 8-bit pool's attention in the norm over a sequence's outputs, which a wrong
+scale, a missing tile or a weight of a merge cannot hide in (``test_quant_errors.py`` shows
+that on the CPU), and what its queries and probabilities keep of their bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from infrared_amd import kernels
+from oracle import quant
+from test_gpu_quant import device_tables, filled, gen
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+HALF = [torch.bfloat16, torch.float16]
+
+
+def check(out, q, values, table, bs, cached, scale, dtype, round_p, what=None):
+    """A sequence's outputs within the bound of their roundings."""
+    o, spread, reach = quant.attend_spread(q, values, table, bs, cached, scale)
+    off, bound = float((out.double().cpu() - o).norm()), quant.error_bound(o, spread, reach, dtype, round_p)
+    assert off <= bound, (what, off / float(o.norm()), bound / float(o.norm()))
+
+
+def chunks(cached, new):
+    """Device metadata of packed chunks."""
+    cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    return cu, torch.tensor(cached, dtype=torch.int32, device=DEV)
+
+
+# ---- prefill: the probabilities and the output are rounded to the dtype, nothing else
+
+
+@pytest.mark.parametrize("plan", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq, h, d, bs", [(28, 4, 128, 16), (14, 2, 64, 16), (8, 8, 64, 64), (20, 1, 128, 48)])
+def test_prefill(plan, dtype, hq, h, d, bs):
+    cached, new = [0, 37, 0, 512, 1, 130], [1, 70, 200, 1, 0, 65]
+    pool, tables, values = filled(hq, dtype, [c + n for c, n in zip(cached, new)], h, d, bs)
+    total = sum(new)
+    q = torch.randn(total, 2 * hq, d, generator=gen(12), device=DEV).to(dtype)[:, :hq]
+    cu, start = chunks(cached, new)
+    bt = device_tables(tables)
+    p = kernels.prefill_plan(cu, start, bt, total, max(new), bs, hq, h, d, dtype=dtype) if plan else None
+    out = kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, start, max(new), bs, d**-0.5,
+                                err_flags=pool.err_flags, plan=p, kv_scales=pool.kv_scales[0])
+    pool.check_errors()
+    row = 0
+    for t, c, n in zip(tables, cached, new):
+        if n:
+            check(out[row : row + n], q[row : row + n], values, t, bs, c, d**-0.5, dtype, 1.0, (c, n))
+        row += n
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq, h", [(8, 4), (130, 1)])
+def test_prefill_over_many_workgroups_and_wide_groups(dtype, hq, h):
+    bs, d = 16, 64
+    cached, new = [6000, 0, 300], [700, 900, 257]
+    pool, tables, values = filled(31, dtype, [c + n for c, n in zip(cached, new)], h, d, bs)
+    total = sum(new)
+    q = torch.randn(total, hq, d, generator=gen(13), device=DEV).to(dtype)
+    cu, start = chunks(cached, new)
+    bt = device_tables(tables)
+    plan = kernels.prefill_plan(cu, start, bt, total, max(new), bs, hq, h, d, dtype=dtype)
+    heads = slice(0, hq) if hq <= 8 else slice(hq - 3, hq)  # (the oracle's cost)
+    for p in (plan, None):
+        out = kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, start, max(new), bs, d**-0.5, plan=p,
+                                    kv_scales=pool.kv_scales[0])
+        row = 0
+        for t, c, n in zip(tables, cached, new):
+            check(out[row : row + n, heads], q[row : row + n, heads], values, t, bs, c, d**-0.5, dtype, 1.0, (hq, c))
+            row += n
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_of_large_scores(d, dtype, wide):
+    """Scores of some hundred, of queries of the dtype and of fp32: what a query or a sum of
+    products loses shows in every probability."""
+    bs, hq, h, n, cached = 16, 6, 2, 90, 1500
+    pool, tables, values = filled(35, dtype, [cached + n], h, d, bs)
+    q = 12.0 * torch.randn(n, hq, d, generator=gen(15), device=DEV)
+    if not wide:
+        q = q.to(dtype)
+    cu, start = chunks([cached], [n])
+    bt = device_tables(tables)
+    for plan in (None, kernels.prefill_plan(cu, start, bt, n, n, bs, hq, h, d, dtype=dtype)):
+        out = torch.empty(n, hq, d, dtype=dtype, device=DEV)
+        kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, start, n, bs, d**-0.5, out=out, plan=plan,
+                              kv_scales=pool.kv_scales[0])
+        check(out, q, values, tables[0], bs, cached, d**-0.5, dtype, 1.0)
+
+
+# ---- queries that one element dwarfs
+
+
+def without_channel(seed, dtype, lens, h, d, bs, channel):
+    """``filled`` whose keys are zero in a channel."""
+    pool, tables, values = filled(seed, dtype, lens, h, d, bs)
+    raw = pool.k[0].view(torch.uint8)
+    written = (raw != 0x7F).any(-1).any(-1)
+    raw[written, :, channel] = 0
+    values[0, :, :, channel] = 0.0
+    return pool, tables, values
+
+
+def others_beside_a_large_one(path, hq, h, d, dtype, wide):
+    """One element of a query is 30,000 (in bf16 and fp32 also a million) times the others, and
+    no key has anything there: the scores are of the others alone, to their own bits. In fp32
+    the large one is past fp16's range."""
+    bs, lens, channel = 16, [700, 33, 250, 64], 5
+    pool, tables, values = without_channel(36 + d, dtype, lens, h, d, bs, channel)
+    q = torch.randn(len(lens), hq, d, generator=gen(16), device=DEV)
+    q[:, :, channel] = 3e4
+    if wide or dtype == torch.bfloat16:
+        q[1:, :, channel] = -1e6
+    if not wide:
+        q = q.to(dtype)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    bt, out = device_tables(tables), torch.empty(len(lens), hq, d, dtype=dtype, device=DEV)
+    attend(path, pool, q, bt, ctx, d**-0.5, out)
+    rest = q.clone()
+    rest[:, :, channel] = 0.0  # (reach is that of the others too)
+    for i, n in enumerate(lens):
+        check(out[i : i + 1], rest[i : i + 1], values, tables[i], bs, n - 1, d**-0.5, dtype, 1.0, i)
+
+
+def attend(path, pool, q, bt, ctx, scale, out):
+    """One token of each sequence by the decode, planned or not, or the prefill, with a plan or without."""
+    n, hq, d = q.shape
+    bs, h = pool.block_size, pool.num_kv_heads
+    if path in ("decode", "planned"):
+        run = {"err_flags": pool.err_flags, "kv_scales": pool.kv_scales[0], "out": out}
+        if path == "decode":
+            kernels.paged_decode(q, pool.k[0], pool.v[0], bt, ctx, bs, scale, **run)
+        else:
+            plan = kernels.decode_plan(bt, ctx, hq, pool.k[0], bs, err_flags=pool.err_flags)
+            kernels.paged_decode_planned(q, pool.k[0], pool.v[0], plan, scale, **run)
+    else:
+        cu, plan = torch.arange(n + 1, dtype=torch.int32, device=DEV), None
+        if path == "prefill_plan":
+            plan = kernels.prefill_plan(cu, ctx - 1, bt, n, 1, bs, hq, h, d, dtype=pool.dtype)
+        kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, ctx - 1, 1, bs, scale, plan=plan, out=out,
+                              err_flags=pool.err_flags, kv_scales=pool.kv_scales[0])
+    pool.check_errors()
+
+
+def fp32_queries(path, size, dtype):
+    """Queries whose numbers leave fp16's range on either side, with the scale that makes up for
+    it; a query of zeros attends all keys alike."""
+    hq, h, d, bs, lens = 14, 2, 64, 16, [300, 5, 64, 40]
+    pool, tables, values = filled(37, dtype, lens, h, d, bs)
+    q = size * torch.randn(len(lens), hq, d, generator=gen(17), device=DEV)
+    q[3] = 0.0
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = torch.empty(len(lens), hq, d, dtype=dtype, device=DEV)
+    scale = d**-0.5 / size
+    attend(path, pool, q, device_tables(tables), ctx, scale, out)
+    for i, n in enumerate(lens):
+        check(out[i : i + 1], q[i : i + 1], values, tables[i], bs, n - 1, scale, dtype, 1.0, i)
+
+
+@pytest.mark.parametrize("path", ["prefill", "prefill_plan"])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq, h, d", [(28, 4, 128), (14, 2, 64)])
+def test_prefill_of_a_large_element(hq, h, d, dtype, wide, path):
+    others_beside_a_large_one(path, hq, h, d, dtype, wide)
+
+
+@pytest.mark.parametrize("path", ["prefill", "prefill_plan"])
+@pytest.mark.parametrize("size", [1e-30, 1e-7, 1e6, 1e30])
+@pytest.mark.parametrize("dtype", HALF)
+def test_prefill_of_fp32_queries_of_any_size(path, size, dtype):
+    fp32_queries(path, size, dtype)
