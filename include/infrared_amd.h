@@ -661,7 +661,8 @@ int ir_paged_gather_q8(const void* k_cache, const void* v_cache, const float* sc
  * Attention over the 8-bit pool: ir_paged_decode, ir_paged_decode_planned and
  * ir_paged_prefill of the values that a layer holds, dtype being that of the pool and out.
  * q_dtype: dtype, or IR_DTYPE_F32 with a 16-bit dtype for queries that were not rounded to
- * it; they are used to 14 bits at least.
+ * it; they are used to 2^-18 of each element, in f16 to 2^-24 of it or 2^-39 of the largest of
+ * its row.
  * Workspaces, counters and plans are theirs (a decode plan is built with
  * IR_DTYPE_E4M3 and the layer's strides; partition_tokens 0 is
  * ir_paged_decode_default_partition, at least 128). The step's new rows are written first

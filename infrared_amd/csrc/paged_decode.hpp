@@ -123,31 +123,37 @@ struct CacheFormat<DT, D, true> {
 };
 
 // A query operand in registers; with QF (an fp32 query of a 16-bit pool) first the 16
-// elements of a step as they are loaded, x then rest, and after split() two pieces.
+// elements of a step as they are loaded, x then rest, and after split() two pieces of the
+// dtype times the power of two that unit takes back.
 template <int DT, int D, bool QF>
 struct QueryRegs {
   uint32_t x[TileShape<DT, D>::KDW];
   __device__ __forceinline__ void split() {}
+  __device__ __forceinline__ float scaled(float scale) const { return scale; }
 };
 template <int DT, int D>
 struct QueryRegs<DT, D, true> {
   static constexpr int N = TileShape<DT, D>::KDW;
   uint32_t x[N], rest[N];
+  float unit;
+  // (all lanes of the wavefront: the four lane groups hold a row together)
   __device__ __forceinline__ void split() {
-    uint32_t hi[N], lo[N];
+    float v[2 * N], most = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {  // elements 2i, 2i + 1 of the lane's
-      const float a = __uint_as_float(2 * i < N ? x[2 * i] : rest[2 * i - N]);
-      const float b = __uint_as_float(2 * i < N ? x[2 * i + 1] : rest[2 * i + 1 - N]);
-      hi[i] = Elem<DT>::pack2(a, b);
-      lo[i] = Elem<DT>::pack2(a - Elem<DT>::lo(hi[i]), b - Elem<DT>::hi(hi[i]));
+    for (int i = 0; i < 2 * N; ++i) {
+      v[i] = __uint_as_float(i < N ? x[i] : rest[i - N]);
+      most = fmaxf(most, fabsf(v[i]));
     }
+    const int up = row_shift(wave_max_groups_swap(most));
+    unit = pow2(-up);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      x[i] = hi[i];
-      rest[i] = lo[i];
+      const Pieces p = split2<DT>(v[2 * i] * pow2(up), v[2 * i + 1] * pow2(up));
+      x[i] = p.hi;
+      rest[i] = p.lo;
     }
   }
+  __device__ __forceinline__ float scaled(float scale) const { return scale * unit; }
 };
 
 // Issues a code tile's loads; the tile's first row is at tk / tv.
@@ -270,17 +276,19 @@ __device__ __forceinline__ void compute_tile(const Tile<DT, D>& tl, const uint32
 // The same for a tile of codes. The K codes go through LDS as they are and turn into
 // the operand there: lane group g of step j holds elements 64 j + 16 g .. + 15 of its
 // key (load_query_codes: the same of the query), one 16-byte read each. They are used
-// without their scale, which score_scale (times scale * log2 e) holds; the V codes
-// are multiplied by theirs, both exact.
+// without their scale, which multiplies the score beside scale_log2 (scale * log2 e); the
+// V codes are multiplied by theirs, both exact.
 //
-// QF: a 16-bit pool's query is fp32 and held in two pieces of the dtype, its rounded
-// value and what that leaves, off by 2^-16 of it (f16: 2^-22) instead of 2^-8 (2^-11).
+// QF: a 16-bit pool's query is fp32 and held in two pieces of the dtype, its rounded value and
+// that of what it leaves, off by 2^-18 of an element (f16: 2^-24, or 2^-39 of the row's
+// largest where the pieces are subnormal) instead of 2^-9 (2^-12).
 template <int DT, int D, bool QF>
 __device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const QueryRegs<DT, D, QF>& q, uint32_t kmask,
-                                              float score_scale, float v_scale, uint8_t* kst, int lane, State<D>& st,
-                                              bool col_on = true) {
+                                              float scale_log2, float k_scale, float v_scale, uint8_t* kst, int lane,
+                                              State<D>& st, bool col_on = true) {
   typedef TileShape<DT, D> Sh;
   constexpr int CPR = D / 16;  // 16-byte chunks per row
+  const float score_scale = q.scaled(scale_log2) * k_scale;
   const int g = lane >> 4, t = staged_token(lane & 15);
 #pragma unroll
   for (int i = 0; i < CodeTile<D>::NI; ++i) {
@@ -411,7 +419,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
         const int ii = min(i, last);
         const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[0]), ii));
         const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[1]), ii));
-        compute_codes<DT, D, QF>(tl, qr, mask, a.scale_log2 * ks, vs, kst, lane, st);
+        compute_codes<DT, D, QF>(tl, qr, mask, a.scale_log2, ks, vs, kst, lane, st);
       } else
         compute_tile<DT, D>(tl, qr.x, mask, a.scale_log2, kst, lane, st);
     };

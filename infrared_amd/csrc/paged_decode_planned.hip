@@ -727,7 +727,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       if constexpr (Q8) {
         const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
         const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
-        compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2 * ks, vs, kstage[w], lane, st, con[r]);
+        compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, ks, vs, kstage[w], lane, st, con[r]);
       } else {
         compute_tile<DT, D>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
       }

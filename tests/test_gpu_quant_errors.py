@@ -177,3 +177,18 @@ def test_prefill_of_a_large_element(hq, h, d, dtype, wide, path):
 @pytest.mark.parametrize("dtype", HALF)
 def test_prefill_of_fp32_queries_of_any_size(path, size, dtype):
     fp32_queries(path, size, dtype)
+
+
+@pytest.mark.parametrize("path", ["decode", "planned"])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq, h, d", [(28, 4, 128), (14, 2, 64)])
+def test_decode_of_a_large_element(hq, h, d, dtype, wide, path):
+    others_beside_a_large_one(path, hq, h, d, dtype, wide)
+
+
+@pytest.mark.parametrize("path", ["decode", "planned"])
+@pytest.mark.parametrize("size", [1e-30, 1e-7, 1e6, 1e30])
+@pytest.mark.parametrize("dtype", HALF)
+def test_decode_of_fp32_queries_of_any_size(path, size, dtype):
+    fp32_queries(path, size, dtype)
