@@ -248,14 +248,17 @@ constexpr float kRescaleSlack = 8.f;
 // O^T += V^T . P^T. Unless FULL, `vok[r]` says whether key row 4g+r may be
 // read; rows that may not are zeroed so 0 * V never meets a NaN pattern in
 // stale pool memory. FULL tiles (every key present) skip that masking.
-// SWAP: the column's maximum over lane groups by lane swaps instead of LDS.
-template <int DT, int D, bool FULL, bool SWAP = false>
+// Q8 (tiles of an 8-bit cache): the column's maximum over lane groups by lane swaps instead
+// of LDS, and the probabilities of a 16-bit dtype in two pieces of it (off by 2^-18, fp16
+// 2^-24), so that the output's rounding is all that shows. A product of 32 k-slots holds both
+// pieces, the V rows twice, and takes as long as one of 16.
+template <int DT, int D, bool FULL, bool Q8 = false>
 __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t (&vin)[4][TileShape<DT, D>::VDW],
                                            const bool (&vok)[4], State<D>& st) {
   typedef TileShape<DT, D> Sh;
   constexpr int TILES = Sh::TILES;
   float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-  mx = SWAP ? wave_max_groups_swap(mx) : wave_max_groups(mx);
+  mx = Q8 ? wave_max_groups_swap(mx) : wave_max_groups(mx);
   const bool grow = mx > st.m + kRescaleSlack;
   if (__any(grow)) {
     const float m_new = grow ? mx : st.m;
@@ -275,9 +278,8 @@ __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t 
 #pragma unroll
     for (int i = 0; i < Sh::VDW; ++i) v[r][i] = (FULL || vok[r]) ? vin[r][i] : 0u;
   if constexpr (Sh::k16) {
-    // P rounded to the input dtype, as softmax(...).to(q.dtype) does.
-    using E = Elem<DT>;
-    const u32x2 pb = {E::pack2(p[0], p[1]), E::pack2(p[2], p[3])};
+    // P rounded to the input dtype, as softmax(...).to(q.dtype) does (Q8: p0.hi, p1.hi).
+    const Pieces p0 = split2<DT>(p[0], p[1]), p1 = split2<DT>(p[2], p[3]);
 #pragma unroll
     for (int n = 0; n < TILES; ++n) {
       // element n of rows 4g..4g+3 -> the 4 k-slots of this lane (transpose)
@@ -290,8 +292,10 @@ __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t 
         lo = (v[0][wdw] >> 16) | (v[1][wdw] & 0xffff0000u);
         hi = (v[2][wdw] >> 16) | (v[3][wdw] & 0xffff0000u);
       }
-      const u32x2 va = {lo, hi};
-      st.acc[n] = mfma_k16<DT>(va, pb, st.acc[n]);
+      if constexpr (Q8)
+        st.acc[n] = mfma_k32<DT>(u32x4{lo, hi, lo, hi}, u32x4{p0.hi, p1.hi, p0.lo, p1.lo}, st.acc[n]);
+      else
+        st.acc[n] = mfma_k16<DT>(u32x2{lo, hi}, u32x2{p0.hi, p1.hi}, st.acc[n]);
     }
   } else {
     // fp32: one 16x16x4 product per key row; k-slot = lane group.

@@ -141,6 +141,16 @@ __device__ __forceinline__ float sum2<IR_DTYPE_F16>(uint32_t w, float acc) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), acc, false);
 }
 
+// a and b, fp32, in two pieces of dtype DT each: hi their rounding, lo that of what it leaves.
+struct Pieces {
+  uint32_t hi, lo;
+};
+template <int DT>
+__device__ __forceinline__ Pieces split2(float a, float b) {
+  const uint32_t hi = Elem<DT>::pack2(a, b);
+  return {hi, Elem<DT>::pack2(a - Elem<DT>::lo(hi), b - Elem<DT>::hi(hi))};
+}
+
 // 16x16x16, 16-bit inputs: 4 elements (2 dwords) of A and B per lane.
 template <int DT>
 __device__ __forceinline__ f32x4 mfma_k16(u32x2 a, u32x2 b, f32x4 c);

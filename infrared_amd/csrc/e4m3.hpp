@@ -56,14 +56,4 @@ __device__ __forceinline__ f32x2 decode2_f32(uint32_t w, float scale) {
 // the most room below it (k in [-113, 126], so that 2^k and 2^-k are normal numbers).
 __device__ __forceinline__ int row_shift(float most) { return max(-113, min(126, 14 - exponent_of(most))); }
 
-// a and b, fp32, in two pieces of dtype DT each: hi their rounding, lo that of what it leaves.
-struct Pieces {
-  uint32_t hi, lo;
-};
-template <int DT>
-__device__ __forceinline__ Pieces split2(float a, float b) {
-  const uint32_t hi = Elem<DT>::pack2(a, b);
-  return {hi, Elem<DT>::pack2(a - Elem<DT>::lo(hi), b - Elem<DT>::hi(hi))};
-}
-
 }  // namespace ir

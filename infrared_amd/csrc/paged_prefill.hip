@@ -619,7 +619,8 @@ void paged_prefill_kernel(PrefillArgs a) {
                            E::pack2(cur[ct][2 * st + 1][0], cur[ct][2 * st + 1][1]),
                            E::pack2(cur[ct][2 * st + 1][2], cur[ct][2 * st + 1][3])};
         // the running sum adds the rounded probabilities the PV product uses,
-        // two per instruction
+        // two per instruction (Q8: two pieces of each, as the decode has them, are
+        // twice the PV products: 368 us against 298 for 8 chunks of 512 tokens)
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[ct] = sum2<DT>(pb[ct][st][e], l[ct]);
       }

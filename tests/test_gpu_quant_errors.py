@@ -9,7 +9,7 @@ import torch
 
 from infrared_amd import kernels
 from oracle import quant
-from test_gpu_quant import device_tables, filled, gen
+from test_gpu_quant import device_tables, filled, gen, run_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,46 @@ def test_decode_of_a_large_element(hq, h, d, dtype, wide, path):
 @pytest.mark.parametrize("dtype", HALF)
 def test_decode_of_fp32_queries_of_any_size(path, size, dtype):
     fp32_queries(path, size, dtype)
+
+
+# ---- decode: the output is rounded, the probabilities keep what shows in it
+
+
+@pytest.mark.parametrize("planned", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq, h, d, bs", [(28, 4, 128, 16), (14, 2, 64, 16), (8, 8, 64, 32), (20, 1, 128, 48),
+                                          (33, 1, 64, 16)])
+def test_decode(planned, dtype, wide, hq, h, d, bs):
+    lens = [1, 2, 15, 16, 17, 33, 300, 1100, 64, 0, 5]
+    pool, tables, values = filled(hq + d, dtype, lens, h, d, bs)
+    q = torch.randn(len(lens), hq, d, generator=gen(9), device=DEV)
+    kw = {"out": torch.empty(len(lens), hq, d, dtype=dtype, device=DEV)} if wide else {}
+    q = q if wide else q.to(dtype)
+    out = run_decode(pool, q, device_tables(tables), torch.tensor(lens, dtype=torch.int32, device=DEV), planned, **kw)
+    pool.check_errors()
+    for i, n in enumerate(lens):
+        if n:
+            check(out[i : i + 1], q[i : i + 1], values, tables[i], bs, n - 1, d**-0.5, dtype, 0.0, n)
+        else:
+            assert not out[i].any()
+
+
+@pytest.mark.parametrize("dtype, hq, h, d, lens", [
+    (torch.bfloat16, 28, 4, 128, [9000, 700, 4097, 2500]), (torch.bfloat16, 28, 4, 128, [20011]),
+    (torch.float16, 14, 2, 64, [9000, 0, 17]), (torch.bfloat16, 40, 2, 64, [8191, 4000]),
+])
+def test_decode_of_long_contexts(dtype, hq, h, d, lens):
+    """Contexts cut into parts, merged at arrival or by a launch of their own; pairs."""
+    bs = 16
+    pool, tables, values = filled(23, dtype, lens, h, d, bs)
+    tables.insert(1, tables[0][:200])
+    lens = [lens[0], 200 * bs - 3, *lens[1:]]
+    q = torch.randn(len(lens), hq, d, generator=gen(10), device=DEV).to(dtype)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for planned in (True, False):
+        out = run_decode(pool, q, device_tables(tables), ctx, planned)
+        pool.check_errors()
+        for i, n in enumerate(lens):
+            if n:
+                check(out[i : i + 1], q[i : i + 1], values, tables[i], bs, n - 1, d**-0.5, dtype, 0.0, (planned, n))
