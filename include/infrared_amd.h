@@ -53,8 +53,9 @@ enum {
   IR_ERR_BLOCK_RANGE = 2,    /* block id outside [0, num_blocks) (block masked) */
   IR_ERR_CONTEXT_RANGE = 4,  /* context_len > max_blocks*block_size (clamped) or < 0 */
   IR_ERR_GATHER_RANGE = 8,   /* gather slot outside [0, num_slots) (key masked) */
-  IR_ERR_PLAN = 16,          /* a decode plan with sequence pairs run without IR_PLAN_SHARE_GROUPS
-                                (nothing written) */
+  IR_ERR_PLAN = 16,          /* a decode plan with sequence pairs run without IR_PLAN_SHARE_GROUPS,
+                                or one for IR_DTYPE_E4M3 run by another dtype's call or the
+                                reverse (nothing written) */
   IR_ERR_WRITE_SLOT = 32     /* a fused prefill's new token written elsewhere than its block-table
                                 slot (the call attended the new row itself) */
 };
@@ -264,7 +265,9 @@ int ir_paged_decode_noalloc(const void* q, int64_t q_seq_stride, int64_t q_head_
  *   wholly inside both contexts) are read once for the pair. Runs of
  *   consecutive sharing sequences pair from their start. Outputs are the same
  *   attention (each column sees exactly its sequence's keys). A plan that
- *   holds pairs run without the flag writes nothing and sets IR_ERR_PLAN.
+ *   holds pairs run without the flag writes nothing and sets IR_ERR_PLAN, and so
+ *   does one built for IR_DTYPE_E4M3 run by ir_paged_decode_planned, or one built for
+ *   another dtype run by ir_paged_decode_planned_q8.
  */
 int64_t ir_paged_decode_plan_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
                                    int max_blocks_per_seq, int block_size);

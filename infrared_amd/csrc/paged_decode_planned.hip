@@ -52,11 +52,13 @@ constexpr int kPlanWaves = 4;       // streaming wavefronts per workgroup
 // sequences of 512..4096 keys: 45.1 us with four, 33.5 with eight, whatever the number
 // of tiles in flight; twelve are short of registers, 46.5).
 constexpr int kCodeWaves = 8;
+constexpr int kCodePlan = 1 << 16;  // (above any number of pairs)
 constexpr int kPlanRun = 64;        // tile facts per wavefront and run (one per lane)
 constexpr int kPlanMinTiles = 16;   // smallest slice
 
 // Plan regions (byte offsets, 256-byte aligned):
-//   hdr[8]             T, R, number of sequences with no usable key, number of pairs
+//   hdr[8]             T, R, number of sequences with no usable key, number of pairs (kCodePlan
+//                      added in a plan of kCodeWaves wavefronts, whose regions lie elsewhere)
 //   seq_pre[B + 1]     list tiles before sequence b, per unit
 //   empty[B]           sequences with no usable key
 //   share[B]           shared 16-key tiles of sequences b, b + 1 (ir_paged_decode_plan's pair scan)
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(NW * 64) void paged_decode_plan_kernel(PlanArgs p) 
     hdr[0] = T;
     hdr[1] = R;
     hdr[2] = s_nempty;
-    hdr[3] = s_npairs;
+    hdr[3] = s_npairs + (NW == kCodeWaves ? kCodePlan : 0);
   }
   int32_t* wh = (int32_t*)(p.plan + p.ly.whdr) + ((int64_t)grp * NW + w) * 8;
   if (lo >= hi) {
@@ -516,8 +518,9 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   const int n_ups = a.n_ups;
 
   // ---- 1. everything the wavefront needs, requested at once
-  // (a plan with pairs needs the pair kernel: its flag empties this
-  // workgroup's slice rather than branching, so no read waits on it)
+  // (a plan with pairs needs the pair kernel, and one of the other kind of cache has its
+  // slices and tiles elsewhere: a wrong plan's flag empties this workgroup's slice rather
+  // than branching, so no read waits on it; what is read before lies within either kind)
   const int32_t* hdr = (const int32_t*)plan;
   const int32_t* wh = (const int32_t*)(plan + o_whdr) + ((int64_t)grp * NW + w) * 8;
   const u32x2* facts = (const u32x2*)(plan + ly.facts);
@@ -526,7 +529,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   const int pre0 = tid <= B ? sp[tid] : 0;  // every sequence's when B < NT
   const int pair0 = PAIRS && tid < B ? pp[tid] : 0;
   const u32x4 h4 = *(const u32x4*)hdr;
-  const int R = (int)h4[1], hdr_pairs = (int)h4[3];
+  const int R = (int)h4[1], hdr_pairs = (int)h4[3] - (Q8 ? kCodePlan : 0);
   // the wavefront's header in two 16-byte reads (the plan is 256-byte
   // aligned), so the select below cannot become a skipped load
   const u32x4 wh0 = *(const u32x4*)wh, wh1 = *(const u32x4*)(wh + 4);
@@ -535,7 +538,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   // (one round trip) instead of each behind the last one's use
   asm volatile("" ::"s"(R), "s"(hdr_pairs), "s"(wh0[0]), "s"(wh0[1]), "s"(wh0[2]), "s"(wh0[3]), "s"(wh1[0]),
                "s"(wh1[1]), "s"(wh1[2]), "v"(f0[0]), "v"(f0[1]), "v"(pre0), "v"(pair0));
-  const bool wrong_plan = !PAIRS && hdr_pairs != 0;
+  const bool wrong_plan = PAIRS ? (uint32_t)hdr_pairs >= kCodePlan : hdr_pairs != 0;
   const int wlo = (int)wh0[0], cnt_w = (int)wh0[1], fl = (int)wh0[2], ll = (int)wh0[3];
   const int lo = (int)wh1[0], u_first = (int)wh1[2];
   const int hi = wrong_plan ? lo : (int)wh1[1];
@@ -567,7 +570,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   }
   __syncthreads();
   if (wrong_plan && grp == 0 && tid == 0) flag_error(a.err, IR_ERR_PLAN);
-  if (lo >= hi) return;  // uniform: past the end of the list (or a plan with pairs)
+  if (lo >= hi) return;  // uniform: past the end of the list (or a wrong plan)
 
   struct Lbl {
     int u, b, j, us, ue;
@@ -889,7 +892,8 @@ __global__ __launch_bounds__(kMergeThreads) void paged_decode_planned_merge(cons
   const int32_t* hdr = (const int32_t*)plan;
   const int32_t* pre = (const int32_t*)(plan + o_seq_pre);
   const int R = hdr[1];
-  if (hdr[3] != 0 && !pairs) return;  // (flagged by the run)
+  const int hdr_pairs = hdr[3] - kCodePlan;
+  if (pairs ? (uint32_t)hdr_pairs >= kCodePlan : hdr_pairs != 0) return;  // (flagged by the run)
   const int u = blockIdx.x, col = blockIdx.y;
   const int b = u / a.n_ups, j = u - b * a.n_ups;
   const int ts = pre[b + 1] - pre[b];

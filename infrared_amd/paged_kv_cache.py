@@ -57,7 +57,7 @@ _ERR_NAMES = {
     ERR_BLOCK_RANGE: "block id outside the pool",
     ERR_CONTEXT_RANGE: "context length outside the block table",
     ERR_GATHER_RANGE: "gather slot outside the pool",
-    ERR_PLAN: "decode plan with sequence pairs run without share groups",
+    ERR_PLAN: "decode plan with sequence pairs run without share groups, or of another kind of pool",
     ERR_WRITE_SLOT: "new token written elsewhere than its block-table slot",
 }
 

@@ -4,10 +4,13 @@ that on the CPU), and what its queries and probabilities keep of their bits."""
 
 from __future__ import annotations
 
+import dataclasses
+
 import pytest
 import torch
 
-from infrared_amd import kernels
+from infrared_amd import PagedKVPool, kernels
+from infrared_amd._lib import ERR_PLAN
 from oracle import quant
 from test_gpu_quant import device_tables, filled, gen, run_decode
 
@@ -235,3 +238,30 @@ def test_decode_of_long_contexts(dtype, hq, h, d, lens):
         for i, n in enumerate(lens):
             if n:
                 check(out[i : i + 1], q[i : i + 1], values, tables[i], bs, n - 1, d**-0.5, dtype, 0.0, (planned, n))
+
+
+# ---- plans of the other kind of pool
+
+
+@pytest.mark.parametrize("share", [False, True])
+@pytest.mark.parametrize("lens", [[4000], [700, 900, 300] * 20])
+def test_a_plan_of_another_kind_of_pool_writes_nothing(lens, share):
+    """Plans of 8-bit and of other pools lie differently in memory: a run over the other's flags it
+    and touches neither the output nor the counters, in the launch that merges too."""
+    hq, h, d, bs, dtype = 8, 2, 64, 16, torch.bfloat16
+    pool, tables, _ = filled(61, dtype, lens, h, d, bs)
+    plain = PagedKVPool(1, pool.num_blocks, bs, h, d, dtype)
+    bt, ctx = device_tables(tables), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = torch.randn(len(lens), hq, d, generator=gen(62), device=DEV).to(dtype)
+    plans = [kernels.decode_plan(bt, ctx, hq, p.k[0], bs, share_groups=share) for p in (pool, plain)]
+    as_other = [dataclasses.replace(a, buf=b.buf) for a, b in (plans, plans[::-1])]
+    ctr = torch.zeros(kernels.decode_num_counters(len(lens), hq, h), dtype=torch.int32, device=DEV)
+    for p, plan, kw in ((pool, as_other[0], {"kv_scales": pool.kv_scales[0]}), (plain, as_other[1], {})):
+        out, err = torch.full_like(q, 3.0), torch.zeros(1, dtype=torch.int32, device=DEV)
+        kernels.paged_decode_planned(q, p.k[0], p.v[0], plan, d**-0.5, out=out, err_flags=err, counters=ctr, **kw)
+        torch.cuda.synchronize()
+        assert err.item() == ERR_PLAN and bool((out == 3.0).all()) and not ctr.any()
+        right = plans[0] if kw else plans[1]
+        err.zero_()
+        kernels.paged_decode_planned(q, p.k[0], p.v[0], right, d**-0.5, out=out, err_flags=err, counters=ctr, **kw)
+        assert err.item() == 0 and not (out == 3.0).all()
