@@ -164,6 +164,11 @@ class MixedStep:
         self.pool, self.batch, self.inputs, self.scale = pool, batch, inputs, scale
         self.overlap = overlap
         self.quant = isinstance(pool, QuantPagedKVPool)
+        if self.quant:  # (the kernels take a layer's scales for those of their rows' dtype)
+            for name in ("q_dec", "q_pre", "k_new", "v_new"):
+                dtype = getattr(inputs, name).dtype
+                if dtype != pool.dtype:
+                    raise RuntimeError(f"MixedStep: {name} is {dtype}, the 8-bit pool's dtype is {pool.dtype}")
         self.fused = fused and not overlap and not self.quant
         dev = pool.device
         self.out_dec = torch.empty_like(inputs.q_dec)
