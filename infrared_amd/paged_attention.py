@@ -327,8 +327,9 @@ def _prefill(q, pool, layer_idx: int, block_tables, cu_seqlens_q, q_start, max_q
     b, sq, hq, d = q.shape
     h_kv = pool.k.shape[-2]
     nseq = q_start.shape[0]
+    rows = q.reshape(b * sq, hq, d)
     if out is None:
-        out = _out_for(q.reshape(b * sq, hq, d), pool)
+        out = _out_for(rows, pool)
     dtype = q.dtype if out is None else out.dtype
     plan = getattr(holder, "prefill_plan", None)
     if plan is not None and plan.f32 != (dtype == torch.float32):
@@ -344,7 +345,7 @@ def _prefill(q, pool, layer_idx: int, block_tables, cu_seqlens_q, q_start, max_q
             pass
     k_layer, v_layer, scales = _layer(pool, layer_idx)
     return kernels.paged_prefill(
-        q.reshape(b * sq, hq, d), k_layer, v_layer, block_tables, cu_seqlens_q, q_start, max_q,
+        rows, k_layer, v_layer, block_tables, cu_seqlens_q, q_start, max_q,
         pool.block_size, scale, out=out, err_flags=err, plan=plan, new_kv=new_kv, src_row0=src_row0,
         kv_scales=scales,
     ).view(b, sq, hq, d)
