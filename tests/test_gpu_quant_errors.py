@@ -9,10 +9,11 @@ import dataclasses
 import pytest
 import torch
 
-from infrared_amd import PagedKVPool, kernels
+from infrared_amd import PagedKVPool, QuantPagedKVPool, kernels, metadata, rope_paged_attention
 from infrared_amd._lib import ERR_PLAN
+from infrared_amd.mixed_step import MixedConfig, MixedStep, make_mixed_case
 from oracle import quant
-from test_gpu_quant import device_tables, filled, gen, run_decode
+from test_gpu_quant import device_tables, filled, gen, rotation, rows, run_decode, step_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -238,6 +239,116 @@ def test_decode_of_long_contexts(dtype, hq, h, d, lens):
         for i, n in enumerate(lens):
             if n:
                 check(out[i : i + 1], q[i : i + 1], values, tables[i], bs, n - 1, d**-0.5, dtype, 0.0, (planned, n))
+
+
+# ---- together
+
+
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+def test_a_sequence_through_the_seam(dtype, normed):
+    """Prefill chunks, then decodes, through ``rope_paged_attention``, against attention in 64 bits of
+    the queries as they leave the rotation over the values read back."""
+    hq, h, d, bs = 14, 2, 64, 16
+    g = gen(16)
+    pool = QuantPagedKVPool(1, 40, bs, h, d, dtype, strict=True)
+    tables = [list(range(20, 30)), list(range(3, 13)), list(range(30, 40))]
+    wq, wk = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+    norms = {"q_norm": wq, "k_norm": wk, "eps": 1e-5} if normed else {}
+    cached = [0, 0, 0]
+    for step in ([40, 3, 0], [1, 60, 0], [33, 1, 9], [1, 1, 1], [1, 1, 1]):
+        live = [i for i, n in enumerate(step) if n]
+        new, was = [step[i] for i in live], [cached[i] for i in live]
+        decode = max(new) == 1
+        context = metadata.decode_context if decode else metadata.prefill_context
+        paged, mask = context(pool, [tables[i] for i in live], was, *(() if decode else (new,)))
+        b, n = (len(live), 1) if decode else (1, sum(new))
+        q, k, v, cos, sin = step_inputs(g, b, n, hq, h, d, dtype)
+        out = rope_paged_attention(q, k, v, cos, sin, paged, mask, 0, d**-0.5, hq // h, **norms).reshape(-1, hq, d)
+        spare = QuantPagedKVPool(1, 40, bs, h, d, dtype)
+        qr = torch.empty(b * n, hq, d, device=DEV)
+        kernels.rope_kv_scatter_q8(q.reshape(-1, hq, d), k.reshape(-1, h, d), v.reshape(-1, h, d), cos.reshape(-1, d),
+                                   sin.reshape(-1, d), spare.k[0], spare.v[0], spare.kv_scales[0], paged.write_slots,
+                                   bs, *(norms.values()), q_out=qr)
+        values = torch.stack(pool.gather(0, torch.arange(pool.num_slots, device=DEV))).double().cpu()
+        row = 0
+        for i, m, c in zip(live, new, was):
+            check(out[row : row + m], qr[row : row + m], values, tables[i], bs, c, d**-0.5, dtype, 1.0, (step, i))
+            row += m
+        cached = [c + n for c, n in zip(cached, step)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_mixed_step(dtype):
+    cfg = MixedConfig("t", 1, 70, 20, 300, 3, 40, 33, 28, 4, 128, 16, dtype, seed=2)
+    _, plain, batch, inputs = make_mixed_case(cfg, DEV)
+    pool = QuantPagedKVPool(1, plain.num_blocks, 16, 4, 128, dtype)
+    slots = torch.arange(pool.num_slots, device=DEV)
+    pool.write(0, plain.k[0], plain.v[0], slots)
+    step = MixedStep(pool, batch, inputs, cfg.scale)
+    step.eager()
+    assert int(step.err.item()) == 0
+    values = torch.stack(pool.gather(0, slots)).double().cpu()
+    for i in range(0, 70, 3):
+        check(step.out_dec[0, i : i + 1], inputs.q_dec[0, i : i + 1], values, batch.dec_tables[i].tolist(), 16,
+              int(batch.dec_ctx[i]) - 1, cfg.scale, dtype, 0.0, i)
+    for i in range(3):
+        t = slice(40 * i, 40 * i + 40)
+        check(step.out_pre[0, t], inputs.q_pre[0, t], values, batch.pre_tables[i].tolist(), 16, 33, cfg.scale, dtype, 1.0)
+
+
+# ---- writes whose workgroups take several blocks in turn
+
+
+@pytest.mark.parametrize("mode", ["plain", "rotated", "normed"])
+@pytest.mark.parametrize("n, window", [(70, 2), (260, 8), (520, 16)])
+def test_write_of_windows_of_some_tokens(n, window, mode):
+    """Every token of a window may own a block: shuffled tokens with slots given twice, skipped and past
+    the pool; one token a block; runs that begin inside blocks. 64 KV heads make 32 workgroups a token."""
+    h, hq, d, bs, dtype = 64, 2, 64, 16, torch.bfloat16
+    assert max(1, n * (2 * h // 4) // 1024) == window
+    g, blocks = gen(n), 640
+    pool, want = QuantPagedKVPool(1, blocks, bs, h, d, dtype), quant.QuantCache(blocks, bs, h, d, dtype)
+    total = pool.num_slots
+    shuffled = torch.randint(0, 40 * bs, (n,), generator=g, device=DEV)
+    shuffled[::9] = -1
+    shuffled[6] = total
+    shuffled[1::2] = shuffled[0::2][: len(shuffled[1::2])]  # (given twice, next to each other)
+    decode = torch.randperm(blocks, generator=g, device=DEV)[:n] * bs + torch.randint(0, bs, (n,), generator=g, device=DEV)
+    runs = torch.arange(n, device=DEV) + 7
+    calls = [(shuffled, True), (runs, False), (runs.flip(0), False)]
+    if mode == "plain" or n == 70:  # (the oracle's cost)
+        calls.append((decode, False))
+    for slots, bad in calls:
+        q, k, v = rows(g, n, hq + 2 * h, d, dtype, 2.0).split([hq, h, h], 1)
+        if mode == "plain":
+            pool.write(0, k, v, slots)
+            want.write(k, v, slots)
+        else:
+            w = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+            cos, sin = rotation(g, n, d)
+            norms = (*w, 1e-6) if mode == "normed" else ()
+            kernels.rope_kv_scatter_q8(q, k, v, cos, sin, pool.k[0], pool.v[0], pool.kv_scales[0], slots, bs, *norms,
+                                       err_flags=pool.err_flags)
+            # the keys as the pool takes them: the same call's over a 32-bit pool (normed: fp32, of
+            # rows that fp32 holds exactly), the last row of a slot given twice where it comes to rest
+            wide = torch.float32 if mode == "normed" else dtype
+            turned = torch.empty(n, h, d, dtype=wide, device=DEV)
+            x = [t.to(wide) for t in (k, k, v)]
+            spare_k, spare_v = torch.empty(2, n, h, d, dtype=wide, device=DEV)
+            if norms:
+                kernels.qk_norm_rope_kv_scatter(*x, w[1].to(wide), w[1].to(wide), 1e-6, cos, sin, spare_k, spare_v,
+                                                torch.arange(n, device=DEV), q_out=turned)
+            else:
+                kernels.rope_kv_scatter(*x, cos, sin, spare_k, spare_v, torch.arange(n, device=DEV), q_out=turned)
+            want.write(turned, v, slots)
+        if bad:
+            with pytest.raises(IndexError, match="slot"):
+                pool.check_errors()
+        pool.check_errors()
+        assert torch.equal(pool.kv_scales[0].double().cpu(), torch.exp2(want.exps.double()))
+        k, v = pool.gather(0, torch.arange(total, device=DEV))
+        assert torch.equal(torch.stack([k, v]).double().cpu(), want.values)
 
 
 # ---- plans of the other kind of pool
