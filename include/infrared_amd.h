@@ -672,27 +672,31 @@ int ir_paged_gather_q8(const void* k_cache, const void* v_cache, const float* sc
  * (ir_kv_scatter_q8): their blocks' scales are not known before, so the prefill has no
  * fused write.
  */
-int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
-                       const void* v_cache, const float* scales, int64_t num_blocks, int block_size,
-                       const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
-                       const int32_t* context_lens, void* out, int64_t out_seq_stride,
-                       int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
-                       int head_dim, float scale, int dtype, int q_dtype, int partition_tokens, int32_t* counters,
-                       int64_t num_counters, void* workspace, int64_t workspace_bytes,
-                       int32_t* err_flags, ir_stream_t stream);
+int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                       const void* k_cache, const void* v_cache, const float* scales,
+                       int64_t num_blocks, int block_size, const int32_t* block_tables,
+                       int64_t bt_stride, int max_blocks_per_seq, const int32_t* context_lens,
+                       void* out, int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
+                       int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype,
+                       int q_dtype, int partition_tokens, int32_t* counters, int64_t num_counters,
+                       void* workspace, int64_t workspace_bytes, int32_t* err_flags,
+                       ir_stream_t stream);
 int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
-                               const void* k_cache, const void* v_cache, const float* scales, void* out,
-                               int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
-                               int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
-                               int block_size, float scale, int dtype, int q_dtype, int flags, const void* plan,
-                               int32_t* counters, int64_t num_counters, void* workspace,
-                               int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream);
-int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache, const void*
-                        v_cache, const float* scales, int64_t num_blocks, int block_size, const int32_t* block_tables,
-                        int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
-                        int num_seqs, int total_q, int max_q_len, void* out, int64_t out_tok_stride, int64_t
-                        out_head_stride, int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype,
-                        int q_dtype, void* plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
+                               const void* k_cache, const void* v_cache, const float* scales,
+                               void* out, int64_t out_seq_stride, int64_t out_head_stride,
+                               int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                               int max_blocks_per_seq, int block_size, float scale, int dtype,
+                               int q_dtype, int flags, const void* plan, int32_t* counters,
+                               int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                               int32_t* err_flags, ir_stream_t stream);
+int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                        const void* k_cache, const void* v_cache, const float* scales,
+                        int64_t num_blocks, int block_size, const int32_t* block_tables,
+                        int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q,
+                        const int32_t* q_start, int num_seqs, int total_q, int max_q_len, void* out,
+                        int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads,
+                        int num_kv_heads, int head_dim, float scale, int dtype, int q_dtype,
+                        void* plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
 
 /*
  * Read-only HBM streaming roof (a measurement utility; no counterpart in the

@@ -49,7 +49,6 @@ __device__ __forceinline__ void merge_partials(const DecodeArgs& a, int seq, int
 template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH, bool Q8 = false, bool QF = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 ? 1 : 2)))
 void paged_decode_kernel(DecodeArgs a) {
-  typedef TileShape<DT, D> Sh;
   typedef CacheFormat<DT, D, Q8> F;
   __shared__ MergeSmem<NW, D> sm;
   __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][F::STAGE];
@@ -312,12 +311,11 @@ namespace {
 // ir_paged_decode, and with `scales` ir_paged_decode_q8 (a dense layer of codes).
 int decode_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_seq_stride,
                 int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
-                int64_t cache_head_stride,
-                int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
-                int max_blocks_per_seq, const int32_t* context_lens, void* out, int64_t out_seq_stride,
-                int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, float scale,
-                int dtype, int partition_tokens, int32_t* counters, int64_t num_counters, void* workspace,
-                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
+                int64_t cache_head_stride, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                int64_t bt_stride, int max_blocks_per_seq, const int32_t* context_lens, void* out,
+                int64_t out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
+                int head_dim, float scale, int dtype, int partition_tokens, int32_t* counters, int64_t num_counters,
+                void* workspace, int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   const int eb = dtype_bytes(dtype);
   IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
   IR_REQUIRE(q_dtype == dtype || (scales && q_dtype == IR_DTYPE_F32), "%s: unknown q_dtype %d for dtype %d", name,
@@ -447,10 +445,9 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
                                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   return decode_call("ir_paged_decode", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                      cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride,
-                     max_blocks_per_seq,
-                     context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
-                     scale, dtype, partition_tokens, counters, num_counters, workspace, workspace_bytes, err_flags,
-                     stream);
+                     max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
+                     num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
+                     workspace_bytes, err_flags, stream);
 }
 
 extern "C" int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
@@ -463,8 +460,8 @@ extern "C" int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q
                                   int32_t* err_flags, ir_stream_t stream) {
   if (num_seqs == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_decode_q8: null pointer");
-  return decode_call("ir_paged_decode_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache, head_dim,
-                     num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
+  return decode_call("ir_paged_decode_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                     head_dim, num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
                      max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
                      num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
                      workspace_bytes, err_flags, stream);

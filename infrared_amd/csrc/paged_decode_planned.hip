@@ -997,6 +997,8 @@ extern "C" int64_t ir_paged_decode_plan_bytes(int num_seqs, int num_q_heads, int
                                               int block_size) {
   if (!plannable(num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size)) return 0;
   const int n_ups = num_kv_heads * n_hg_of(num_q_heads, num_kv_heads);
+  // (of the larger kind, whichever is built: a run reads its wavefront's part of the plan before
+  // it knows whether the plan is of its kind)
   return plan_layout(num_seqs, device_cus(), t_cap_of(num_seqs, n_ups, max_blocks_per_seq, block_size),
                      std::max(kPlanWaves, kCodeWaves))
       .total;
@@ -1068,12 +1070,11 @@ namespace {
 // ir_paged_decode_planned, and with `scales` ir_paged_decode_planned_q8 (a dense
 // layer of codes).
 int planned_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_seq_stride,
-                 int64_t q_head_stride,
-                 const void* k_cache, const void* v_cache, int64_t cache_slot_stride, void* out,
-                 int64_t out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
-                 int head_dim, int max_blocks_per_seq, int block_size, float scale, int dtype, int flags,
-                 const void* plan, int32_t* counters, int64_t num_counters, void* workspace, int64_t workspace_bytes,
-                 int32_t* err_flags, ir_stream_t stream) {
+                 int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
+                 void* out, int64_t out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads,
+                 int num_kv_heads, int head_dim, int max_blocks_per_seq, int block_size, float scale, int dtype,
+                 int flags, const void* plan, int32_t* counters, int64_t num_counters, void* workspace,
+                 int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   const int eb = dtype_bytes(dtype);
   IR_REQUIRE(eb > 0, "%s: unknown dtype %d", name, dtype);
   IR_REQUIRE(q_dtype == dtype || (scales && q_dtype == IR_DTYPE_F32), "%s: unknown q_dtype %d for dtype %d", name,
@@ -1180,18 +1181,16 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
   return planned_call("ir_paged_decode_planned", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                       cache_slot_stride, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads,
                       head_dim, max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters,
-                      workspace,
-                      workspace_bytes, err_flags, stream);
+                      workspace, workspace_bytes, err_flags, stream);
 }
 
-extern "C" int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void*
-                                          k_cache, const void* v_cache, const float* scales, void* out, int64_t
-                                          out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads, int
-                                          num_kv_heads, int head_dim, int max_blocks_per_seq, int block_size, float
-                                          scale, int dtype, int q_dtype, int flags, const void* plan, int32_t*
-                                          counters, int64_t num_counters, void* workspace, int64_t workspace_bytes,
-                                          int32_t* err_flags,
-                                          ir_stream_t stream) {
+extern "C" int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                                          const void* k_cache, const void* v_cache, const float* scales, void* out,
+                                          int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
+                                          int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
+                                          int block_size, float scale, int dtype, int q_dtype, int flags,
+                                          const void* plan, int32_t* counters, int64_t num_counters, void* workspace,
+                                          int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   IR_REQUIRE(scales, "ir_paged_decode_planned_q8: null pointer");
   return planned_call("ir_paged_decode_planned_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                       head_dim, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,

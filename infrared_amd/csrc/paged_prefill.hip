@@ -1815,14 +1815,13 @@ namespace {
 // ir_paged_prefill, and with `scales` ir_paged_prefill_q8 (a dense layer of codes).
 int prefill_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_tok_stride,
                  int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
-                 int64_t cache_head_stride,
-                 int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride, int
-                 max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q,
-                 int max_q_len, void* out, int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads, int
-                 num_kv_heads, int head_dim, float scale, int dtype, void* plan, int64_t plan_bytes, const void* k_new,
-                 int64_t k_new_tok_stride, int64_t k_new_head_stride, const void* v_new, int64_t v_new_tok_stride,
-                 int64_t v_new_head_stride, const int64_t* write_slots, int64_t n_write, int64_t src_row0, int32_t*
-                 err_flags, ir_stream_t stream) {
+                 int64_t cache_head_stride, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                 int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
+                 int num_seqs, int total_q, int max_q_len, void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                 int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype, void* plan,
+                 int64_t plan_bytes, const void* k_new, int64_t k_new_tok_stride, int64_t k_new_head_stride,
+                 const void* v_new, int64_t v_new_tok_stride, int64_t v_new_head_stride, const int64_t* write_slots,
+                 int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
   IR_REQUIRE(dtype == IR_DTYPE_BF16 || dtype == IR_DTYPE_F16 || dtype == IR_DTYPE_F32,
              "%s: unknown dtype %d", name, dtype);
   const bool f32 = dtype == IR_DTYPE_F32;
@@ -1956,27 +1955,27 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
                                 int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
   return prefill_call("ir_paged_prefill", nullptr, dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
                       cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride,
-                      max_blocks_per_seq,
-                      cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride, out_head_stride,
-                      num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, k_new, k_new_tok_stride,
-                      k_new_head_stride, v_new, v_new_tok_stride, v_new_head_stride, write_slots, n_write, src_row0,
-                      err_flags, stream);
+                      max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
+                      out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, k_new,
+                      k_new_tok_stride, k_new_head_stride, v_new, v_new_tok_stride, v_new_head_stride, write_slots,
+                      n_write, src_row0, err_flags, stream);
 }
 
 extern "C" int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
-                                   const void* v_cache, const float* scales, int64_t num_blocks, int block_size, const
-                                   int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq, const int32_t*
-                                   cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q, int max_q_len,
-                                   void* out, int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads, int
-                                   num_kv_heads, int head_dim, float scale, int dtype, int q_dtype, void* plan,
-                                   int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream) {
+                                   const void* v_cache, const float* scales, int64_t num_blocks, int block_size,
+                                   const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                                   const int32_t* cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q,
+                                   int max_q_len, void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                                   int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype,
+                                   int q_dtype, void* plan, int64_t plan_bytes, int32_t* err_flags,
+                                   ir_stream_t stream) {
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_prefill_q8: null pointer");
   return prefill_call("ir_paged_prefill_q8", scales, q_dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
                       head_dim, num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
                       max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
-                      out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, nullptr, 0,
-                      0, nullptr, 0, 0, nullptr, 0, 0, err_flags, stream);
+                      out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, nullptr,
+                      0, 0, nullptr, 0, 0, nullptr, 0, 0, err_flags, stream);
 }
 
 extern "C" int ir_paged_prefill_plan(const int32_t* cu_seqlens_q, const int32_t* q_start, const int32_t* block_tables,
