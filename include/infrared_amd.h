@@ -35,7 +35,8 @@ enum {
   IR_DTYPE_F32 = 0,
   IR_DTYPE_F16 = 1,
   IR_DTYPE_BF16 = 2,
-  IR_DTYPE_E4M3 = 3 /* the codes of an 8-bit pool; only where a call says so */
+  IR_DTYPE_E4M3 = 3, /* the codes of an 8-bit pool; only where a call says so */
+  IR_DTYPE_E2M1 = 4  /* the codes of a 4-bit pool; likewise */
 };
 
 /* return codes */
@@ -54,8 +55,8 @@ enum {
   IR_ERR_CONTEXT_RANGE = 4,  /* context_len > max_blocks*block_size (clamped) or < 0 */
   IR_ERR_GATHER_RANGE = 8,   /* gather slot outside [0, num_slots) (key masked) */
   IR_ERR_PLAN = 16,          /* a decode plan with sequence pairs run without IR_PLAN_SHARE_GROUPS,
-                                or one for IR_DTYPE_E4M3 run by another dtype's call or the
-                                reverse (nothing written) */
+                                or one for IR_DTYPE_E4M3 or IR_DTYPE_E2M1 run by another
+                                dtype's call or the reverse (nothing written) */
   IR_ERR_WRITE_SLOT = 32     /* a fused prefill's new token written elsewhere than its block-table
                                 slot (the call attended the new row itself) */
 };
@@ -248,7 +249,8 @@ int ir_paged_decode_noalloc(const void* q, int64_t q_seq_stride, int64_t q_head_
  *   which the run leaves at zero.
  * ir_paged_decode_plan: writes the plan for (block_tables, context_lens) and a
  *   pool with the given slot/head strides (elements) and dtype (IR_DTYPE_E4M3 for
- *   an 8-bit pool, strides head_dim and num_blocks * block_size * head_dim). Context
+ *   an 8-bit pool, strides head_dim and num_blocks * block_size * head_dim;
+ *   IR_DTYPE_E2M1 for a 4-bit pool, half of both, in bytes). Context
  *   lengths outside [0, max_blocks * block_size] are clamped and flagged
  *   (IR_ERR_CONTEXT_RANGE); block ids outside [0, num_blocks) are flagged
  *   (IR_ERR_BLOCK_RANGE) and their keys masked, as in ir_paged_decode.
@@ -266,8 +268,9 @@ int ir_paged_decode_noalloc(const void* q, int64_t q_seq_stride, int64_t q_head_
  *   consecutive sharing sequences pair from their start. Outputs are the same
  *   attention (each column sees exactly its sequence's keys). A plan that
  *   holds pairs run without the flag writes nothing and sets IR_ERR_PLAN, and so
- *   does one built for IR_DTYPE_E4M3 run by ir_paged_decode_planned, or one built for
- *   another dtype run by ir_paged_decode_planned_q8.
+ *   does one built for IR_DTYPE_E4M3 run by any call but ir_paged_decode_planned_q8, or
+ *   one built for another dtype run by that; likewise IR_DTYPE_E2M1 and
+ *   ir_paged_decode_planned_q4.
  */
 int64_t ir_paged_decode_plan_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
                                    int max_blocks_per_seq, int block_size);
@@ -697,6 +700,148 @@ int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stri
                         int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads,
                         int num_kv_heads, int head_dim, float scale, int dtype, int q_dtype,
                         void* plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
+
+/*
+ * The 4-bit K/V pool. Of each token, KV head and K or V, groups of 32 consecutive
+ * channels share a scale 2^k; a value is code * 2^k with e2m1 codes (OCP: 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and their negatives). One layer is dense:
+ *   k_cache, v_cache: [num_kv_heads][num_blocks * block_size / 16] tiles of 16 tokens,
+ *                     8 * head_dim bytes each, whose order within a tile is the kernels'
+ *                     (csrc/e2m1.hpp); tokens share no byte;
+ *   scales:           [num_kv_heads][num_blocks * block_size / 16][head_dim] bytes, a
+ *                     tile's K scales, then its V scales. A byte is k + 127, and 255 says
+ *                     that the group's 32 values are NaN.
+ * block_size a multiple of 16, at most 1024; head_dim in {64, 128}; caches and scales
+ * 16-byte aligned; num_blocks * block_size < 2^31. dtype is the pool's, as with the 8-bit
+ * pool above; every value the pool holds is exactly a number of it.
+ *
+ * ir_kv_scatter_q4: ir_kv_scatter into such a layer (slots alike; of rows given the same
+ * slot the last is written in calls of up to 1,024 tokens, in longer ones they must be
+ * identical). A group's scale is the least 2^k with
+ * amax <= 7 * 2^k, k in [-100, 125] (f16: [-23, 13]): 7 is where the largest magnitude would
+ * round past 6, so that each value is off by half a step of the codes at most. Codes are
+ * rounded to nearest even; magnitudes past 6 * 2^125 (f16: 49152) saturate; a group that
+ * holds a NaN or an infinity becomes NaN. Nothing but the written tokens changes, so
+ * calls and workgroups may write one block's tokens in any order.
+ *
+ * ir_rope_kv_scatter_q4: ir_rope_kv_scatter (weights null), or ir_qk_norm_rope_kv_scatter
+ * (weights given), into such a layer, one launch; q_out_dtype as in ir_rope_kv_scatter_q8.
+ *
+ * ir_gather_slots_q4, ir_paged_gather_q4: ir_gather_slots and ir_paged_gather of such a
+ * layer, values of dtype; outputs 16-byte aligned.
+ */
+int ir_kv_scatter_q4(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, void* k_cache, void* v_cache,
+                     uint8_t* scales, int64_t num_blocks, int block_size, const int64_t* slot_mapping,
+                     int64_t n_tokens, int num_kv_heads, int head_dim, int dtype, int32_t* err_flags,
+                     ir_stream_t stream);
+int ir_rope_kv_scatter_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                          int64_t qo_tok_stride, int64_t qo_head_stride, const void* k,
+                          int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_tok_stride, int64_t v_head_stride, const void* q_weight,
+                          const void* k_weight, float eps, const float* cos, const float* sin,
+                          int64_t cs_tok_stride, void* k_cache, void* v_cache, uint8_t* scales,
+                          int64_t num_blocks, int block_size, const int64_t* slot_mapping,
+                          int64_t n_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                          int q_out_dtype, int32_t* err_flags, ir_stream_t stream);
+int ir_gather_slots_q4(const void* k_cache, const void* v_cache, const uint8_t* scales, int64_t num_blocks,
+                       int block_size, const int64_t* slots, int64_t n, int num_kv_heads, int head_dim,
+                       int dtype, void* out_k, void* out_v, int32_t* err_flags, ir_stream_t stream);
+int ir_paged_gather_q4(const void* k_cache, const void* v_cache, const uint8_t* scales, int64_t num_blocks,
+                       int block_size, const int32_t* block_tables, int64_t bt_stride,
+                       int max_blocks_per_seq, const int32_t* context_lens, int num_seqs, int max_ctx,
+                       int num_kv_heads, int head_dim, int dtype, void* out_k, void* out_v,
+                       int32_t* err_flags, ir_stream_t stream);
+
+/*
+ * Attention over the 4-bit pool: the calls of the 8-bit pool, arguments alike (q_dtype
+ * too; a decode plan is built with IR_DTYPE_E2M1 and the layer's strides).
+ */
+int ir_paged_decode_q4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                       const void* k_cache, const void* v_cache, const uint8_t* scales,
+                       int64_t num_blocks, int block_size, const int32_t* block_tables,
+                       int64_t bt_stride, int max_blocks_per_seq, const int32_t* context_lens,
+                       void* out, int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
+                       int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype,
+                       int q_dtype, int partition_tokens, int32_t* counters, int64_t num_counters,
+                       void* workspace, int64_t workspace_bytes, int32_t* err_flags,
+                       ir_stream_t stream);
+int ir_paged_decode_planned_q4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                               const void* k_cache, const void* v_cache, const uint8_t* scales,
+                               void* out, int64_t out_seq_stride, int64_t out_head_stride,
+                               int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                               int max_blocks_per_seq, int block_size, float scale, int dtype,
+                               int q_dtype, int flags, const void* plan, int32_t* counters,
+                               int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                               int32_t* err_flags, ir_stream_t stream);
+int ir_paged_prefill_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                        const void* k_cache, const void* v_cache, const uint8_t* scales,
+                        int64_t num_blocks, int block_size, const int32_t* block_tables,
+                        int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q,
+                        const int32_t* q_start, int num_seqs, int total_q, int max_q_len, void* out,
+                        int64_t out_tok_stride, int64_t out_head_stride, int num_q_heads,
+                        int num_kv_heads, int head_dim, float scale, int dtype, int q_dtype,
+                        void* plan, int64_t plan_bytes, int32_t* err_flags, ir_stream_t stream);
+
+/*
+ * Rotary embedding by positions with several axes (time, height and width of images
+ * and video; one axis is the usual rotation). Pair j of a head, elements j and j + D/2,
+ * turns by positions[axis of j][i] * (its frequency). With y = x, or the per-head norm
+ * x * rsqrt(mean(x^2) + eps) * weight where weights are given:
+ *   out[j]       = scaling * (y[j] * cos - y[j + D/2] * sin),
+ *   out[j + D/2] = scaling * (y[j + D/2] * cos + y[j] * sin),
+ * in fp32, rounded to the output's dtype once.
+ *   positions: int64 [num_axes][n_tokens], pos_axis_stride elements between axes; any
+ *              value, also negative.
+ *   pairs:     device array of head_dim / 2 entries, 16-byte aligned: step = the
+ *              frequency in turns (radians / 2 pi) times 2^64, modulo 2^64; axis in
+ *              [0, num_axes) (another is taken for the nearest of them). position * step
+ *              modulo 2^64 is the angle as a fraction of a turn, off by at most
+ *              |position| * 2^-65 turns however far the position.
+ *   num_axes:  1..IR_ROTARY_MAX_AXES.
+ *   q_out_dtype: dtype, or IR_DTYPE_F32.
+ *
+ * ir_rope_axes: rows q [n_tokens, num_q_heads, head_dim] to q_out and k to k_out (either
+ * may have no heads and null pointers; outputs may alias their inputs where the dtypes
+ * agree); head_dim a multiple of 16 up to 256, with norms 64 or 128.
+ * ir_rope_axes_kv_scatter: k goes to the pool's slots instead and v beside it, as
+ * ir_qk_norm_rope_kv_scatter does; head_dim in {64, 128}.
+ * ir_rope_axes_kv_scatter_q4: the same into a layer of a 4-bit pool (the keys are
+ * quantised as they leave the rotation, from fp32).
+ */
+enum { IR_ROTARY_MAX_AXES = 8 };
+typedef struct {
+  uint64_t step;
+  int32_t axis;
+  int32_t reserved;
+} ir_rotary_pair;
+int ir_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                 int64_t qo_tok_stride, int64_t qo_head_stride, const void* k, int64_t k_tok_stride,
+                 int64_t k_head_stride, void* k_out, int64_t ko_tok_stride, int64_t ko_head_stride,
+                 const void* q_weight, const void* k_weight, float eps, const int64_t* positions,
+                 int64_t pos_axis_stride, int num_axes, const ir_rotary_pair* pairs, float scaling,
+                 int64_t n_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                 int q_out_dtype, ir_stream_t stream);
+int ir_rope_axes_kv_scatter(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                            int64_t qo_tok_stride, int64_t qo_head_stride, const void* k,
+                            int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                            int64_t v_tok_stride, int64_t v_head_stride, const void* q_weight,
+                            const void* k_weight, float eps, const int64_t* positions,
+                            int64_t pos_axis_stride, int num_axes, const ir_rotary_pair* pairs,
+                            float scaling, void* k_cache, void* v_cache, int64_t cache_slot_stride,
+                            int64_t cache_head_stride, int64_t num_slots, const int64_t* slot_mapping,
+                            int64_t n_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                            int q_out_dtype, int32_t* err_flags, ir_stream_t stream);
+int ir_rope_axes_kv_scatter_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                               int64_t qo_tok_stride, int64_t qo_head_stride, const void* k,
+                               int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                               int64_t v_tok_stride, int64_t v_head_stride, const void* q_weight,
+                               const void* k_weight, float eps, const int64_t* positions,
+                               int64_t pos_axis_stride, int num_axes, const ir_rotary_pair* pairs,
+                               float scaling, void* k_cache, void* v_cache, uint8_t* scales,
+                               int64_t num_blocks, int block_size, const int64_t* slot_mapping,
+                               int64_t n_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                               int dtype, int q_out_dtype, int32_t* err_flags, ir_stream_t stream);
 
 /*
  * Read-only HBM streaming roof (a measurement utility; no counterpart in the

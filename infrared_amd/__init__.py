@@ -6,8 +6,18 @@ names and call contracts, and run hand-written HIP kernels through a C ABI
 (``include/infrared_amd.h``, ``libinfrared_amd.so``).
 """
 
-from infrared_amd.paged_attention import paged_attention, rope_paged_attention
-from infrared_amd.paged_kv_cache import PagedContext, PagedKVPool, QuantPagedKVPool
+from infrared_amd.paged_attention import paged_attention, rope_axes_paged_attention, rope_paged_attention
+from infrared_amd.paged_kv_cache import PagedContext, PagedKVPool, Quant4PagedKVPool, QuantPagedKVPool
+from infrared_amd.rotary import RotaryAxes
 
-__all__ = ["PagedContext", "PagedKVPool", "QuantPagedKVPool", "paged_attention", "rope_paged_attention"]
+__all__ = [
+    "PagedContext",
+    "PagedKVPool",
+    "Quant4PagedKVPool",
+    "QuantPagedKVPool",
+    "RotaryAxes",
+    "paged_attention",
+    "rope_axes_paged_attention",
+    "rope_paged_attention",
+]
 __version__ = "0.1.0"

@@ -19,6 +19,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libinfrared
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 DTYPE_E4M3 = 3  # the codes of an 8-bit pool: decode plans only
+DTYPE_E2M1 = 4  # likewise of a 4-bit pool
+ROTARY_MAX_AXES = 8
 _DTYPE_CODES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
 # err_flags bits (IR_ERR_*)
@@ -175,6 +177,58 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_i32,
          _c_i32, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "ir_kv_scatter_q4": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32,
+         _c_i32, _c_p, _c_p],
+    ),
+    "ir_rope_kv_scatter_q4": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
+         _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_p, _c_p],
+    ),
+    "ir_gather_slots_q4": (
+        _c_i32,
+        [_c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "ir_paged_gather_q4": (
+        _c_i32,
+        [_c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p,
+         _c_p, _c_p, _c_p],
+    ),
+    "ir_paged_decode_q4": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i64, _c_i64,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "ir_paged_decode_planned_q4": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_f32, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "ir_paged_prefill_q4": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_i32,
+         _c_i32, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_i32, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "ir_rope_axes": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
+         _c_p, _c_i64, _c_i32, _c_p, _c_f32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p],
+    ),
+    "ir_rope_axes_kv_scatter": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
+         _c_p, _c_i64, _c_i32, _c_p, _c_f32, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_i32, _c_p, _c_p],
+    ),
+    "ir_rope_axes_kv_scatter_q4": (
+        _c_i32,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_f32,
+         _c_p, _c_i64, _c_i32, _c_p, _c_f32, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_i32, _c_p, _c_p],
     ),
 }
 

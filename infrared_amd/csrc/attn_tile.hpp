@@ -17,6 +17,9 @@
 
 namespace ir {
 
+// What a cache holds: the dtype itself, 8-bit codes or 4-bit ones.
+enum { kElements = 0, kCodes8 = 1, kCodes4 = 2 };
+
 template <int DT, int D>
 struct TileShape {
   static constexpr bool k16 = DT != IR_DTYPE_F32;
@@ -244,6 +247,13 @@ __device__ __forceinline__ f32x4 qk_tile(const uint32_t (&k)[TileShape<DT, D>::K
 // max (a wave-uniform branch).
 constexpr float kRescaleSlack = 8.f;
 
+// Over a 4-bit cache fp16 probabilities are held 2^7 times larger, at most 2^15 with the
+// slack: below 2^-14 an fp16 number loses bits, and a tenth of the cache's values are 0, so
+// that an output can be all small probabilities' (2^-32 of the largest is then lost of each, not
+// 2^-25). Sums and maxima carry the factor along, so it is free and cancels.
+template <int DT>
+constexpr float kProbUp = DT == IR_DTYPE_F16 ? 7.f : 0.f;
+
 // Online-softmax update with base-2 scores sv (-inf = key absent) followed by
 // O^T += V^T . P^T. Unless FULL, `vok[r]` says whether key row 4g+r may be
 // read; rows that may not are zeroed so 0 * V never meets a NaN pattern in
@@ -252,16 +262,17 @@ constexpr float kRescaleSlack = 8.f;
 // of LDS, and the probabilities of a 16-bit dtype in two pieces of it (off by 2^-18, fp16
 // 2^-24), so that the output's rounding is all that shows. A product of 32 k-slots holds both
 // pieces, the V rows twice, and takes as long as one of 16.
-template <int DT, int D, bool FULL, bool Q8 = false>
+// UP: probabilities are held 2^UP times larger (st.m is the maximum less UP).
+template <int DT, int D, bool FULL, bool Q8 = false, int UP = 0>
 __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t (&vin)[4][TileShape<DT, D>::VDW],
                                            const bool (&vok)[4], State<D>& st) {
   typedef TileShape<DT, D> Sh;
   constexpr int TILES = Sh::TILES;
   float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
   mx = Q8 ? wave_max_groups_swap(mx) : wave_max_groups(mx);
-  const bool grow = mx > st.m + kRescaleSlack;
+  const bool grow = mx > st.m + (kRescaleSlack + UP);
   if (__any(grow)) {
-    const float m_new = grow ? mx : st.m;
+    const float m_new = grow ? mx - UP : st.m;
     const float alpha = fast_exp2(st.m - m_new);  // 1 if unchanged, 0 from the start value
     st.l *= alpha;
 #pragma unroll

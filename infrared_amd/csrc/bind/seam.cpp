@@ -66,20 +66,39 @@ void check_tables(const char* name, const Tensor& bt, const Tensor& ctx) {
   require(ctx.is_contiguous(), name, ": context_lens must be contiguous");
 }
 
-// One layer of an 8-bit pool: dense codes [num_slots, num_kv_heads, head_dim] in
-// head-major storage, scales [num_kv_heads, num_blocks, 2].
-void code_layer(const char* name, const Tensor& kc, const Tensor& vc, const Tensor& scales, int64_t block_size) {
+// Whether a layer's scales are a 4-bit pool's (else an 8-bit one's).
+bool four_bits(const Tensor& scales) { return scales.scalar_type() == at::kByte; }
+
+// The width of a cache's heads: a 4-bit pool's rows are half as many bytes.
+int64_t head_width(const Tensor& kc, bool four) { return four ? 2 * kc.size(2) : kc.size(2); }
+
+// One layer of a pool of codes: dense codes [num_slots, num_kv_heads, head_dim] (4 bits:
+// head_dim / 2 bytes) in head-major storage, scales [num_kv_heads, num_blocks, 2] (4 bits:
+// [num_kv_heads, num_slots / 16, head_dim] bytes).
+void code_layer(const char* name, const Tensor& kc, const Tensor& vc, const Tensor& scales, int64_t block_size,
+                bool four) {
   require_device({&kc, &vc, &scales});
   cache_layer(name, kc);
-  require(kc.scalar_type() == at::kFloat8_e4m3fn && vc.scalar_type() == at::kFloat8_e4m3fn, name,
-          ": kv_scales go with caches of float8_e4m3fn codes, got ", kc.scalar_type(), " and ", vc.scalar_type());
+  if (four)
+    require(kc.scalar_type() == at::kByte && vc.scalar_type() == at::kByte, name,
+            ": uint8 kv_scales go with caches of uint8 4-bit codes, got ", kc.scalar_type(), " and ", vc.scalar_type());
+  else
+    require(kc.scalar_type() == at::kFloat8_e4m3fn && vc.scalar_type() == at::kFloat8_e4m3fn, name,
+            ": kv_scales go with caches of float8_e4m3fn codes, got ", kc.scalar_type(), " and ", vc.scalar_type());
   require(vc.sizes() == kc.sizes() && vc.strides() == kc.strides(), name,
           ": k_cache and v_cache must have the same shape and strides");
   require(kc.stride(0) == kc.size(2) && (kc.size(1) == 1 || kc.stride(1) == kc.size(0) * kc.size(2)), name,
           ": a cache of codes must be dense [num_kv_heads, num_slots, head_dim] storage");
-  require(scales.scalar_type() == at::kFloat && scales.dim() == 3 && scales.is_contiguous() &&
-              scales.size(0) == kc.size(1) && scales.size(1) * block_size == kc.size(0) && scales.size(2) == 2,
-          name, ": kv_scales must be contiguous fp32 [num_kv_heads, num_blocks, 2]");
+  if (four) {
+    require(kc.size(0) % block_size == 0, name, ": ", kc.size(0), " slots are not whole blocks of ", block_size);
+    require(four_bits(scales) && scales.dim() == 3 && scales.is_contiguous() && scales.size(0) == kc.size(1) &&
+                scales.size(1) * 16 == kc.size(0) && scales.size(2) == 2 * kc.size(2),
+            name, ": kv_scales must be contiguous uint8 [num_kv_heads, num_slots / 16, head_dim]");
+  } else {
+    require(scales.scalar_type() == at::kFloat && scales.dim() == 3 && scales.is_contiguous() &&
+                scales.size(0) == kc.size(1) && scales.size(1) * block_size == kc.size(0) && scales.size(2) == 2,
+            name, ": kv_scales must be contiguous fp32 [num_kv_heads, num_blocks, 2]");
+  }
 }
 
 // An output the caller gave for `like`'s shape (strides are the kernel's to check). One of
@@ -136,7 +155,7 @@ void kv_scatter(const Tensor& kc, const Tensor& vc, const Tensor& k, const Tenso
         "ir_kv_scatter");
 }
 
-// (scales: of an 8-bit pool's layer)
+// (scales: of a layer of a pool of codes)
 Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const OptTensor& scales, const Tensor& bt,
                    const Tensor& ctx, int64_t block_size, double scale, const OptTensor& out_, int64_t partition,
                    const OptTensor& workspace, const OptTensor& err, const OptTensor& counters, int64_t stream) {
@@ -146,9 +165,10 @@ Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const Op
   require(q.dim() == 3, "paged_decode: q must be [B, H_q, D], got ", q.sizes());
   check_block_size("paged_decode: ", block_size);
   const int b = (int)q.size(0), hq = (int)q.size(1), d = (int)q.size(2), h_kv = (int)kc.size(1);
-  require(d == kc.size(2) && (scales || q.scalar_type() == kc.scalar_type()) && vc.sizes() == kc.sizes(),
+  const bool four = scales && four_bits(*scales);
+  if (scales) code_layer("paged_decode", kc, vc, *scales, block_size, four);
+  require(d == head_width(kc, four) && (scales || q.scalar_type() == kc.scalar_type()) && vc.sizes() == kc.sizes(),
           "paged_decode: q / pool shape or dtype mismatch");
-  if (scales) code_layer("paged_decode", kc, vc, *scales, block_size);
   if (scales && out_) given_out("paged_decode", *out_, q, Wide::kLike);
   require(bt.size(0) == b, "paged_decode: block_tables rows != batch");
   unit_last("paged_decode q", q);
@@ -162,6 +182,16 @@ Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const Op
     ws = scratch(workspace, need, q);
     n_ctr = ir_paged_decode_num_counters(b, hq, h_kv);
     ctr = counters_for(counters, n_ctr, q);
+  }
+  if (four) {
+    check(ir_paged_decode_q4(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                             (const uint8_t*)scales->data_ptr(), kc.size(0) / bs, bs, (const int32_t*)bt.data_ptr(),
+                             bt.stride(0), max_blocks, (const int32_t*)ctx.data_ptr(), out.data_ptr(), out.stride(0),
+                             out.stride(1), b, hq, h_kv, d, (float)scale, dtype_code(out), dtype_code(q),
+                             partition > 0 ? part : 0, need > 0 ? (int32_t*)ctr.data_ptr() : nullptr, n_ctr,
+                             need > 0 ? ws.data_ptr() : nullptr, need, (int32_t*)ptr(err), stream_of(stream)),
+          "ir_paged_decode_q4");
+    return out;
   }
   if (scales) {
     check(ir_paged_decode_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
@@ -216,15 +246,25 @@ Tensor planned_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const O
           "paged_decode_planned: pool layout differs from the plan's");
   require(vc.sizes() == kc.sizes() && vc.strides() == kc.strides(),
           "paged_decode_planned: v_cache must match k_cache's shape and strides");
-  require(d == kc.size(2) && (scales || q.scalar_type() == kc.scalar_type()),
+  const bool four = scales && four_bits(*scales);
+  if (scales) code_layer("paged_decode_planned", kc, vc, *scales, bs, four);
+  require(d == head_width(kc, four) && (scales || q.scalar_type() == kc.scalar_type()),
           "paged_decode_planned: q / pool shape or dtype mismatch");
-  if (scales) code_layer("paged_decode_planned", kc, vc, *scales, bs);
   if (scales && out_) given_out("paged_decode_planned", *out_, q, Wide::kLike);
   unit_last("paged_decode_planned q", q);
   const Tensor out = out_ ? *out_ : at::empty({b, hq, d}, q.options());
   const Tensor ws = scratch(workspace, ir_paged_decode_planned_workspace_bytes(b, hq, (int)p_hkv, d), q);
   const int64_t n_ctr = ir_paged_decode_num_counters(b, hq, (int)p_hkv);
   const Tensor ctr = counters_for(counters, n_ctr, q);
+  if (four) {
+    check(ir_paged_decode_planned_q4(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                                     (const uint8_t*)scales->data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+                                     b, hq, (int)p_hkv, d, (int)max_blocks, (int)bs, (float)scale, dtype_code(out),
+                                     dtype_code(q), (int)flags, plan_buf.data_ptr(), (int32_t*)ctr.data_ptr(), n_ctr,
+                                     ws.data_ptr(), ws.numel(), (int32_t*)ptr(err), stream_of(stream)),
+          "ir_paged_decode_planned_q4");
+    return out;
+  }
   if (scales) {
     check(ir_paged_decode_planned_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                                      (const float*)scales->data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), b,
@@ -339,21 +379,30 @@ Tensor rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const 
   return qo;
 }
 
-void kv_scatter_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales, const Tensor& k, const Tensor& v,
-                   const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
-  check_block_size("kv_scatter_q8: ", block_size);
-  code_layer("kv_scatter_q8", kc, vc, scales, block_size);
+void kv_scatter_codes(const char* name, bool four, const Tensor& kc, const Tensor& vc, const Tensor& scales,
+                      const Tensor& k, const Tensor& v, const Tensor& slots, int64_t block_size, const OptTensor& err,
+                      int64_t stream) {
+  check_block_size((std::string(name) + ": ").c_str(), block_size);
+  code_layer(name, kc, vc, scales, block_size, four);
   require_device({&kc, &k, &v, &slots});
-  require(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == kc.size(1) && k.size(2) == kc.size(2),
-          "kv_scatter_q8: k ", k.sizes(), " / v ", v.sizes(), " do not match pool rows ", kc.sizes().slice(1));
-  require(v.scalar_type() == k.scalar_type(), "kv_scatter_q8: dtype mismatch (", k.scalar_type(), ", ",
-          v.scalar_type(), ")");
+  require(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == kc.size(1) && k.size(2) == head_width(kc, four), name,
+          ": k ", k.sizes(), " / v ", v.sizes(), " do not match pool rows [", kc.size(1), ", ", head_width(kc, four),
+          "]");
+  require(v.scalar_type() == k.scalar_type(), name, ": dtype mismatch (", k.scalar_type(), ", ", v.scalar_type(), ")");
   const int64_t n = k.size(0);
-  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n,
-          "kv_scatter_q8: slots must be int64 [", n, "], got ", slots.scalar_type(), " ", slots.sizes());
-  unit_last("kv_scatter_q8 k", k);
-  unit_last("kv_scatter_q8 v", v);
+  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name,
+          ": slots must be int64 [", n, "], got ", slots.scalar_type(), " ", slots.sizes());
+  unit_last(name, k);
+  unit_last(name, v);
   const Tensor s = slots.contiguous();
+  if (four) {
+    check(ir_kv_scatter_q4(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                           kc.data_ptr(), vc.data_ptr(), (uint8_t*)scales.data_ptr(), kc.size(0) / block_size,
+                           (int)block_size, (const int64_t*)s.data_ptr(), n, (int)k.size(1), (int)k.size(2),
+                           dtype_code(k), (int32_t*)ptr(err), stream_of(stream)),
+          "ir_kv_scatter_q4");
+    return;
+  }
   check(ir_kv_scatter_q8(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), kc.data_ptr(),
                          vc.data_ptr(), (float*)scales.data_ptr(), scales.size(1), (int)block_size,
                          (const int64_t*)s.data_ptr(), n, (int)k.size(1), (int)k.size(2), dtype_code(k),
@@ -361,7 +410,17 @@ void kv_scatter_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales, con
         "ir_kv_scatter_q8");
 }
 
-// A layer of an 8-bit pool's tensors (the checks are the layer's).
+void kv_scatter_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales, const Tensor& k, const Tensor& v,
+                   const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
+  kv_scatter_codes("kv_scatter_q8", false, kc, vc, scales, k, v, slots, block_size, err, stream);
+}
+
+void kv_scatter_q4(const Tensor& kc, const Tensor& vc, const Tensor& scales, const Tensor& k, const Tensor& v,
+                   const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
+  kv_scatter_codes("kv_scatter_q4", true, kc, vc, scales, k, v, slots, block_size, err, stream);
+}
+
+// A layer of a pool of codes' tensors (the checks are the layer's).
 Tensor layer_of(const Tensor& t, int64_t layer) { return t.select(0, layer); }
 
 void pool_write_q8(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales, int64_t layer, const Tensor& k,
@@ -370,23 +429,48 @@ void pool_write_q8(const Tensor& k_pool, const Tensor& v_pool, const Tensor& sca
                 stream);
 }
 
-std::tuple<Tensor, Tensor> gather_slots_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales,
-                                           const Tensor& slots, int64_t block_size, at::ScalarType dtype,
-                                           const OptTensor& err, int64_t stream) {
-  check_block_size("gather_slots_q8: ", block_size);
-  code_layer("gather_slots_q8", kc, vc, scales, block_size);
+void pool_write_q4(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales, int64_t layer, const Tensor& k,
+                   const Tensor& v, const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
+  kv_scatter_q4(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), k, v, slots, block_size, err,
+                stream);
+}
+
+std::tuple<Tensor, Tensor> gather_slots_codes(const char* name, bool four, const Tensor& kc, const Tensor& vc,
+                                              const Tensor& scales, const Tensor& slots, int64_t block_size,
+                                              at::ScalarType dtype, const OptTensor& err, int64_t stream) {
+  check_block_size((std::string(name) + ": ").c_str(), block_size);
+  code_layer(name, kc, vc, scales, block_size, four);
   require_device({&kc, &slots});
-  require(slots.scalar_type() == at::kLong, "gather_slots_q8: slots must be int64");
+  require(slots.scalar_type() == at::kLong, name, ": slots must be int64");
   const Tensor flat = slots.contiguous();
-  const int64_t h = kc.size(1), d = kc.size(2);
+  const int64_t h = kc.size(1), d = head_width(kc, four);
   std::vector<int64_t> shape = slots.sizes().vec();
   shape.insert(shape.end(), {h, d});
   const Tensor ok = at::empty(shape, kc.options().dtype(dtype)), ov = at::empty_like(ok);
+  if (four) {
+    check(ir_gather_slots_q4(kc.data_ptr(), vc.data_ptr(), (const uint8_t*)scales.data_ptr(), kc.size(0) / block_size,
+                             (int)block_size, (const int64_t*)flat.data_ptr(), flat.numel(), (int)h, (int)d,
+                             dtype_code(ok), ok.data_ptr(), ov.data_ptr(), (int32_t*)ptr(err), stream_of(stream)),
+          "ir_gather_slots_q4");
+    return {ok, ov};
+  }
   check(ir_gather_slots_q8(kc.data_ptr(), vc.data_ptr(), (const float*)scales.data_ptr(), scales.size(1),
                            (int)block_size, (const int64_t*)flat.data_ptr(), flat.numel(), (int)h, (int)d,
                            dtype_code(ok), ok.data_ptr(), ov.data_ptr(), (int32_t*)ptr(err), stream_of(stream)),
         "ir_gather_slots_q8");
   return {ok, ov};
+}
+
+std::tuple<Tensor, Tensor> gather_slots_q8(const Tensor& kc, const Tensor& vc, const Tensor& scales,
+                                           const Tensor& slots, int64_t block_size, at::ScalarType dtype,
+                                           const OptTensor& err, int64_t stream) {
+  return gather_slots_codes("gather_slots_q8", false, kc, vc, scales, slots, block_size, dtype, err, stream);
+}
+
+std::tuple<Tensor, Tensor> gather_slots_q4(const Tensor& kc, const Tensor& vc, const Tensor& scales,
+                                           const Tensor& slots, int64_t block_size, at::ScalarType dtype,
+                                           const OptTensor& err, int64_t stream) {
+  return gather_slots_codes("gather_slots_q4", true, kc, vc, scales, slots, block_size, dtype, err, stream);
 }
 
 std::tuple<Tensor, Tensor> pool_gather_q8(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales,
@@ -396,23 +480,31 @@ std::tuple<Tensor, Tensor> pool_gather_q8(const Tensor& k_pool, const Tensor& v_
                          dtype, err, stream);
 }
 
-// ir_qk_norm_rope_kv_scatter, and with scales (an 8-bit pool's layer) ir_rope_kv_scatter_q8,
-// whose norms may be absent.
+std::tuple<Tensor, Tensor> pool_gather_q4(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales,
+                                          int64_t layer, const Tensor& slots, int64_t block_size, at::ScalarType dtype,
+                                          const OptTensor& err, int64_t stream) {
+  return gather_slots_q4(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), slots, block_size,
+                         dtype, err, stream);
+}
+
+// ir_qk_norm_rope_kv_scatter, and with scales (a layer of a pool of codes)
+// ir_rope_kv_scatter_q8 or _q4, whose norms may be absent.
 Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& wq,
                             const OptTensor& wk, double eps, const Tensor& cos, const Tensor& sin, const Tensor& kc,
                             const Tensor& vc, const OptTensor& scales, int64_t block_size, const Tensor& slots,
                             const OptTensor& q_out_, const OptTensor& err, int64_t stream) {
-  const char* name = scales ? "rope_kv_scatter_q8" : "qk_norm_rope_kv_scatter";
+  const bool four = scales && four_bits(*scales);
+  const char* name = four ? "rope_kv_scatter_q4" : scales ? "rope_kv_scatter_q8" : "qk_norm_rope_kv_scatter";
   require_device({&q, &k, &v, &cos, &sin, &kc, &vc, &slots});
   cache_layer(name, kc);
   if (scales) {
-    check_block_size("rope_kv_scatter_q8: ", block_size);
-    code_layer(name, kc, vc, *scales, block_size);
+    check_block_size(four ? "rope_kv_scatter_q4: " : "rope_kv_scatter_q8: ", block_size);
+    code_layer(name, kc, vc, *scales, block_size, four);
   }
   require(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes(), name,
           ": q [N, H_q, D], k and v [N, H_kv, D] expected");
   const int64_t n = q.size(0), d = q.size(2);
-  require(k.size(0) == n && k.size(2) == d && k.size(1) == kc.size(1) && d == kc.size(2), name,
+  require(k.size(0) == n && k.size(2) == d && k.size(1) == kc.size(1) && d == head_width(kc, four), name,
           ": k/v rows do not match q or the pool");
   require(q.scalar_type() == k.scalar_type() && v.scalar_type() == k.scalar_type() &&
               (scales || kc.scalar_type() == k.scalar_type()),
@@ -441,6 +533,17 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
   }
   const Tensor qo = q_out_ ? *q_out_ : at::empty_like(q);
   const Tensor s = slots.contiguous();
+  if (four) {
+    check(ir_rope_kv_scatter_q4(q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+                                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                ptr(wq), ptr(wk), (float)eps, (const float*)cos.data_ptr(),
+                                (const float*)sin.data_ptr(), cos.stride(0), kc.data_ptr(), vc.data_ptr(),
+                                (uint8_t*)scales->data_ptr(), kc.size(0) / block_size, (int)block_size,
+                                (const int64_t*)s.data_ptr(), n, (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q),
+                                dtype_code(qo), (int32_t*)ptr(err), stream_of(stream)),
+          "ir_rope_kv_scatter_q4");
+    return qo;
+  }
   if (scales) {
     check(ir_rope_kv_scatter_q8(q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
                                 k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
@@ -460,6 +563,102 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
                                    (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q), (int32_t*)ptr(err),
                                    stream_of(stream)),
         "ir_qk_norm_rope_kv_scatter");
+  return qo;
+}
+
+// The rows, norms and positions that the rotations by axes share; positions [axes, N].
+// Returns them with contiguous rows.
+Tensor check_axes(const char* name, const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
+                  const Tensor& positions, const Tensor& pairs) {
+  require_device({&q, &k, &positions, &pairs});
+  require(q.dim() == 3 && k.dim() == 3 && k.size(0) == q.size(0) && k.size(2) == q.size(2), name,
+          ": q [N, H_q, D] and k [N, H_kv, D] expected, got ", q.sizes(), " and ", k.sizes());
+  require(q.scalar_type() == k.scalar_type(), name, ": dtype mismatch (", q.scalar_type(), ", ", k.scalar_type(), ")");
+  const int64_t d = q.size(2);
+  require(pairs.scalar_type() == at::kLong && pairs.dim() == 2 && pairs.size(0) * 2 == d && pairs.size(1) == 2 &&
+              pairs.is_contiguous(),
+          name, ": the rotary's pairs are for heads of ", pairs.dim() ? 2 * pairs.size(0) : 0, ", q has ", d);
+  require(positions.scalar_type() == at::kLong && positions.dim() == 2 && positions.size(1) == q.size(0), name,
+          ": positions must be int64 [axes, ", q.size(0), "], got ", positions.scalar_type(), " ", positions.sizes());
+  require(wq.has_value() == wk.has_value(), name, ": one norm weight without the other");
+  if (wq) {
+    require_device({&q, &*wq, &*wk});
+    for (const auto& [which, t] : {std::pair<const char*, const Tensor*>{"q_norm", &*wq}, {"k_norm", &*wk}})
+      require(t->dim() == 1 && t->size(0) == d && t->is_contiguous() && t->scalar_type() == q.scalar_type(), name, ": ",
+              which, " must be contiguous [", d, "] of ", q.scalar_type());
+  }
+  unit_last(name, q);
+  unit_last(name, k);
+  return positions.size(1) <= 1 || positions.stride(1) == 1 ? positions : positions.contiguous();
+}
+
+std::tuple<Tensor, Tensor> rope_axes(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& pairs,
+                                     double scaling, const OptTensor& wq, const OptTensor& wk, double eps,
+                                     const OptTensor& q_out_, const OptTensor& k_out_, int64_t stream) {
+  const char* name = "rope_axes";
+  const Tensor pos = check_axes(name, q, k, wq, wk, positions, pairs);
+  if (q_out_) given_out(name, *q_out_, q, Wide::kOut);
+  if (k_out_) {
+    given_out(name, *k_out_, k, Wide::kOut);
+    require(k_out_->scalar_type() == k.scalar_type(), name, ": k_out must be of ", k.scalar_type());
+  }
+  const Tensor qo = q_out_ ? *q_out_ : at::empty(q.sizes(), q.options());
+  const Tensor ko = k_out_ ? *k_out_ : at::empty(k.sizes(), k.options());
+  check(ir_rope_axes(q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k.data_ptr(),
+                     k.stride(0), k.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), ptr(wq), ptr(wk), (float)eps,
+                     (const int64_t*)pos.data_ptr(), pos.stride(0), (int)pos.size(0),
+                     (const ir_rotary_pair*)pairs.data_ptr(), (float)scaling, q.size(0), (int)q.size(1),
+                     (int)k.size(1), (int)q.size(2), dtype_code(q), dtype_code(qo), stream_of(stream)),
+        "ir_rope_axes");
+  return {qo, ko};
+}
+
+Tensor rope_axes_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
+                            const Tensor& pairs, double scaling, const Tensor& kc, const Tensor& vc,
+                            const OptTensor& scales, int64_t block_size, const Tensor& slots, const OptTensor& wq,
+                            const OptTensor& wk, double eps, const OptTensor& q_out_, const OptTensor& err,
+                            int64_t stream) {
+  const char* name = "rope_axes_kv_scatter";
+  const Tensor pos = check_axes(name, q, k, wq, wk, positions, pairs);
+  require_device({&q, &v, &kc, &vc, &slots});
+  cache_layer(name, kc);
+  const bool four = scales.has_value();
+  if (four) {
+    check_block_size("rope_axes_kv_scatter: ", block_size);
+    code_layer(name, kc, vc, *scales, block_size, true);
+  }
+  const int64_t n = q.size(0), d = q.size(2);
+  require(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), name, ": k and v differ");
+  require(k.size(1) == kc.size(1) && d == head_width(kc, four) && (four || kc.scalar_type() == k.scalar_type()), name,
+          ": k/v rows do not match the pool");
+  require(vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && vc.scalar_type() == kc.scalar_type(), name,
+          ": k_cache and v_cache must share shape, strides and dtype");
+  require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name,
+          ": slots must be int64 [", n, "], got ", slots.scalar_type(), " ", slots.sizes());
+  unit_last(name, v);
+  if (q_out_) given_out(name, *q_out_, q, Wide::kOut);
+  const Tensor qo = q_out_ ? *q_out_ : at::empty(q.sizes(), q.options());
+  const Tensor s = slots.contiguous();
+  if (four) {
+    check(ir_rope_axes_kv_scatter_q4(
+              q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k.data_ptr(),
+              k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), ptr(wq), ptr(wk), (float)eps,
+              (const int64_t*)pos.data_ptr(), pos.stride(0), (int)pos.size(0),
+              (const ir_rotary_pair*)pairs.data_ptr(), (float)scaling, kc.data_ptr(), vc.data_ptr(),
+              (uint8_t*)scales->data_ptr(), kc.size(0) / block_size, (int)block_size, (const int64_t*)s.data_ptr(), n,
+              (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q), dtype_code(qo), (int32_t*)ptr(err),
+              stream_of(stream)),
+          "ir_rope_axes_kv_scatter_q4");
+    return qo;
+  }
+  check(ir_rope_axes_kv_scatter(
+            q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k.data_ptr(),
+            k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), ptr(wq), ptr(wk), (float)eps,
+            (const int64_t*)pos.data_ptr(), pos.stride(0), (int)pos.size(0), (const ir_rotary_pair*)pairs.data_ptr(),
+            (float)scaling, kc.data_ptr(), vc.data_ptr(), kc.stride(0), kc.stride(1), kc.size(0),
+            (const int64_t*)s.data_ptr(), n, (int)q.size(1), (int)k.size(1), (int)d, dtype_code(q), dtype_code(qo),
+            (int32_t*)ptr(err), stream_of(stream)),
+        "ir_rope_axes_kv_scatter");
   return qo;
 }
 
@@ -519,9 +718,10 @@ Tensor paged_prefill_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, con
   require_device({&q, &kc, &vc, &bt, &cu, &q_start});
   require(q.dim() == 3, "paged_prefill: q must be [total_q, H_q, D], got ", q.sizes());
   check_block_size("paged_prefill: ", block_size);
-  code_layer("paged_prefill", kc, vc, scales, block_size);
+  const bool four = four_bits(scales);
+  code_layer("paged_prefill", kc, vc, scales, block_size, four);
   const int hq = (int)q.size(1), d = (int)q.size(2), h_kv = (int)kc.size(1);
-  require(d == kc.size(2), "paged_prefill: q / pool shape mismatch");
+  require(d == head_width(kc, four), "paged_prefill: q / pool shape mismatch");
   require(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.stride(1) == 1,
           "paged_prefill: block_tables must be int32 [B, max_blocks] with unit column stride");
   const int64_t b = bt.size(0);
@@ -533,6 +733,17 @@ Tensor paged_prefill_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, con
   if (plan_buf) require_device({&q, &*plan_buf});
   if (out_) given_out("paged_prefill", *out_, q, Wide::kLike);
   const Tensor out = out_ ? *out_ : at::empty(q.sizes(), q.options());
+  if (four) {
+    check(ir_paged_prefill_q4(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                              (const uint8_t*)scales.data_ptr(), kc.size(0) / block_size, (int)block_size,
+                              (const int32_t*)bt.data_ptr(), bt.stride(0), (int)bt.size(1),
+                              (const int32_t*)cu.data_ptr(), (const int32_t*)q_start.data_ptr(), (int)b,
+                              (int)q.size(0), (int)max_q_len, out.data_ptr(), out.stride(0), out.stride(1), hq, h_kv,
+                              d, (float)scale, dtype_code(out), dtype_code(q), ptr(plan_buf),
+                              plan_buf ? plan_buf->numel() : 0, (int32_t*)ptr(err), stream_of(stream)),
+          "ir_paged_prefill_q4");
+    return out;
+  }
   check(ir_paged_prefill_q8(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                             (const float*)scales.data_ptr(), scales.size(1), (int)block_size,
                             (const int32_t*)bt.data_ptr(), bt.stride(0), (int)bt.size(1), (const int32_t*)cu.data_ptr(),
@@ -584,6 +795,12 @@ PYBIND11_MODULE(_seam, m) {
   m.def("pool_write_q8", &pool_write_q8, nogil());
   m.def("pool_gather_q8", &pool_gather_q8, nogil());
   m.def("norm_rope_kv_scatter", &norm_rope_kv_scatter, nogil());
+  m.def("kv_scatter_q4", &kv_scatter_q4, nogil());
+  m.def("gather_slots_q4", &gather_slots_q4, nogil());
+  m.def("pool_write_q4", &pool_write_q4, nogil());
+  m.def("pool_gather_q4", &pool_gather_q4, nogil());
+  m.def("rope_axes", &rope_axes, nogil());
+  m.def("rope_axes_kv_scatter", &rope_axes_kv_scatter, nogil());
   m.def("paged_decode_q8", &paged_decode_q8, nogil());
   m.def("paged_decode_planned_q8", &paged_decode_planned_q8, nogil());
   m.def("paged_prefill_q8", &paged_prefill_q8, nogil());

@@ -4,7 +4,8 @@
 //   rotate_half(y) = (-y2, y1) over the halves of head_dim,
 // in fp32 throughout and rounded once, where it is stored. Without norms
 // (ROTATE) the rotation is ir_rope_kv_scatter's, which rounds the tables, each
-// product and the sum to the dtype as the reference's tensor operations do.
+// product and the sum to the dtype as the reference's tensor operations do. kRowsTurn is
+// the rotation in fp32, as with norms, of rows that have none.
 //
 // head_dim / 16 lanes share a row: each holds 8 elements of its first half and
 // the 8 of the second half that the rotation pairs them with, so only the sum of
@@ -15,7 +16,7 @@
 
 namespace ir {
 
-enum { kRowsPlain = 0, kRowsRotate = 1, kRowsNorm = 2 };
+enum { kRowsPlain = 0, kRowsRotate = 1, kRowsNorm = 2, kRowsTurn = 3 };
 
 struct RowArgs {
   const uint8_t* q;
@@ -39,7 +40,12 @@ struct RowArgs {
 };
 
 // Checks a C call's row arguments (strides in elements of eb bytes, q_out's of qo_eb; the norm
-// weights both given or both null) and fills r; an IR_E* code on refusal.
+// weights both given or both null) and fills r; an IR_E* code on refusal. fill_rows: those
+// but the tables and slots (k and v null where there are none).
+int fill_rows(const char* name, RowArgs& r, const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok,
+              int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
+              int64_t v_head, const void* q_weight, const void* k_weight, float eps, int64_t n_tokens,
+              int num_q_heads, int num_kv_heads, int eb, int qo_eb);
 int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, int64_t q_head, void* q_out,
                   int64_t qo_tok, int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v,
                   int64_t v_tok, int64_t v_head, const void* q_weight, const void* k_weight, float eps,
@@ -108,14 +114,18 @@ template <int DT, int D, int MODE>
 __device__ __forceinline__ void transform_row(float (&x)[16], const float (&w)[16], float eps,
                                               const Angles<DT, D, MODE>& t) {
 #pragma clang fp contract(off)
-  if constexpr (MODE == kRowsNorm) {
-    float ss = 0.f;
+  if constexpr (MODE == kRowsNorm || MODE == kRowsTurn) {
+    if constexpr (MODE == kRowsNorm) {
+      float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
-    const float r = rsqrtf(row_sum<D / 16>(ss) * (1.f / D) + eps);
+      for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
+      const float r = rsqrtf(row_sum<D / 16>(ss) * (1.f / D) + eps);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = x[e] * r * w[e];
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float a = x[e] * r * w[e], b = x[8 + e] * r * w[8 + e];
+      const float a = x[e], b = x[8 + e];
       x[e] = __builtin_fmaf(a, t.c[e], -b * t.s[e]);
       x[8 + e] = __builtin_fmaf(b, t.c[8 + e], a * t.s[8 + e]);
     }

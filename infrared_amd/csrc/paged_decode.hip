@@ -46,10 +46,10 @@ __device__ __forceinline__ void merge_partials(const DecodeArgs& a, int seq, int
 // 16-bit dtypes: two wavefronts per SIMD (<= 256 registers each) keep two
 // resident workgroups' worth of loads in flight per CU. fp32 tiles are twice
 // the registers and run one per SIMD.
-template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH, bool Q8 = false, bool QF = false>
+template <int DT, int D, bool BS16, int NW, bool FUSED, int DEPTH, int FMT = kElements, bool QF = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 ? 1 : 2)))
 void paged_decode_kernel(DecodeArgs a) {
-  typedef CacheFormat<DT, D, Q8> F;
+  typedef CacheFormat<DT, D, FMT> F;
   __shared__ MergeSmem<NW, D> sm;
   __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][F::STAGE];
   __shared__ int s_last;
@@ -80,17 +80,18 @@ void paged_decode_kernel(DecodeArgs a) {
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
   const uint8_t* kc = (const uint8_t*)a.kc + (int64_t)kvh * a.c_head * F::EB;
   const uint8_t* vc = (const uint8_t*)a.vc + (int64_t)kvh * a.c_head * F::EB;
-  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
+  const f32x2* scales = FMT == kCodes8 ? a.scales + kvh * a.num_blocks : nullptr;
+  const uint8_t* scales4 = FMT == kCodes4 ? a.scales4 + kvh * a.c_head / 8 : nullptr;
   const typename F::Offsets lo = F::offsets(lane, a.c_slot * F::EB);
   QueryRegs<DT, D, QF> qr;
-  load_query_for<DT, D, Q8>(a, seq, kvh * a.n_rep + h_local, h_local < a.n_rep, g, qr);
+  load_query_for<DT, D, FMT>(a, seq, kvh * a.n_rep + h_local, h_local < a.n_rep, g, qr);
   qr.split();
 
   State<D> st;
   state_init(st);
   bool bad = false;
-  attend_tiles<DT, D, BS16, NW, DEPTH, Q8, QF>(a, bt_row, kc, vc, scales, lo, qr, tile_lo, tile_hi, t_end, kstage[w],
-                                               lane, w, st, bad);
+  attend_tiles<DT, D, BS16, NW, DEPTH, FMT, QF>(a, bt_row, kc, vc, scales, scales4, lo, qr, tile_lo, tile_hi, t_end,
+                                                kstage[w], lane, w, st, bad);
   if (bad) flag_error(a.err, IR_ERR_BLOCK_RANGE);
   st.l = wave_sum_groups(st.l);
 
@@ -253,16 +254,37 @@ int launch_decode(const DecodeArgs& a, bool bs16, bool fused, hipStream_t s) {
 // heads of 128: 11.9 and 9.1). A workspace sized for the default partition is enough.
 constexpr int kCodePartition = 128;
 
-template <int DT, int D, bool QF>
-int launch_decode_q8(const DecodeArgs& a, bool fused, hipStream_t s) {
+template <int DT, int D, int FMT, bool QF>
+int launch_decode_codes(const char* name, const DecodeArgs& a, bool fused, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * a.n_hg), (unsigned)a.max_parts);
   if (fused || a.max_parts == 1) {
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, true, 2, true, QF>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, true, 2, FMT, QF>), grid, dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, false, 2, true, QF>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, false, 2, FMT, QF>), grid, dim3(256), 0, s, a);
     hipLaunchKernelGGL((paged_decode_reduce<DT, D>), dim3(grid.x), dim3(256), 0, s, a);
   }
-  return check_launch("ir_paged_decode_q8");
+  return check_launch(name);
+}
+
+template <int DT, int FMT, bool QF>
+int launch_decode_codes_d(const char* name, int head_dim, const DecodeArgs& a, bool fused, hipStream_t s) {
+  return head_dim == 128 ? launch_decode_codes<DT, 128, FMT, QF>(name, a, fused, s)
+                         : launch_decode_codes<DT, 64, FMT, QF>(name, a, fused, s);
+}
+
+template <int FMT>
+int dispatch_decode_codes(const char* name, int dtype, bool qf, int head_dim, const DecodeArgs& a, bool fused,
+                          hipStream_t s) {
+  switch (dtype) {
+    case IR_DTYPE_BF16:
+      return qf ? launch_decode_codes_d<IR_DTYPE_BF16, FMT, true>(name, head_dim, a, fused, s)
+                : launch_decode_codes_d<IR_DTYPE_BF16, FMT, false>(name, head_dim, a, fused, s);
+    case IR_DTYPE_F16:
+      return qf ? launch_decode_codes_d<IR_DTYPE_F16, FMT, true>(name, head_dim, a, fused, s)
+                : launch_decode_codes_d<IR_DTYPE_F16, FMT, false>(name, head_dim, a, fused, s);
+    default:
+      return launch_decode_codes_d<IR_DTYPE_F32, FMT, false>(name, head_dim, a, fused, s);
+  }
 }
 
 }  // namespace
@@ -308,8 +330,9 @@ extern "C" int64_t ir_paged_decode_num_counters(int num_seqs, int num_q_heads, i
 
 namespace {
 
-// ir_paged_decode, and with `scales` ir_paged_decode_q8 (a dense layer of codes).
-int decode_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_seq_stride,
+// ir_paged_decode, and with `scales` ir_paged_decode_q8 or _q4 (a dense layer of codes; fmt
+// says of which).
+int decode_call(const char* name, int fmt, const void* scales, int q_dtype, const void* q, int64_t q_seq_stride,
                 int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
                 int64_t cache_head_stride, int64_t num_blocks, int block_size, const int32_t* block_tables,
                 int64_t bt_stride, int max_blocks_per_seq, const int32_t* context_lens, void* out,
@@ -350,11 +373,13 @@ int decode_call(const char* name, const float* scales, int q_dtype, const void* 
   const bool bs16 = block_size % 16 == 0;
   if (scales) {
     IR_REQUIRE(bs16, "%s: block size %d must be a multiple of 16", name, block_size);
-    IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+    const unsigned al = fmt == kCodes4 ? 16 : 8;
+    IR_REQUIRE(((uintptr_t)scales & (al - 1)) == 0, "%s: scales must be %u-byte aligned", name, al);
   }
 
   DecodeArgs a;
   a.scales = (const f32x2*)scales;
+  a.scales4 = (const uint8_t*)scales;
   a.block16 = 0;
   a.merge_later = 0;
   a.q = q;
@@ -407,17 +432,8 @@ int decode_call(const char* name, const float* scales, int q_dtype, const void* 
   hipStream_t s = (hipStream_t)stream;
   if (scales) {
     const bool qf = q_dtype != dtype;
-#define IR_DECODE_Q8(DT_, QF_) \
-  (head_dim == 128 ? launch_decode_q8<DT_, 128, QF_>(a, fused, s) : launch_decode_q8<DT_, 64, QF_>(a, fused, s))
-    switch (dtype) {
-      case IR_DTYPE_BF16:
-        return qf ? IR_DECODE_Q8(IR_DTYPE_BF16, true) : IR_DECODE_Q8(IR_DTYPE_BF16, false);
-      case IR_DTYPE_F16:
-        return qf ? IR_DECODE_Q8(IR_DTYPE_F16, true) : IR_DECODE_Q8(IR_DTYPE_F16, false);
-      default:
-        return IR_DECODE_Q8(IR_DTYPE_F32, false);
-    }
-#undef IR_DECODE_Q8
+    return fmt == kCodes4 ? dispatch_decode_codes<kCodes4>(name, dtype, qf, head_dim, a, fused, s)
+                          : dispatch_decode_codes<kCodes8>(name, dtype, qf, head_dim, a, fused, s);
   }
   switch (dtype) {
     case IR_DTYPE_BF16:
@@ -443,7 +459,7 @@ extern "C" int ir_paged_decode(const void* q, int64_t q_seq_stride, int64_t q_he
                                int head_dim, float scale, int dtype, int partition_tokens,
                                int32_t* counters, int64_t num_counters, void* workspace,
                                int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
-  return decode_call("ir_paged_decode", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+  return decode_call("ir_paged_decode", kElements, nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                      cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride,
                      max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
                      num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
@@ -460,8 +476,25 @@ extern "C" int ir_paged_decode_q8(const void* q, int64_t q_seq_stride, int64_t q
                                   int32_t* err_flags, ir_stream_t stream) {
   if (num_seqs == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_decode_q8: null pointer");
-  return decode_call("ir_paged_decode_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+  return decode_call("ir_paged_decode_q8", kCodes8, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                      head_dim, num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
+                     max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
+                     num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
+                     workspace_bytes, err_flags, stream);
+}
+
+extern "C" int ir_paged_decode_q4(const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* k_cache,
+                                  const void* v_cache, const uint8_t* scales, int64_t num_blocks, int block_size,
+                                  const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                                  const int32_t* context_lens, void* out, int64_t out_seq_stride,
+                                  int64_t out_head_stride, int num_seqs, int num_q_heads, int num_kv_heads,
+                                  int head_dim, float scale, int dtype, int q_dtype, int partition_tokens,
+                                  int32_t* counters, int64_t num_counters, void* workspace, int64_t workspace_bytes,
+                                  int32_t* err_flags, ir_stream_t stream) {
+  if (num_seqs == 0) return ok();
+  IR_REQUIRE(scales, "ir_paged_decode_q4: null pointer");
+  return decode_call("ir_paged_decode_q4", kCodes4, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                     head_dim / 2, num_blocks * block_size * (head_dim / 2), num_blocks, block_size, block_tables, bt_stride,
                      max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
                      num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
                      workspace_bytes, err_flags, stream);

@@ -31,7 +31,7 @@
 #include <type_traits>
 
 #include "attn_tile.hpp"
-#include "e4m3.hpp"
+#include "e2m1.hpp"
 
 namespace ir {
 
@@ -63,6 +63,8 @@ struct DecodeArgs {
   // 8-bit caches: (K, V) scales [kv_head][block], 16-byte units of a block's codes
   const f32x2* scales;
   uint32_t block16;
+  // 4-bit caches: scales [kv_head][tile][D]
+  const uint8_t* scales4;
   int merge_later;  // the planned call's partial rows are merged by a launch of their own
 };
 
@@ -100,8 +102,16 @@ struct CodeTile {
   uint32_t v[4][NI];
 };
 
-// What a kernel streams: tiles of the dtype itself, or of codes.
-template <int DT, int D, bool Q8>
+// A tile of a 4-bit cache as a lane loads it (e2m1.hpp): a third of the 8-bit one's
+// registers, and the operands' order from the start, so that K needs no LDS.
+template <int D>
+struct Code4Tile {
+  uint32_t k[D / 32], v[D / 32];
+  uint32_t ks, vs;  // a byte for the lane's row of K, one for each of its rows of V
+};
+
+// What a kernel streams, by the cache's format.
+template <int DT, int D, int FMT>
 struct CacheFormat {
   typedef Tile<DT, D> Raw;
   typedef LaneOffsets<DT, D> Offsets;
@@ -112,7 +122,7 @@ struct CacheFormat {
   }
 };
 template <int DT, int D>
-struct CacheFormat<DT, D, true> {
+struct CacheFormat<DT, D, kCodes8> {
   typedef CodeTile<D> Raw;
   struct Offsets {
     uint32_t k, v;  // of this lane in a tile
@@ -121,6 +131,21 @@ struct CacheFormat<DT, D, true> {
   static constexpr int STAGE = 16 * D;
   __device__ __forceinline__ static Offsets offsets(int lane, int64_t) {
     return Offsets{(uint32_t)lane * 16u, (uint32_t)lane * (D / 16)};
+  }
+};
+template <int DT, int D>
+struct CacheFormat<DT, D, kCodes4> {
+  typedef Code4Tile<D> Raw;
+  struct Offsets {
+    uint32_t codes, ks, vs;  // of this lane in a tile's codes and scales
+  };
+  static constexpr int EB = 1;      // (strides are in bytes)
+  static constexpr int STAGE = 16;  // (K needs no staging)
+  __device__ __forceinline__ static Offsets offsets(int lane, int64_t) {
+    const int g = lane >> 4, c = lane & 15;
+    // (rows of both operands are in the order that Tile4's scales have)
+    return Offsets{(uint32_t)(lane * Tile4<D>::LB), (uint32_t)(16 * (D == 128 ? g : g >> 1) + c),
+                   (uint32_t)(D / 2 + 4 * (Tile4<D>::NG * g + c / (16 / Tile4<D>::NG)))};
   }
 };
 
@@ -161,7 +186,7 @@ struct QueryRegs<DT, D, true> {
 // Issues a code tile's loads; the tile's first row is at tk / tv.
 template <int DT, int D>
 __device__ __forceinline__ void issue_codes(const uint8_t* tk, const uint8_t* tv,
-                                            const typename CacheFormat<DT, D, true>::Offsets& lo, CodeTile<D>& tl) {
+                                            const typename CacheFormat<DT, D, kCodes8>::Offsets& lo, CodeTile<D>& tl) {
 #pragma unroll
   for (int i = 0; i < CodeTile<D>::NI; ++i) {
     const u32x4 x = __builtin_nontemporal_load((const u32x4*)(tk + lo.k + 1024 * i));
@@ -180,6 +205,19 @@ __device__ __forceinline__ void issue_codes(const uint8_t* tk, const uint8_t* tv
       tl.v[r][0] = __builtin_nontemporal_load((const uint32_t*)(tv + lo.v + 4 * D * r));
     }
   }
+}
+
+// Issues a 4-bit tile's loads; its codes are `at` bytes past kc / vc, 8 times as far as its
+// scales past sc.
+template <int DT, int D>
+__device__ __forceinline__ void issue_codes4(const uint8_t* kc, const uint8_t* vc, const uint8_t* sc, int64_t at,
+                                             const typename CacheFormat<DT, D, kCodes4>::Offsets& lo,
+                                             Code4Tile<D>& tl) {
+  const uint8_t *tk = kc + at, *tv = vc + at, *ts = sc + at / 8;
+  load_dwords_nt<D / 32, true>(tk + lo.codes, tl.k);
+  load_dwords_nt<D / 32, true>(tv + lo.codes, tl.v);
+  tl.ks = __builtin_nontemporal_load(ts + lo.ks);
+  tl.vs = __builtin_nontemporal_load((const uint32_t*)(ts + lo.vs));
 }
 
 // Issues the loads of the tile starting at key t0 and returns a 4-bit mask of
@@ -359,6 +397,62 @@ __device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const Query
   }
 }
 
+// The same for a 4-bit tile. The conversions take a group's scale with them, so the
+// scores need none: a lane's K is one group's, its four rows of V a group each. QF as above.
+template <int DT, int D, bool QF>
+__device__ __forceinline__ void compute_codes4(const Code4Tile<D>& tl, const QueryRegs<DT, D, QF>& q, uint32_t kmask,
+                                               float scale_log2, State<D>& st, bool col_on = true) {
+  typedef TileShape<DT, D> Sh;
+  constexpr int W = Sh::k16 ? 4 : 8;  // dwords of eight elements
+  const float score_scale = q.scaled(scale_log2), ks = scale_of_byte(tl.ks);
+  uint32_t kop[Sh::KDW];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    uint32_t x[W];
+    decode8_e2m1<DT>(tl.k[j], ks, x);
+#pragma unroll
+    for (int i = 0; i < W; ++i) kop[W * j + i] = x[i];
+  }
+  f32x4 s = qk_tile<DT, D>(kop, q.x);
+  if constexpr (QF) s += qk_tile<DT, D>(kop, q.rest);
+  uint32_t v[4][Sh::VDW];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float vs = scale_of_byte((tl.vs >> (8 * r)) & 0xffu);
+    if constexpr (D == 128) {
+      decode8_e2m1<DT>(tl.v[r], vs, v[r]);
+    } else if constexpr (Sh::k16) {
+      const uint32_t w = tl.v[r >> 1] >> (16 * (r & 1));
+      v[r][0] = decode2_e2m1<DT, 0>(w, vs);
+      v[r][1] = decode2_e2m1<DT, 1>(w, vs);
+    } else {
+      const uint32_t w = tl.v[r >> 1] >> (16 * (r & 1));
+      const f32x2 a = decode2_e2m1_f32<0>(w, vs), b = decode2_e2m1_f32<1>(w, vs);
+      v[r][0] = __float_as_uint(a[0]);
+      v[r][1] = __float_as_uint(a[1]);
+      v[r][2] = __float_as_uint(b[0]);
+      v[r][3] = __float_as_uint(b[1]);
+    }
+  }
+  float sv[4];
+  bool vok[4];
+  if (__all(kmask == 0xfu)) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vok[r] = true;
+      sv[r] = col_on ? s[r] * score_scale : kNegInf;
+    }
+    softmax_pv<DT, D, true, true, (int)kProbUp<DT>>(sv, v, vok, st);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vok[r] = (kmask >> r) & 1u;
+      sv[r] = vok[r] && col_on ? s[r] * score_scale : kNegInf;
+    }
+    softmax_pv<DT, D, false, true, (int)kProbUp<DT>>(sv, v, vok, st);
+  }
+}
+
 // Context length of `seq`, clamped to what its block table can hold (flagged).
 __device__ __forceinline__ int clamp_ctx(const DecodeArgs& a, int seq, bool report) {
   int ctx = a.ctx[seq];
@@ -374,14 +468,14 @@ __device__ __forceinline__ int clamp_ctx(const DecodeArgs& a, int seq, bool repo
 // (wavefront w takes tiles tile_lo + w, tile_lo + w + NW, ...) into st. Keys
 // at or past t_end are masked. Runs of up to NW * kMaxWaveTiles tiles: each
 // run fetches its block ids once, one per lane.
-template <int DT, int D, bool BS16, int NW, int DEPTH, bool Q8, bool QF>
+template <int DT, int D, bool BS16, int NW, int DEPTH, int FMT, bool QF>
 __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t* bt_row, const uint8_t* kc,
-                                             const uint8_t* vc, const f32x2* scales,
-                                             const typename CacheFormat<DT, D, Q8>::Offsets& lo,
+                                             const uint8_t* vc, const f32x2* scales, const uint8_t* scales4,
+                                             const typename CacheFormat<DT, D, FMT>::Offsets& lo,
                                              const QueryRegs<DT, D, QF>& qr, int tile_lo, int tile_hi, int t_end,
                                              uint8_t* kst, int lane, int w, State<D>& st, bool& bad) {
-  static_assert(BS16 || !Q8, "a block of codes holds whole tiles");
-  typedef typename CacheFormat<DT, D, Q8>::Raw Raw;
+  static_assert(BS16 || FMT == kElements, "a block of codes holds whole tiles");
+  typedef typename CacheFormat<DT, D, FMT>::Raw Raw;
   constexpr int RUN = NW * kMaxWaveTiles;
   for (int r0 = tile_lo; r0 < tile_hi; r0 += RUN) {
     const int ntiles = min(tile_hi - r0, RUN);
@@ -393,17 +487,18 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
       if (lane < my_tiles) bid_lane = bt_row[(t_begin + 16 * (w + NW * lane)) / a.bs];
     }
     f32x2 sc = {0.f, 0.f};  // scales of this lane's tile
-    if constexpr (Q8) {
+    if constexpr (FMT == kCodes8) {
       if (lane < my_tiles && bid_lane >= 0 && (int64_t)bid_lane < a.num_blocks) sc = scales[bid_lane];
     }
     auto issue = [&](int i, Raw& tl) -> uint32_t {
       const int32_t bid = BS16 ? __builtin_amdgcn_readlane(bid_lane, i) : 0;
-      if constexpr (Q8) {
+      if constexpr (FMT != kElements) {
         const int g = lane >> 4, t0 = t_begin + 16 * (w + NW * i), blk = t0 / a.bs;
         const bool ok = bid >= 0 && (int64_t)bid < a.num_blocks;
         bad |= !ok;
         const int64_t at = ok ? ((int64_t)bid * a.bs + (t0 - blk * a.bs)) * D : 0;
-        issue_codes<DT, D>(kc + at, vc + at, lo, tl);
+        if constexpr (FMT == kCodes4) issue_codes4<DT, D>(kc, vc, scales4, at / 2, lo, tl);
+        else issue_codes<DT, D>(kc + at, vc + at, lo, tl);
         uint32_t m = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) m |= (ok && t0 + 4 * r + g < t_end) ? (1u << r) : 0u;
@@ -417,7 +512,9 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     Raw ring[DEPTH];
     uint32_t mk[DEPTH];
     auto compute = [&](const Raw& tl, int i, uint32_t mask) {
-      if constexpr (Q8) {
+      if constexpr (FMT == kCodes4) {
+        compute_codes4<DT, D, QF>(tl, qr, mask, a.scale_log2, st);
+      } else if constexpr (FMT == kCodes8) {
         const int ii = min(i, last);
         const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[0]), ii));
         const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[1]), ii));
@@ -463,19 +560,22 @@ __device__ __forceinline__ void load_query(const DecodeArgs& a, int seq, int qh,
     zero_dwords(qr);
 }
 
-// The query operand that goes with code tiles (compute_codes), before its split().
-template <int DT, int D, bool QF>
+// The query operand that goes with code tiles (compute_codes; K4: compute_codes4, whose lane
+// group holds a quarter of the row in one run), before its split().
+template <int DT, int D, bool QF, bool K4>
 __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
                                                  QueryRegs<DT, D, QF>& q) {
   typedef TileShape<DT, D> Sh;
   constexpr int EB = QF ? 4 : Sh::EB;
   constexpr int DW = 4 * EB;  // dwords of 16 elements
-  const uint8_t* row = (const uint8_t*)a.q + ((int64_t)seq * a.q_seq + (int64_t)qh * a.q_head + 16 * g) * EB;
+  constexpr int STEP = K4 ? 16 : 64;
+  const uint8_t* row =
+      (const uint8_t*)a.q + ((int64_t)seq * a.q_seq + (int64_t)qh * a.q_head + (K4 ? D / 4 : 16) * g) * EB;
 #pragma unroll
   for (int j = 0; j < D / 64; ++j)
 #pragma unroll
     for (int i = 0; i < DW; i += 4) {
-      const u32x4 x = head_ok ? *(const u32x4*)(row + 64 * j * EB + 4 * i) : u32x4{0u, 0u, 0u, 0u};
+      const u32x4 x = head_ok ? *(const u32x4*)(row + STEP * j * EB + 4 * i) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = DW * j + i + e;
@@ -489,11 +589,11 @@ __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, i
     }
 }
 
-template <int DT, int D, bool Q8, bool QF>
+template <int DT, int D, int FMT, bool QF>
 __device__ __forceinline__ void load_query_for(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
                                                QueryRegs<DT, D, QF>& q) {
-  static_assert(Q8 || !QF, "16-bit caches take queries of their dtype");
-  if constexpr (Q8) load_query_codes<DT, D>(a, seq, qh, head_ok, g, q);
+  static_assert(FMT != kElements || !QF, "16-bit caches take queries of their dtype");
+  if constexpr (FMT != kElements) load_query_codes<DT, D, QF, FMT == kCodes4>(a, seq, qh, head_ok, g, q);
   else load_query<DT, D>(a, seq, qh, head_ok, g, q.x);
 }
 

@@ -52,13 +52,19 @@ constexpr int kPlanWaves = 4;       // streaming wavefronts per workgroup
 // sequences of 512..4096 keys: 45.1 us with four, 33.5 with eight, whatever the number
 // of tiles in flight; twelve are short of registers, 46.5).
 constexpr int kCodeWaves = 8;
+// Of a call over a 4-bit cache.
+constexpr int kCode4Waves = 8;
+constexpr int kMaxWaves = std::max(kPlanWaves, std::max(kCodeWaves, kCode4Waves));
 constexpr int kCodePlan = 1 << 16;  // (above any number of pairs)
+
+// A plan's wavefronts by the format of the cache it is for.
+constexpr int plan_waves(int fmt) { return fmt == kCodes4 ? kCode4Waves : fmt == kCodes8 ? kCodeWaves : kPlanWaves; }
 constexpr int kPlanRun = 64;        // tile facts per wavefront and run (one per lane)
 constexpr int kPlanMinTiles = 16;   // smallest slice
 
 // Plan regions (byte offsets, 256-byte aligned):
-//   hdr[8]             T, R, number of sequences with no usable key, number of pairs (kCodePlan
-//                      added in a plan of kCodeWaves wavefronts, whose regions lie elsewhere)
+//   hdr[8]             T, R, number of sequences with no usable key, number of pairs (plus kCodePlan
+//                      times the cache's format, whose wavefronts say where the regions lie)
 //   seq_pre[B + 1]     list tiles before sequence b, per unit
 //   empty[B]           sequences with no usable key
 //   share[B]           shared 16-key tiles of sequences b, b + 1 (ir_paged_decode_plan's pair scan)
@@ -261,9 +267,9 @@ __global__ __launch_bounds__(kPairThreads) void paged_decode_pair_kernel(PlanArg
 // prefix sum, one int32 per sequence), finds its slice, and writes its
 // wavefronts' headers and tile facts; workgroup 0 also writes the header, the
 // prefix sums, the list of sequences with no usable key and the pairs.
-template <int NW>
-__global__ __launch_bounds__(NW * 64) void paged_decode_plan_kernel(PlanArgs p) {
-  constexpr int NT = NW * 64;
+template <int FMT>
+__global__ __launch_bounds__(plan_waves(FMT) * 64) void paged_decode_plan_kernel(PlanArgs p) {
+  constexpr int NW = plan_waves(FMT), NT = NW * 64;
   __shared__ int s_pre[kPlanMaxSeqs + 1];
   __shared__ int s_ctx[kPlanMaxSeqs];
   __shared__ int s_share[kPlanMaxSeqs];  // shared tiles of pair (b, b + 1) / of a pair's first sequence
@@ -377,7 +383,7 @@ __global__ __launch_bounds__(NW * 64) void paged_decode_plan_kernel(PlanArgs p) 
     hdr[0] = T;
     hdr[1] = R;
     hdr[2] = s_nempty;
-    hdr[3] = s_npairs + (NW == kCodeWaves ? kCodePlan : 0);
+    hdr[3] = s_npairs + FMT * kCodePlan;
   }
   int32_t* wh = (int32_t*)(p.plan + p.ly.whdr) + ((int64_t)grp * NW + w) * 8;
   if (lo >= hi) {
@@ -491,14 +497,15 @@ __device__ __forceinline__ void slot_read(const float* row, int g, f32x4 (&acc)[
 // arguments over in SGPRs at wave start, so the plan reads do not wait for a
 // kernel-argument load.
 //
-// Q8: the tiles are codes; a run's lanes also fetch the scales of their tiles, whose
+// kCodes8: the tiles are codes; a run's lanes also fetch the scales of their tiles, whose
 // block the tile's pool offset gives (the layer is dense), ahead of the tiles' own loads.
-template <int DT, int D, int NW, int DEPTH, bool PAIRS, bool Q8 = false, bool QF = false>
+// kCodes4: a tile's scales are loaded with it.
+template <int DT, int D, int NW, int DEPTH, bool PAIRS, int FMT = kElements, bool QF = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 && NW == 4 ? 1 : 2)))
 void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32_t o_pair, uint32_t o_whdr,
                                  uint32_t o_first, int B, DecodeArgs a, PlanLayout ly) {
   typedef TileShape<DT, D> Sh;
-  typedef CacheFormat<DT, D, Q8> F;
+  typedef CacheFormat<DT, D, FMT> F;
   constexpr int EB = Sh::EB;
   constexpr int NT = NW * 64;
   constexpr int TILES = D / 16;
@@ -529,7 +536,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   const int pre0 = tid <= B ? sp[tid] : 0;  // every sequence's when B < NT
   const int pair0 = PAIRS && tid < B ? pp[tid] : 0;
   const u32x4 h4 = *(const u32x4*)hdr;
-  const int R = (int)h4[1], hdr_pairs = (int)h4[3] - (Q8 ? kCodePlan : 0);
+  const int R = (int)h4[1], hdr_pairs = (int)h4[3] - FMT * kCodePlan;
   // the wavefront's header in two 16-byte reads (the plan is 256-byte
   // aligned), so the select below cannot become a skipped load
   const u32x4 wh0 = *(const u32x4*)wh, wh1 = *(const u32x4*)(wh + 4);
@@ -593,11 +600,11 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     const int kvh = a.n_hg == 1 ? j : fdiv(j, a.n_hg);
     if (paired(b)) {  // columns 0..n_rep-1: sequence b, n_rep..2 n_rep-1: b + 1
       const int second = c >= a.n_rep;
-      load_query_for<DT, D, Q8>(a, b + second, kvh * a.n_rep + c - second * a.n_rep, c < 2 * a.n_rep, g, dst);
+      load_query_for<DT, D, FMT>(a, b + second, kvh * a.n_rep + c - second * a.n_rep, c < 2 * a.n_rep, g, dst);
       return;
     }
     const int hl = hg * 16 + c;
-    load_query_for<DT, D, Q8>(a, b, kvh * a.n_rep + hl, hl < a.n_rep, g, dst);
+    load_query_for<DT, D, FMT>(a, b, kvh * a.n_rep + hl, hl < a.n_rep, g, dst);
   };
   QueryRegs<DT, D, QF> qr, qn;
   int q_lbl = -1, qn_lbl = -1;
@@ -681,7 +688,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     const int cnt = min(kPlanRun, cnt_w - r0);
     const int last = cnt - 1;
     f32x2 sc = {0.f, 0.f};
-    if constexpr (Q8) {
+    if constexpr (FMT == kCodes8) {
       if (lane < cnt) sc = a.scales[info_off / a.block16];
     }
     // Issues the loads of tile i of the run (`real`: i is known to be a tile of
@@ -694,7 +701,9 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       const uint32_t off = (uint32_t)__builtin_amdgcn_readlane((int)info_off, ii);
       const uint32_t meta = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, ii);
       if (real || i <= last) {
-        if constexpr (Q8) issue_codes<DT, D>(kc + ((uint64_t)off << 4), vc + ((uint64_t)off << 4), lo_off, tl);
+        if constexpr (FMT == kCodes4) issue_codes4<DT, D>(kc, vc, a.scales4, (int64_t)off << 4, lo_off, tl);
+        else if constexpr (FMT == kCodes8)
+          issue_codes<DT, D>(kc + ((uint64_t)off << 4), vc + ((uint64_t)off << 4), lo_off, tl);
         else issue_tile<DT, D>(kc, vc, off, lo_off, tl);
       }
       lb = (int)(meta >> 7);
@@ -727,7 +736,9 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
           qn_lbl = cur + 1;
         }
       }
-      if constexpr (Q8) {
+      if constexpr (FMT == kCodes4) {
+        compute_codes4<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, st, con[r]);
+      } else if constexpr (FMT == kCodes8) {
         const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
         const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
         compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, ks, vs, kstage[w], lane, st, con[r]);
@@ -796,7 +807,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       if (d0 == 0) store_dev2(r_ml, rr * 8, f32x2{stg.m[k][hc], stg.l[k][hc]});
     }
   }
-  if constexpr (Q8) {
+  if constexpr (FMT != kElements) {
     if (a.merge_later) {
       if (pend >= 0) write_out(label(pend));
       return;
@@ -886,13 +897,14 @@ constexpr int kMergeThreads = 256;
 
 template <int DT, int D>
 __global__ __launch_bounds__(kMergeThreads) void paged_decode_planned_merge(const uint8_t* plan, uint32_t o_seq_pre,
-                                                                            uint32_t o_pair, int pairs, DecodeArgs a) {
+                                                                            uint32_t o_pair, int pairs, int fmt,
+                                                                            DecodeArgs a) {
   constexpr int EB = TileShape<DT, D>::EB, LPR = D / 4, G = kMergeThreads / LPR;
   __shared__ float s_part[G][D + 2];
   const int32_t* hdr = (const int32_t*)plan;
   const int32_t* pre = (const int32_t*)(plan + o_seq_pre);
   const int R = hdr[1];
-  const int hdr_pairs = hdr[3] - kCodePlan;
+  const int hdr_pairs = hdr[3] - fmt * kCodePlan;
   if (pairs ? (uint32_t)hdr_pairs >= kCodePlan : hdr_pairs != 0) return;  // (flagged by the run)
   const int u = blockIdx.x, col = blockIdx.y;
   const int b = u / a.n_ups, j = u - b * a.n_ups;
@@ -948,20 +960,45 @@ __global__ __launch_bounds__(kMergeThreads) void paged_decode_planned_merge(cons
              L > 0.f ? 1.f / L : 0.f);
 }
 
-template <int DT, int D, bool QF>
-void launch_planned_q8(const DecodeArgs& a, const uint8_t* plan, const PlanLayout& ly, int grid, bool pairs,
-                       hipStream_t s) {
+template <int DT, int D, int FMT, bool QF>
+void launch_planned_codes(const DecodeArgs& a, const uint8_t* plan, const PlanLayout& ly, int grid, bool pairs,
+                          hipStream_t s) {
   const uint32_t o_sp = (uint32_t)ly.seq_pre, o_pr = (uint32_t)ly.pair, o_wh = (uint32_t)ly.whdr,
                  o_fi = (uint32_t)ly.first;
+  constexpr int NW = plan_waves(FMT), DEPTH = FMT == kCodes4 ? 2 : 1;
   if (pairs)
-    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, true, true, QF>), dim3(grid),
-                       dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, NW, DEPTH, true, FMT, QF>), dim3(grid), dim3(NW * 64), 0, s,
+                       plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
   else
-    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, kCodeWaves, 1, false, true, QF>), dim3(grid),
-                       dim3(kCodeWaves * 64), 0, s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
+    hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, NW, DEPTH, false, FMT, QF>), dim3(grid), dim3(NW * 64), 0,
+                       s, plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
   if (a.merge_later)
     hipLaunchKernelGGL((paged_decode_planned_merge<DT, D>), dim3(a.num_seqs * a.n_ups, std::min(16, 2 * a.n_rep)),
-                       dim3(kMergeThreads), 0, s, plan, o_sp, o_pr, pairs ? 1 : 0, a);
+                       dim3(kMergeThreads), 0, s, plan, o_sp, o_pr, pairs ? 1 : 0, FMT, a);
+}
+
+template <int DT, int FMT, bool QF>
+void launch_planned_codes_d(int head_dim, const DecodeArgs& a, const uint8_t* plan, const PlanLayout& ly, int grid,
+                            bool pairs, hipStream_t s) {
+  if (head_dim == 128) launch_planned_codes<DT, 128, FMT, QF>(a, plan, ly, grid, pairs, s);
+  else launch_planned_codes<DT, 64, FMT, QF>(a, plan, ly, grid, pairs, s);
+}
+
+template <int FMT>
+void dispatch_planned_codes(int dtype, bool qf, int head_dim, const DecodeArgs& a, const uint8_t* plan,
+                            const PlanLayout& ly, int grid, bool pairs, hipStream_t s) {
+  switch (dtype) {
+    case IR_DTYPE_BF16:
+      qf ? launch_planned_codes_d<IR_DTYPE_BF16, FMT, true>(head_dim, a, plan, ly, grid, pairs, s)
+         : launch_planned_codes_d<IR_DTYPE_BF16, FMT, false>(head_dim, a, plan, ly, grid, pairs, s);
+      break;
+    case IR_DTYPE_F16:
+      qf ? launch_planned_codes_d<IR_DTYPE_F16, FMT, true>(head_dim, a, plan, ly, grid, pairs, s)
+         : launch_planned_codes_d<IR_DTYPE_F16, FMT, false>(head_dim, a, plan, ly, grid, pairs, s);
+      break;
+    default:
+      launch_planned_codes_d<IR_DTYPE_F32, FMT, false>(head_dim, a, plan, ly, grid, pairs, s);
+  }
 }
 
 // Pairs fit one unit's 16 MFMA columns when a KV head has at most 8 query
@@ -1000,7 +1037,7 @@ extern "C" int64_t ir_paged_decode_plan_bytes(int num_seqs, int num_q_heads, int
   // (of the larger kind, whichever is built: a run reads its wavefront's part of the plan before
   // it knows whether the plan is of its kind)
   return plan_layout(num_seqs, device_cus(), t_cap_of(num_seqs, n_ups, max_blocks_per_seq, block_size),
-                     std::max(kPlanWaves, kCodeWaves))
+                     kMaxWaves)
       .total;
 }
 
@@ -1016,7 +1053,8 @@ extern "C" int ir_paged_decode_plan(const int32_t* block_tables, int64_t bt_stri
                                     int block_size, int64_t num_blocks, int64_t cache_slot_stride,
                                     int64_t cache_head_stride, int dtype, int flags, void* plan, int64_t plan_bytes,
                                     int32_t* err_flags, ir_stream_t stream) {
-  const int eb = dtype == IR_DTYPE_E4M3 ? 1 : dtype_bytes(dtype);
+  const int fmt = dtype == IR_DTYPE_E2M1 ? kCodes4 : dtype == IR_DTYPE_E4M3 ? kCodes8 : kElements;
+  const int eb = fmt != kElements ? 1 : dtype_bytes(dtype);  // (of the unit that strides are in)
   IR_REQUIRE(eb > 0, "ir_paged_decode_plan: unknown dtype %d", dtype);
   IR_REQUIRE((flags & ~IR_PLAN_SHARE_GROUPS) == 0, "ir_paged_decode_plan: unknown flags 0x%x", flags);
   IR_REQUIRE(plannable(num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size),
@@ -1050,26 +1088,22 @@ extern "C" int ir_paged_decode_plan(const int32_t* block_tables, int64_t bt_stri
   p.pairs = (flags & IR_PLAN_SHARE_GROUPS) && pairs_fit(num_q_heads, num_kv_heads);
   p.plan = (uint8_t*)plan;
   const int grid = device_cus();
-  const bool codes = dtype == IR_DTYPE_E4M3;
-  p.ly = plan_layout(num_seqs, grid, t_cap_of(num_seqs, p.n_ups, max_blocks_per_seq, block_size),
-                     codes ? kCodeWaves : kPlanWaves);
+  p.ly = plan_layout(num_seqs, grid, t_cap_of(num_seqs, p.n_ups, max_blocks_per_seq, block_size), plan_waves(fmt));
   p.err = err_flags;
   if (p.pairs)
     hipLaunchKernelGGL(paged_decode_pair_kernel, dim3(num_seqs), dim3(kPairThreads), 0, (hipStream_t)stream, p);
-  if (codes)
-    hipLaunchKernelGGL((paged_decode_plan_kernel<kCodeWaves>), dim3(grid), dim3(kCodeWaves * 64), 0,
-                       (hipStream_t)stream, p);
-  else
-    hipLaunchKernelGGL((paged_decode_plan_kernel<kPlanWaves>), dim3(grid), dim3(kPlanWaves * 64), 0,
-                       (hipStream_t)stream, p);
+  const dim3 g(grid), block(plan_waves(fmt) * 64);
+  if (fmt == kCodes4) hipLaunchKernelGGL((paged_decode_plan_kernel<kCodes4>), g, block, 0, (hipStream_t)stream, p);
+  else if (fmt == kCodes8) hipLaunchKernelGGL((paged_decode_plan_kernel<kCodes8>), g, block, 0, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL((paged_decode_plan_kernel<kElements>), g, block, 0, (hipStream_t)stream, p);
   return check_launch("ir_paged_decode_plan");
 }
 
 namespace {
 
-// ir_paged_decode_planned, and with `scales` ir_paged_decode_planned_q8 (a dense
-// layer of codes).
-int planned_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_seq_stride,
+// ir_paged_decode_planned, and with `scales` ir_paged_decode_planned_q8 or _q4 (a dense
+// layer of codes; fmt says of which).
+int planned_call(const char* name, int fmt, const void* scales, int q_dtype, const void* q, int64_t q_seq_stride,
                  int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
                  void* out, int64_t out_seq_stride, int64_t out_head_stride, int num_seqs, int num_q_heads,
                  int num_kv_heads, int head_dim, int max_blocks_per_seq, int block_size, float scale, int dtype,
@@ -1123,6 +1157,7 @@ int planned_call(const char* name, const float* scales, int q_dtype, const void*
   a.scale_log2 = scale * kLog2e;
   a.err = err_flags;
   a.scales = (const f32x2*)scales;
+  a.scales4 = (const uint8_t*)scales;
   a.block16 = (uint32_t)(block_size * (head_dim / 16));
   a.merge_later = scales && units * kMergeSlices <= grid;
   a.counters = counters;
@@ -1130,27 +1165,16 @@ int planned_call(const char* name, const float* scales, int q_dtype, const void*
   a.ws_ml = (float*)((uint8_t*)workspace + ws.acc_bytes);
   const PlanLayout ly =
       plan_layout(num_seqs, grid, t_cap_of(num_seqs, a.n_ups, max_blocks_per_seq, block_size),
-                  scales ? kCodeWaves : kPlanWaves);
+                  plan_waves(fmt));
   const uint8_t* pl = (const uint8_t*)plan;
   hipStream_t s = (hipStream_t)stream;
   const bool pairs = (flags & IR_PLAN_SHARE_GROUPS) && pairs_fit(num_q_heads, num_kv_heads);
   if (scales) {
-    IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+    const unsigned al = fmt == kCodes4 ? 16 : 8;
+    IR_REQUIRE(((uintptr_t)scales & (al - 1)) == 0, "%s: scales must be %u-byte aligned", name, al);
     const bool qf = q_dtype != dtype;
-#define IR_PLANNED_Q8(DT_, QF_)                                                   \
-  (head_dim == 128 ? launch_planned_q8<DT_, 128, QF_>(a, pl, ly, grid, pairs, s) \
-                   : launch_planned_q8<DT_, 64, QF_>(a, pl, ly, grid, pairs, s))
-    switch (dtype) {
-      case IR_DTYPE_BF16:
-        qf ? IR_PLANNED_Q8(IR_DTYPE_BF16, true) : IR_PLANNED_Q8(IR_DTYPE_BF16, false);
-        break;
-      case IR_DTYPE_F16:
-        qf ? IR_PLANNED_Q8(IR_DTYPE_F16, true) : IR_PLANNED_Q8(IR_DTYPE_F16, false);
-        break;
-      default:
-        IR_PLANNED_Q8(IR_DTYPE_F32, false);
-    }
-#undef IR_PLANNED_Q8
+    if (fmt == kCodes4) dispatch_planned_codes<kCodes4>(dtype, qf, head_dim, a, pl, ly, grid, pairs, s);
+    else dispatch_planned_codes<kCodes8>(dtype, qf, head_dim, a, pl, ly, grid, pairs, s);
     return check_launch(name);
   }
   switch (dtype) {
@@ -1178,7 +1202,7 @@ extern "C" int ir_paged_decode_planned(const void* q, int64_t q_seq_stride, int6
                                        int block_size, float scale, int dtype, int flags, const void* plan,
                                        int32_t* counters, int64_t num_counters, void* workspace,
                                        int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
-  return planned_call("ir_paged_decode_planned", nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+  return planned_call("ir_paged_decode_planned", kElements, nullptr, dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                       cache_slot_stride, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads,
                       head_dim, max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters,
                       workspace, workspace_bytes, err_flags, stream);
@@ -1192,8 +1216,22 @@ extern "C" int ir_paged_decode_planned_q8(const void* q, int64_t q_seq_stride, i
                                           const void* plan, int32_t* counters, int64_t num_counters, void* workspace,
                                           int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   IR_REQUIRE(scales, "ir_paged_decode_planned_q8: null pointer");
-  return planned_call("ir_paged_decode_planned_q8", scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+  return planned_call("ir_paged_decode_planned_q8", kCodes8, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
                       head_dim, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                      max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
+                      workspace_bytes, err_flags, stream);
+}
+
+extern "C" int ir_paged_decode_planned_q4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                                          const void* k_cache, const void* v_cache, const uint8_t* scales, void* out,
+                                          int64_t out_seq_stride, int64_t out_head_stride, int num_seqs,
+                                          int num_q_heads, int num_kv_heads, int head_dim, int max_blocks_per_seq,
+                                          int block_size, float scale, int dtype, int q_dtype, int flags,
+                                          const void* plan, int32_t* counters, int64_t num_counters, void* workspace,
+                                          int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
+  IR_REQUIRE(scales, "ir_paged_decode_planned_q4: null pointer");
+  return planned_call("ir_paged_decode_planned_q4", kCodes4, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
+                      head_dim / 2, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
                       max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
                       workspace_bytes, err_flags, stream);
 }

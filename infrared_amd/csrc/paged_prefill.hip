@@ -69,7 +69,7 @@
 #include <type_traits>
 
 #include "attn_tile.hpp"
-#include "e4m3.hpp"
+#include "e2m1.hpp"
 #include "status.hpp"
 
 namespace ir {
@@ -125,6 +125,7 @@ struct PrefillArgs {
   int64_t n_work;  // attending workgroups (the grid less the writers)
   // 8-bit caches: (K, V) scales [kv head][block] (null: the caches are of the dtype)
   const f32x2* scales;
+  const uint8_t* scales4;  // 4-bit caches: [kv head][tile][D]
 };
 
 // 16-byte pieces a writer lane moves, all loads in flight before any store.
@@ -189,13 +190,14 @@ struct PShape {
 // and <= 256 registers, so two 4-wavefront workgroups share a CU).
 constexpr int kLockstep = 0, kRing2 = 2;
 
-// Q8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
+// kCodes8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
 // key's K and of its V with the key's scales, which turn into the dtype's elements,
-// exactly, where they are stored to LDS. The queries are used as they are given, in QP
+// exactly, where they are stored to LDS. kCodes4 (e2m1.hpp): 16 codes of a key's K and, as they
+// lie in a tile, 8 of two keys' V (4 of four at head_dim 64), likewise. CODES, either: The queries are used as they are given, in QP
 // pieces of the dtype: one for queries of it, so that a score is the sum of exact products in
 // fp32, two for fp32 queries (below). scale * log2 e is multiplied with a score less the
 // running maximum, in fp32, where its exponential is taken.
-template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, bool Q8 = false, int QP = 1>
+template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, int FMT = kElements, int QP = 1>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
   typedef PShape<D, NW, CTW> S;
@@ -203,7 +205,8 @@ void paged_prefill_kernel(PrefillArgs a) {
   constexpr int CT = S::CT, BN = S::BN, NT = S::NT;
   constexpr int RING = SCHED == kRing2 ? 2 : 3;
   constexpr bool WIDE = QP == 2;  // fp32 queries of a 16-bit pool
-  static_assert(Q8 || !WIDE, "16-bit caches take queries of their dtype");
+  constexpr bool CODES = FMT != kElements, C4 = FMT == kCodes4;
+  static_assert(CODES || !WIDE, "16-bit caches take queries of their dtype");
   __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][BN * S::KROW];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[RING][BN * S::KROW];
   __shared__ int32_t bt_lds[kBtCache];
@@ -276,11 +279,12 @@ void paged_prefill_kernel(PrefillArgs a) {
     return Col{tq0 + t, kvh * a.n_rep + (j - t * a.n_rep), t < TQ && tq0 + t < q_len};
   };
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
-  typedef typename std::conditional<Q8, uint8_t, uint16_t>::type Elt;  // cache element
+  typedef typename std::conditional<CODES, uint8_t, uint16_t>::type Elt;  // cache element
   const Elt* kc = (const Elt*)a.kc + (int64_t)kvh * a.c_head;
   const Elt* vc = (const Elt*)a.vc + (int64_t)kvh * a.c_head;
-  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
-  static_assert(!(FUSED && Q8), "new rows are quantised before they are attended");
+  const f32x2* scales = FMT == kCodes8 ? a.scales + kvh * a.num_blocks : nullptr;
+  const uint8_t* scales4 = C4 ? a.scales4 + (int64_t)kvh * a.c_head / 8 : nullptr;
+  static_assert(!(FUSED && CODES), "new rows are quantised before they are attended");
 
   // ---- Q^T operands: lane (g, c) holds d = 32 ks + 8 g .. +7 of its column,
   // multiplied by scale * log2(e) and rounded back to the input dtype, so the
@@ -294,7 +298,7 @@ void paged_prefill_kernel(PrefillArgs a) {
   // that leaves: off by 2^-18 of an element in bf16; in fp16 by 2^-24 of it or, where the pieces
   // are subnormal, 2^-39 of the row's largest. unit takes the power back.
   u32x4 qreg[CT][S::KS], qrest[WIDE ? CT : 1][S::KS];
-  float unit[CT];  // Q8: factor of a column's scores to base-2 exponents
+  float unit[CT];  // CODES: factor of a column's scores to base-2 exponents
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const Col col = column(ct);
@@ -327,7 +331,7 @@ void paged_prefill_kernel(PrefillArgs a) {
     const uint16_t* qrow = (const uint16_t*)a.q + q_off;
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
-      if constexpr (EARLY || Q8) {
+      if constexpr (EARLY || CODES) {
         const u32x4 x = *(const u32x4*)(qrow + ks * 32 + 8 * g);  // (a valid row when !col.ok)
         qreg[ct][ks] = col.ok ? x : u32x4{0u, 0u, 0u, 0u};
       } else {
@@ -380,22 +384,26 @@ void paged_prefill_kernel(PrefillArgs a) {
 
   // K and V of a key share its slot: each thread loads the same 16-byte
   // piece of both
-  constexpr int PE = Q8 ? 16 : 8;                // elements of a piece
+  constexpr int PE = CODES ? 16 : 8;             // elements of a piece
   constexpr int PIECES = BN * D / PE;            // pieces of a tile
   constexpr int KPT = (PIECES + NT - 1) / NT;    // of a thread
-  u32x4 kreg[KPT], vreg[KPT];
-  f32x2 screg[KPT];  // Q8: the pieces' scales
+  typedef typename std::conditional<C4, u32x2, u32x4>::type Piece;
+  typedef typename std::conditional<C4, u32x2, f32x2>::type PieceScale;  // of K and of V
+  // whether its key may be used; kCodes4: how many of its 16 keys may
+  typedef typename std::conditional<C4, int, bool>::type Use;
+  Piece kreg[KPT], vreg[KPT];
+  PieceScale screg[KPT];  // CODES: the pieces' scales
   // whether each load in flight reads a usable key: applied when the tile is
   // stored (zero_unless), not when it is loaded, so the loads stay in flight
   // through the next tile's math instead of being waited for at once
-  bool kuse[KPT];
+  Use kuse[KPT];
   // Global loads of key tile kb into registers (whole workgroup, uniform call).
   // In a fused call, a tile holding the sequence's new keys reads those keys
   // from the call's new rows (the writers fill their slots concurrently).
   const uint16_t* kn = a.k_new ? (const uint16_t*)a.k_new + (int64_t)kvh * a.kn_head : nullptr;
   const uint16_t* vn = a.v_new ? (const uint16_t*)a.v_new + (int64_t)kvh * a.vn_head : nullptr;
   const int64_t new_row0 = a.src_row0 + q_lo - p0;  // row of new key k: new_row0 + k
-  auto load_into = [&](int kb, u32x4 (&kr)[KPT], u32x4 (&vr)[KPT], f32x2 (&sc)[KPT], bool (&ku)[KPT]) {
+  auto load_into = [&](int kb, Piece (&kr)[KPT], Piece (&vr)[KPT], PieceScale (&sc)[KPT], Use (&ku)[KPT]) {
     const int k0 = kb * BN;
     const int k_last = min(k0 + BN, kmax) - 1;
     const int last_blk = FAST ? k_last >> a.bs_shift : k_last / a.bs;
@@ -427,6 +435,27 @@ void paged_prefill_kernel(PrefillArgs a) {
         return;
       }
     }
+    if constexpr (C4) {
+      // piece q: 8 bytes of the 16-token tile q / D, in the order of memory
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) {
+        const int q = tid + NT * i;
+        if (PIECES % NT == 0 || q < PIECES) {
+          const int t0 = 16 * (q / D), p = q % D, row = 8 * p / Tile4<D>::LB, gg = row >> 4, cc = row & 15;
+          bool use;
+          const int64_t at = slot_of(k0 + t0, use, block);
+          const uint8_t* ts = scales4 + at / 8;
+          kr[i] = *(const u32x2*)(kc + at + 8 * p);
+          vr[i] = *(const u32x2*)(vc + at + 8 * p);
+          sc[i][0] = ts[16 * (D == 128 ? gg : gg >> 1) + cc];
+          const uint8_t* vs = ts + D / 2 + 4 * (Tile4<D>::NG * gg + cc / (16 / Tile4<D>::NG));
+          if constexpr (D == 128) sc[i][1] = *(const uint16_t*)(vs + 2 * (p & 1));
+          else sc[i][1] = *(const uint32_t*)vs;
+          ku[i] = use ? min(16, kmax - (k0 + t0)) : 0;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       const int q = tid + NT * i;
@@ -434,9 +463,11 @@ void paged_prefill_kernel(PrefillArgs a) {
         const int key = q / (D / PE), part = q % (D / PE);
         bool use;
         const int64_t sl = slot_of(k0 + key, use, block);
-        kr[i] = *(const u32x4*)(kc + sl + part * PE);
-        vr[i] = *(const u32x4*)(vc + sl + part * PE);
-        if constexpr (Q8) sc[i] = scales[block];  // (block 0's for an unusable key, whose codes become 0)
+        if constexpr (!C4) {
+          kr[i] = *(const u32x4*)(kc + sl + part * PE);
+          vr[i] = *(const u32x4*)(vc + sl + part * PE);
+          if constexpr (FMT == kCodes8) sc[i] = scales[block];  // (block 0's for an unusable key, whose codes become 0)
+        }
         ku[i] = use;
       }
     }
@@ -444,18 +475,58 @@ void paged_prefill_kernel(PrefillArgs a) {
   auto load_regs = [&](int kb) { load_into(kb, kreg, vreg, screg, kuse); };
   // Registers -> LDS buffer `buf`: K and V tiles both row-major [64 keys][D]
   // (+32 bytes a row).
-  auto store_from = [&](int buf, const u32x4 (&kr)[KPT], const u32x4 (&vr)[KPT], const f32x2 (&sc)[KPT],
-                        const bool (&ku)[KPT]) {
+  auto store_from = [&](int buf, const Piece (&kr)[KPT], const Piece (&vr)[KPT], const PieceScale (&sc)[KPT],
+                        const Use (&ku)[KPT]) {
+    if constexpr (C4) {
+      constexpr int VT = 256 / D;  // keys of a V piece, 16 / VT channels of each
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) {
+        const int q = tid + NT * i;
+        if (q < PIECES) {
+          const int t0 = 16 * (q / D), p = q % D, row = 8 * p / Tile4<D>::LB, gg = row >> 4, cc = row & 15;
+          const int half = D == 128 ? p & 1 : 0, t = staged_token(cc);
+          const bool keep = t < ku[i];
+          uint16_t* kp = &ks_lds[buf][(t0 + t) * S::KROW + D / 4 * gg + 16 * half];
+          const float ks = scale_of_byte(sc[i][0]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[4];
+            decode8_e2m1<DT>(kr[i][h], ks, x);
+            *(u32x4*)(kp + 8 * h) = zero_unless(u32x4{x[0], x[1], x[2], x[3]}, keep);
+          }
+#pragma unroll
+          for (int r = 0; r < VT; ++r) {
+            const int tv = 4 * (VT * half + r) + gg;
+            const float vs = scale_of_byte((sc[i][1] >> (8 * r)) & 0xffu);
+            uint16_t* vp = &vs_lds[buf][(t0 + tv) * S::KROW + D / 16 * cc];
+            if constexpr (D == 128) {
+              uint32_t x[4];
+              decode8_e2m1<DT>(vr[i][r], vs, x);
+              *(u32x4*)vp = zero_unless(u32x4{x[0], x[1], x[2], x[3]}, tv < ku[i]);
+            } else {
+              const uint32_t w = vr[i][r >> 1] >> (16 * (r & 1));
+              const bool kv = tv < ku[i];
+              *(u32x2*)vp = u32x2{kv ? decode2_e2m1<DT, 0>(w, vs) : 0u, kv ? decode2_e2m1<DT, 1>(w, vs) : 0u};
+            }
+          }
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       const int q = tid + NT * i;
       if (q < PIECES) {
         const int key = q / (D / PE), part = q % (D / PE);
-        const u32x4 k4 = zero_unless(kr[i], ku[i]), v4 = zero_unless(vr[i], ku[i]);
-        const f32x2 s2 = Q8 && ku[i] ? sc[i] : f32x2{1.f, 1.f};
+        u32x4 k4{}, v4{};
+        if constexpr (!C4) {
+          k4 = zero_unless(kr[i], ku[i]);
+          v4 = zero_unless(vr[i], ku[i]);
+        }
         uint16_t* kp = &ks_lds[buf][key * S::KROW + part * PE];
         uint16_t* vp = &vs_lds[buf][key * S::KROW + part * PE];
-        if constexpr (Q8) {
+        if constexpr (FMT == kCodes8) {
+          const f32x2 s2 = ku[i] ? sc[i] : f32x2{1.f, 1.f};
           auto wide = [](uint16_t* to, u32x4 x, float scale) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -490,7 +561,7 @@ void paged_prefill_kernel(PrefillArgs a) {
   };
 
   // ---- online softmax state, per column tile: lane owns column c of it.
-  // negm[ct] holds -m (the running base-2 max, in Q8 that of the products; 0 before the first tile) in
+  // negm[ct] holds -m (the running base-2 max, in CODES that of the products; 0 before the first tile) in
   // all four slots: it is the accumulator a tile's score MFMAs start from, so
   // the scores arrive as s - m and need only the exponential.
   f32x4 acc[CT][S::DTL], negm[CT];
@@ -553,11 +624,11 @@ void paged_prefill_kernel(PrefillArgs a) {
       for (int kt = 0; kt < 4; ++kt)
         mx = fmaxf(mx, fmaxf(fmaxf(cur[ct][kt][0], cur[ct][kt][1]), fmaxf(cur[ct][kt][2], cur[ct][kt][3])));
       mx = wave_max_groups_swap(mx);  // relative to m; finite on the first tile (key 0 is always visible)
-      const bool grow = first || (Q8 ? mx * unit[ct] : mx) > kRescaleSlack;
+      const bool grow = first || (CODES ? mx * unit[ct] : mx) > kRescaleSlack;
       if (__any(grow)) {
         const float d = grow ? mx : 0.f;  // the max moves up by d
         if (!first) {
-          const float alpha = fast_exp2(Q8 ? -d * unit[ct] : -d);
+          const float alpha = fast_exp2(CODES ? -d * unit[ct] : -d);
           l[ct] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < S::DTL; ++dt) acc[ct][dt] *= alpha;
@@ -579,11 +650,11 @@ void paged_prefill_kernel(PrefillArgs a) {
     // Program order is kept step by step (sched_barrier): each step's K operand
     // was read one step earlier, its MFMAs go to the matrix pipe and the
     // exponentials of SPS scores fill the VALU meanwhile.
-    // Q8: a wavefront in its products, or on the way to them, goes before one in its
+    // CODES: a wavefront in its products, or on the way to them, goes before one in its
     // exponentials. Two workgroups share a CU, and the matrix pipe runs on while the VALU is the
     // other's (8 chunks of 512 tokens, 28 / 4 heads of 128: 338 us without, 333 the other way
     // round, 305 so; 325 with the stores of the next tile to LDS at low priority too).
-    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
+    if constexpr (CODES) __builtin_amdgcn_s_setprio(0);
     constexpr int NQK = 4 * S::KS, SPS = CT * 16 / NQK;
     auto k_operand = [&](int t) {
       return *(const u32x4*)&kn[((t % 4) * 16 + c) * S::KROW + (t / 4) * 32 + 8 * g];
@@ -603,7 +674,9 @@ void paged_prefill_kernel(PrefillArgs a) {
       for (int j = 0; j < SPS; ++j) {
         const int i = t * SPS + j;
         const int ct = i / 16, kt = (i % 16) / 4, r = i % 4;
-        cur[ct][kt][r] = fast_exp2(Q8 ? cur[ct][kt][r] * unit[ct] : cur[ct][kt][r]);
+        cur[ct][kt][r] = fast_exp2(C4      ? __builtin_fmaf(cur[ct][kt][r], unit[ct], kProbUp<DT>)
+                                   : CODES ? cur[ct][kt][r] * unit[ct]
+                                           : cur[ct][kt][r]);
       }
       // (no scheduling barrier)
     }
@@ -619,7 +692,7 @@ void paged_prefill_kernel(PrefillArgs a) {
                            E::pack2(cur[ct][2 * st + 1][0], cur[ct][2 * st + 1][1]),
                            E::pack2(cur[ct][2 * st + 1][2], cur[ct][2 * st + 1][3])};
         // the running sum adds the rounded probabilities the PV product uses,
-        // two per instruction (Q8: two pieces of each, as the decode has them, are
+        // two per instruction (CODES: two pieces of each, as the decode has them, are
         // twice the PV products: 368 us against 298 for 8 chunks of 512 tokens)
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[ct] = sum2<DT>(pb[ct][st][e], l[ct]);
@@ -631,7 +704,7 @@ void paged_prefill_kernel(PrefillArgs a) {
     auto v_operand = [&](int t) {
       return v_operand_tr(vb_lds, t);
     };
-    if constexpr (Q8) __builtin_amdgcn_s_setprio(1);
+    if constexpr (CODES) __builtin_amdgcn_s_setprio(1);
     u32x4 vring[kOperandAhead];
 #pragma unroll
     for (int t = 0; t < kOperandAhead; ++t) vring[t] = v_operand(t);
@@ -656,9 +729,9 @@ void paged_prefill_kernel(PrefillArgs a) {
     // block ids are, with Q's loads.
     constexpr int R = 4;
     if (t_lo < t_hi) {
-      u32x4 kr[R][KPT], vr[R][KPT];
-      f32x2 sc8[R][KPT];
-      bool ku[R][KPT];
+      Piece kr[R][KPT], vr[R][KPT];
+      PieceScale sc8[R][KPT];
+      Use ku[R][KPT];
       const int bt0 = FAST ? (t_lo * BN) >> a.bs_shift : (t_lo * BN) / a.bs;
       if (FUSED && t_lo * BN >= p0) {  // uniform
         load_into(t_lo, kr[0], vr[0], sc8[0], ku[0]);
@@ -674,7 +747,7 @@ void paged_prefill_kernel(PrefillArgs a) {
       __syncthreads();
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        if constexpr (Q8) continue;
+        if constexpr (CODES) continue;
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
           const u32x4 x = qreg[ct][ks];
@@ -818,7 +891,7 @@ void paged_prefill_kernel(PrefillArgs a) {
   const int row_step = a.num_kv_heads * COLS;  // rows between parts of one item
   const int row_base = (pbase * a.num_kv_heads + kvh) * COLS;  // part 0, column 0
   float lsum[CT];
-  auto top = [&](int qt) { return Q8 ? -negm[qt][0] * unit[qt] : -negm[qt][0]; };  // in base 2
+  auto top = [&](int qt) { return CODES ? -negm[qt][0] * unit[qt] : -negm[qt][0]; };  // in base 2
 #pragma unroll
   for (int qt = 0; qt < CT; ++qt) {
     lsum[qt] = wave_sum_groups_swap(l[qt]);
@@ -915,10 +988,11 @@ void paged_prefill_kernel(PrefillArgs a) {
 constexpr int kF32Threads = 256;
 constexpr int kF32Cols = 64;
 
-template <int D, bool FAST, bool Q8 = false>
+template <int D, bool FAST, int FMT = kElements>
 __global__ __launch_bounds__(kF32Threads) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_prefill_f32_kernel(PrefillArgs a) {
   constexpr int NT = kF32Threads, BN = 64, MT = D / 16, DT4 = D / 4;
+  constexpr bool CODES = FMT != kElements, C4 = FMT == kCodes4;
   constexpr int KROW = D + 4;           // floats per K row in LDS
   constexpr int VROW = BN + 4;          // floats per V^T row (one d, 64 keys)
   constexpr int BPT = (BN / 4) * DT4 / NT;  // 4-key x 4-d blocks of a tile per thread
@@ -994,11 +1068,12 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
   }
 
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
-  typedef typename std::conditional<Q8, uint8_t, float>::type Elt;  // cache element
-  typedef typename std::conditional<Q8, uint32_t, f32x4>::type Four;
+  typedef typename std::conditional<CODES, uint8_t, float>::type Elt;  // cache element
+  typedef typename std::conditional<CODES, uint32_t, f32x4>::type Four;  // (kCodes4: in its low half)
   const Elt* kc = (const Elt*)a.kc + (int64_t)kvh * a.c_head;
   const Elt* vc = (const Elt*)a.vc + (int64_t)kvh * a.c_head;
-  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
+  const f32x2* scales = FMT == kCodes8 ? a.scales + kvh * a.num_blocks : nullptr;
+  const uint8_t* scales4 = C4 ? a.scales4 + (int64_t)kvh * a.c_head / 8 : nullptr;
   const int nblk_needed = (kmax + a.bs - 1) / a.bs;
   int bt_base = 0;
   auto fill_bt = [&](int base) {
@@ -1033,10 +1108,14 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
   // a tile's 4-key x 4-d blocks: block b = tid + NT i holds keys 4 (b / DT4)
   // .. +3 at d = 4 (b % DT4) .. +3
   Four kr[BPT][4], vr[BPT][4];
-  f32x2 sc[BPT];  // Q8: the scales of the four keys, which share a block
+  f32x2 sc[BPT];  // kCodes8: the scales of the four keys, which share a block
+  uint32_t sk[BPT][4], sv[BPT][4];  // kCodes4: of each
   bool ku[BPT][4];
   auto widen = [](Four x, float scale) -> f32x4 {
-    if constexpr (Q8) {
+    if constexpr (C4) {
+      const f32x2 lo = decode2_e2m1_f32<0>(x, scale), hi = decode2_e2m1_f32<1>(x, scale);
+      return f32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else if constexpr (FMT == kCodes8) {
       const f32x2 lo = decode2_f32<false>(x, scale), hi = decode2_f32<true>(x, scale);
       return f32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
@@ -1051,6 +1130,24 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < BPT; ++i) {
       const int b = tid + NT * i, key4 = b / DT4, d4 = b - key4 * DT4;
+      if constexpr (C4) {
+        typedef Tile4<D> T;
+        const int k16 = k0 + 4 * (key4 & ~3);  // the keys' tile
+        bool use;
+        int32_t block;
+        const int64_t at = slot_of(k16, use, block);
+        const uint8_t* ts = scales4 + at / 8;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = 4 * (key4 & 3) + e;
+          kr[i][e] = *(const uint16_t*)(kc + at + T::k(t, d4 >> 1) + 2 * (d4 & 1));
+          vr[i][e] = *(const uint16_t*)(vc + at + (D == 128 ? T::v(t, d4 >> 1) + 2 * (d4 & 1) : T::v(t, d4)));
+          sk[i][e] = ts[T::k_scale(t, d4 >> 3)];
+          sv[i][e] = ts[T::v_scale(t, d4 >> 3)];
+          ku[i][e] = use && k16 + t < kmax;
+        }
+        continue;
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         bool use;
@@ -1059,7 +1156,7 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
         kr[i][e] = *(const Four*)(kc + sl + 4 * d4);
         vr[i][e] = *(const Four*)(vc + sl + 4 * d4);
         ku[i][e] = use;
-        if (Q8 && e == 0) sc[i] = scales[block];
+        if (FMT == kCodes8 && e == 0) sc[i] = scales[block];
       }
     }
   };
@@ -1068,10 +1165,14 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < BPT; ++i) {
       const int b = tid + NT * i, key4 = b / DT4, d4 = b - key4 * DT4;
-      const float k_scale = Q8 ? sc[i][0] : 1.f, v_scale = Q8 ? sc[i][1] : 1.f;
+      float k_scale = FMT == kCodes8 ? sc[i][0] : 1.f, v_scale = FMT == kCodes8 ? sc[i][1] : 1.f;
       f32x4 v4[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        if constexpr (C4) {
+          k_scale = scale_of_byte(sk[i][e]);
+          v_scale = scale_of_byte(sv[i][e]);
+        }
         *(f32x4*)&ks[(4 * key4 + e) * KROW + 4 * d4] = ku[i][e] ? widen(kr[i][e], k_scale) : zero;
         v4[e] = widen(vr[i][e], v_scale);
       }
@@ -1245,10 +1346,14 @@ int launch_prefill_f32(PrefillArgs a, hipStream_t s) {
   const bool fast = a.bs_shift >= 0 && slots < (1 << 23) && a.c_slot < (1 << 23) &&
                     (slots * a.c_slot + a.c_head * a.num_kv_heads) < ((int64_t)1 << 31);
   const dim3 g((unsigned)grid), block(kF32Threads);
-  if (a.scales && fast)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, true>), g, block, 0, s, a);
+  if (a.scales4 && fast)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, kCodes4>), g, block, 0, s, a);
+  else if (a.scales4)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, kCodes4>), g, block, 0, s, a);
+  else if (a.scales && fast)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, kCodes8>), g, block, 0, s, a);
   else if (a.scales)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, true>), g, block, 0, s, a);
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, kCodes8>), g, block, 0, s, a);
   else if (fast)
     hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true>), g, block, 0, s, a);
   else
@@ -1766,30 +1871,36 @@ int launch_prefill(PrefillArgs a, int sched, hipStream_t s) {
   return check_launch("ir_paged_prefill");
 }
 
-// An 8-bit cache: launch_prefill's shapes by the same rules (2-deep rings), the
+// A cache of codes: launch_prefill's shapes by the same rules (2-deep rings), the
 // step's rows already written.
-template <int DT, int D, int QP>
-int launch_prefill_q8(const PrefillArgs& a, hipStream_t s) {
+template <int DT, int D, int FMT, int QP>
+int launch_prefill_codes(const char* name, const PrefillArgs& a, hipStream_t s) {
   const int64_t grid = a.items ? a.n_items_grid : (int64_t)a.n_qblocks * a.num_kv_heads * a.num_seqs;
   if (grid <= 0) return ok();
-  if (grid > 0x7fffffff)
-    return fail(IR_EINVAL, "ir_paged_prefill_q8: grid of %lld workgroups too large", (long long)grid);
+  if (grid > 0x7fffffff) return fail(IR_EINVAL, "%s: grid of %lld workgroups too large", name, (long long)grid);
   const int64_t slots = a.num_blocks * a.bs;
   const bool fast = a.bs_shift >= 0 && slots < (1 << 23) &&
                     (slots * a.c_slot + a.c_head * a.num_kv_heads) < ((int64_t)1 << 31);
-#define IR_PREFILL_Q8(NW_, CT_)                                                                                    \
-  do {                                                                                                            \
-    const dim3 g((unsigned)grid), block(NW_ * 64);                                                                \
-    if (fast)                                                                                                     \
-      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, true, NW_, CT_, kRing2, false, true, QP>), g, block, 0, s, a);  \
-    else                                                                                                          \
-      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, false, NW_, CT_, kRing2, false, true, QP>), g, block, 0, s, a); \
+#define IR_PREFILL_CODES(NW_, CT_)                                                                                   \
+  do {                                                                                                               \
+    const dim3 g((unsigned)grid), block(NW_ * 64);                                                                   \
+    if (fast)                                                                                                        \
+      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, true, NW_, CT_, kRing2, false, FMT, QP>), g, block, 0, s, a);  \
+    else                                                                                                             \
+      hipLaunchKernelGGL((paged_prefill_kernel<DT, D, false, NW_, CT_, kRing2, false, FMT, QP>), g, block, 0, s, a); \
   } while (0)
-  if (a.nw == 4 && !a.items && grid <= device_cus()) IR_PREFILL_Q8(8, 1);
-  else if (a.nw == 4) IR_PREFILL_Q8(4, 2);
-  else IR_PREFILL_Q8(8, 2);
-#undef IR_PREFILL_Q8
-  return check_launch("ir_paged_prefill_q8");
+  if (a.nw == 4 && !a.items && grid <= device_cus()) IR_PREFILL_CODES(8, 1);
+  else if (a.nw == 4) IR_PREFILL_CODES(4, 2);
+  else IR_PREFILL_CODES(8, 2);
+#undef IR_PREFILL_CODES
+  return check_launch(name);
+}
+
+template <int DT, int FMT>
+int dispatch_prefill_codes(const char* name, int head_dim, bool wide, const PrefillArgs& a, hipStream_t s) {
+  if (head_dim == 128)
+    return wide ? launch_prefill_codes<DT, 128, FMT, 2>(name, a, s) : launch_prefill_codes<DT, 128, FMT, 1>(name, a, s);
+  return wide ? launch_prefill_codes<DT, 64, FMT, 2>(name, a, s) : launch_prefill_codes<DT, 64, FMT, 1>(name, a, s);
 }
 
 }  // namespace
@@ -1812,8 +1923,9 @@ extern "C" int ir_paged_prefill_plan_xcds(void) { return plan_xcds(); }
 
 namespace {
 
-// ir_paged_prefill, and with `scales` ir_paged_prefill_q8 (a dense layer of codes).
-int prefill_call(const char* name, const float* scales, int q_dtype, const void* q, int64_t q_tok_stride,
+// ir_paged_prefill, and with `scales` ir_paged_prefill_q8 or _q4 (a dense layer of codes; fmt
+// says of which).
+int prefill_call(const char* name, int fmt, const void* scales, int q_dtype, const void* q, int64_t q_tok_stride,
                  int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t cache_slot_stride,
                  int64_t cache_head_stride, int64_t num_blocks, int block_size, const int32_t* block_tables,
                  int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
@@ -1854,7 +1966,8 @@ int prefill_call(const char* name, const float* scales, int q_dtype, const void*
              "%s: q/cache strides must be multiples of 16 bytes, out strides of %d bytes", name, 4 * eb);
   if (scales) {
     IR_REQUIRE(block_size % 16 == 0, "%s: block size %d must be a multiple of 16", name, block_size);
-    IR_REQUIRE(((uintptr_t)scales & 7u) == 0, "%s: scales must be 8-byte aligned", name);
+    const unsigned al = fmt == kCodes4 ? 16 : 8;
+    IR_REQUIRE(((uintptr_t)scales & (al - 1)) == 0, "%s: scales must be %u-byte aligned", name, al);
   }
   PrefillArgs a;
   memset(&a, 0, sizeof(a));
@@ -1916,7 +2029,8 @@ int prefill_call(const char* name, const float* scales, int q_dtype, const void*
     a.n_write = n_write;
     a.src_row0 = src_row0;
   }
-  a.scales = (const f32x2*)scales;
+  a.scales = fmt == kCodes8 ? (const f32x2*)scales : nullptr;
+  a.scales4 = fmt == kCodes4 ? (const uint8_t*)scales : nullptr;
   a.out = out;
   a.o_tok = out_tok_stride;
   a.o_head = out_head_stride;
@@ -1927,11 +2041,11 @@ int prefill_call(const char* name, const float* scales, int q_dtype, const void*
   hipStream_t s = (hipStream_t)stream;
   if (scales && !f32) {
     const bool wide = q_dtype == IR_DTYPE_F32;
-#define IR_PREFILL_Q8(DT_, QP_) \
-  (head_dim == 128 ? launch_prefill_q8<DT_, 128, QP_>(a, s) : launch_prefill_q8<DT_, 64, QP_>(a, s))
-    if (dtype == IR_DTYPE_F16) return wide ? IR_PREFILL_Q8(IR_DTYPE_F16, 2) : IR_PREFILL_Q8(IR_DTYPE_F16, 1);
-    return wide ? IR_PREFILL_Q8(IR_DTYPE_BF16, 2) : IR_PREFILL_Q8(IR_DTYPE_BF16, 1);
-#undef IR_PREFILL_Q8
+    if (fmt == kCodes4)
+      return dtype == IR_DTYPE_F16 ? dispatch_prefill_codes<IR_DTYPE_F16, kCodes4>(name, head_dim, wide, a, s)
+                                   : dispatch_prefill_codes<IR_DTYPE_BF16, kCodes4>(name, head_dim, wide, a, s);
+    return dtype == IR_DTYPE_F16 ? dispatch_prefill_codes<IR_DTYPE_F16, kCodes8>(name, head_dim, wide, a, s)
+                                 : dispatch_prefill_codes<IR_DTYPE_BF16, kCodes8>(name, head_dim, wide, a, s);
   }
   if (f32) return head_dim == 128 ? launch_prefill_f32<128>(a, s) : launch_prefill_f32<64>(a, s);
   if (dtype == IR_DTYPE_BF16)
@@ -1953,7 +2067,7 @@ extern "C" int ir_paged_prefill(const void* q, int64_t q_tok_stride, int64_t q_h
                                 int64_t k_new_tok_stride, int64_t k_new_head_stride, const void* v_new,
                                 int64_t v_new_tok_stride, int64_t v_new_head_stride, const int64_t* write_slots,
                                 int64_t n_write, int64_t src_row0, int32_t* err_flags, ir_stream_t stream) {
-  return prefill_call("ir_paged_prefill", nullptr, dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
+  return prefill_call("ir_paged_prefill", kElements, nullptr, dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
                       cache_slot_stride, cache_head_stride, num_blocks, block_size, block_tables, bt_stride,
                       max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
                       out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, k_new,
@@ -1971,8 +2085,25 @@ extern "C" int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t 
                                    ir_stream_t stream) {
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_prefill_q8: null pointer");
-  return prefill_call("ir_paged_prefill_q8", scales, q_dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
+  return prefill_call("ir_paged_prefill_q8", kCodes8, scales, q_dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
                       head_dim, num_blocks * block_size * head_dim, num_blocks, block_size, block_tables, bt_stride,
+                      max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
+                      out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, nullptr,
+                      0, 0, nullptr, 0, 0, nullptr, 0, 0, err_flags, stream);
+}
+
+extern "C" int ir_paged_prefill_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
+                                   const void* v_cache, const uint8_t* scales, int64_t num_blocks, int block_size,
+                                   const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                                   const int32_t* cu_seqlens_q, const int32_t* q_start, int num_seqs, int total_q,
+                                   int max_q_len, void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                                   int num_q_heads, int num_kv_heads, int head_dim, float scale, int dtype,
+                                   int q_dtype, void* plan, int64_t plan_bytes, int32_t* err_flags,
+                                   ir_stream_t stream) {
+  if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
+  IR_REQUIRE(scales, "ir_paged_prefill_q4: null pointer");
+  return prefill_call("ir_paged_prefill_q4", kCodes4, scales, q_dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
+                      head_dim / 2, num_blocks * block_size * (head_dim / 2), num_blocks, block_size, block_tables, bt_stride,
                       max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,
                       out_head_stride, num_q_heads, num_kv_heads, head_dim, scale, dtype, plan, plan_bytes, nullptr,
                       0, 0, nullptr, 0, 0, nullptr, 0, 0, err_flags, stream);

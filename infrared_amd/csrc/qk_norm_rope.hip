@@ -87,19 +87,16 @@ int launch_norm_rope(NormRopeArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, int64_t q_head, void* q_out,
-                  int64_t qo_tok, int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v,
-                  int64_t v_tok, int64_t v_head, const void* q_weight, const void* k_weight, float eps,
-                  const float* cos, const float* sin, int64_t cs_tok, const int64_t* slots, int64_t n_tokens,
-                  int num_q_heads, int num_kv_heads, int eb, int qo_eb) {
-  IR_REQUIRE(k && v && cos && sin && slots && (num_q_heads == 0 || (q && q_out)), "%s: null pointer", name);
-  IR_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cos) && aligned16(sin) &&
-                 (num_q_heads == 0 || (aligned16(q) && aligned16(q_out))),
+int fill_rows(const char* name, RowArgs& r, const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok,
+              int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
+              int64_t v_head, const void* q_weight, const void* k_weight, float eps, int64_t n_tokens,
+              int num_q_heads, int num_kv_heads, int eb, int qo_eb) {
+  IR_REQUIRE(num_q_heads == 0 || (q && q_out), "%s: null pointer", name);
+  IR_REQUIRE(aligned16(k) && aligned16(v) && (num_q_heads == 0 || (aligned16(q) && aligned16(q_out))),
              "%s: tensors must be 16-byte aligned", name);
   IR_REQUIRE(!q_weight == !k_weight, "%s: one norm weight without the other", name);
   IR_REQUIRE(aligned16(q_weight) && aligned16(k_weight), "%s: norm weights must be 16-byte aligned", name);
   IR_REQUIRE(!q_weight || eps >= 0.f, "%s: eps must not be negative", name);
-  IR_REQUIRE(cs_tok % 4 == 0, "%s: cos/sin row stride must be a multiple of 4 elements", name);
   for (int64_t st : {qo_tok, qo_head})
     IR_REQUIRE((st * qo_eb) % 16 == 0, "%s: strides must be multiples of 16 bytes", name);
   for (int64_t st : {q_tok, q_head, k_tok, k_head, v_tok, v_head})
@@ -117,16 +114,30 @@ int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, in
   r.v = (const uint8_t*)v;
   r.v_tok = v_tok * eb;
   r.v_head = v_head * eb;
-  r.cos = cos;
-  r.sin = sin;
-  r.cs_tok = cs_tok;
   r.q_weight = (const uint8_t*)q_weight;
   r.k_weight = (const uint8_t*)k_weight;
   r.eps = eps;
-  r.slots = slots;
   r.n_tokens = n_tokens;
   r.num_q_heads = num_q_heads;
   r.num_kv_heads = num_kv_heads;
+  return IR_OK;
+}
+
+int fill_row_args(const char* name, RowArgs& r, const void* q, int64_t q_tok, int64_t q_head, void* q_out,
+                  int64_t qo_tok, int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head, const void* v,
+                  int64_t v_tok, int64_t v_head, const void* q_weight, const void* k_weight, float eps,
+                  const float* cos, const float* sin, int64_t cs_tok, const int64_t* slots, int64_t n_tokens,
+                  int num_q_heads, int num_kv_heads, int eb, int qo_eb) {
+  IR_REQUIRE(k && v && cos && sin && slots && (num_q_heads == 0 || (q && q_out)), "%s: null pointer", name);
+  IR_REQUIRE(aligned16(cos) && aligned16(sin), "%s: tensors must be 16-byte aligned", name);
+  IR_REQUIRE(cs_tok % 4 == 0, "%s: cos/sin row stride must be a multiple of 4 elements", name);
+  const int rc = fill_rows(name, r, q, q_tok, q_head, q_out, qo_tok, qo_head, k, k_tok, k_head, v, v_tok, v_head,
+                           q_weight, k_weight, eps, n_tokens, num_q_heads, num_kv_heads, eb, qo_eb);
+  if (rc != IR_OK) return rc;
+  r.cos = cos;
+  r.sin = sin;
+  r.cs_tok = cs_tok;
+  r.slots = slots;
   return IR_OK;
 }
 

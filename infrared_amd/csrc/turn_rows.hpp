@@ -1,0 +1,206 @@
+// The kernel of the row-wise calls whose keys and values go to a 4-bit pool, or whose
+// angles come from positions with several axes: one pass over the step's rows, the row
+// mathematics norm_rope.hpp's.
+//
+// A wavefront takes one token and 64 / (head_dim / 16) of its rows (q, then k, then v) at
+// a time, its lanes holding their part of the token's angles in registers for all of
+// them. Bound by memory: every row is read once and written once.
+#pragma once
+
+#include "e2m1.hpp"
+#include "norm_rope.hpp"
+
+namespace ir {
+
+enum { kAnglesNone = 0, kAnglesTables = 1, kAnglesPositions = 2 };
+enum { kToRows = 0, kToCache = 1, kToCodes4 = 2 };  // where keys go; values go with them, or nowhere
+
+constexpr int kMaxPairs = 128;  // of a head
+// Tokens of a call up to which a slot may be given twice: a decode step's, whose padding
+// repeats a row (all slots are read by each token's wavefronts, with its own).
+constexpr int kLastWins = 1024;
+constexpr int kTurnWaves = 4;
+
+struct TurnArgs {
+  RowArgs r;
+  // kAnglesPositions
+  const int64_t* pos;
+  int64_t pos_axis;
+  int num_axes;
+  const ir_rotary_pair* pairs;
+  float scaling;
+  int head_dim;
+  // kToRows, bytes
+  uint8_t* ko;
+  int64_t ko_tok, ko_head;
+  // kToCache (bytes), kToCodes4 (dense)
+  uint8_t* kc;
+  uint8_t* vc;
+  int64_t c_slot, c_head;
+  uint8_t* scales;
+  int64_t num_slots;
+  int chunks, chunk_rows;  // wavefronts per token, rows of each
+  int32_t* err;
+};
+
+// cos and sin of a token's pairs, one pair a lane, to the wavefront's LDS. position *
+// step modulo 2^64 is the angle as a fraction of a turn: the wrap-around is the reduction,
+// exact however far the position, and the signed upper half of it is half a turn at most.
+__device__ __forceinline__ void angles_of(const TurnArgs& a, int64_t tok, int lane, int pairs, float* cs) {
+  for (int j = lane; j < pairs; j += 64) {
+    const u32x4 p = *(const u32x4*)(a.pairs + j);
+    const uint64_t step = ((uint64_t)p[1] << 32) | p[0];
+    const int axis = max(0, min((int)p[2], a.num_axes - 1));
+    const uint64_t turn = (uint64_t)a.pos[axis * a.pos_axis + tok] * step + 0x80000000u;
+    float s, c;
+    sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
+    cs[j] = c * a.scaling;
+    cs[kMaxPairs + j] = s * a.scaling;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// D 0: a.head_dim (rows without norms only).
+template <int DT, int D, int MODE, int ANG, int DST>
+__global__ __launch_bounds__(kTurnWaves * 64) void turn_rows_kernel(TurnArgs a) {
+  typedef Chunk8<DT> C;
+  static_assert(D != 0 || (MODE == kRowsTurn && DST == kToRows), "the head's width is known for norms and pools");
+  __shared__ __attribute__((aligned(16))) float s_cs[ANG == kAnglesPositions ? kTurnWaves : 1][2 * kMaxPairs];
+  const int hd = D ? D : a.head_dim, lpr = hd / 16, half = hd / 2 * C::EB;
+  const int G = 64 / lpr;  // rows of a wavefront at a time
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, grp = lane / lpr, ci = lane - grp * lpr;
+  const int64_t wave = (int64_t)blockIdx.x * kTurnWaves + w;
+  const int64_t tok = wave / a.chunks;
+  if (tok >= a.r.n_tokens) return;
+  const int nq = a.r.num_q_heads, nkv = a.r.num_kv_heads, rows = nq + (DST == kToRows ? nkv : 2 * nkv);
+  const int row0 = (int)(wave - tok * a.chunks) * a.chunk_rows;
+  const int row_end = min(rows, row0 + a.chunk_rows);
+  int64_t slot = 0;
+  bool kv_ok = true;
+  if constexpr (DST != kToRows) {
+    slot = a.r.slots[tok];
+    kv_ok = slot >= 0 && slot < a.num_slots;
+    if (slot >= a.num_slots && lane == 0 && row0 == 0) flag_error(a.err, IR_ERR_SLOT_RANGE);
+  }
+  if constexpr (DST == kToCodes4) {
+    // of rows given the same slot the last is written: a mixture of two would have one's
+    // codes at the other's scales
+    if (a.r.n_tokens <= kLastWins) {
+      bool later = false;
+      for (int64_t j = tok + 1 + lane; j < a.r.n_tokens; j += 64) later |= a.r.slots[j] == slot;
+      if (__any(later)) kv_ok = false;
+    }
+  }
+  Angles<DT, D, MODE> t;
+  if constexpr (ANG == kAnglesTables) t.load(a.r.cos + tok * a.r.cs_tok, a.r.sin + tok * a.r.cs_tok, ci);
+  if constexpr (ANG == kAnglesPositions) {
+    angles_of(a, tok, lane, hd / 2, s_cs[w]);
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 c = *(const f32x4*)&s_cs[w][8 * ci + e], s = *(const f32x4*)&s_cs[w][kMaxPairs + 8 * ci + e];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        t.c[e + i] = t.c[8 + e + i] = c[i];
+        t.s[e + i] = t.s[8 + e + i] = s[i];
+      }
+    }
+  }
+  typename C::Raw wraw[2][2];  // norm weights of q and k
+  if constexpr (MODE == kRowsNorm) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* p = (i ? a.r.k_weight : a.r.q_weight) + ci * 8 * C::EB;
+      C::raw_load(p, wraw[i][0]);
+      C::raw_load(p + half, wraw[i][1]);
+    }
+  }
+  for (int row = row0 + grp; row < row_end && grp < G; row += G) {
+    const bool is_q = row < nq, is_v = row >= nq + nkv;
+    const int h = is_q ? row : is_v ? row - nq - nkv : row - nq;
+    if (!is_q && !kv_ok) continue;  // (a row's lanes go together)
+    const uint8_t* src = (is_q   ? a.r.q + tok * a.r.q_tok + h * a.r.q_head
+                          : is_v ? a.r.v + tok * a.r.v_tok + h * a.r.v_head
+                                 : a.r.k + tok * a.r.k_tok + h * a.r.k_head) +
+                         ci * 8 * C::EB;
+    typename C::Raw lo, hi;
+    C::raw_load(src, lo);
+    C::raw_load(src + half, hi);
+    if constexpr (DST == kToCache) {
+      if (is_v) {
+        uint8_t* dst = a.vc + slot * a.c_slot + h * a.c_head + ci * 8 * C::EB;
+        C::raw_store_nt(dst, lo);
+        C::raw_store_nt(dst + half, hi);
+        continue;
+      }
+    }
+    float x[16], wt[16];
+    auto unpack = [](const typename C::Raw& l, const typename C::Raw& u, float(&to)[16]) {
+      float p[8], q[8];
+      C::unpack(l, p);
+      C::unpack(u, q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        to[e] = p[e];
+        to[8 + e] = q[e];
+      }
+    };
+    unpack(lo, hi, x);
+    if constexpr (MODE != kRowsPlain) {
+      if (!is_v) {
+        if constexpr (MODE == kRowsNorm) unpack(wraw[is_q ? 0 : 1][0], wraw[is_q ? 0 : 1][1], wt);
+        transform_row<DT, D, MODE>(x, wt, a.r.eps, t);
+      }
+    }
+    if constexpr (DST == kToCodes4) {
+      if (!is_q) {
+        const int64_t tile = h * (a.num_slots >> 4) + (slot >> 4);
+        store_row_e2m1<DT, D>(x, (is_v ? a.vc : a.kc) + tile * Tile4<D>::CODES, a.scales + tile * Tile4<D>::SCALES,
+                              (int)(slot & 15), ci, is_v);
+        continue;
+      }
+    }
+    float x0[8], x1[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x0[e] = x[e];
+      x1[e] = x[8 + e];
+    }
+    if (is_q && a.r.qo_wide) {
+      typedef Chunk8<IR_DTYPE_F32> W;
+      uint8_t* dst = a.r.qo + tok * a.r.qo_tok + h * a.r.qo_head + ci * 32;
+      W::store_nt(dst, x0);
+      W::store_nt(dst + hd * 2, x1);
+      continue;
+    }
+    uint8_t* dst = (is_q               ? a.r.qo + tok * a.r.qo_tok + h * a.r.qo_head
+                    : DST == kToCache ? a.kc + slot * a.c_slot + h * a.c_head
+                                      : a.ko + tok * a.ko_tok + h * a.ko_head) +
+                   ci * 8 * C::EB;
+    C::store_nt(dst, x0);
+    C::store_nt(dst + half, x1);
+  }
+}
+
+// Wavefronts of a token: one for all its rows once the tokens alone fill the device, which
+// then have their angles once a token; below that one for each run of rows, so that a
+// decode step's few tokens are a single pass (qk_norm_rope.hip has both measured).
+constexpr int64_t kTurnTokensForDevice = 2048;
+
+template <int DT, int D, int MODE, int ANG, int DST>
+int launch_turn(const char* name, TurnArgs a, hipStream_t s) {
+  const int rows = a.r.num_q_heads + (DST == kToRows ? 1 : 2) * a.r.num_kv_heads;
+  if (rows == 0) return ok();
+  const int g = 64 / ((D ? D : a.head_dim) / 16);
+  const int runs = (rows + g - 1) / g;
+  a.chunks = a.r.n_tokens >= kTurnTokensForDevice ? 1 : runs;
+  a.chunk_rows = a.chunks == 1 ? rows : g;
+  IR_REQUIRE(a.r.n_tokens <= 0x7fffffff, "%s: too many tokens", name);
+  const int64_t grid = (a.r.n_tokens * a.chunks + kTurnWaves - 1) / kTurnWaves;
+  IR_REQUIRE(grid <= 0x7fffffff, "%s: too many tokens", name);
+  hipLaunchKernelGGL((turn_rows_kernel<DT, D, MODE, ANG, DST>), dim3((unsigned)grid), dim3(kTurnWaves * 64), 0, s, a);
+  return check_launch(name);
+}
+
+}  // namespace ir

@@ -13,9 +13,22 @@ from dataclasses import dataclass
 
 import torch
 
-from infrared_amd._lib import DTYPE_E4M3, check, dtype_code, lib, ptr, require_device, seam, stream_of, stream_ptr
+from infrared_amd._lib import (
+    DTYPE_E2M1,
+    DTYPE_E4M3,
+    check,
+    dtype_code,
+    lib,
+    ptr,
+    require_device,
+    seam,
+    stream_of,
+    stream_ptr,
+)
+from infrared_amd.rotary import RotaryAxes
 
 CODES = torch.float8_e4m3fn  # dtype of an 8-bit pool's caches
+CODES4 = torch.uint8  # dtype of a 4-bit pool's caches (two codes a byte) and of its scales
 
 
 def _last_dim_contiguous(name: str, t: torch.Tensor) -> None:
@@ -170,6 +183,82 @@ def paged_gather_q8(
     return out[0], out[1]
 
 
+def kv_scatter_q4(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    err_flags: torch.Tensor | None = None,
+) -> None:
+    """:func:`kv_scatter` into one layer of a 4-bit pool (``Quant4PagedKVPool.write``
+    semantics): ``k_cache``/``v_cache`` uint8 ``[num_slots, H_kv, D / 2]`` in head-major
+    storage, ``kv_scales`` uint8 ``[H_kv, num_slots / 16, D]``."""
+    seam().kv_scatter_q4(k_cache, v_cache, kv_scales, k, v, slots, int(block_size), err_flags, stream_of(k_cache))
+
+
+def gather_slots_q4(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    dtype: torch.dtype,
+    err_flags: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`gather_slots` of a layer of a 4-bit pool, as values of ``dtype`` (the
+    pool's, of which each is exactly a number)."""
+    return seam().gather_slots_q4(k_cache, v_cache, kv_scales, slots, int(block_size), dtype, err_flags,
+                                  stream_of(k_cache))
+
+
+def paged_gather_q4(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    max_ctx: int,
+    dtype: torch.dtype,
+    err_flags: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`paged_gather` of a layer of a 4-bit pool, as values of ``dtype``."""
+    dev = require_device(k_cache, v_cache, kv_scales, block_tables, context_lens)
+    _code4_layer("paged_gather_q4", k_cache, v_cache, kv_scales, block_size)
+    _check_tables("paged_gather_q4", block_tables, context_lens)
+    b = block_tables.shape[0]
+    slots, h, d = k_cache.shape[0], k_cache.shape[1], 2 * k_cache.shape[2]
+    out = torch.empty(2, b, max_ctx, h, d, dtype=dtype, device=dev)
+    rc = lib().ir_paged_gather_q4(
+        ptr(k_cache), ptr(v_cache), ptr(kv_scales), slots // block_size, block_size, ptr(block_tables),
+        block_tables.stride(0), block_tables.shape[1], ptr(context_lens), b, max_ctx, h, d, dtype_code(dtype),
+        ptr(out[0]), ptr(out[1]), ptr(err_flags), stream_ptr(dev),
+    )
+    check(rc, "ir_paged_gather_q4")
+    return out[0], out[1]
+
+
+def _code4_layer(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: torch.Tensor,
+                 block_size: int) -> None:
+    _cache_layer(name, k_cache)
+    slots, h, row = k_cache.shape
+    if k_cache.dtype != CODES4 or v_cache.dtype != CODES4:
+        raise RuntimeError(f"{name}: uint8 kv_scales go with caches of uint8 4-bit codes, got {k_cache.dtype}, "
+                           f"{v_cache.dtype}")
+    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+        raise RuntimeError(f"{name}: k_cache and v_cache must have the same shape and strides")
+    if k_cache.stride(0) != row or (h > 1 and k_cache.stride(1) != slots * row):
+        raise RuntimeError(f"{name}: a cache of codes must be dense [num_kv_heads, num_slots, head_dim] storage")
+    if block_size <= 0 or slots % block_size:
+        raise RuntimeError(f"{name}: {slots} slots are not whole blocks of {block_size}")
+    if (kv_scales.dtype != torch.uint8 or not kv_scales.is_contiguous()
+            or kv_scales.shape != (h, slots // 16, 2 * row)):
+        raise RuntimeError(f"{name}: kv_scales must be contiguous uint8 [num_kv_heads, num_slots / 16, head_dim]")
+
+
 def _check_tables(name: str, block_tables: torch.Tensor, context_lens: torch.Tensor) -> None:
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1:
         raise RuntimeError(f"{name}: block_tables must be int32 [B, max_blocks] with contiguous rows")
@@ -219,7 +308,7 @@ def paged_decode(
     zero-filled before first use; every call leaves them at zero) are allocated
     when not given and the longest possible context needs more than one
     partition. ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn)
-    with these scales; ``q`` is of the pool's dtype, or fp32 (queries that were not
+    or, if uint8, of a 4-bit one with these scales; ``q`` is of the pool's dtype, or fp32 (queries that were not
     rounded to it) with ``out`` of it.
     """
     if kv_scales is not None:
@@ -256,6 +345,9 @@ class DecodePlan:
         return (self.buf, (self.num_seqs, self.num_q_heads, self.num_kv_heads, self.max_blocks, self.block_size,
                            self.num_blocks, self.slot_stride, self.head_stride),
                 self.dtype, PLAN_SHARE_GROUPS if self.share_groups else 0)
+
+
+_CODE_DTYPES = {CODES: DTYPE_E4M3, CODES4: DTYPE_E2M1}
 
 
 def decode_plan_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_blocks: int, block_size: int) -> int:
@@ -306,7 +398,7 @@ def decode_plan(
 ) -> DecodePlan:
     """Builds the balanced decode schedule of ``(block_tables, context_lens)``
     for query heads ``num_q_heads`` over pool layers shaped like ``k_cache``
-    ``[num_slots, H_kv, D]`` (any layer: all share the strides).
+    ``[num_slots, H_kv, D]`` (any layer: all share the strides; of a pool of codes, its codes).
     ``share_groups``: consecutive sequences whose tables begin with the same
     block ids (a shared cached prefix) run as pairs, one unit per KV head with
     both sequences' query heads, so the shared blocks are read once (taken when
@@ -326,7 +418,7 @@ def decode_plan(
     rc = lib().ir_paged_decode_plan(
         ptr(block_tables), block_tables.stride(0), max_blocks, ptr(context_lens), b, num_q_heads, h_kv,
         block_size, k_cache.shape[0] // block_size, k_cache.stride(0), k_cache.stride(1),
-        DTYPE_E4M3 if k_cache.dtype == CODES else dtype_code(k_cache.dtype),
+        _CODE_DTYPES[k_cache.dtype] if k_cache.dtype in _CODE_DTYPES else dtype_code(k_cache.dtype),
         PLAN_SHARE_GROUPS if share_groups else 0, ptr(buf), buf.numel(), ptr(err_flags),
         stream_ptr(dev),
     )
@@ -350,7 +442,7 @@ def paged_decode_planned(
     """:func:`paged_decode` over a plan: ``q`` ``[B, H_q, D]`` -> ``[B, H_q, D]``.
     ``workspace`` (uint8 scratch) and ``counters`` (int32 zeros, left at zero)
     are allocated when not given. ``kv_scales``, and ``q``'s dtype with them: as there,
-    the plan built for the float8_e4m3fn layer."""
+    the plan built for the layer of codes."""
     if kv_scales is not None:
         return seam().paged_decode_planned_q8(q, k_cache, v_cache, kv_scales, *plan.native(), scale, out, workspace,
                                               err_flags, counters, stream_of(q))
@@ -448,8 +540,85 @@ def rope_kv_scatter_q8(
     (normed keys from fp32, without a rounding to the dtype before). A ``q_out`` of fp32
     takes the queries as they leave the rotation, for an attention that is given them
     so."""
+    if kv_scales.dtype == CODES4:
+        raise RuntimeError("rope_kv_scatter_q8: kv_scales are a 4-bit pool's (rope_kv_scatter_q4 takes them)")
     return seam().norm_rope_kv_scatter(q, k, v, q_norm, k_norm, eps, cos, sin, k_cache, v_cache, kv_scales,
                                        int(block_size), slots, q_out, err_flags, stream_of(q))
+
+
+def rope_kv_scatter_q4(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    slots: torch.Tensor,
+    block_size: int,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 0.0,
+    q_out: torch.Tensor | None = None,
+    err_flags: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`rope_kv_scatter_q8` into one layer of a 4-bit pool: the rotated keys and
+    the values are quantised as :func:`kv_scatter_q4` does, in the same launch."""
+    if kv_scales.dtype != CODES4:
+        raise RuntimeError(f"rope_kv_scatter_q4: kv_scales must be uint8, got {kv_scales.dtype}")
+    return seam().norm_rope_kv_scatter(q, k, v, q_norm, k_norm, eps, cos, sin, k_cache, v_cache, kv_scales,
+                                       int(block_size), slots, q_out, err_flags, stream_of(q))
+
+
+def rope_axes(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    rotary: RotaryAxes,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary embedding of the rows ``q`` ``[N, H_q, D]`` and ``k`` ``[N, H_kv, D]`` by
+    ``positions`` int64 ``[axes, N]`` (or ``[N]`` for one axis): pair ``j`` of a head turns by
+    ``positions[rotary.axis_of[j]] * rotary.inv_freq[j]``. fp32 throughout, however far
+    the positions, rounded to the dtype once. Returns the rotated rows; outputs that are
+    given may be the inputs themselves, and ``q_out`` may be fp32 beside 16-bit rows.
+
+    ``q_norm``, ``k_norm`` (``[D]`` of the rows' dtype, both or neither): per-head norms
+    before the rotation, ``x * rsqrt(mean(x^2) + eps) * weight``, in the same launch
+    (``D`` 64 or 128; without norms a multiple of 16 up to 256)."""
+    pos, pairs = rotary.bind("rope_axes", positions, q)
+    return seam().rope_axes(q, k, pos, pairs, rotary.scaling, q_norm, k_norm, eps, q_out, k_out, stream_of(q))
+
+
+def rope_axes_kv_scatter(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    rotary: RotaryAxes,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    q_out: torch.Tensor | None = None,
+    err_flags: torch.Tensor | None = None,
+    kv_scales: torch.Tensor | None = None,
+    block_size: int = 0,
+) -> torch.Tensor:
+    """:func:`rope_axes` with the rotated ``k`` and ``v`` written into the pool layer at
+    ``slots`` (as :func:`kv_scatter`) instead of returned, one launch; ``head_dim`` 64 or
+    128. ``kv_scales`` (uint8, with the pool's ``block_size``): the caches are a layer of a
+    4-bit pool, and the keys are quantised from fp32 as they leave the rotation."""
+    pos, pairs = rotary.bind("rope_axes_kv_scatter", positions, q)
+    return seam().rope_axes_kv_scatter(q, k, v, pos, pairs, rotary.scaling, k_cache, v_cache, kv_scales,
+                                       int(block_size), slots, q_norm, k_norm, eps, q_out, err_flags, stream_of(q))
 
 
 PLAN_SHARE_GROUPS = 1  # IR_PLAN_SHARE_GROUPS
@@ -607,10 +776,10 @@ def paged_prefill(
     src_row0 + total_q - 1`` are this call's query tokens, whose keys are then
     read from those rows (``ERR_WRITE_SLOT`` is flagged where a token's write
     slot is not its block-table slot).
-    ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn) with these
-    scales; ``q`` is of the pool's dtype, or fp32 (queries that were not rounded to it)
-    with ``out`` of it. Its new rows are written before (:func:`kv_scatter_q8`), so
-    there is no ``new_kv``.
+    ``kv_scales``: the caches are a layer of an 8-bit pool (float8_e4m3fn) or, if uint8, of
+    a 4-bit one with these scales; ``q`` is of the pool's dtype, or fp32 (queries that were
+    not rounded to it) with ``out`` of it. Its new rows are written before
+    (:func:`kv_scatter_q8`, :func:`kv_scatter_q4`), so there is no ``new_kv``.
     """
     stream = stream_of(q)
     if plan is not None:
@@ -624,7 +793,8 @@ def paged_prefill(
                                + ("fp32" if plan.f32 else "16-bit") + f" calls, q is {q.dtype}")
     if kv_scales is not None:
         if new_kv is not None:
-            raise RuntimeError("paged_prefill: new_kv cannot be written to an 8-bit cache by the same launch")
+            raise RuntimeError(f"paged_prefill: new_kv cannot be written to {'a 4' if kv_scales.dtype == CODES4 else 'an 8'}"
+                               "-bit cache by the same launch")
         return seam().paged_prefill_q8(q, k_cache, v_cache, kv_scales, block_tables, cu_seqlens_q, q_start,
                                        int(max_q_len), block_size, scale, out, err_flags,
                                        None if plan is None else plan.buf, stream)
@@ -853,10 +1023,13 @@ def hbm_read_granule() -> int:
 __all__ = [
     "kv_scatter",
     "kv_scatter_q8",
+    "kv_scatter_q4",
     "gather_slots",
     "gather_slots_q8",
+    "gather_slots_q4",
     "paged_gather",
     "paged_gather_q8",
+    "paged_gather_q4",
     "paged_decode",
     "paged_attention_masked",
     "paged_prefill",
@@ -866,6 +1039,9 @@ __all__ = [
     "prefill_plan_pays",
     "rope_kv_scatter",
     "rope_kv_scatter_q8",
+    "rope_kv_scatter_q4",
+    "rope_axes",
+    "rope_axes_kv_scatter",
     "qk_norm_rope_kv_scatter",
     "decode_workspace_bytes",
     "default_partition",

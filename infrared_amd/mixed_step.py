@@ -29,7 +29,7 @@ decode rows + 4 x 256-token chunks: 187.5 against 177.5 us per layer, with a
 prefill workgroup (~78 KB of LDS) fitting beside each decode workgroup
 (72 KB), so the loss is the branches' cost, not CUs held by the prefill.
 
-Over a ``QuantPagedKVPool`` the write is always its own launch (``fused`` is off):
+Over a ``QuantPagedKVPool`` or ``Quant4PagedKVPool`` the write is always its own launch (``fused`` is off):
 the chunks attend what the pool holds.
 
 The per-layer projections around attention are not part of this path; the
@@ -45,7 +45,7 @@ import torch
 
 from infrared_amd import kernels, metadata
 from infrared_amd.hip_graph import capturing
-from infrared_amd.paged_kv_cache import PagedKVPool, QuantPagedKVPool
+from infrared_amd.paged_kv_cache import PagedKVPool, Quant4PagedKVPool, QuantPagedKVPool
 
 
 @dataclass(frozen=True)
@@ -168,7 +168,7 @@ class MixedStep:
             for name in ("q_dec", "q_pre", "k_new", "v_new"):
                 dtype = getattr(inputs, name).dtype
                 if dtype != pool.dtype:
-                    raise RuntimeError(f"MixedStep: {name} is {dtype}, the 8-bit pool's dtype is {pool.dtype}")
+                    raise RuntimeError(f"MixedStep: {name} is {dtype}, the {pool.bits}-bit pool's dtype is {pool.dtype}")
         self.fused = fused and not overlap and not self.quant
         dev = pool.device
         self.out_dec = torch.empty_like(inputs.q_dec)
@@ -208,8 +208,8 @@ class MixedStep:
         pool, rows = self.pool, (self.inputs.k_new[layer, lo:hi], self.inputs.v_new[layer, lo:hi])
         slots = self.batch.write_slots[lo:hi]
         if self.quant:
-            kernels.kv_scatter_q8(pool.k[layer], pool.v[layer], pool.kv_scales[layer], *rows, slots, pool.block_size,
-                                  self.err)
+            write = kernels.kv_scatter_q4 if isinstance(pool, Quant4PagedKVPool) else kernels.kv_scatter_q8
+            write(pool.k[layer], pool.v[layer], pool.kv_scales[layer], *rows, slots, pool.block_size, self.err)
         else:
             kernels.kv_scatter(pool.k[layer], pool.v[layer], *rows, slots, self.err)
 

@@ -40,8 +40,8 @@ calls once per layer (``infrared/model/layers.py:178-180``):
      exactly as the reference's naive path does
      (``infrared/model/triton_attention.py:110-129``).
 
-Over a ``QuantPagedKVPool`` the write quantises and the first two of these attend
-through the scales; the ones that start from ``gather_slots`` are refused.
+Over a ``QuantPagedKVPool`` or ``Quant4PagedKVPool`` the write quantises and the first two of
+these attend through the scales; the ones that start from ``gather_slots`` are refused.
 
 ``paged`` may be this package's ``PagedContext`` or any object with the same
 attributes (the reference's own ``PagedContext`` works: it simply lacks the
@@ -55,7 +55,8 @@ import torch
 
 from infrared_amd import kernels
 from infrared_amd._lib import seam, stream_of
-from infrared_amd.paged_kv_cache import PagedKVPool, QuantPagedKVPool
+from infrared_amd.paged_kv_cache import PagedKVPool, Quant4PagedKVPool, QuantPagedKVPool
+from infrared_amd.rotary import RotaryAxes
 
 _POOL_WRITE = PagedKVPool.write
 
@@ -115,19 +116,12 @@ def rope_paged_attention(
     ``q_norm``, ``k_norm`` (``[D]``, of the activations' dtype, both or neither):
     queries and keys are normed per head before the rotation, ``x * rsqrt(mean(x^2) +
     eps) * weight``, in the same kernel, which then stays in fp32 and rounds once
-    (``ir_qk_norm_rope_kv_scatter``; ``ir_rope_kv_scatter_q8`` for an 8-bit pool, whose
-    attention takes the queries unrounded).
+    (``ir_qk_norm_rope_kv_scatter``; ``ir_rope_kv_scatter_q8`` or ``_q4`` for a pool of codes,
+    whose attention takes the queries unrounded).
     """
     pool = paged.pool
-    h_kv, d = k.shape[-2], k.shape[-1]
-    b, sq, hq, dq = q.shape
-    if dq != d or hq != h_kv * n_rep:
-        raise RuntimeError(
-            f"rope_paged_attention: q {tuple(q.shape)} inconsistent with k {tuple(k.shape)} and n_rep={n_rep}"
-        )
-    if (q_norm is None) != (k_norm is None):
-        raise RuntimeError("rope_paged_attention: q_norm and k_norm go together")
-    rows = (q.reshape(b * sq, hq, d), k.reshape(b * sq, h_kv, d), v.reshape(b * sq, h_kv, d))
+    rows = _step_rows("rope_paged_attention", q, k, v, n_rep, q_norm, k_norm)
+    b, sq, hq, d = q.shape
     angles = (cos.reshape(b * sq, d), sin.reshape(b * sq, d))
     k_layer, v_layer, scales = _layer(pool, layer_idx)
     caches = (k_layer, v_layer)
@@ -137,8 +131,9 @@ def rope_paged_attention(
         # normed queries stay fp32 up to the scores, as normed keys do up to their codes: a
         # rounding of theirs would be as large an error of the outputs as all others
         q_out = None if q_norm is None else torch.empty(b * sq, hq, d, dtype=torch.float32, device=q.device)
-        q_rot = kernels.rope_kv_scatter_q8(*rows, *angles, *caches, scales, paged.write_slots,
-                                           pool.block_size, q_norm, k_norm, eps, q_out, err_flags=err)
+        write = kernels.rope_kv_scatter_q4 if isinstance(pool, Quant4PagedKVPool) else kernels.rope_kv_scatter_q8
+        q_rot = write(*rows, *angles, *caches, scales, paged.write_slots, pool.block_size, q_norm, k_norm, eps, q_out,
+                      err_flags=err)
     elif q_norm is not None:
         q_rot = kernels.qk_norm_rope_kv_scatter(*rows, q_norm, k_norm, eps, *angles, *caches, paged.write_slots,
                                                 err_flags=err)
@@ -147,16 +142,77 @@ def rope_paged_attention(
     return _attend(q_rot.view(b, sq, hq, d), paged, mask, layer_idx, scale)
 
 
+def rope_axes_paged_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    rotary: RotaryAxes,
+    paged,
+    mask: torch.Tensor | None,
+    layer_idx: int,
+    scale: float,
+    n_rep: int,
+    *,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> torch.Tensor:
+    """:func:`rope_paged_attention` for tokens with a position for each of several axes:
+    the rotation is ``rotary``'s, by ``positions`` int64 ``[axes, B, Sq]`` (``[B, Sq]`` for one
+    axis), fused with the optional norms and the K/V write (``ir_rope_axes_kv_scatter``), in
+    fp32 and rounded once.
+
+    Over a 4-bit pool the same launch quantises the keys, from fp32, and its attention
+    takes the queries unrounded. Over an 8-bit pool the rotation is a launch of its own
+    (``ir_rope_axes``) and the pool's write follows.
+    """
+    pool = paged.pool
+    name = "rope_axes_paged_attention"
+    rows = _step_rows(name, q, k, v, n_rep, q_norm, k_norm)
+    b, sq, hq, d = q.shape
+    if positions.shape[-2:] != (b, sq) or positions.dim() not in (2, 3):
+        raise RuntimeError(f"{name}: positions {tuple(positions.shape)} for rows [{b}, {sq}]; [axes, B, Sq] expected")
+    positions = positions.reshape(-1, b * sq)
+    k_layer, v_layer, scales = _layer(pool, layer_idx)
+    err = getattr(pool, "err_flags", None)
+    q_out = None
+    if scales is not None:
+        _check_quant(pool, q, paged)
+        # (the queries stay fp32 up to the scores, as in rope_paged_attention)
+        q_out = torch.empty(b * sq, hq, d, dtype=torch.float32, device=q.device)
+    if scales is not None and not isinstance(pool, Quant4PagedKVPool):
+        q_rot, k_rot = kernels.rope_axes(rows[0], rows[1], positions, rotary, q_norm, k_norm, eps, q_out)
+        pool.write(layer_idx, k_rot, rows[2], paged.write_slots)
+    else:
+        q_rot = kernels.rope_axes_kv_scatter(*rows, positions, rotary, k_layer, v_layer, paged.write_slots, q_norm,
+                                             k_norm, eps, q_out, err, scales,
+                                             0 if scales is None else pool.block_size)
+    return _attend(q_rot.view(b, sq, hq, d), paged, mask, layer_idx, scale)
+
+
+def _step_rows(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_rep: int,
+               q_norm: torch.Tensor | None, k_norm: torch.Tensor | None) -> tuple[torch.Tensor, ...]:
+    """``q``, ``k`` and ``v`` ``[B, Sq, H, D]`` as rows, checked against each other."""
+    h_kv, d = k.shape[-2], k.shape[-1]
+    b, sq, hq, dq = q.shape
+    if dq != d or hq != h_kv * n_rep:
+        raise RuntimeError(f"{name}: q {tuple(q.shape)} inconsistent with k {tuple(k.shape)} and n_rep={n_rep}")
+    if (q_norm is None) != (k_norm is None):
+        raise RuntimeError(f"{name}: q_norm and k_norm go together")
+    return q.reshape(b * sq, hq, d), k.reshape(b * sq, h_kv, d), v.reshape(b * sq, h_kv, d)
+
+
 def _check_quant(pool: QuantPagedKVPool, q: torch.Tensor, paged) -> None:
-    """Refuses, before anything is written, what an 8-bit pool has no kernel for."""
+    """Refuses, before anything is written, what a pool of codes has no kernel for."""
     if q.dtype != pool.dtype:
-        raise RuntimeError(f"paged_attention: q is {q.dtype}, the 8-bit pool's dtype is {pool.dtype}")
+        raise RuntimeError(f"paged_attention: q is {q.dtype}, the {pool.bits}-bit pool's dtype is {pool.dtype}")
     tables = paged.use_triton and getattr(paged, "block_tables", None) is not None
     packed = getattr(paged, "cu_seqlens_q", None) is not None and getattr(paged, "q_start", None) is not None
     if not tables or not (packed or (getattr(paged, "context_lens", None) is not None and q.shape[1] == 1)):
         raise RuntimeError(
-            "paged_attention: an 8-bit pool is attended through block_tables, with context_lens for a single-token "
-            "decode or cu_seqlens_q and q_start for packed chunks (metadata.decode_context, prefill_context)"
+            f"paged_attention: {'an 8' if pool.bits == 8 else 'a 4'}-bit pool is attended through block_tables, with "
+            "context_lens for a single-token decode or cu_seqlens_q and q_start for packed chunks (metadata.decode_context, prefill_context)"
         )
 
 
@@ -411,7 +467,7 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
 
 
 def _out_for(q: torch.Tensor, pool) -> torch.Tensor | None:
-    """The output for rows ``q`` ``[N, H_q, D]`` of fp32 that attend an 8-bit pool of
+    """The output for rows ``q`` ``[N, H_q, D]`` of fp32 that attend a pool of codes of
     another dtype; None where it is of ``q``'s."""
     if not isinstance(pool, QuantPagedKVPool) or q.dtype == pool.dtype:
         return None
@@ -419,7 +475,7 @@ def _out_for(q: torch.Tensor, pool) -> torch.Tensor | None:
 
 
 def _layer(pool, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """The layer's K, V and, of an 8-bit pool, scales."""
+    """The layer's K, V and, of a pool of codes, scales."""
     if isinstance(pool, QuantPagedKVPool):
         return pool.layer(layer_idx)
     return pool.k[layer_idx], pool.v[layer_idx], None

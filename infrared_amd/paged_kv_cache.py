@@ -352,6 +352,8 @@ class QuantPagedKVPool(PagedKVPool):
     or 128.
     """
 
+    bits = 8
+
     def __init__(
         self,
         num_layers: int,
@@ -364,13 +366,7 @@ class QuantPagedKVPool(PagedKVPool):
         *,
         strict: bool = False,
     ) -> None:
-        dtype_code(dtype)
-        if block_size <= 0 or block_size % 16 or block_size > 1024:
-            raise ValueError(f"an 8-bit pool's block size is a multiple of 16, at most 1024; got {block_size}")
-        if head_dim not in (64, 128):
-            raise ValueError(f"an 8-bit pool's head_dim is 64 or 128; got {head_dim}")
-        if num_blocks * block_size >= 2**31:
-            raise ValueError(f"{num_blocks} blocks of {block_size} tokens exceed 2^31 slots")
+        self._check_shape(num_blocks, block_size, head_dim, dtype)
         super().__init__(num_layers, num_blocks, block_size, num_kv_heads, head_dim, kernels.CODES, device,
                          strict=strict)
         self.dtype = dtype
@@ -378,6 +374,17 @@ class QuantPagedKVPool(PagedKVPool):
         # (empty blocks have the least scale: whatever is written first sets it)
         self.kv_scales = torch.full((num_layers, num_kv_heads, num_blocks, 2),
                                     2.0 ** (-15 if dtype == torch.float16 else -100), device=self.device)
+
+    @classmethod
+    def _check_shape(cls, num_blocks: int, block_size: int, head_dim: int, dtype: torch.dtype) -> None:
+        dtype_code(dtype)
+        a = "an" if cls.bits == 8 else "a"
+        if block_size <= 0 or block_size % 16 or block_size > 1024:
+            raise ValueError(f"{a} {cls.bits}-bit pool's block size is a multiple of 16, at most 1024; got {block_size}")
+        if head_dim not in (64, 128):
+            raise ValueError(f"{a} {cls.bits}-bit pool's head_dim is 64 or 128; got {head_dim}")
+        if num_blocks * block_size >= 2**31:
+            raise ValueError(f"{num_blocks} blocks of {block_size} tokens exceed 2^31 slots")
 
     def layer(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """One layer's ``(k, v, kv_scales)`` (views, made once for the tensors the pool has)."""
@@ -413,6 +420,84 @@ class QuantPagedKVPool(PagedKVPool):
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """``PagedKVPool.gather_blocks`` of the values the codes stand for, in ``dtype``."""
         out = kernels.paged_gather_q8(
+            self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], block_tables, context_lens,
+            self.block_size, max_ctx, self.dtype, self.err_flags,
+        )
+        if self.strict:
+            self.check_errors()
+        return out
+
+
+class Quant4PagedKVPool(QuantPagedKVPool):
+    """A K/V pool held in 4 bits: a quarter of a 16-bit one's memory and a sixteenth for
+    scales, and as much less for its attention to read.
+
+    Used as the 8-bit pool is, ``dtype`` alike. Groups of 32 channels of a token's head,
+    K or V, share a scale, a power of two; a value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a
+    sign, times it. ``k`` / ``v`` uint8 ``[num_layers, num_slots, num_kv_heads, head_dim / 2]``
+    hold two codes a byte in head-major storage, in tiles of 16 slots whose order is the
+    kernels' (``write`` and ``gather`` address slots, indexing does not), ``kv_scales`` uint8
+    ``[num_layers, num_kv_heads, num_slots / 16, head_dim]`` the scales' exponents plus 127
+    (255: the group is NaN).
+
+    ``write`` quantises (``ir_kv_scatter_q4``): a group's scale is the least with which its largest
+    magnitude is at most 7, every value is rounded to the nearest code, the largest to 6, and
+    a group with a NaN or an infinity becomes NaN. A token's scales are its own, so a
+    write changes nothing but its slots, whatever else is in their blocks. Of equal slots the
+    last is written in calls of up to 1,024 tokens; in longer ones their rows must be equal.
+    """
+
+    bits = 4
+
+    def __init__(
+        self,
+        num_layers: int,
+        num_blocks: int,
+        block_size: int,
+        num_kv_heads: int,
+        head_dim: int,
+        dtype: torch.dtype,
+        device: torch.device | str = "cuda",
+        *,
+        strict: bool = False,
+    ) -> None:
+        self._check_shape(num_blocks, block_size, head_dim, dtype)
+        PagedKVPool.__init__(self, num_layers, num_blocks, block_size, num_kv_heads, head_dim // 2, kernels.CODES4,
+                             device, strict=strict)
+        self.head_dim = head_dim
+        self.dtype = dtype
+        self._layers = None
+        # (what was never written is 0 at the least scale)
+        self.kv_scales = torch.full((num_layers, num_kv_heads, self.num_slots // 16, head_dim),
+                                    127 - (23 if dtype == torch.float16 else 100), dtype=torch.uint8, device=self.device)
+
+    def write(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Quantises this step's K/V (``[N, num_kv_heads, head_dim]`` of ``dtype``) into ``slots``
+        (``[N]`` int64; negative: skipped)."""
+        if k.dtype != self.dtype:
+            raise RuntimeError(f"Quant4PagedKVPool.write: k is {k.dtype}, the pool's dtype is {self.dtype}")
+        seam().pool_write_q4(self.k, self.v, self.kv_scales, layer_idx, k, v, slots, self.block_size, self.err_flags,
+                             stream_of(self.k))
+        if self.strict:
+            self.check_errors()
+
+    def gather(self, layer_idx: int, gather_slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """``PagedKVPool.gather`` of the values the codes stand for, in ``dtype``."""
+        out = seam().pool_gather_q4(self.k, self.v, self.kv_scales, layer_idx, gather_slots, self.block_size,
+                                    self.dtype, self.err_flags, stream_of(self.k))
+        if self.strict:
+            self.check_errors()
+        return out
+
+    def gather_blocks(
+        self,
+        layer_idx: int,
+        block_tables: torch.Tensor,
+        context_lens: torch.Tensor,
+        max_ctx: int,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """``PagedKVPool.gather_blocks`` of the values the codes stand for, in ``dtype``."""
+        out = kernels.paged_gather_q4(
             self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], block_tables, context_lens,
             self.block_size, max_ctx, self.dtype, self.err_flags,
         )
