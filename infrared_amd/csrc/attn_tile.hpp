@@ -262,17 +262,16 @@ constexpr float kProbUp = DT == IR_DTYPE_F16 ? 7.f : 0.f;
 // of LDS, and the probabilities of a 16-bit dtype in two pieces of it (off by 2^-18, fp16
 // 2^-24), so that the output's rounding is all that shows. A product of 32 k-slots holds both
 // pieces, the V rows twice, and takes as long as one of 16.
-// UP: probabilities are held 2^UP times larger (st.m is the maximum less UP).
-template <int DT, int D, bool FULL, bool Q8 = false, int UP = 0>
+template <int DT, int D, bool FULL, bool Q8 = false>
 __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t (&vin)[4][TileShape<DT, D>::VDW],
                                            const bool (&vok)[4], State<D>& st) {
   typedef TileShape<DT, D> Sh;
   constexpr int TILES = Sh::TILES;
   float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
   mx = Q8 ? wave_max_groups_swap(mx) : wave_max_groups(mx);
-  const bool grow = mx > st.m + (kRescaleSlack + UP);
+  const bool grow = mx > st.m + kRescaleSlack;
   if (__any(grow)) {
-    const float m_new = grow ? mx - UP : st.m;
+    const float m_new = grow ? mx : st.m;
     const float alpha = fast_exp2(st.m - m_new);  // 1 if unchanged, 0 from the start value
     st.l *= alpha;
 #pragma unroll

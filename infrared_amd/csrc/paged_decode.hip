@@ -55,7 +55,7 @@ void paged_decode_kernel(DecodeArgs a) {
   __shared__ int s_last;
 
   const int lane = threadIdx.x & 63;
-  const int w = threadIdx.x >> 6;
+  const int w = FMT == kCodes4 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x >> 6;
   const int g = lane >> 4;
   const int c = lane & 15;
 
@@ -84,14 +84,18 @@ void paged_decode_kernel(DecodeArgs a) {
   const uint8_t* scales4 = FMT == kCodes4 ? a.scales4 + kvh * a.c_head / 8 : nullptr;
   const typename F::Offsets lo = F::offsets(lane, a.c_slot * F::EB);
   QueryRegs<DT, D, QF> qr;
-  load_query_for<DT, D, FMT>(a, seq, kvh * a.n_rep + h_local, h_local < a.n_rep, g, qr);
-  qr.split();
+  load_query_for<DT, D, FMT>(a, seq, kvh * a.n_rep + (FMT == kCodes4 ? min(h_local, a.n_rep - 1) : h_local),
+                             h_local < a.n_rep, g, qr);
+  if (FMT != kCodes4) qr.split();
 
   State<D> st;
   state_init(st);
   bool bad = false;
-  attend_tiles<DT, D, BS16, NW, DEPTH, FMT, QF>(a, bt_row, kc, vc, scales, scales4, lo, qr, tile_lo, tile_hi, t_end,
-                                                kstage[w], lane, w, st, bad);
+  if constexpr (FMT == kCodes4)
+    attend_tiles4<DT, D, NW, QF>(a, bt_row, kc, vc, scales4, lo, qr, tile_lo, tile_hi, t_end, lane, w, st, bad);
+  else
+    attend_tiles<DT, D, BS16, NW, DEPTH, FMT, QF>(a, bt_row, kc, vc, scales, lo, qr, tile_lo, tile_hi, t_end, kstage[w],
+                                                  lane, w, st, bad);
   if (bad) flag_error(a.err, IR_ERR_BLOCK_RANGE);
   st.l = wave_sum_groups(st.l);
 

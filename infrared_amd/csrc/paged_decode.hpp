@@ -156,6 +156,10 @@ template <int DT, int D, bool QF>
 struct QueryRegs {
   uint32_t x[TileShape<DT, D>::KDW];
   __device__ __forceinline__ void split() {}
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (uint32_t& e : x) e ^= TileShape<DT, D>::k16 ? 0x80008000u : 0x80000000u;
+  }
   __device__ __forceinline__ float scaled(float scale) const { return scale; }
 };
 template <int DT, int D>
@@ -163,6 +167,13 @@ struct QueryRegs<DT, D, true> {
   static constexpr int N = TileShape<DT, D>::KDW;
   uint32_t x[N], rest[N];
   float unit;
+  __device__ __forceinline__ void negate() {  // (before split())
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x[i] ^= 0x80000000u;
+      rest[i] ^= 0x80000000u;
+    }
+  }
   // (all lanes of the wavefront: the four lane groups hold a row together)
   __device__ __forceinline__ void split() {
     float v[2 * N], most = 0.f;
@@ -207,16 +218,20 @@ __device__ __forceinline__ void issue_codes(const uint8_t* tk, const uint8_t* tv
   }
 }
 
-// Issues a 4-bit tile's loads; its codes are `at` bytes past kc / vc, 8 times as far as its
-// scales past sc.
+// Issues the loads of a 4-bit tile's K, and of its V; its codes are `at` bytes past kc / vc, 8
+// times as far as its scales past sc.
 template <int DT, int D>
-__device__ __forceinline__ void issue_codes4(const uint8_t* kc, const uint8_t* vc, const uint8_t* sc, int64_t at,
-                                             const typename CacheFormat<DT, D, kCodes4>::Offsets& lo,
-                                             Code4Tile<D>& tl) {
-  const uint8_t *tk = kc + at, *tv = vc + at, *ts = sc + at / 8;
+__device__ __forceinline__ void issue_k4(const uint8_t* kc, const uint8_t* sc, int64_t at,
+                                         const typename CacheFormat<DT, D, kCodes4>::Offsets& lo, Code4Tile<D>& tl) {
+  const uint8_t *tk = kc + at, *ts = sc + at / 8;
   load_dwords_nt<D / 32, true>(tk + lo.codes, tl.k);
-  load_dwords_nt<D / 32, true>(tv + lo.codes, tl.v);
   tl.ks = __builtin_nontemporal_load(ts + lo.ks);
+}
+template <int DT, int D>
+__device__ __forceinline__ void issue_v4(const uint8_t* vc, const uint8_t* sc, int64_t at,
+                                         const typename CacheFormat<DT, D, kCodes4>::Offsets& lo, Code4Tile<D>& tl) {
+  const uint8_t *tv = vc + at, *ts = sc + at / 8;
+  load_dwords_nt<D / 32, true>(tv + lo.codes, tl.v);
   tl.vs = __builtin_nontemporal_load((const uint32_t*)(ts + lo.vs));
 }
 
@@ -397,60 +412,146 @@ __device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const Query
   }
 }
 
-// The same for a 4-bit tile. The conversions take a group's scale with them, so the
-// scores need none: a lane's K is one group's, its four rows of V a group each. QF as above.
-template <int DT, int D, bool QF>
-__device__ __forceinline__ void compute_codes4(const Code4Tile<D>& tl, const QueryRegs<DT, D, QF>& q, uint32_t kmask,
-                                               float scale_log2, State<D>& st, bool col_on = true) {
+// A pair of 4-bit tiles in registers.
+template <int D>
+struct Pair4 {
+  Code4Tile<D> a, b;
+};
+
+// The same for 4-bit tiles, two of them (32 keys) at a time. The conversions take a group's
+// scale with them, so the scores need none: a lane's K is one group's, its four rows of V a
+// group each. QF as above.
+//
+// What bounds the loop is issuing instructions: a wavefront issues one every 8 cycles, two on a
+// SIMD one every 5, and a tile at a time, with the products of softmax_pv, took some 310 a
+// tile (64 sequences of 512..4096 keys 28.6 us, whatever the number of tiles in flight). So
+// - the common path compares each lane's own scores with the running maximum: only where
+//   one is past the slack are they reduced over the lanes;
+// - the scores stay as the products gave them, and one multiply-add makes them exponents;
+// - a product of 32 k-slots takes 8 keys of a lane, one permutation making each dword of its V
+//   operand, and the probabilities' two pieces are two products with the same V.
+// The codes are dead once they are numbers, so the next pair's loads go into the same
+// registers: its K's as soon as the scores are there (next_k), its V's behind the products (next_v).
+//
+// valid_a, valid_b: the tiles' usable keys; col_a, col_b: whether the lane's column attends the tile;
+// whole: it is all of them. An absent key's scales become 0, what it holds finite.
+template <int DT, int D, bool QF, typename NextK, typename NextV>
+__device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D, QF>& q, bool whole, int valid_a,
+                                              int valid_b, bool col_a, bool col_b, float scale_log2, int lane,
+                                              State<D>& st, NextK next_k, NextV next_v) {
   typedef TileShape<DT, D> Sh;
   constexpr int W = Sh::k16 ? 4 : 8;  // dwords of eight elements
-  const float score_scale = q.scaled(scale_log2), ks = scale_of_byte(tl.ks);
-  uint32_t kop[Sh::KDW];
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    uint32_t x[W];
-    decode8_e2m1<DT>(tl.k[j], ks, x);
-#pragma unroll
-    for (int i = 0; i < W; ++i) kop[W * j + i] = x[i];
+  constexpr float UP = kProbUp<DT>;
+  Code4Tile<D>&ta = x.a, &tb = x.b;
+  const int g = lane >> 4;
+  if (!whole) {
+    const int key = staged_token(lane & 15);
+    ta.ks = key < valid_a ? ta.ks : 0u;
+    tb.ks = key < valid_b ? tb.ks : 0u;
+    auto rows = [&](int valid) {  // bytes of the usable ones of the rows 4 r + g
+      const int n = (valid - g + 3) >> 2;
+      return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1u;
+    };
+    ta.vs &= rows(valid_a);
+    tb.vs &= rows(valid_b);
   }
-  f32x4 s = qk_tile<DT, D>(kop, q.x);
-  if constexpr (QF) s += qk_tile<DT, D>(kop, q.rest);
-  uint32_t v[4][Sh::VDW];
+  auto scores = [&](const Code4Tile<D>& t) {
+    uint32_t kop[Sh::KDW];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      uint32_t x[W];
+      decode8_e2m1<DT>(t.k[j], scale_of_byte(t.ks), x);
+#pragma unroll
+      for (int i = 0; i < W; ++i) kop[W * j + i] = x[i];
+    }
+    f32x4 s = qk_tile<DT, D>(kop, q.x);
+    if constexpr (QF) s += qk_tile<DT, D>(kop, q.rest);
+    return s;
+  };
+  const f32x4 sa = scores(ta), sb = scores(tb);
+  next_k();
+  // (not 0: an absent key's score is infinite; a negative scale is in the queries' signs)
+  const float c = fmaxf(q.scaled(fabsf(scale_log2)), __FLT_MIN__);
+  float p[8];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const float vs = scale_of_byte((tl.vs >> (8 * r)) & 0xffu);
-    if constexpr (D == 128) {
-      decode8_e2m1<DT>(tl.v[r], vs, v[r]);
-    } else if constexpr (Sh::k16) {
-      const uint32_t w = tl.v[r >> 1] >> (16 * (r & 1));
-      v[r][0] = decode2_e2m1<DT, 0>(w, vs);
-      v[r][1] = decode2_e2m1<DT, 1>(w, vs);
+    p[r] = sa[r];
+    p[4 + r] = sb[r];
+  }
+  if (!whole) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] = 4 * r + g < valid_a && col_a ? p[r] : kNegInf;
+      p[4 + r] = 4 * r + g < valid_b && col_b ? p[4 + r] : kNegInf;
+    }
+  }
+  float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+  if (__any(mx * c > st.m + (kRescaleSlack + UP))) {
+    mx = wave_max_groups_swap(mx) * c;
+    const float m_new = mx > st.m + (kRescaleSlack + UP) ? mx - UP : st.m;
+    const float alpha = fast_exp2(st.m - m_new);  // 1 if unchanged, 0 from the start value
+    st.l *= alpha;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) st.acc[n] *= alpha;
+    st.m = m_new;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = fast_exp2(__builtin_fmaf(p[i], c, -st.m));
+  st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+  // dword I of a row of V: elements 2 I, 2 I + 1 of the lane's key R of tile t (two dwords in fp32)
+  auto value = [&](const Code4Tile<D>& t, auto row, auto dw) {
+    constexpr int R = decltype(row)::value, I = decltype(dw)::value;
+    constexpr int B = D == 128 ? I : 2 * (R & 1) + I;  // byte of its dword of codes
+    const uint32_t w = t.v[D == 128 ? R : R >> 1];
+    const float vs = scale_of_byte<R>(t.vs);
+    if constexpr (Sh::k16) {
+      return decode2_e2m1<DT, B>(w, vs);
     } else {
-      const uint32_t w = tl.v[r >> 1] >> (16 * (r & 1));
-      const f32x2 a = decode2_e2m1_f32<0>(w, vs), b = decode2_e2m1_f32<1>(w, vs);
-      v[r][0] = __float_as_uint(a[0]);
-      v[r][1] = __float_as_uint(a[1]);
-      v[r][2] = __float_as_uint(b[0]);
-      v[r][3] = __float_as_uint(b[1]);
+      return decode2_e2m1_f32<B>(w, vs);
+    }
+  };
+  u32x4 hi, lo;
+  if constexpr (Sh::k16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const Pieces w = split2<DT>(p[2 * i], p[2 * i + 1]);
+      hi[i] = w.hi;
+      lo[i] = w.lo;
     }
   }
-  float sv[4];
-  bool vok[4];
-  if (__all(kmask == 0xfu)) {
+  auto products = [&](auto dw) {
+    constexpr int I = decltype(dw)::value;
+    typedef std::integral_constant<int, 0> R0;
+    typedef std::integral_constant<int, 1> R1;
+    typedef std::integral_constant<int, 2> R2;
+    typedef std::integral_constant<int, 3> R3;
+    const auto v0 = value(ta, R0{}, dw), v1 = value(ta, R1{}, dw), v2 = value(ta, R2{}, dw), v3 = value(ta, R3{}, dw);
+    const auto v4 = value(tb, R0{}, dw), v5 = value(tb, R1{}, dw), v6 = value(tb, R2{}, dw), v7 = value(tb, R3{}, dw);
+    if constexpr (Sh::k16) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      vok[r] = true;
-      sv[r] = col_on ? s[r] * score_scale : kNegInf;
-    }
-    softmax_pv<DT, D, true, true, (int)kProbUp<DT>>(sv, v, vok, st);
-  } else {
+      for (int odd = 0; odd < 2; ++odd) {
+        const uint32_t sel = odd ? 0x07060302u : 0x05040100u;
+        const u32x4 x = {__builtin_amdgcn_perm(v1, v0, sel), __builtin_amdgcn_perm(v3, v2, sel),
+                         __builtin_amdgcn_perm(v5, v4, sel), __builtin_amdgcn_perm(v7, v6, sel)};
+        st.acc[2 * I + odd] = mfma_k32<DT>(x, hi, st.acc[2 * I + odd]);
+        st.acc[2 * I + odd] = mfma_k32<DT>(x, lo, st.acc[2 * I + odd]);
+      }
+    } else {
+      const f32x2 v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      vok[r] = (kmask >> r) & 1u;
-      sv[r] = vok[r] && col_on ? s[r] * score_scale : kNegInf;
+      for (int i = 0; i < 8; ++i) {
+        st.acc[2 * I] = mfma_f32_k4(v[i][0], p[i], st.acc[2 * I]);
+        st.acc[2 * I + 1] = mfma_f32_k4(v[i][1], p[i], st.acc[2 * I + 1]);
+      }
     }
-    softmax_pv<DT, D, false, true, (int)kProbUp<DT>>(sv, v, vok, st);
+  };
+  products(std::integral_constant<int, 0>{});
+  products(std::integral_constant<int, 1>{});
+  if constexpr (D == 128) {
+    products(std::integral_constant<int, 2>{});
+    products(std::integral_constant<int, 3>{});
   }
+  next_v();
 }
 
 // Context length of `seq`, clamped to what its block table can hold (flagged).
@@ -470,11 +571,11 @@ __device__ __forceinline__ int clamp_ctx(const DecodeArgs& a, int seq, bool repo
 // run fetches its block ids once, one per lane.
 template <int DT, int D, bool BS16, int NW, int DEPTH, int FMT, bool QF>
 __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t* bt_row, const uint8_t* kc,
-                                             const uint8_t* vc, const f32x2* scales, const uint8_t* scales4,
+                                             const uint8_t* vc, const f32x2* scales,
                                              const typename CacheFormat<DT, D, FMT>::Offsets& lo,
                                              const QueryRegs<DT, D, QF>& qr, int tile_lo, int tile_hi, int t_end,
                                              uint8_t* kst, int lane, int w, State<D>& st, bool& bad) {
-  static_assert(BS16 || FMT == kElements, "a block of codes holds whole tiles");
+  static_assert(FMT == kElements || (FMT == kCodes8 && BS16), "a block of codes holds whole tiles");
   typedef typename CacheFormat<DT, D, FMT>::Raw Raw;
   constexpr int RUN = NW * kMaxWaveTiles;
   for (int r0 = tile_lo; r0 < tile_hi; r0 += RUN) {
@@ -492,13 +593,12 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     }
     auto issue = [&](int i, Raw& tl) -> uint32_t {
       const int32_t bid = BS16 ? __builtin_amdgcn_readlane(bid_lane, i) : 0;
-      if constexpr (FMT != kElements) {
+      if constexpr (FMT == kCodes8) {
         const int g = lane >> 4, t0 = t_begin + 16 * (w + NW * i), blk = t0 / a.bs;
         const bool ok = bid >= 0 && (int64_t)bid < a.num_blocks;
         bad |= !ok;
         const int64_t at = ok ? ((int64_t)bid * a.bs + (t0 - blk * a.bs)) * D : 0;
-        if constexpr (FMT == kCodes4) issue_codes4<DT, D>(kc, vc, scales4, at / 2, lo, tl);
-        else issue_codes<DT, D>(kc + at, vc + at, lo, tl);
+        issue_codes<DT, D>(kc + at, vc + at, lo, tl);
         uint32_t m = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) m |= (ok && t0 + 4 * r + g < t_end) ? (1u << r) : 0u;
@@ -512,9 +612,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     Raw ring[DEPTH];
     uint32_t mk[DEPTH];
     auto compute = [&](const Raw& tl, int i, uint32_t mask) {
-      if constexpr (FMT == kCodes4) {
-        compute_codes4<DT, D, QF>(tl, qr, mask, a.scale_log2, st);
-      } else if constexpr (FMT == kCodes8) {
+      if constexpr (FMT == kCodes8) {
         const int ii = min(i, last);
         const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[0]), ii));
         const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[1]), ii));
@@ -548,6 +646,75 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
   }
 }
 
+// Makes a loaded query of code tiles the operand (K4: with the scale's sign, see compute_pair4).
+template <int DT, int D, int FMT, bool QF>
+__device__ __forceinline__ void query_ready(const DecodeArgs& a, QueryRegs<DT, D, QF>& q) {
+  if (FMT == kCodes4 && a.scale_log2 < 0.f) q.negate();
+  q.split();
+}
+
+// attend_tiles of a 4-bit cache: the wavefront's tiles two by two, tile_lo + 2 (w + i NW) and
+// the next. qr: as loaded.
+template <int DT, int D, int NW, bool QF>
+__device__ __forceinline__ void attend_tiles4(const DecodeArgs& a, const int32_t* bt_row, const uint8_t* kc,
+                                              const uint8_t* vc, const uint8_t* scales,
+                                              const typename CacheFormat<DT, D, kCodes4>::Offsets& lo,
+                                              QueryRegs<DT, D, QF>& qr, int tile_lo, int tile_hi, int t_end,
+                                              int lane, int w, State<D>& st, bool& bad) {
+  constexpr int RUN = NW * kMaxWaveTiles;
+  const int g = lane >> 4;
+  for (int r0 = tile_lo; r0 < tile_hi; r0 += RUN) {
+    const int ntiles = min(tile_hi - r0, RUN);
+    const int pairs = (ntiles + 1) / 2, my_pairs = pairs > w ? (pairs - w + NW - 1) / NW : 0;
+    if (my_pairs <= 0) break;
+    auto tile_of = [&](int i) { return r0 + 2 * (w + NW * (i >> 1)) + (i & 1); };  // of the wavefront's i-th
+    int32_t bid_lane = 0;
+    if (tile_of(lane) < r0 + ntiles) bid_lane = bt_row[16 * tile_of(lane) / a.bs];
+    // A tile's place and its usable keys (one past the end or of a bad block: the pool's first
+    // tile, none of it).
+    struct Spot {
+      int64_t at;
+      int valid;
+    };
+    auto spot = [&](int i) {
+      const int t0 = 16 * tile_of(i), blk = t0 / a.bs;
+      const int32_t bid = __builtin_amdgcn_readlane(bid_lane, i);
+      const bool in = tile_of(i) < r0 + ntiles, ok = in && bid >= 0 && (int64_t)bid < a.num_blocks;
+      bad |= in && !ok;
+      return Spot{ok ? ((int64_t)bid * a.bs + (t0 - blk * a.bs)) * (D / 2) : 0, ok ? min(16, t_end - t0) : 0};
+    };
+    Pair4<D> x;
+    Spot sa = spot(0), sb = spot(1);
+    issue_k4<DT, D>(kc, scales, sa.at, lo, x.a);
+    issue_k4<DT, D>(kc, scales, sb.at, lo, x.b);
+    issue_v4<DT, D>(vc, scales, sa.at, lo, x.a);
+    issue_v4<DT, D>(vc, scales, sb.at, lo, x.b);
+    if (r0 == tile_lo) query_ready<DT, D, kCodes4, QF>(a, qr);
+    auto step = [&](int i, auto more) {
+      const int va = sa.valid, vb = sb.valid;
+      if constexpr (decltype(more)::value) {
+        sa = spot(2 * i + 2);
+        sb = spot(2 * i + 3);
+      }
+      auto next_k = [&] {
+        if constexpr (decltype(more)::value) {
+          issue_k4<DT, D>(kc, scales, sa.at, lo, x.a);
+          issue_k4<DT, D>(kc, scales, sb.at, lo, x.b);
+        }
+      };
+      auto next_v = [&] {
+        if constexpr (decltype(more)::value) {
+          issue_v4<DT, D>(vc, scales, sa.at, lo, x.a);
+          issue_v4<DT, D>(vc, scales, sb.at, lo, x.b);
+        }
+      };
+      compute_pair4<DT, D, QF>(x, qr, va == 16 && vb == 16, va, vb, true, true, a.scale_log2, lane, st, next_k, next_v);
+    };
+    for (int i = 0; i + 1 < my_pairs; ++i) step(i, std::true_type{});
+    step(my_pairs - 1, std::false_type{});  // (nothing is issued past the end)
+  }
+}
+
 // Q^T operand of (seq, query head qh), same k-slot assignment as the K loads;
 // padded heads are zero.
 template <int DT, int D>
@@ -560,8 +727,9 @@ __device__ __forceinline__ void load_query(const DecodeArgs& a, int seq, int qh,
     zero_dwords(qr);
 }
 
-// The query operand that goes with code tiles (compute_codes; K4: compute_codes4, whose lane
-// group holds a quarter of the row in one run), before its split().
+// The query operand that goes with code tiles (compute_codes; K4: compute_pair4, whose lane
+// group holds a quarter of the row in one run, and where a padded head is another's number:
+// nothing between these loads and the tiles' has to wait or branch), before its split().
 template <int DT, int D, bool QF, bool K4>
 __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, int qh, bool head_ok, int g,
                                                  QueryRegs<DT, D, QF>& q) {
@@ -575,7 +743,7 @@ __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, i
   for (int j = 0; j < D / 64; ++j)
 #pragma unroll
     for (int i = 0; i < DW; i += 4) {
-      const u32x4 x = head_ok ? *(const u32x4*)(row + STEP * j * EB + 4 * i) : u32x4{0u, 0u, 0u, 0u};
+      const u32x4 x = K4 || head_ok ? *(const u32x4*)(row + STEP * j * EB + 4 * i) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = DW * j + i + e;

@@ -52,7 +52,8 @@ constexpr int kPlanWaves = 4;       // streaming wavefronts per workgroup
 // sequences of 512..4096 keys: 45.1 us with four, 33.5 with eight, whatever the number
 // of tiles in flight; twelve are short of registers, 46.5).
 constexpr int kCodeWaves = 8;
-// Of a call over a 4-bit cache.
+// Of a call over a 4-bit cache: as many (64 sequences of 512..4096 keys, 28 / 4 heads of 128:
+// 27.7 us with four, 25.4 with eight, 26.1 with twelve).
 constexpr int kCode4Waves = 8;
 constexpr int kMaxWaves = std::max(kPlanWaves, std::max(kCodeWaves, kCode4Waves));
 constexpr int kCodePlan = 1 << 16;  // (above any number of pairs)
@@ -433,11 +434,11 @@ __global__ __launch_bounds__(plan_waves(FMT) * 64) void paged_decode_plan_kernel
       const int kvh = p.n_hg == 1 ? j : fdiv(j, p.n_hg);
       // which sequence's keys the tile holds, and which column halves see it
       int sq = b, tok0 = ti * 16;
-      uint32_t cm = 1u;
+      uint32_t cm = FMT == kCodes4 ? 3u : 1u;  // (4 bits: a unit of one sequence has no other half)
       if (s_lead[b] > 0) {
         const int S = s_share[b], ta = tiles0(b);
-        if (ti < S) cm = 3u;
-        else if (ti >= ta) {
+        cm = ti < S ? 3u : 1u;
+        if (ti >= ta) {
           sq = b + 1;
           tok0 = (ti - ta + S) * 16;
           cm = 2u;
@@ -499,7 +500,11 @@ __device__ __forceinline__ void slot_read(const float* row, int g, f32x4 (&acc)[
 //
 // kCodes8: the tiles are codes; a run's lanes also fetch the scales of their tiles, whose
 // block the tile's pool offset gives (the layer is dense), ahead of the tiles' own loads.
-// kCodes4: a tile's scales are loaded with it.
+// kCodes4: a tile's scales are loaded with it, and the states of a unit that several wavefronts
+// of the workgroup share are joined by all of it. (64 sequences, 28 / 4 heads of 128: every key
+// takes 136 bytes, and a call of L keys a sequence 8 us + 1 us for every 6.2 MB, 30.3 us at
+// L = 4096, 4.7 TB/s. The 8 us: the launch 2.7, the plan's and the first tiles' round trips 2,
+// joining and writing 2.5.)
 template <int DT, int D, int NW, int DEPTH, bool PAIRS, int FMT = kElements, bool QF = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DT == IR_DTYPE_F32 && NW == 4 ? 1 : 2)))
 void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32_t o_pair, uint32_t o_whdr,
@@ -509,12 +514,16 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   constexpr int EB = Sh::EB;
   constexpr int NT = NW * 64;
   constexpr int TILES = D / 16;
-  __shared__ WaveSlots<NW, D> sl;
-  __shared__ WaveSlots<2, D> stg;  // this slice's cross-workgroup partials: [0] first unit, [1] last unit
+  // (JOIN: slots NW.. hold the states of owners, and nothing is staged)
+  constexpr bool JOIN = FMT == kCodes4;
+  __shared__ WaveSlots<JOIN ? 2 * NW : NW, D> sl;
+  // this slice's cross-workgroup partials: [0] first unit, [1] last unit
+  __shared__ WaveSlots<JOIN ? 1 : 2, JOIN ? 4 : D> stg;
   __shared__ __attribute__((aligned(16))) uint8_t kstage[NW][F::STAGE];
   __shared__ int s_pre[kPlanMaxSeqs + 1];
   __shared__ int s_pair[PAIRS ? kPlanMaxSeqs : 1];
   __shared__ int s_fl[NW];
+  __shared__ int s_own[JOIN ? 2 * NW : 1];  // the unit whose owner's state the slot holds
   __shared__ int s_stg[2];
   __shared__ int s_last[2];
 
@@ -556,6 +565,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     for (int b = tid + NT; b < B; b += NT) s_pair[b] = pp[b];
   }
   if (tid < NW) s_fl[tid] = -1;
+  if (JOIN && tid < 2 * NW) s_own[tid] = -1;
   if (tid < 2) s_stg[tid] = -1;
 
   // sequences with no usable key get a zero output row (workgroup 0)
@@ -600,15 +610,17 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     const int kvh = a.n_hg == 1 ? j : fdiv(j, a.n_hg);
     if (paired(b)) {  // columns 0..n_rep-1: sequence b, n_rep..2 n_rep-1: b + 1
       const int second = c >= a.n_rep;
-      load_query_for<DT, D, FMT>(a, b + second, kvh * a.n_rep + c - second * a.n_rep, c < 2 * a.n_rep, g, dst);
+      const int hl = c - second * a.n_rep;
+      load_query_for<DT, D, FMT>(a, b + second, kvh * a.n_rep + (JOIN ? min(hl, a.n_rep - 1) : hl), c < 2 * a.n_rep, g,
+                                 dst);
       return;
     }
-    const int hl = hg * 16 + c;
+    const int hl = JOIN ? min(hg * 16 + c, a.n_rep - 1) : hg * 16 + c;
     load_query_for<DT, D, FMT>(a, b, kvh * a.n_rep + hl, hl < a.n_rep, g, dst);
   };
   QueryRegs<DT, D, QF> qr, qn;
   int q_lbl = -1, qn_lbl = -1;
-  if (QF) {  // (split when it is needed, not as soon as it is here)
+  if (QF || JOIN) {  // (made ready when it is needed, not as soon as it is here)
     if (cnt_w > 0) q_of(fl, qn);
     qn_lbl = fl;
   } else if (cnt_w > 0) {
@@ -657,6 +669,10 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     slot_write<D>(stg.acc[k][c], stg.m[k], stg.l[k], st, g, c);
     if (lane == 0) s_stg[k] = u;
   };
+  auto slot_of = [&](int slot, int* owner, int u) {
+    slot_write<D>(sl.acc[slot][c], sl.m[slot], sl.l[slot], st, g, c);
+    if (lane == 0) *owner = u;
+  };
   auto wave_finish = [&](int u, bool at_end) {
     st.l = wave_sum_groups(st.l);
     const Lbl x = label(u);
@@ -667,13 +683,14 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       }
       write_out(x);
     } else if (max(x.us, lo) < wlo) {
-      slot_write<D>(sl.acc[w][c], sl.m[w], sl.l[w], st, g, c);
-      if (lane == 0) s_fl[w] = u;
+      slot_of(w, &s_fl[w], u);
     } else if (x.ue > whi) {
-      keep = u;
+      if constexpr (JOIN) slot_of(NW + w, &s_own[NW + w], u);
+      else keep = u;
       return;
-    } else {
-      stage_partial(u, 0);
+    } else {  // (the slice's first unit, its only part here: the wavefront's slot is free)
+      if constexpr (JOIN) slot_of(w, &s_own[w], u);
+      else stage_partial(u, 0);
     }
     if (!at_end) state_init(st);
   };
@@ -687,83 +704,136 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
     }
     const int cnt = min(kPlanRun, cnt_w - r0);
     const int last = cnt - 1;
-    f32x2 sc = {0.f, 0.f};
-    if constexpr (FMT == kCodes8) {
-      if (lane < cnt) sc = a.scales[info_off / a.block16];
-    }
-    // Issues the loads of tile i of the run (`real`: i is known to be a tile of
-    // the run). Past the run's end (the ring's last DEPTH issues, never
-    // computed) it issues nothing: the end phase reuses the ring's registers,
-    // and a load still in flight into them would hold it up (padding loads
-    // cost 0.7 us per call this way).
-    auto issue = [&](int i, typename F::Raw& tl, int& lb, bool& con, bool real) -> uint32_t {
-      const int ii = real || i <= last ? i : last;
-      const uint32_t off = (uint32_t)__builtin_amdgcn_readlane((int)info_off, ii);
-      const uint32_t meta = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, ii);
-      if (real || i <= last) {
-        if constexpr (FMT == kCodes4) issue_codes4<DT, D>(kc, vc, a.scales4, (int64_t)off << 4, lo_off, tl);
-        else if constexpr (FMT == kCodes8)
-          issue_codes<DT, D>(kc + ((uint64_t)off << 4), vc + ((uint64_t)off << 4), lo_off, tl);
-        else issue_tile<DT, D>(kc, vc, off, lo_off, tl);
+    // Makes unit `to` the current one: the one before it is finished, its query is at hand.
+    auto enter = [&](int to) __attribute__((always_inline)) {
+      if (to == cur) return;
+      if (cur >= 0) wave_finish(cur, false);
+      cur = to;
+      if (q_lbl != cur) {
+        if (qn_lbl == cur) qr = qn;
+        else q_of(cur, qr);
+        query_ready<DT, D, FMT, QF>(a, qr);
+        q_lbl = cur;
       }
-      lb = (int)(meta >> 7);
-      // this lane's column half sees the tile (column mask bits 5, 6)
-      con = !PAIRS || ((meta >> (c >= a.n_rep ? 6 : 5)) & 1u);
-      const int valid = (int)(meta & 31u);
-      uint32_t m = 0;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) m |= (4 * r + g < valid) ? (1u << r) : 0u;
-      return m;
-    };
-    typename F::Raw ring[DEPTH];
-    uint32_t mk[DEPTH];
-    int lb[DEPTH];
-    bool con[DEPTH];
-    // Computes ring slot r, which holds tile i, switching units (and queries) at a
-    // label change.
-    auto step = [&](int r, int i) {
-      if (lb[r] != cur) {
-        if (cur >= 0) wave_finish(cur, false);
-        cur = lb[r];
-        if (q_lbl != cur) {
-          if (qn_lbl == cur) qr = qn;
-          else q_of(cur, qr);
-          qr.split();
-          q_lbl = cur;
-        }
-        if (cur + 1 <= ll && qn_lbl != cur + 1) {
-          q_of(cur + 1, qn);
-          qn_lbl = cur + 1;
-        }
-      }
-      if constexpr (FMT == kCodes4) {
-        compute_codes4<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, st, con[r]);
-      } else if constexpr (FMT == kCodes8) {
-        const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
-        const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
-        compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, ks, vs, kstage[w], lane, st, con[r]);
-      } else {
-        compute_tile<DT, D>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
+      if (cur + 1 <= ll && qn_lbl != cur + 1) {
+        q_of(cur + 1, qn);
+        qn_lbl = cur + 1;
       }
     };
-#pragma unroll
-    for (int r = 0; r < DEPTH; ++r) mk[r] = issue(r, ring[r], lb[r], con[r], false);
-    int i = 0;
-    // Steady state: every issue is a real tile and the body has no branch
-    // around it (the branch cost 0.9 us per call on 64 sequences, even with
-    // one tile in flight); then the last DEPTH..2 DEPTH - 1 tiles.
-    for (; i + 2 * DEPTH <= cnt; i += DEPTH) {
-#pragma unroll
-      for (int r = 0; r < DEPTH; ++r) {
-        step(r, i + r);
-        mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], true);
+    if constexpr (FMT == kCodes4) {
+      // Two tiles of a unit at a time (compute_pair4), the next pair's loads in flight. (Two or
+      // three pairs ahead: 64 sequences of 512..4096 keys no faster, three of 40,000..90,000
+      // slower by 4%.)
+      Pair4<D> x;
+      int64_t at_a, at_b;
+      uint32_t ma, mb;
+      int next = 0;  // first tile that no pair has yet
+      auto spot = [&] {  // (the last tile of an odd unit is loaded twice, the second time without keys)
+        const int j = min(next + 1, last);
+        const uint32_t oa = (uint32_t)__builtin_amdgcn_readlane((int)info_off, next);
+        const uint32_t ob = (uint32_t)__builtin_amdgcn_readlane((int)info_off, j);
+        ma = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, next);
+        mb = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, j);
+        const bool two = next < last && ma >> 7 == mb >> 7;
+        at_a = (int64_t)oa << 4;
+        at_b = (int64_t)(two ? ob : oa) << 4;
+        mb = two ? mb : ma & ~31u;
+        next += two ? 2 : 1;
+      };
+      auto issue_k = [&] {
+        issue_k4<DT, D>(kc, a.scales4, at_a, lo_off, x.a);
+        issue_k4<DT, D>(kc, a.scales4, at_b, lo_off, x.b);
+      };
+      auto issue_v = [&] {
+        issue_v4<DT, D>(vc, a.scales4, at_a, lo_off, x.a);
+        issue_v4<DT, D>(vc, a.scales4, at_b, lo_off, x.b);
+      };
+      auto step = [&](auto more) __attribute__((always_inline)) {
+        const uint32_t na = ma, nb = mb;
+        enter((int)(na >> 7));
+        if constexpr (decltype(more)::value) spot();
+        auto next_k = [&] {
+          if constexpr (decltype(more)::value) issue_k();
+        };
+        auto next_v = [&] {
+          if constexpr (decltype(more)::value) issue_v();
+        };
+        constexpr uint32_t kAll = 3u << 5 | 16u;  // every key, every column
+        const bool whole = (na & 127u) == kAll && (nb & 127u) == kAll;
+        const int half = PAIRS && c >= a.n_rep ? 6 : 5;
+        compute_pair4<DT, D, QF>(x, qr, whole, na & 31u, nb & 31u, (na >> half) & 1u, (nb >> half) & 1u, a.scale_log2,
+                                 lane, st, next_k, next_v);
+      };
+      spot();
+      issue_k();
+      issue_v();
+      // (no branch around the loop's loads, and nothing is issued past the end)
+      while (next <= last) step(std::true_type{});
+      step(std::false_type{});
+    } else {
+      f32x2 sc = {0.f, 0.f};
+      if constexpr (FMT == kCodes8) {
+        if (lane < cnt) sc = a.scales[info_off / a.block16];
       }
-    }
-    for (; i < cnt; i += DEPTH) {
-#pragma unroll
-      for (int r = 0; r < DEPTH; ++r) {
-        if (i + r < cnt) step(r, i + r);
-        mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], false);
+      // Issues the loads of tile i of the run (`real`: i is known to be a tile of
+      // the run). Past the run's end (the ring's last DEPTH issues, never
+      // computed) it issues nothing: the end phase reuses the ring's registers,
+      // and a load still in flight into them would hold it up (padding loads
+      // cost 0.7 us per call this way).
+      auto issue = [&](int i, typename F::Raw& tl, int& lb, bool& con, bool real) -> uint32_t {
+        const int ii = real || i <= last ? i : last;
+        const uint32_t off = (uint32_t)__builtin_amdgcn_readlane((int)info_off, ii);
+        const uint32_t meta = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, ii);
+        if (real || i <= last) {
+          if constexpr (FMT == kCodes8)
+            issue_codes<DT, D>(kc + ((uint64_t)off << 4), vc + ((uint64_t)off << 4), lo_off, tl);
+          else if constexpr (FMT == kElements)
+            issue_tile<DT, D>(kc, vc, off, lo_off, tl);
+        }
+        lb = (int)(meta >> 7);
+        // this lane's column half sees the tile (column mask bits 5, 6)
+        con = !PAIRS || ((meta >> (c >= a.n_rep ? 6 : 5)) & 1u);
+        const int valid = (int)(meta & 31u);
+        uint32_t m = 0;
+  #pragma unroll
+        for (int r = 0; r < 4; ++r) m |= (4 * r + g < valid) ? (1u << r) : 0u;
+        return m;
+      };
+      typename F::Raw ring[DEPTH];
+      uint32_t mk[DEPTH];
+      int lb[DEPTH];
+      bool con[DEPTH];
+      // Computes ring slot r, which holds tile i, switching units (and queries) at a
+      // label change.
+      auto step = [&](int r, int i) {
+        enter(lb[r]);
+        if constexpr (FMT == kCodes8) {
+          const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
+          const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
+          compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, ks, vs, kstage[w], lane, st, con[r]);
+        } else {
+          compute_tile<DT, D>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
+        }
+      };
+  #pragma unroll
+      for (int r = 0; r < DEPTH; ++r) mk[r] = issue(r, ring[r], lb[r], con[r], false);
+      int i = 0;
+      // Steady state: every issue is a real tile and the body has no branch
+      // around it (the branch cost 0.9 us per call on 64 sequences, even with
+      // one tile in flight); then the last DEPTH..2 DEPTH - 1 tiles.
+      for (; i + 2 * DEPTH <= cnt; i += DEPTH) {
+  #pragma unroll
+        for (int r = 0; r < DEPTH; ++r) {
+          step(r, i + r);
+          mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], true);
+        }
+      }
+      for (; i < cnt; i += DEPTH) {
+  #pragma unroll
+        for (int r = 0; r < DEPTH; ++r) {
+          if (i + r < cnt) step(r, i + r);
+          mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], false);
+        }
       }
     }
   }
@@ -771,40 +841,104 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   __syncthreads();
 
   // ---- 3. owners of units that run on into later quarters fold their slots in
-  if (keep >= 0) {
-    const Lbl x = label(keep);
+  const __amdgpu_buffer_rsrc_t r_o = dev_rsrc(a.ws_o), r_ml = dev_rsrc(a.ws_ml);
+  int U0 = -1, U1 = -1;
+  if constexpr (JOIN) {
+    // The whole workgroup joins a unit's slots, a thread four columns of a row, and writes what
+    // comes of it (1.9 us a call where the owner's wavefront read its seven slots of 8 KB alone);
+    // several units are dealt to groups of wavefronts.
+    const int own = lane < 2 * NW ? s_own[lane] : -1, member = lane < NW ? s_fl[lane] : -1;
+    uint32_t owners = (uint32_t)__ballot(own >= 0);
+    const int units = __builtin_popcount(owners);
+    const int groups = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : NW;
+    for (int k = 0; owners; ++k, owners &= owners - 1) {
+      const int o = __builtin_ctz(owners);
+      const int u = __builtin_amdgcn_readlane(own, o);
+      const Lbl x = label(u);
+      const bool whole = x.us >= lo && x.ue <= hi;
+      if (!whole) (u == u_first ? U0 : U1) = u;
+      if ((k ^ w) & (groups - 1)) continue;
+      const uint32_t members = (uint32_t)__ballot(member == u);
+      const int nh = n_cols(x);
+      for (int it = (w / groups) * 64 + lane; it < nh * (D / 4); it += NT / groups) {
+        const int hc = it / (D / 4);
+        const int d0 = (it - hc * (D / 4)) * 4;
+        float m[NW], ls[NW], M = sl.m[o][hc];
+        f32x4 v[NW];
 #pragma unroll
-    for (int w2 = 1; w2 < NW; ++w2) {
-      if (w2 <= w || s_fl[w2] != keep) continue;
-      f32x4 acc2[TILES];
-      slot_read<D>(sl.acc[w2][c], g, acc2);
-      fold_state(st, sl.m[w2][c], sl.l[w2][c], acc2);
+        for (int i = 0; i < NW; ++i) {  // (all requested at once; in a slot that is no member's place the owner's)
+          const int at = (members >> i) & 1u ? i : o;
+          m[i] = sl.m[at][hc];
+          ls[i] = sl.l[at][hc];
+          v[i] = *(const f32x4*)&sl.acc[at][hc][d0];
+        }
+        const float m0 = M;
+        float l = sl.l[o][hc];
+        f32x4 acc = *(const f32x4*)&sl.acc[o][hc][d0];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) M = fmaxf(M, m[i]);
+        const float f0 = fast_exp2(m0 - M);
+        l *= f0;
+        acc *= f0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          const float f = fast_exp2(m[i] - M);
+          const f32x4 with = acc + f * v[i];
+          const bool in = (members >> i) & 1u;
+          l = in ? l + f * ls[i] : l;
+          acc = in ? with : acc;
+        }
+        if (whole) {
+          int sq, h;
+          out_of(x, hc, sq, h);
+          const float o4[4] = {acc[0], acc[1], acc[2], acc[3]};
+          store4<DT>((uint8_t*)a.out + ((int64_t)sq * a.o_seq + (int64_t)h * a.o_head + d0) * EB, o4,
+                     l > 0.f ? 1.f / l : 0.f);
+        } else {
+          const int rr = (grp + u) * 16 + hc;  // < 2^22 rows (plannable), so byte offsets fit int
+          store_dev4(r_o, (rr * D + d0) * 4, acc);
+          if (d0 == 0) store_dev2(r_ml, rr * 8, f32x2{M, l});
+        }
+      }
     }
-    if (x.us >= lo && x.ue <= hi) pend = keep;
-    else stage_partial(keep, keep == u_first ? 0 : 1);
+  } else {
+    if (keep >= 0) {
+      const Lbl x = label(keep);
+#pragma unroll
+      for (int w2 = 1; w2 < NW; ++w2) {
+        if (w2 <= w || s_fl[w2] != keep) continue;
+        f32x4 acc2[TILES];
+        slot_read<D>(sl.acc[w2][c], g, acc2);
+        fold_state(st, sl.m[w2][c], sl.l[w2][c], acc2);
+      }
+      if (x.us >= lo && x.ue <= hi) pend = keep;
+      else stage_partial(keep, keep == u_first ? 0 : 1);
+    }
+    __syncthreads();
+    U0 = s_stg[0];
+    U1 = s_stg[1];
   }
-  __syncthreads();
 
   // ---- 4. cross-workgroup partials (16-byte device-scope stores), arrivals and
   // the last arrival's merge
-  const int U0 = s_stg[0], U1 = s_stg[1];
   if (U0 < 0 && U1 < 0) {
     if (pend >= 0) write_out(label(pend));
     return;
   }
-  const __amdgpu_buffer_rsrc_t r_o = dev_rsrc(a.ws_o), r_ml = dev_rsrc(a.ws_ml);
+  if constexpr (!JOIN) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int u = k == 0 ? U0 : U1;
-    if (u < 0) continue;
-    const Lbl x = label(u);
-    const int nh = n_cols(x);
-    for (int it = tid; it < nh * (D / 4); it += NT) {
-      const int hc = it / (D / 4);
-      const int d0 = (it - hc * (D / 4)) * 4;
-      const int rr = (grp + u) * 16 + hc;  // < 2^22 rows (plannable), so byte offsets fit int
-      store_dev4(r_o, (rr * D + d0) * 4, *(const f32x4*)&stg.acc[k][hc][d0]);
-      if (d0 == 0) store_dev2(r_ml, rr * 8, f32x2{stg.m[k][hc], stg.l[k][hc]});
+    for (int k = 0; k < 2; ++k) {
+      const int u = k == 0 ? U0 : U1;
+      if (u < 0) continue;
+      const Lbl x = label(u);
+      const int nh = n_cols(x);
+      for (int it = tid; it < nh * (D / 4); it += NT) {
+        const int hc = it / (D / 4);
+        const int d0 = (it - hc * (D / 4)) * 4;
+        const int rr = (grp + u) * 16 + hc;  // < 2^22 rows (plannable), so byte offsets fit int
+        store_dev4(r_o, (rr * D + d0) * 4, *(const f32x4*)&stg.acc[k][hc][d0]);
+        if (d0 == 0) store_dev2(r_ml, rr * 8, f32x2{stg.m[k][hc], stg.l[k][hc]});
+      }
     }
   }
   if constexpr (FMT != kElements) {
@@ -965,7 +1099,7 @@ void launch_planned_codes(const DecodeArgs& a, const uint8_t* plan, const PlanLa
                           hipStream_t s) {
   const uint32_t o_sp = (uint32_t)ly.seq_pre, o_pr = (uint32_t)ly.pair, o_wh = (uint32_t)ly.whdr,
                  o_fi = (uint32_t)ly.first;
-  constexpr int NW = plan_waves(FMT), DEPTH = FMT == kCodes4 ? 2 : 1;
+  constexpr int NW = plan_waves(FMT), DEPTH = 1;
   if (pairs)
     hipLaunchKernelGGL((paged_decode_planned_kernel<DT, D, NW, DEPTH, true, FMT, QF>), dim3(grid), dim3(NW * 64), 0, s,
                        plan, o_sp, o_pr, o_wh, o_fi, a.num_seqs, a, ly);
