@@ -100,8 +100,13 @@ class RotaryAxes:
 
     def bind(self, name: str, positions: torch.Tensor, like: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """``positions`` as ``[axes, N]`` and the pairs on ``like``'s device, checked."""
+        held = self._pairs.get(like.device)
+        if held is None:
+            held = self.pairs(like.device)
+        if positions.dim() == 2 and positions.shape[0] == self.num_axes:
+            return positions, held
         if positions.dim() == 1:
             positions = positions[None]
         if positions.dim() != 2 or positions.shape[0] < self.num_axes:
             raise RuntimeError(f"{name}: positions {tuple(positions.shape)} for a rotary of {self.num_axes} axes")
-        return positions[: self.num_axes], self.pairs(like.device)
+        return positions[: self.num_axes], held
