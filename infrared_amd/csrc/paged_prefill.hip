@@ -391,6 +391,18 @@ void paged_prefill_kernel(PrefillArgs a) {
   typedef typename std::conditional<C4, u32x2, f32x2>::type PieceScale;  // of K and of V
   // whether its key may be used; kCodes4: how many of its 16 keys may
   typedef typename std::conditional<C4, int, bool>::type Use;
+  // kCodes4: the 8-byte piece of a tile's K, and of its V, that thread q % D of the tile takes (not
+  // the same: lane (gg, cc) of the tile's order, of its 16 bytes in D = 128 the half). The lanes
+  // that write LDS together have one key's K, and one key's V, side by side, so that their
+  // addresses meet in no bank (in the order of memory they are rows apart, four to a bank).
+  struct Place {
+    int gg, cc, half;
+  };
+  auto k_place = [](int q) { return D == 128 ? Place{(q >> 1) & 3, (q % D) >> 3, q & 1} : Place{q & 3, (q % D) >> 2, 0}; };
+  auto v_place = [](int q) {
+    return D == 128 ? Place{(q % D) >> 5, q & 15, (q >> 4) & 1} : Place{(q % D) >> 4, q & 15, 0};
+  };
+  auto piece_at = [](Place p) { return Tile4<D>::LB * (16 * p.gg + p.cc) + 8 * p.half; };
   Piece kreg[KPT], vreg[KPT];
   PieceScale screg[KPT];  // CODES: the pieces' scales
   // whether each load in flight reads a usable key: applied when the tile is
@@ -436,20 +448,21 @@ void paged_prefill_kernel(PrefillArgs a) {
       }
     }
     if constexpr (C4) {
-      // piece q: 8 bytes of the 16-token tile q / D, in the order of memory
+      typedef Tile4<D> T;
 #pragma unroll
       for (int i = 0; i < KPT; ++i) {
         const int q = tid + NT * i;
         if (PIECES % NT == 0 || q < PIECES) {
-          const int t0 = 16 * (q / D), p = q % D, row = 8 * p / Tile4<D>::LB, gg = row >> 4, cc = row & 15;
+          const int t0 = 16 * (q / D);
+          const Place pk = k_place(q), pv = v_place(q);
           bool use;
           const int64_t at = slot_of(k0 + t0, use, block);
           const uint8_t* ts = scales4 + at / 8;
-          kr[i] = *(const u32x2*)(kc + at + 8 * p);
-          vr[i] = *(const u32x2*)(vc + at + 8 * p);
-          sc[i][0] = ts[16 * (D == 128 ? gg : gg >> 1) + cc];
-          const uint8_t* vs = ts + D / 2 + 4 * (Tile4<D>::NG * gg + cc / (16 / Tile4<D>::NG));
-          if constexpr (D == 128) sc[i][1] = *(const uint16_t*)(vs + 2 * (p & 1));
+          kr[i] = *(const u32x2*)(kc + at + piece_at(pk));
+          vr[i] = *(const u32x2*)(vc + at + piece_at(pv));
+          sc[i][0] = ts[16 * (D == 128 ? pk.gg : pk.gg >> 1) + pk.cc];
+          const uint8_t* vs = ts + D / 2 + 4 * (T::NG * pv.gg + pv.cc / (16 / T::NG));
+          if constexpr (D == 128) sc[i][1] = *(const uint16_t*)(vs + 2 * pv.half);
           else sc[i][1] = *(const uint32_t*)vs;
           ku[i] = use ? min(16, kmax - (k0 + t0)) : 0;
         }
@@ -483,31 +496,40 @@ void paged_prefill_kernel(PrefillArgs a) {
       for (int i = 0; i < KPT; ++i) {
         const int q = tid + NT * i;
         if (q < PIECES) {
-          const int t0 = 16 * (q / D), p = q % D, row = 8 * p / Tile4<D>::LB, gg = row >> 4, cc = row & 15;
-          const int half = D == 128 ? p & 1 : 0, t = staged_token(cc);
-          const bool keep = t < ku[i];
-          uint16_t* kp = &ks_lds[buf][(t0 + t) * S::KROW + D / 4 * gg + 16 * half];
-          const float ks = scale_of_byte(sc[i][0]);
+          const int t0 = 16 * (q / D);
+          const Place pk = k_place(q), pv = v_place(q);
+          const int tk = staged_token(pk.cc), tv = 4 * VT * pv.half + pv.gg;  // V's keys: tv, tv + 4, ..
+          // (the scales of keys that may not be used become 0, whatever their codes)
+          const float ks = scale_of_byte(tk < ku[i] ? sc[i][0] : 0u);
+          uint32_t w = sc[i][1];
+#pragma unroll
+          for (int r = 0; r < VT; ++r) w &= tv + 4 * r < ku[i] ? ~0u : ~(0xffu << (8 * r));
+          uint16_t* kp = &ks_lds[buf][(t0 + tk) * S::KROW + D / 4 * pk.gg + 16 * pk.half];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t x[4];
             decode8_e2m1<DT>(kr[i][h], ks, x);
-            *(u32x4*)(kp + 8 * h) = zero_unless(u32x4{x[0], x[1], x[2], x[3]}, keep);
+            *(u32x4*)(kp + 8 * h) = u32x4{x[0], x[1], x[2], x[3]};
           }
-#pragma unroll
-          for (int r = 0; r < VT; ++r) {
-            const int tv = 4 * (VT * half + r) + gg;
-            const float vs = scale_of_byte((sc[i][1] >> (8 * r)) & 0xffu);
-            uint16_t* vp = &vs_lds[buf][(t0 + tv) * S::KROW + D / 16 * cc];
+          uint16_t* vp = &vs_lds[buf][(t0 + tv) * S::KROW + D / 16 * pv.cc];
+          auto v_row = [&](auto row) {
+            constexpr int R = decltype(row)::value;
+            const float vs = scale_of_byte<R>(w);
             if constexpr (D == 128) {
               uint32_t x[4];
-              decode8_e2m1<DT>(vr[i][r], vs, x);
-              *(u32x4*)vp = zero_unless(u32x4{x[0], x[1], x[2], x[3]}, tv < ku[i]);
+              decode8_e2m1<DT>(vr[i][R], vs, x);
+              *(u32x4*)(vp + 4 * R * S::KROW) = u32x4{x[0], x[1], x[2], x[3]};
             } else {
-              const uint32_t w = vr[i][r >> 1] >> (16 * (r & 1));
-              const bool kv = tv < ku[i];
-              *(u32x2*)vp = u32x2{kv ? decode2_e2m1<DT, 0>(w, vs) : 0u, kv ? decode2_e2m1<DT, 1>(w, vs) : 0u};
+              const uint32_t y = vr[i][R >> 1];
+              *(u32x2*)(vp + 4 * R * S::KROW) =
+                  u32x2{decode2_e2m1<DT, 2 * (R & 1)>(y, vs), decode2_e2m1<DT, 2 * (R & 1) + 1>(y, vs)};
             }
+          };
+          v_row(std::integral_constant<int, 0>{});
+          v_row(std::integral_constant<int, 1>{});
+          if constexpr (VT == 4) {
+            v_row(std::integral_constant<int, 2>{});
+            v_row(std::integral_constant<int, 3>{});
           }
         }
       }
