@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void kv_read_q4_kernel(ReadArgs a) {
   typedef Chunk8<DT> C;
   typedef Tile4<D> T;
   constexpr int PIECES = D / 8;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t idx = (int64_t)near_block(blockIdx.x) * 256 + threadIdx.x;
   const int64_t rh = idx / PIECES;
   const int piece = (int)(idx - rh * PIECES);
   const int64_t row = rh / a.num_kv_heads;
@@ -124,7 +124,7 @@ int dispatch_write(const char* name, const TurnArgs& a, int mode, int head_dim, 
 
 int launch_read(const char* name, const ReadArgs& a, int head_dim, int dtype, hipStream_t s) {
   const int64_t lanes = a.n * a.num_kv_heads * (head_dim / 8);
-  const int64_t grid = (lanes + 255) / 256;
+  const int64_t grid = near_blocks((lanes + 255) / 256);
   IR_REQUIRE(grid <= 0x7fffffff, "%s: too many rows", name);
   const dim3 g((unsigned)grid), b(256);
 #define IR_READ(DT)                                                          \
