@@ -382,7 +382,7 @@ Tensor rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, const 
 void kv_scatter_codes(const char* name, bool four, const Tensor& kc, const Tensor& vc, const Tensor& scales,
                       const Tensor& k, const Tensor& v, const Tensor& slots, int64_t block_size, const OptTensor& err,
                       int64_t stream) {
-  check_block_size((std::string(name) + ": ").c_str(), block_size);
+  check_block_size(four ? "kv_scatter_q4: " : "kv_scatter_q8: ", block_size);
   code_layer(name, kc, vc, scales, block_size, four);
   require_device({&kc, &k, &v, &slots});
   require(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == kc.size(1) && k.size(2) == head_width(kc, four), name,
@@ -429,16 +429,10 @@ void pool_write_q8(const Tensor& k_pool, const Tensor& v_pool, const Tensor& sca
                 stream);
 }
 
-void pool_write_q4(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales, int64_t layer, const Tensor& k,
-                   const Tensor& v, const Tensor& slots, int64_t block_size, const OptTensor& err, int64_t stream) {
-  kv_scatter_q4(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), k, v, slots, block_size, err,
-                stream);
-}
-
 std::tuple<Tensor, Tensor> gather_slots_codes(const char* name, bool four, const Tensor& kc, const Tensor& vc,
                                               const Tensor& scales, const Tensor& slots, int64_t block_size,
                                               at::ScalarType dtype, const OptTensor& err, int64_t stream) {
-  check_block_size((std::string(name) + ": ").c_str(), block_size);
+  check_block_size(four ? "gather_slots_q4: " : "gather_slots_q8: ", block_size);
   code_layer(name, kc, vc, scales, block_size, four);
   require_device({&kc, &slots});
   require(slots.scalar_type() == at::kLong, name, ": slots must be int64");
@@ -477,13 +471,6 @@ std::tuple<Tensor, Tensor> pool_gather_q8(const Tensor& k_pool, const Tensor& v_
                                           int64_t layer, const Tensor& slots, int64_t block_size, at::ScalarType dtype,
                                           const OptTensor& err, int64_t stream) {
   return gather_slots_q8(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), slots, block_size,
-                         dtype, err, stream);
-}
-
-std::tuple<Tensor, Tensor> pool_gather_q4(const Tensor& k_pool, const Tensor& v_pool, const Tensor& scales,
-                                          int64_t layer, const Tensor& slots, int64_t block_size, at::ScalarType dtype,
-                                          const OptTensor& err, int64_t stream) {
-  return gather_slots_q4(layer_of(k_pool, layer), layer_of(v_pool, layer), layer_of(scales, layer), slots, block_size,
                          dtype, err, stream);
 }
 
@@ -797,8 +784,6 @@ PYBIND11_MODULE(_seam, m) {
   m.def("norm_rope_kv_scatter", &norm_rope_kv_scatter, nogil());
   m.def("kv_scatter_q4", &kv_scatter_q4, nogil());
   m.def("gather_slots_q4", &gather_slots_q4, nogil());
-  m.def("pool_write_q4", &pool_write_q4, nogil());
-  m.def("pool_gather_q4", &pool_gather_q4, nogil());
   m.def("rope_axes", &rope_axes, nogil());
   m.def("rope_axes_kv_scatter", &rope_axes_kv_scatter, nogil());
   m.def("paged_decode_q8", &paged_decode_q8, nogil());

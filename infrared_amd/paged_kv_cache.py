@@ -476,15 +476,16 @@ class Quant4PagedKVPool(QuantPagedKVPool):
         (``[N]`` int64; negative: skipped)."""
         if k.dtype != self.dtype:
             raise RuntimeError(f"Quant4PagedKVPool.write: k is {k.dtype}, the pool's dtype is {self.dtype}")
-        seam().pool_write_q4(self.k, self.v, self.kv_scales, layer_idx, k, v, slots, self.block_size, self.err_flags,
-                             stream_of(self.k))
+        k_layer, v_layer, scales = self.layer(layer_idx)
+        seam().kv_scatter_q4(k_layer, v_layer, scales, k, v, slots, self.block_size, self.err_flags, stream_of(k_layer))
         if self.strict:
             self.check_errors()
 
     def gather(self, layer_idx: int, gather_slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """``PagedKVPool.gather`` of the values the codes stand for, in ``dtype``."""
-        out = seam().pool_gather_q4(self.k, self.v, self.kv_scales, layer_idx, gather_slots, self.block_size,
-                                    self.dtype, self.err_flags, stream_of(self.k))
+        k_layer, v_layer, scales = self.layer(layer_idx)
+        out = seam().gather_slots_q4(k_layer, v_layer, scales, gather_slots, self.block_size, self.dtype,
+                                     self.err_flags, stream_of(k_layer))
         if self.strict:
             self.check_errors()
         return out
@@ -497,10 +498,8 @@ class Quant4PagedKVPool(QuantPagedKVPool):
         max_ctx: int,
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """``PagedKVPool.gather_blocks`` of the values the codes stand for, in ``dtype``."""
-        out = kernels.paged_gather_q4(
-            self.k[layer_idx], self.v[layer_idx], self.kv_scales[layer_idx], block_tables, context_lens,
-            self.block_size, max_ctx, self.dtype, self.err_flags,
-        )
+        out = kernels.paged_gather_q4(*self.layer(layer_idx), block_tables, context_lens, self.block_size, max_ctx,
+                                      self.dtype, self.err_flags)
         if self.strict:
             self.check_errors()
         return out
