@@ -3,7 +3,9 @@
 // and the wrappers' shape checks, stride reads and 25-argument foreign calls cost
 // more than that on the host in Python (33 us a layer).
 //
-// `stream` is the raw handle of torch's current stream on the tensors' device.
+// `stream` is the raw handle of torch's current stream on the tensors' device, which calls
+// that a pool of codes or a rotation by axes can reach make the current one (the handle may be
+// the null stream's, which is the current device's).
 // Errors are RuntimeError with the same messages wherever the call came from.
 #include <torch/extension.h>
 
@@ -160,6 +162,7 @@ Tensor decode_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const Op
                    const Tensor& ctx, int64_t block_size, double scale, const OptTensor& out_, int64_t partition,
                    const OptTensor& workspace, const OptTensor& err, const OptTensor& counters, int64_t stream) {
   require_device({&q, &kc, &vc, &bt, &ctx});
+  const c10::DeviceGuard on(q.device());
   cache_layer("paged_decode", kc);
   check_tables("paged_decode", bt, ctx);
   require(q.dim() == 3, "paged_decode: q must be [B, H_q, D], got ", q.sizes());
@@ -235,6 +238,7 @@ Tensor planned_call(const Tensor& q, const Tensor& kc, const Tensor& vc, const O
                     const OptTensor& out_, const OptTensor& workspace, const OptTensor& err, const OptTensor& counters,
                     int64_t stream) {
   require_device({&q, &kc, &vc, &plan_buf});
+  const c10::DeviceGuard on(q.device());
   cache_layer("paged_decode_planned", kc);
   require(q.dim() == 3, "paged_decode_planned: q must be [B, H_q, D], got ", q.sizes());
   const auto& [seqs, p_hq, p_hkv, max_blocks, bs, num_blocks, slot_stride, head_stride] = p;
@@ -385,6 +389,7 @@ void kv_scatter_codes(const char* name, bool four, const Tensor& kc, const Tenso
   check_block_size(four ? "kv_scatter_q4: " : "kv_scatter_q8: ", block_size);
   code_layer(name, kc, vc, scales, block_size, four);
   require_device({&kc, &k, &v, &slots});
+  const c10::DeviceGuard on(kc.device());
   require(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == kc.size(1) && k.size(2) == head_width(kc, four), name,
           ": k ", k.sizes(), " / v ", v.sizes(), " do not match pool rows [", kc.size(1), ", ", head_width(kc, four),
           "]");
@@ -435,6 +440,7 @@ std::tuple<Tensor, Tensor> gather_slots_codes(const char* name, bool four, const
   check_block_size(four ? "gather_slots_q4: " : "gather_slots_q8: ", block_size);
   code_layer(name, kc, vc, scales, block_size, four);
   require_device({&kc, &slots});
+  const c10::DeviceGuard on(kc.device());
   require(slots.scalar_type() == at::kLong, name, ": slots must be int64");
   const Tensor flat = slots.contiguous();
   const int64_t h = kc.size(1), d = head_width(kc, four);
@@ -483,6 +489,7 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
   const bool four = scales && four_bits(*scales);
   const char* name = four ? "rope_kv_scatter_q4" : scales ? "rope_kv_scatter_q8" : "qk_norm_rope_kv_scatter";
   require_device({&q, &k, &v, &cos, &sin, &kc, &vc, &slots});
+  const c10::DeviceGuard on(q.device());
   cache_layer(name, kc);
   if (scales) {
     check_block_size(four ? "rope_kv_scatter_q4: " : "rope_kv_scatter_q8: ", block_size);
@@ -584,6 +591,7 @@ std::tuple<Tensor, Tensor> rope_axes(const Tensor& q, const Tensor& k, const Ten
                                      const OptTensor& q_out_, const OptTensor& k_out_, int64_t stream) {
   const char* name = "rope_axes";
   const Tensor pos = check_axes(name, q, k, wq, wk, positions, pairs);
+  const c10::DeviceGuard on(q.device());
   if (q_out_) given_out(name, *q_out_, q, Wide::kOut);
   if (k_out_) {
     given_out(name, *k_out_, k, Wide::kOut);
@@ -608,6 +616,7 @@ Tensor rope_axes_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
   const char* name = "rope_axes_kv_scatter";
   const Tensor pos = check_axes(name, q, k, wq, wk, positions, pairs);
   require_device({&q, &v, &kc, &vc, &slots});
+  const c10::DeviceGuard on(q.device());
   cache_layer(name, kc);
   const bool four = scales.has_value();
   if (four) {
@@ -703,6 +712,7 @@ Tensor paged_prefill_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, con
                         const Tensor& cu, const Tensor& q_start, int64_t max_q_len, int64_t block_size, double scale,
                         const OptTensor& out_, const OptTensor& err, const OptTensor& plan_buf, int64_t stream) {
   require_device({&q, &kc, &vc, &bt, &cu, &q_start});
+  const c10::DeviceGuard on(q.device());
   require(q.dim() == 3, "paged_prefill: q must be [total_q, H_q, D], got ", q.sizes());
   check_block_size("paged_prefill: ", block_size);
   const bool four = four_bits(scales);

@@ -8,6 +8,7 @@
 // the unit to finish -- found with an arrival counter -- merges with
 // log-sum-exp weights before it resets the counter (or, with
 // IR_DECODE_MERGE=kernel, a second launch merges them).
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -497,9 +498,10 @@ extern "C" int ir_paged_decode_q4(const void* q, int64_t q_seq_stride, int64_t q
                                   int32_t* err_flags, ir_stream_t stream) {
   if (num_seqs == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_decode_q4: null pointer");
+  IR_REQUIRE(isfinite(scale), "ir_paged_decode_q4: scale must be finite");
   return decode_call("ir_paged_decode_q4", kCodes4, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
-                     head_dim / 2, num_blocks * block_size * (head_dim / 2), num_blocks, block_size, block_tables, bt_stride,
-                     max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
+                     head_dim / 2, num_blocks * block_size * (head_dim / 2), num_blocks, block_size, block_tables,
+                     bt_stride, max_blocks_per_seq, context_lens, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads,
                      num_kv_heads, head_dim, scale, dtype, partition_tokens, counters, num_counters, workspace,
                      workspace_bytes, err_flags, stream);
 }

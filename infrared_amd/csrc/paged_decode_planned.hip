@@ -34,6 +34,7 @@
 // and the last of the unit's slices merges the rows with log-sum-exp weights
 // and resets the counter, so a call is one launch and the counters are zero
 // again after it.
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -1364,8 +1365,9 @@ extern "C" int ir_paged_decode_planned_q4(const void* q, int64_t q_seq_stride, i
                                           const void* plan, int32_t* counters, int64_t num_counters, void* workspace,
                                           int64_t workspace_bytes, int32_t* err_flags, ir_stream_t stream) {
   IR_REQUIRE(scales, "ir_paged_decode_planned_q4: null pointer");
-  return planned_call("ir_paged_decode_planned_q4", kCodes4, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache, v_cache,
-                      head_dim / 2, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
+  IR_REQUIRE(isfinite(scale), "ir_paged_decode_planned_q4: scale must be finite");
+  return planned_call("ir_paged_decode_planned_q4", kCodes4, scales, q_dtype, q, q_seq_stride, q_head_stride, k_cache,
+                      v_cache, head_dim / 2, out, out_seq_stride, out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim,
                       max_blocks_per_seq, block_size, scale, dtype, flags, plan, counters, num_counters, workspace,
                       workspace_bytes, err_flags, stream);
 }

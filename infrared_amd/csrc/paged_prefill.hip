@@ -61,6 +61,7 @@
 // gathered history (infrared/model/triton_attention.py:110-129), streaming as
 // in infrared/model/triton_attention.py:135-177; probabilities are rounded to
 // the input dtype before the PV product, as softmax(...).to(q.dtype) does.
+#include <float.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -2124,6 +2125,7 @@ extern "C" int ir_paged_prefill_q4(const void* q, int64_t q_tok_stride, int64_t 
                                    ir_stream_t stream) {
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return ok();
   IR_REQUIRE(scales, "ir_paged_prefill_q4: null pointer");
+  IR_REQUIRE(scale <= FLT_MAX, "ir_paged_prefill_q4: scale must be finite");
   return prefill_call("ir_paged_prefill_q4", kCodes4, scales, q_dtype, q, q_tok_stride, q_head_stride, k_cache, v_cache,
                       head_dim / 2, num_blocks * block_size * (head_dim / 2), num_blocks, block_size, block_tables, bt_stride,
                       max_blocks_per_seq, cu_seqlens_q, q_start, num_seqs, total_q, max_q_len, out, out_tok_stride,

@@ -19,6 +19,7 @@ from infrared_amd._lib import (
     check,
     dtype_code,
     lib,
+    on_device,
     ptr,
     require_device,
     seam,
@@ -232,11 +233,12 @@ def paged_gather_q4(
     b = block_tables.shape[0]
     slots, h, d = k_cache.shape[0], k_cache.shape[1], 2 * k_cache.shape[2]
     out = torch.empty(2, b, max_ctx, h, d, dtype=dtype, device=dev)
-    rc = lib().ir_paged_gather_q4(
-        ptr(k_cache), ptr(v_cache), ptr(kv_scales), slots // block_size, block_size, ptr(block_tables),
-        block_tables.stride(0), block_tables.shape[1], ptr(context_lens), b, max_ctx, h, d, dtype_code(dtype),
-        ptr(out[0]), ptr(out[1]), ptr(err_flags), stream_ptr(dev),
-    )
+    with on_device(dev):
+        rc = lib().ir_paged_gather_q4(
+            ptr(k_cache), ptr(v_cache), ptr(kv_scales), slots // block_size, block_size, ptr(block_tables),
+            block_tables.stride(0), block_tables.shape[1], ptr(context_lens), b, max_ctx, h, d, dtype_code(dtype),
+            ptr(out[0]), ptr(out[1]), ptr(err_flags), stream_ptr(dev),
+        )
     check(rc, "ir_paged_gather_q4")
     return out[0], out[1]
 
@@ -415,13 +417,14 @@ def decode_plan(
         buf = torch.empty(need, dtype=torch.uint8, device=dev)
     if buf.dtype != torch.uint8 or buf.data_ptr() % 256:
         raise RuntimeError("decode_plan: buf must be a 256-byte aligned uint8 tensor")
-    rc = lib().ir_paged_decode_plan(
-        ptr(block_tables), block_tables.stride(0), max_blocks, ptr(context_lens), b, num_q_heads, h_kv,
-        block_size, k_cache.shape[0] // block_size, k_cache.stride(0), k_cache.stride(1),
-        _CODE_DTYPES[k_cache.dtype] if k_cache.dtype in _CODE_DTYPES else dtype_code(k_cache.dtype),
-        PLAN_SHARE_GROUPS if share_groups else 0, ptr(buf), buf.numel(), ptr(err_flags),
-        stream_ptr(dev),
-    )
+    with on_device(dev):
+        rc = lib().ir_paged_decode_plan(
+            ptr(block_tables), block_tables.stride(0), max_blocks, ptr(context_lens), b, num_q_heads, h_kv,
+            block_size, k_cache.shape[0] // block_size, k_cache.stride(0), k_cache.stride(1),
+            _CODE_DTYPES[k_cache.dtype] if k_cache.dtype in _CODE_DTYPES else dtype_code(k_cache.dtype),
+            PLAN_SHARE_GROUPS if share_groups else 0, ptr(buf), buf.numel(), ptr(err_flags),
+            stream_ptr(dev),
+        )
     check(rc, "ir_paged_decode_plan")
     return DecodePlan(buf, b, num_q_heads, h_kv, max_blocks, block_size, k_cache.shape[0] // block_size,
                       k_cache.stride(0), k_cache.stride(1), k_cache.dtype, bool(share_groups))
@@ -735,12 +738,13 @@ def prefill_plan(
     if buf.dtype != torch.uint8 or buf.data_ptr() % 256:
         raise RuntimeError("prefill_plan: buf must be a 256-byte aligned uint8 tensor")
     max_blocks = block_tables.shape[1]
-    rc = lib().ir_paged_prefill_plan(
-        ptr(cu_seqlens_q), ptr(q_start), ptr(block_tables), max(block_tables.stride(0), max_blocks), b,
-        int(total_q), int(max_q_len), int(max_blocks), int(block_size), num_q_heads, num_kv_heads, head_dim,
-        (PLAN_SHARE_GROUPS if share_groups else 0) | (PLAN_F32 if f32 else 0), ptr(buf), buf.numel(),
-        stream_ptr(dev),
-    )
+    with on_device(dev):
+        rc = lib().ir_paged_prefill_plan(
+            ptr(cu_seqlens_q), ptr(q_start), ptr(block_tables), max(block_tables.stride(0), max_blocks), b,
+            int(total_q), int(max_q_len), int(max_blocks), int(block_size), num_q_heads, num_kv_heads, head_dim,
+            (PLAN_SHARE_GROUPS if share_groups else 0) | (PLAN_F32 if f32 else 0), ptr(buf), buf.numel(),
+            stream_ptr(dev),
+        )
     check(rc, "ir_paged_prefill_plan")
     return PrefillPlan(buf, b, int(max_q_len), num_q_heads, num_kv_heads, head_dim, f32)
 

@@ -371,6 +371,58 @@ def test_decode_of_many_sequences():
         check_decode(out, q, values, tables, lens, bs, dtype)
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("dtype, hq, h, d", [(torch.bfloat16, 28, 4, 128), (torch.float32, 10, 2, 64)])
+def test_decode_joins_units_of_several_wavefronts(dtype, hq, h, d, shared):
+    """Sequences of about a wavefront's, several wavefronts' and more than a workgroup's share of
+    the keys: one to eight units of a workgroup are joined, others cross to the next."""
+    bs = 16
+    for lens in ([320] * 60 + [17, 700, 2500, 1], [(i * 97) % 400 + 1 for i in range(150)], [1100, 1090, 3, 1300]):
+        pool, tables, values = filled(29, dtype, lens, h, d, bs)
+        if shared:
+            for i in range(0, len(lens) - 1, 3):  # every third sequence begins as the one before it
+                n = min(lens[i], lens[i + 1]) // bs
+                tables[i + 1][:n] = tables[i][:n]
+        q = torch.randn(len(lens), hq, d, generator=gen(30), device=DEV).to(dtype)
+        ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        bt = device_tables(tables)
+        out = run_decode(pool, q, bt, ctx, True)
+        pool.check_errors()
+        check_decode(out, q, values, tables, lens, bs, dtype)
+        assert torch.equal(out, run_decode(pool, q, bt, ctx, True))
+
+
+# (the bounds of check_decode; a negative scale's scores are those of the opposite queries)
+@pytest.mark.parametrize("planned", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1e-40, 0.7])
+def test_decode_at_any_scale(planned, dtype, scale):
+    bs, hq, h, d = 16, 14, 2, 64
+    lens = [1, 40, 333, 0]
+    pool, tables, values = filled(31, dtype, lens, h, d, bs)
+    ctx, bt = torch.tensor(lens, dtype=torch.int32, device=DEV), device_tables(tables)
+    for q_dtype in {dtype, torch.float32}:
+        q = torch.randn(len(lens), hq, d, generator=gen(32), device=DEV).to(q_dtype)
+        kw = {"out": torch.empty(len(lens), hq, d, dtype=dtype, device=DEV), "kv_scales": pool.kv_scales[0]}
+        if planned:
+            plan = kernels.decode_plan(bt, ctx, hq, pool.k[0], bs)
+            out = kernels.paged_decode_planned(q, pool.k[0], pool.v[0], plan, scale, **kw)
+        else:
+            out = kernels.paged_decode(q, pool.k[0], pool.v[0], bt, ctx, bs, scale, **kw)
+        for i, n in enumerate(lens):
+            if n == 0:
+                assert not out[i].any()
+                continue
+            sign = -1.0 if scale < 0 else 1.0
+            o, a, reach = quant.attend(sign * q[i : i + 1], values, tables[i], bs, n - 1, sign * scale)
+            tol = fp32_tolerance(o, a, reach, d) + small_probabilities(values, tables[i], n, bs, hq, dtype)
+            if dtype != torch.float32:
+                # (an fp32 query in two pieces of the dtype: 2^-18 of an element, as above)
+                tol = tol + decode_tolerance(o, a, dtype) + 4 * 2.0**-13 * reach[..., None] * a
+            err = (out[i : i + 1].double().cpu() - o).abs()
+            assert (err <= tol).all(), (q_dtype, i, n, (err / tol).max())
+
+
 @pytest.mark.parametrize("planned", [False, True])
 def test_decode_masks_bad_blocks_and_lengths(planned):
     bs, hq, h, d = 16, 8, 2, 64

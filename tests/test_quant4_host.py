@@ -208,6 +208,13 @@ def test_attention_refusals(fn, kw, text):
     assert text in _lib.lib().ir_last_error()
 
 
+@pytest.mark.parametrize("fn", ["decode", "planned", "prefill"])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf")])
+def test_attention_refuses_a_scale_that_is_no_number(fn, scale):
+    assert _attend(fn, scale=scale) < 0
+    assert b"scale" in _lib.lib().ir_last_error()
+
+
 def test_decode_plan_takes_the_4_bit_layers_strides():
     lib = _lib.lib()
     args = dict(bt=P, bts=4, mb=4, ctx=P, b=1, hq=4, h=2, bs=16, nb=4, cs=64, ch=64 * 64, dt=4, flags=0, plan=None,
