@@ -755,7 +755,9 @@ int ir_paged_gather_q4(const void* k_cache, const void* v_cache, const uint8_t* 
 
 /*
  * Attention over the 4-bit pool: the calls of the 8-bit pool, arguments alike (q_dtype
- * too; a decode plan is built with IR_DTYPE_E2M1 and the layer's strides).
+ * too; a decode plan is built with IR_DTYPE_E2M1 and the layer's strides), but partition_tokens 0
+ * is a partition of its own, no smaller than ir_paged_decode_default_partition's, so that a
+ * workspace sized for 0 is enough, and a scale that is NaN or infinite is refused.
  */
 int ir_paged_decode_q4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
                        const void* k_cache, const void* v_cache, const uint8_t* scales,

@@ -259,16 +259,38 @@ int launch_decode(const DecodeArgs& a, bool bs16, bool fused, hipStream_t s) {
 // heads of 128: 11.9 and 9.1). A workspace sized for the default partition is enough.
 constexpr int kCodePartition = 128;
 
-template <int DT, int D, int FMT, bool QF>
-int launch_decode_codes(const char* name, const DecodeArgs& a, bool fused, hipStream_t s) {
+// Of a 4-bit cache the keys `cap` that a table holds say the partition, no smaller than the default
+// (whose workspace it then fits): up to 512 keys (two pairs of tiles a wavefront) are not split, and of
+// more, a partition's walk and the merge of them all take the least together at some 4 sqrt(cap), in
+// whole runs of four pairs. (One sequence, 28 / 4 heads of 128, us a call in partitions of 128, 256, 512,
+// 1024: 512 keys 6.6, 6.9, 6.5 -; 1024 keys 7.5, 7.1, 8.2, 8.9; 4096: 11.7, 9.5, 9.2, 10.7; 16,000: 30.5,
+// 18.0, 13.5, 13.2.) Up to a unit a CU its workgroups have eight wavefronts (with four those
+// lengths take 6.8, 7.3, 9.4 and 14.0 at their best, 64 sequences of 3,000 keys 33.3 and not 24.8), beyond
+// that four, of which a CU holds more (200 sequences of 50 keys 7.4 and not 12.0, of 300 13.8 and not 19.0).
+
+int partition_codes4(int64_t cap) {
+  return cap <= 512 ? 512 : ((int)(4.25f * sqrtf((float)cap)) + 127) / 128 * 128;
+}
+
+template <int DT, int D, int FMT, bool QF, int NW>
+int launch_decode_codes_w(const char* name, const DecodeArgs& a, bool fused, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * a.n_hg), (unsigned)a.max_parts);
   if (fused || a.max_parts == 1) {
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, true, 2, FMT, QF>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, NW, true, 2, FMT, QF>), grid, dim3(NW * 64), 0, s, a);
   } else {
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, 4, false, 2, FMT, QF>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, true, NW, false, 2, FMT, QF>), grid, dim3(NW * 64), 0, s, a);
     hipLaunchKernelGGL((paged_decode_reduce<DT, D>), dim3(grid.x), dim3(256), 0, s, a);
   }
   return check_launch(name);
+}
+
+template <int DT, int D, int FMT, bool QF>
+int launch_decode_codes(const char* name, const DecodeArgs& a, bool fused, hipStream_t s) {
+  if constexpr (FMT == kCodes4) {
+    if ((int64_t)a.num_seqs * a.num_kv_heads * a.n_hg <= kUnitsForCUs)
+      return launch_decode_codes_w<DT, D, FMT, QF, 8>(name, a, fused, s);
+  }
+  return launch_decode_codes_w<DT, D, FMT, QF, 4>(name, a, fused, s);
 }
 
 template <int DT, int FMT, bool QF>
@@ -366,7 +388,11 @@ int decode_call(const char* name, int fmt, const void* scales, int q_dtype, cons
              "%s: strides must be multiples of 16 bytes", name);
   if (partition_tokens <= 0) {
     partition_tokens = ir_paged_decode_default_partition(num_seqs, num_kv_heads, max_blocks_per_seq, block_size);
-    if (scales) partition_tokens = std::max(partition_tokens, kCodePartition);
+    if (scales) {
+      const int64_t cap = (int64_t)max_blocks_per_seq * block_size;
+      partition_tokens = std::max(partition_tokens, fmt == kCodes4 ? partition_codes4(cap) : kCodePartition);
+      partition_tokens = std::min(partition_tokens, kMaxPartition);
+    }
   }
   IR_REQUIRE(partition_tokens % 16 == 0 && partition_tokens <= kMaxPartition,
              "%s: partition_tokens %d must be a multiple of 16 and at most %d", name, partition_tokens,

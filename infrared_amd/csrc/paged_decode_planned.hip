@@ -796,7 +796,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
         con = !PAIRS || ((meta >> (c >= a.n_rep ? 6 : 5)) & 1u);
         const int valid = (int)(meta & 31u);
         uint32_t m = 0;
-  #pragma unroll
+#pragma unroll
         for (int r = 0; r < 4; ++r) m |= (4 * r + g < valid) ? (1u << r) : 0u;
         return m;
       };
@@ -816,21 +816,21 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
           compute_tile<DT, D>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
         }
       };
-  #pragma unroll
+#pragma unroll
       for (int r = 0; r < DEPTH; ++r) mk[r] = issue(r, ring[r], lb[r], con[r], false);
       int i = 0;
       // Steady state: every issue is a real tile and the body has no branch
       // around it (the branch cost 0.9 us per call on 64 sequences, even with
       // one tile in flight); then the last DEPTH..2 DEPTH - 1 tiles.
       for (; i + 2 * DEPTH <= cnt; i += DEPTH) {
-  #pragma unroll
+#pragma unroll
         for (int r = 0; r < DEPTH; ++r) {
           step(r, i + r);
           mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], true);
         }
       }
       for (; i < cnt; i += DEPTH) {
-  #pragma unroll
+#pragma unroll
         for (int r = 0; r < DEPTH; ++r) {
           if (i + r < cnt) step(r, i + r);
           mk[r] = issue(i + r + DEPTH, ring[r], lb[r], con[r], false);
@@ -867,7 +867,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
         float m[NW], ls[NW], M = sl.m[o][hc];
         f32x4 v[NW];
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {  // (all requested at once; in a slot that is no member's place the owner's)
+        for (int i = 0; i < NW; ++i) {  // (all requested at once; where a slot is no member's, the owner's)
           const int at = (members >> i) & 1u ? i : o;
           m[i] = sl.m[at][hc];
           ls[i] = sl.l[at][hc];
