@@ -5,8 +5,8 @@
 // A wavefront takes one token and 64 / (head_dim / 16) of its rows (q, then k, then v) at
 // a time, its lanes holding their part of the token's angles in registers for all of
 // them. Bound by memory: every row is read once and written once (4,096 tokens of 28 + 2 x 4 rows
-// of 128 in bf16, normed and rotated into a 16-bit pool: 14.0 us, 5.4 TB/s; 64 tokens 3.3 us, the
-// launch and two trips).
+// of 128 in bf16, rotated by axes into a 16-bit pool: 14.0 us, 5.4 TB/s; 64 tokens, normed too, 3.3 us,
+// the launch and two trips).
 #pragma once
 
 #include "e2m1.hpp"
