@@ -151,6 +151,18 @@ __device__ __forceinline__ Pieces split2(float a, float b) {
   return {hi, Elem<DT>::pack2(a - Elem<DT>::lo(hi), b - Elem<DT>::hi(hi))};
 }
 
+// (a, b) as three pieces of bf16 that add up to them exactly: eight bits of the 24 each, by
+// truncation, so that the largest numbers do not become infinite.
+struct Pieces3 {
+  uint32_t hi, mid, lo;
+};
+__device__ __forceinline__ Pieces3 split3(float a, float b) {
+  auto top = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); };
+  auto pair = [](float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); };
+  const float ra = a - top(a), rb = b - top(b);
+  return {pair(a, b), pair(ra, rb), pair(ra - top(ra), rb - top(rb))};
+}
+
 // 16x16x16, 16-bit inputs: 4 elements (2 dwords) of A and B per lane.
 template <int DT>
 __device__ __forceinline__ f32x4 mfma_k16(u32x2 a, u32x2 b, f32x4 c);

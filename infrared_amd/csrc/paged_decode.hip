@@ -310,7 +310,7 @@ int dispatch_decode_codes(const char* name, int dtype, bool qf, int head_dim, co
       return qf ? launch_decode_codes_d<IR_DTYPE_F16, FMT, true>(name, head_dim, a, fused, s)
                 : launch_decode_codes_d<IR_DTYPE_F16, FMT, false>(name, head_dim, a, fused, s);
     default:
-      return launch_decode_codes_d<IR_DTYPE_F32, FMT, false>(name, head_dim, a, fused, s);
+      return launch_decode_codes_d<IR_DTYPE_F32, FMT, FMT == kCodes4>(name, head_dim, a, fused, s);
   }
 }
 

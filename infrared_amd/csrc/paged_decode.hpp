@@ -194,6 +194,34 @@ struct QueryRegs<DT, D, true> {
   __device__ __forceinline__ float scaled(float scale) const { return scale * unit; }
 };
 
+// A query of an fp32 pool of 4-bit codes (compute_pair4): as loaded in x and rest, after split() in three
+// pieces of bf16, exactly.
+template <int D>
+struct QueryRegs<IR_DTYPE_F32, D, true> {
+  static constexpr int N = D / 8;
+  uint32_t x[N], rest[N], low[N];
+  __device__ __forceinline__ void negate() {  // (before split())
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x[i] ^= 0x80000000u;
+      rest[i] ^= 0x80000000u;
+    }
+  }
+  __device__ __forceinline__ void split() {
+    float v[2 * N];
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) v[i] = __uint_as_float(i < N ? x[i] : rest[i - N]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const Pieces3 p = split3(v[2 * i], v[2 * i + 1]);
+      x[i] = p.hi;
+      rest[i] = p.mid;
+      low[i] = p.lo;
+    }
+  }
+  __device__ __forceinline__ float scaled(float scale) const { return scale; }
+};
+
 // Issues a code tile's loads; the tile's first row is at tk / tv.
 template <int DT, int D>
 __device__ __forceinline__ void issue_codes(const uint8_t* tk, const uint8_t* tv,
@@ -431,6 +459,9 @@ struct Pair4 {
 // - a product of 32 k-slots takes 8 keys of a lane, one permutation making each dword of its V
 //   operand, and the probabilities' two pieces are two products with the same V:
 // some 170 a pair, the same call 25.2 us.
+// In an fp32 pool (DT fp32, QF) the numbers of codes are bf16 ones all the same, exactly, and queries and
+// probabilities are three pieces of it, exactly: six products of 32 k-slots that sum in fp32 for 16 of four
+// fp32 ones, each of twice the time (the call in fp32 29.9 us, 57.9 with those).
 // The codes are dead once they are numbers, so the next pair's loads go into the same
 // registers: its K's as soon as the scores are there (next_k), its V's behind the products (next_v).
 //
@@ -440,8 +471,10 @@ template <int DT, int D, bool QF, typename NextK, typename NextV>
 __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D, QF>& q, bool whole, int valid_a,
                                               int valid_b, bool col_a, bool col_b, float scale_log2, int lane,
                                               State<D>& st, NextK next_k, NextV next_v) {
-  typedef TileShape<DT, D> Sh;
-  constexpr int W = Sh::k16 ? 4 : 8;  // dwords of eight elements
+  constexpr bool WIDE = DT == IR_DTYPE_F32;
+  static_assert(!WIDE || QF, "an fp32 pool's queries are fp32 ones in pieces");
+  constexpr int KT = WIDE ? IR_DTYPE_BF16 : DT;  // the operands'
+  typedef TileShape<KT, D> Sh;
   constexpr float UP = kProbUp<DT>;
   Code4Tile<D>&ta = x.a, &tb = x.b;
   const int g = lane >> 4;
@@ -460,13 +493,14 @@ __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D
     uint32_t kop[Sh::KDW];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      uint32_t x[W];
-      decode8_e2m1<DT>(t.k[j], scale_of_byte(t.ks), x);
+      uint32_t x[4];
+      decode8_e2m1<KT>(t.k[j], scale_of_byte(t.ks), x);
 #pragma unroll
-      for (int i = 0; i < W; ++i) kop[W * j + i] = x[i];
+      for (int i = 0; i < 4; ++i) kop[4 * j + i] = x[i];
     }
-    f32x4 s = qk_tile<DT, D>(kop, q.x);
-    if constexpr (QF) s += qk_tile<DT, D>(kop, q.rest);
+    f32x4 s = qk_tile<KT, D>(kop, q.x);
+    if constexpr (QF) s += qk_tile<KT, D>(kop, q.rest);
+    if constexpr (WIDE) s += qk_tile<KT, D>(kop, q.low);
     return s;
   };
   const f32x4 sa = scores(ta), sb = scores(tb);
@@ -499,25 +533,24 @@ __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D
 #pragma unroll
   for (int i = 0; i < 8; ++i) p[i] = fast_exp2(__builtin_fmaf(p[i], c, -st.m));
   st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-  // dword I of a row of V: elements 2 I, 2 I + 1 of the lane's key R of tile t (two dwords in fp32)
+  // dword I of a row of V: elements 2 I, 2 I + 1 of the lane's key R of tile t
   auto value = [&](const Code4Tile<D>& t, auto row, auto dw) {
     constexpr int R = decltype(row)::value, I = decltype(dw)::value;
     constexpr int B = D == 128 ? I : 2 * (R & 1) + I;  // byte of its dword of codes
-    const uint32_t w = t.v[D == 128 ? R : R >> 1];
-    const float vs = scale_of_byte<R>(t.vs);
-    if constexpr (Sh::k16) {
-      return decode2_e2m1<DT, B>(w, vs);
-    } else {
-      return decode2_e2m1_f32<B>(w, vs);
-    }
+    return decode2_e2m1<KT, B>(t.v[D == 128 ? R : R >> 1], scale_of_byte<R>(t.vs));
   };
-  u32x4 hi, lo;
-  if constexpr (Sh::k16) {
+  u32x4 piece[WIDE ? 3 : 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (WIDE) {
+      const Pieces3 w = split3(p[2 * i], p[2 * i + 1]);
+      piece[0][i] = w.hi;
+      piece[1][i] = w.mid;
+      piece[2][i] = w.lo;
+    } else {
       const Pieces w = split2<DT>(p[2 * i], p[2 * i + 1]);
-      hi[i] = w.hi;
-      lo[i] = w.lo;
+      piece[0][i] = w.hi;
+      piece[1][i] = w.lo;
     }
   }
   auto products = [&](auto dw) {
@@ -526,24 +559,15 @@ __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D
     typedef std::integral_constant<int, 1> R1;
     typedef std::integral_constant<int, 2> R2;
     typedef std::integral_constant<int, 3> R3;
-    const auto v0 = value(ta, R0{}, dw), v1 = value(ta, R1{}, dw), v2 = value(ta, R2{}, dw), v3 = value(ta, R3{}, dw);
-    const auto v4 = value(tb, R0{}, dw), v5 = value(tb, R1{}, dw), v6 = value(tb, R2{}, dw), v7 = value(tb, R3{}, dw);
-    if constexpr (Sh::k16) {
+    const uint32_t v0 = value(ta, R0{}, dw), v1 = value(ta, R1{}, dw), v2 = value(ta, R2{}, dw), v3 = value(ta, R3{}, dw);
+    const uint32_t v4 = value(tb, R0{}, dw), v5 = value(tb, R1{}, dw), v6 = value(tb, R2{}, dw), v7 = value(tb, R3{}, dw);
 #pragma unroll
-      for (int odd = 0; odd < 2; ++odd) {
-        const uint32_t sel = odd ? 0x07060302u : 0x05040100u;
-        const u32x4 x = {__builtin_amdgcn_perm(v1, v0, sel), __builtin_amdgcn_perm(v3, v2, sel),
-                         __builtin_amdgcn_perm(v5, v4, sel), __builtin_amdgcn_perm(v7, v6, sel)};
-        st.acc[2 * I + odd] = mfma_k32<DT>(x, hi, st.acc[2 * I + odd]);
-        st.acc[2 * I + odd] = mfma_k32<DT>(x, lo, st.acc[2 * I + odd]);
-      }
-    } else {
-      const f32x2 v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+    for (int odd = 0; odd < 2; ++odd) {
+      const uint32_t sel = odd ? 0x07060302u : 0x05040100u;
+      const u32x4 x = {__builtin_amdgcn_perm(v1, v0, sel), __builtin_amdgcn_perm(v3, v2, sel),
+                       __builtin_amdgcn_perm(v5, v4, sel), __builtin_amdgcn_perm(v7, v6, sel)};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        st.acc[2 * I] = mfma_f32_k4(v[i][0], p[i], st.acc[2 * I]);
-        st.acc[2 * I + 1] = mfma_f32_k4(v[i][1], p[i], st.acc[2 * I + 1]);
-      }
+      for (const u32x4& w : piece) st.acc[2 * I + odd] = mfma_k32<KT>(x, w, st.acc[2 * I + odd]);
     }
   };
   products(std::integral_constant<int, 0>{});
@@ -737,6 +761,7 @@ __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, i
   typedef TileShape<DT, D> Sh;
   constexpr int EB = QF ? 4 : Sh::EB;
   constexpr int DW = 4 * EB;  // dwords of 16 elements
+  constexpr int N = sizeof(q.x) / 4;
   constexpr int STEP = K4 ? 16 : 64;
   const uint8_t* row =
       (const uint8_t*)a.q + ((int64_t)seq * a.q_seq + (int64_t)qh * a.q_head + (K4 ? D / 4 : 16) * g) * EB;
@@ -749,7 +774,7 @@ __device__ __forceinline__ void load_query_codes(const DecodeArgs& a, int seq, i
       for (int e = 0; e < 4; ++e) {
         const int at = DW * j + i + e;
         if constexpr (QF) {
-          if (at >= Sh::KDW) q.rest[at - Sh::KDW] = x[e];
+          if (at >= N) q.rest[at - N] = x[e];
           else q.x[at] = x[e];
         } else {
           q.x[at] = x[e];

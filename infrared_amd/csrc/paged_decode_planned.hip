@@ -1132,7 +1132,7 @@ void dispatch_planned_codes(int dtype, bool qf, int head_dim, const DecodeArgs& 
          : launch_planned_codes_d<IR_DTYPE_F16, FMT, false>(head_dim, a, plan, ly, grid, pairs, s);
       break;
     default:
-      launch_planned_codes_d<IR_DTYPE_F32, FMT, false>(head_dim, a, plan, ly, grid, pairs, s);
+      launch_planned_codes_d<IR_DTYPE_F32, FMT, FMT == kCodes4>(head_dim, a, plan, ly, grid, pairs, s);
   }
 }
 
