@@ -196,17 +196,23 @@ constexpr int kLockstep = 0, kRing2 = 2;
 // exactly, where they are stored to LDS. kCodes4 (e2m1.hpp): 16 codes of a key's K and, as they
 // lie in a tile, 8 of two keys' V (4 of four at head_dim 64), likewise. CODES, either: The queries are used as they are given, in QP
 // pieces of the dtype: one for queries of it, so that a score is the sum of exact products in
-// fp32, two for fp32 queries (below). scale * log2 e is multiplied with a score less the
-// running maximum, in fp32, where its exponential is taken.
+// fp32, two for fp32 queries (below), three for an fp32 pool of 4-bit codes, whose numbers are
+// bf16 ones all the same, exactly: DT is bf16 then, queries and probabilities are three pieces each,
+// exactly, and the output is fp32; three bf16 products take 3 / 16 of the time of the fp32 ones they
+// stand for (8 chunks of 512 tokens after up to 8192 cached, 28 / 4 heads of 128: 684 us, 2516 in fp32
+// products). scale * log2 e is multiplied with a score less the running maximum, in fp32, where its
+// exponential is taken.
 template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, int FMT = kElements, int QP = 1>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
   typedef PShape<D, NW, CTW> S;
-  constexpr int EB = 2;
+  constexpr int OUT = QP == 3 ? IR_DTYPE_F32 : DT;  // of the output
+  constexpr int EB = QP == 3 ? 4 : 2;
   constexpr int CT = S::CT, BN = S::BN, NT = S::NT;
   constexpr int RING = SCHED == kRing2 ? 2 : 3;
-  constexpr bool WIDE = QP == 2;  // fp32 queries of a 16-bit pool
+  constexpr bool WIDE = QP > 1;  // fp32 queries
   constexpr bool CODES = FMT != kElements, C4 = FMT == kCodes4;
+  static_assert(QP < 3 || (C4 && DT == IR_DTYPE_BF16), "three pieces are an fp32 pool of 4-bit codes'");
   static_assert(CODES || !WIDE, "16-bit caches take queries of their dtype");
   __shared__ __attribute__((aligned(16))) uint16_t ks_lds[RING][BN * S::KROW];
   __shared__ __attribute__((aligned(16))) uint16_t vs_lds[RING][BN * S::KROW];
@@ -297,8 +303,9 @@ void paged_prefill_kernel(PrefillArgs a) {
   // WIDE: a row of fp32 queries is multiplied by the power of two that brings its largest
   // magnitude to [2^14, 2^15), and held in two pieces of the dtype, its rounded value and what
   // that leaves: off by 2^-18 of an element in bf16; in fp16 by 2^-24 of it or, where the pieces
-  // are subnormal, 2^-39 of the row's largest. unit takes the power back.
-  u32x4 qreg[CT][S::KS], qrest[WIDE ? CT : 1][S::KS];
+  // are subnormal, 2^-39 of the row's largest. unit takes the power back. (QP 3: to [1, 2), in three
+  // pieces.)
+  u32x4 qreg[CT][S::KS], qrest[WIDE ? CT : 1][S::KS], qlow[QP == 3 ? CT : 1][S::KS];
   float unit[CT];  // CODES: factor of a column's scores to base-2 exponents
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -317,15 +324,23 @@ void paged_prefill_kernel(PrefillArgs a) {
           most = fmaxf(most, fabsf(v[4 * i + j]));
         }
       }
-      const int up = row_shift(wave_max_groups_swap(most));
+      const int shift = row_shift(wave_max_groups_swap(most)), up = QP == 3 ? max(-126, shift - 14) : shift;
       unit[ct] = fmaxf(unit[ct] * pow2(-up), __FLT_MIN__);  // (not 0: a masked score is infinite)
 #pragma unroll
       for (int ks = 0; ks < S::KS; ++ks)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const Pieces p = split2<DT>(v[8 * ks + 2 * i] * pow2(up), v[8 * ks + 2 * i + 1] * pow2(up));
-          qreg[ct][ks][i] = p.hi;
-          qrest[ct][ks][i] = p.lo;
+          const float x0 = v[8 * ks + 2 * i] * pow2(up), x1 = v[8 * ks + 2 * i + 1] * pow2(up);
+          if constexpr (QP == 3) {
+            const Pieces3 p = split3(x0, x1);
+            qreg[ct][ks][i] = p.hi;
+            qrest[ct][ks][i] = p.mid;
+            qlow[ct][ks][i] = p.lo;
+          } else {
+            const Pieces p = split2<DT>(x0, x1);
+            qreg[ct][ks][i] = p.hi;
+            qrest[ct][ks][i] = p.lo;
+          }
         }
       continue;
     }
@@ -610,6 +625,7 @@ void paged_prefill_kernel(PrefillArgs a) {
     for (int ct = 0; ct < CT; ++ct) {
       x[ct][kt] = mfma_k32<DT>(ka, qreg[ct][ks], x[ct][kt]);
       if constexpr (WIDE) x[ct][kt] = mfma_k32<DT>(ka, qrest[ct][ks], x[ct][kt]);
+      if constexpr (QP == 3) x[ct][kt] = mfma_k32<DT>(ka, qlow[ct][ks], x[ct][kt]);
     }
   };
   auto zero_s = [](f32x4 (&x)[CT][4]) {
@@ -706,20 +722,33 @@ void paged_prefill_kernel(PrefillArgs a) {
     }
     // P^T operands of the two 32-key steps: k-slots 0..3 = keys 4g..4g+3 of
     // tile 2st, k-slots 4..7 = keys 4g..4g+3 of tile 2st+1
-    u32x4 pb[CT][2];
+    constexpr int PP = QP == 3 ? 3 : 1;  // pieces of a probability
+    u32x4 pb[PP][CT][2];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        pb[ct][st] = u32x4{E::pack2(cur[ct][2 * st][0], cur[ct][2 * st][1]),
-                           E::pack2(cur[ct][2 * st][2], cur[ct][2 * st][3]),
-                           E::pack2(cur[ct][2 * st + 1][0], cur[ct][2 * st + 1][1]),
-                           E::pack2(cur[ct][2 * st + 1][2], cur[ct][2 * st + 1][3])};
+        if constexpr (QP == 3) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x0 = cur[ct][2 * st + i / 2][2 * (i % 2)], x1 = cur[ct][2 * st + i / 2][2 * (i % 2) + 1];
+            const Pieces3 p = split3(x0, x1);
+            pb[0][ct][st][i] = p.hi;
+            pb[1][ct][st][i] = p.mid;
+            pb[2][ct][st][i] = p.lo;
+            l[ct] += x0 + x1;
+          }
+          continue;
+        }
+        pb[0][ct][st] = u32x4{E::pack2(cur[ct][2 * st][0], cur[ct][2 * st][1]),
+                              E::pack2(cur[ct][2 * st][2], cur[ct][2 * st][3]),
+                              E::pack2(cur[ct][2 * st + 1][0], cur[ct][2 * st + 1][1]),
+                              E::pack2(cur[ct][2 * st + 1][2], cur[ct][2 * st + 1][3])};
         // the running sum adds the rounded probabilities the PV product uses,
         // two per instruction (CODES: two pieces of each, as the decode has them, are
         // twice the PV products: 368 us against 298 for 8 chunks of 512 tokens)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) l[ct] = sum2<DT>(pb[ct][st][e], l[ct]);
+        for (int e = 0; e < 4; ++e) l[ct] = sum2<DT>(pb[0][ct][st][e], l[ct]);
       }
     }
     // O^T += V^T . P^T; V^T operand: d row c of the tile, the same key slots
@@ -738,7 +767,9 @@ void paged_prefill_kernel(PrefillArgs a) {
       if (t + kOperandAhead < 2 * S::DTL) vring[t % kOperandAhead] = v_operand(t + kOperandAhead);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
-        acc[ct][t % S::DTL] = mfma_k32<DT>(va, pb[ct][t / S::DTL], acc[ct][t % S::DTL]);
+#pragma unroll
+        for (int i = 0; i < PP; ++i)
+          acc[ct][t % S::DTL] = mfma_k32<DT>(va, pb[i][ct][t / S::DTL], acc[ct][t % S::DTL]);
     }
   };
 
@@ -899,7 +930,7 @@ void paged_prefill_kernel(PrefillArgs a) {
 #pragma unroll
       for (int dt = 0; dt < S::DTL; ++dt) {
         const float o[4] = {acc[qt][dt][0], acc[qt][dt][1], acc[qt][dt][2], acc[qt][dt][3]};
-        store4<DT>(orow + (dt * 16 + 4 * g) * EB, o, inv);
+        store4<OUT>(orow + (dt * 16 + 4 * g) * EB, o, inv);
       }
     }
     return;
@@ -987,7 +1018,7 @@ void paged_prefill_kernel(PrefillArgs a) {
 #pragma unroll
     for (int dt = 0; dt < S::DTL; ++dt) {
       const float o[4] = {o_run[qt][dt][0], o_run[qt][dt][1], o_run[qt][dt][2], o_run[qt][dt][3]};
-      store4<DT>(orow + (dt * 16 + 4 * g) * EB, o, inv);
+      store4<OUT>(orow + (dt * 16 + 4 * g) * EB, o, inv);
     }
   }
   if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1012,11 +1043,10 @@ void paged_prefill_kernel(PrefillArgs a) {
 constexpr int kF32Threads = 256;
 constexpr int kF32Cols = 64;
 
-template <int D, bool FAST, int FMT = kElements>
+template <int D, bool FAST, bool Q8 = false>
 __global__ __launch_bounds__(kF32Threads) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_prefill_f32_kernel(PrefillArgs a) {
   constexpr int NT = kF32Threads, BN = 64, MT = D / 16, DT4 = D / 4;
-  constexpr bool CODES = FMT != kElements, C4 = FMT == kCodes4;
   constexpr int KROW = D + 4;           // floats per K row in LDS
   constexpr int VROW = BN + 4;          // floats per V^T row (one d, 64 keys)
   constexpr int BPT = (BN / 4) * DT4 / NT;  // 4-key x 4-d blocks of a tile per thread
@@ -1092,12 +1122,11 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
   }
 
   const int32_t* bt_row = a.bt + (int64_t)seq * a.bt_stride;
-  typedef typename std::conditional<CODES, uint8_t, float>::type Elt;  // cache element
-  typedef typename std::conditional<CODES, uint32_t, f32x4>::type Four;  // (kCodes4: in its low half)
+  typedef typename std::conditional<Q8, uint8_t, float>::type Elt;  // cache element
+  typedef typename std::conditional<Q8, uint32_t, f32x4>::type Four;
   const Elt* kc = (const Elt*)a.kc + (int64_t)kvh * a.c_head;
   const Elt* vc = (const Elt*)a.vc + (int64_t)kvh * a.c_head;
-  const f32x2* scales = FMT == kCodes8 ? a.scales + kvh * a.num_blocks : nullptr;
-  const uint8_t* scales4 = C4 ? a.scales4 + (int64_t)kvh * a.c_head / 8 : nullptr;
+  const f32x2* scales = Q8 ? a.scales + kvh * a.num_blocks : nullptr;
   const int nblk_needed = (kmax + a.bs - 1) / a.bs;
   int bt_base = 0;
   auto fill_bt = [&](int base) {
@@ -1132,14 +1161,10 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
   // a tile's 4-key x 4-d blocks: block b = tid + NT i holds keys 4 (b / DT4)
   // .. +3 at d = 4 (b % DT4) .. +3
   Four kr[BPT][4], vr[BPT][4];
-  f32x2 sc[BPT];  // kCodes8: the scales of the four keys, which share a block
-  uint32_t sk[BPT][4], sv[BPT][4];  // kCodes4: of each
+  f32x2 sc[BPT];  // Q8: the scales of the four keys, which share a block
   bool ku[BPT][4];
   auto widen = [](Four x, float scale) -> f32x4 {
-    if constexpr (C4) {
-      const f32x2 lo = decode2_e2m1_f32<0>(x, scale), hi = decode2_e2m1_f32<1>(x, scale);
-      return f32x4{lo[0], lo[1], hi[0], hi[1]};
-    } else if constexpr (FMT == kCodes8) {
+    if constexpr (Q8) {
       const f32x2 lo = decode2_f32<false>(x, scale), hi = decode2_f32<true>(x, scale);
       return f32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
@@ -1154,24 +1179,6 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < BPT; ++i) {
       const int b = tid + NT * i, key4 = b / DT4, d4 = b - key4 * DT4;
-      if constexpr (C4) {
-        typedef Tile4<D> T;
-        const int k16 = k0 + 4 * (key4 & ~3);  // the keys' tile
-        bool use;
-        int32_t block;
-        const int64_t at = slot_of(k16, use, block);
-        const uint8_t* ts = scales4 + at / 8;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = 4 * (key4 & 3) + e;
-          kr[i][e] = *(const uint16_t*)(kc + at + T::k(t, d4 >> 1) + 2 * (d4 & 1));
-          vr[i][e] = *(const uint16_t*)(vc + at + (D == 128 ? T::v(t, d4 >> 1) + 2 * (d4 & 1) : T::v(t, d4)));
-          sk[i][e] = ts[T::k_scale(t, d4 >> 3)];
-          sv[i][e] = ts[T::v_scale(t, d4 >> 3)];
-          ku[i][e] = use && k16 + t < kmax;
-        }
-        continue;
-      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         bool use;
@@ -1180,7 +1187,7 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
         kr[i][e] = *(const Four*)(kc + sl + 4 * d4);
         vr[i][e] = *(const Four*)(vc + sl + 4 * d4);
         ku[i][e] = use;
-        if (FMT == kCodes8 && e == 0) sc[i] = scales[block];
+        if (Q8 && e == 0) sc[i] = scales[block];
       }
     }
   };
@@ -1189,14 +1196,10 @@ void paged_prefill_f32_kernel(PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < BPT; ++i) {
       const int b = tid + NT * i, key4 = b / DT4, d4 = b - key4 * DT4;
-      float k_scale = FMT == kCodes8 ? sc[i][0] : 1.f, v_scale = FMT == kCodes8 ? sc[i][1] : 1.f;
+      const float k_scale = Q8 ? sc[i][0] : 1.f, v_scale = Q8 ? sc[i][1] : 1.f;
       f32x4 v4[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (C4) {
-          k_scale = scale_of_byte(sk[i][e]);
-          v_scale = scale_of_byte(sv[i][e]);
-        }
         *(f32x4*)&ks[(4 * key4 + e) * KROW + 4 * d4] = ku[i][e] ? widen(kr[i][e], k_scale) : zero;
         v4[e] = widen(vr[i][e], v_scale);
       }
@@ -1370,14 +1373,10 @@ int launch_prefill_f32(PrefillArgs a, hipStream_t s) {
   const bool fast = a.bs_shift >= 0 && slots < (1 << 23) && a.c_slot < (1 << 23) &&
                     (slots * a.c_slot + a.c_head * a.num_kv_heads) < ((int64_t)1 << 31);
   const dim3 g((unsigned)grid), block(kF32Threads);
-  if (a.scales4 && fast)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, kCodes4>), g, block, 0, s, a);
-  else if (a.scales4)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, kCodes4>), g, block, 0, s, a);
-  else if (a.scales && fast)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, kCodes8>), g, block, 0, s, a);
+  if (a.scales && fast)
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true, true>), g, block, 0, s, a);
   else if (a.scales)
-    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, kCodes8>), g, block, 0, s, a);
+    hipLaunchKernelGGL((paged_prefill_f32_kernel<D, false, true>), g, block, 0, s, a);
   else if (fast)
     hipLaunchKernelGGL((paged_prefill_f32_kernel<D, true>), g, block, 0, s, a);
   else
@@ -1913,7 +1912,8 @@ int launch_prefill_codes(const char* name, const PrefillArgs& a, hipStream_t s) 
     else                                                                                                             \
       hipLaunchKernelGGL((paged_prefill_kernel<DT, D, false, NW_, CT_, kRing2, false, FMT, QP>), g, block, 0, s, a); \
   } while (0)
-  if (a.nw == 4 && !a.items && grid <= device_cus()) IR_PREFILL_CODES(8, 1);
+  if constexpr (QP == 3) IR_PREFILL_CODES(4, 1);  // 64 columns, as an fp32 plan's items
+  else if (a.nw == 4 && !a.items && grid <= device_cus()) IR_PREFILL_CODES(8, 1);
   else if (a.nw == 4) IR_PREFILL_CODES(4, 2);
   else IR_PREFILL_CODES(8, 2);
 #undef IR_PREFILL_CODES
@@ -2071,6 +2071,9 @@ int prefill_call(const char* name, int fmt, const void* scales, int q_dtype, con
     return dtype == IR_DTYPE_F16 ? dispatch_prefill_codes<IR_DTYPE_F16, kCodes8>(name, head_dim, wide, a, s)
                                  : dispatch_prefill_codes<IR_DTYPE_BF16, kCodes8>(name, head_dim, wide, a, s);
   }
+  if (f32 && fmt == kCodes4)
+    return head_dim == 128 ? launch_prefill_codes<IR_DTYPE_BF16, 128, kCodes4, 3>(name, a, s)
+                           : launch_prefill_codes<IR_DTYPE_BF16, 64, kCodes4, 3>(name, a, s);
   if (f32) return head_dim == 128 ? launch_prefill_f32<128>(a, s) : launch_prefill_f32<64>(a, s);
   if (dtype == IR_DTYPE_BF16)
     return head_dim == 128 ? launch_prefill<IR_DTYPE_BF16, 128>(a, geo.sched, s)
