@@ -722,55 +722,82 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       }
     };
     if constexpr (FMT == kCodes4) {
-      // Two tiles of a unit at a time (compute_pair4), the next pair's loads in flight. (Two or
-      // three pairs ahead: 64 sequences of 512..4096 keys no faster, three of 40,000..90,000
-      // slower by 4%.)
-      Pair4<D> x;
-      int64_t at_a, at_b;
-      uint32_t ma, mb;
+      // Two tiles of a unit at a time (compute_pair4), a pair's loads going out AHEAD pairs before it: at
+      // head_dim 64 a pair is too few bytes to cover their latency (64 sequences of 4,096 keys, 28 / 4
+      // heads: 29.6 us with one ahead, 24.3 with two, 23.6 with three; of 1,024 11.7, 10.7, 11.1), at
+      // 128 more ahead gains nothing (512..4096 keys) or loses 4% (three of 40,000..90,000).
+      // (An fp32 pool's products take three times as long: 20.9 us with one, 22.0 with two.)
+      constexpr int AHEAD = D == 64 && DT != IR_DTYPE_F32 ? 2 : 1;
+      struct Ring {
+        Pair4<D> x;
+        int64_t at_a, at_b;
+        uint32_t ma, mb;
+      } ring[AHEAD];
       int next = 0;  // first tile that no pair has yet
-      auto spot = [&] {  // (the last tile of an odd unit is loaded twice, the second time without keys)
+      auto spot = [&](Ring& r) {  // (the last tile of an odd unit is loaded twice, the second time without keys)
         const int j = min(next + 1, last);
         const uint32_t oa = (uint32_t)__builtin_amdgcn_readlane((int)info_off, next);
         const uint32_t ob = (uint32_t)__builtin_amdgcn_readlane((int)info_off, j);
-        ma = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, next);
-        mb = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, j);
-        const bool two = next < last && ma >> 7 == mb >> 7;
-        at_a = (int64_t)oa << 4;
-        at_b = (int64_t)(two ? ob : oa) << 4;
-        mb = two ? mb : ma & ~31u;
+        r.ma = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, next);
+        r.mb = (uint32_t)__builtin_amdgcn_readlane((int)info_meta, j);
+        const bool two = next < last && r.ma >> 7 == r.mb >> 7;
+        r.at_a = (int64_t)oa << 4;
+        r.at_b = (int64_t)(two ? ob : oa) << 4;
+        r.mb = two ? r.mb : r.ma & ~31u;
         next += two ? 2 : 1;
       };
-      auto issue_k = [&] {
-        issue_k4<DT, D>(kc, a.scales4, at_a, lo_off, x.a);
-        issue_k4<DT, D>(kc, a.scales4, at_b, lo_off, x.b);
+      auto issue_k = [&](Ring& r) {
+        issue_k4<DT, D>(kc, a.scales4, r.at_a, lo_off, r.x.a);
+        issue_k4<DT, D>(kc, a.scales4, r.at_b, lo_off, r.x.b);
       };
-      auto issue_v = [&] {
-        issue_v4<DT, D>(vc, a.scales4, at_a, lo_off, x.a);
-        issue_v4<DT, D>(vc, a.scales4, at_b, lo_off, x.b);
+      auto issue_v = [&](Ring& r) {
+        issue_v4<DT, D>(vc, a.scales4, r.at_a, lo_off, r.x.a);
+        issue_v4<DT, D>(vc, a.scales4, r.at_b, lo_off, r.x.b);
       };
-      auto step = [&](auto more) __attribute__((always_inline)) {
-        const uint32_t na = ma, nb = mb;
+      // Computes ring slot r and, if `more`, issues the next pair into it.
+      auto step = [&](Ring& r, auto more) __attribute__((always_inline)) {
+        const uint32_t na = r.ma, nb = r.mb;
         enter((int)(na >> 7));
-        if constexpr (decltype(more)::value) spot();
+        if (more) spot(r);
         auto next_k = [&] {
-          if constexpr (decltype(more)::value) issue_k();
+          if (more) issue_k(r);
         };
         auto next_v = [&] {
-          if constexpr (decltype(more)::value) issue_v();
+          if (more) issue_v(r);
         };
         constexpr uint32_t kAll = 3u << 5 | 16u;  // every key, every column
         const bool whole = (na & 127u) == kAll && (nb & 127u) == kAll;
         const int half = PAIRS && c >= a.n_rep ? 6 : 5;
-        compute_pair4<DT, D, QF>(x, qr, whole, na & 31u, nb & 31u, (na >> half) & 1u, (nb >> half) & 1u, a.scale_log2,
+        compute_pair4<DT, D, QF>(r.x, qr, whole, na & 31u, nb & 31u, (na >> half) & 1u, (nb >> half) & 1u, a.scale_log2,
                                  lane, st, next_k, next_v);
       };
-      spot();
-      issue_k();
-      issue_v();
-      // (no branch around the loop's loads, and nothing is issued past the end)
-      while (next <= last) step(std::true_type{});
-      step(std::false_type{});
+      int held = 0;  // pairs in the ring
+#pragma unroll
+      for (int r = 0; r < AHEAD; ++r) {
+        if (r > 0 && next > last) break;
+        spot(ring[r]);
+        issue_k(ring[r]);
+        issue_v(ring[r]);
+        ++held;
+      }
+      // (the loop has no branch around its loads, and nothing is issued past the end)
+      while (next + 2 * AHEAD - 2 <= last) {
+#pragma unroll
+        for (int r = 0; r < AHEAD; ++r) step(ring[r], std::true_type{});
+      }
+      if constexpr (AHEAD == 1) {
+        step(ring[0], std::false_type{});
+      } else {
+        while (held > 0) {
+#pragma unroll
+          for (int r = 0; r < AHEAD; ++r) {
+            if (held == 0) break;
+            const bool more = next <= last;
+            step(ring[r], more);
+            held -= !more;
+          }
+        }
+      }
     } else {
       f32x2 sc = {0.f, 0.f};
       if constexpr (FMT == kCodes8) {
