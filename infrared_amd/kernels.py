@@ -361,7 +361,7 @@ _CU_COUNT: dict[int, int] = {}
 
 
 def decode_plan_pays(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_blocks: int, block_size: int,
-                     device: torch.device | str | int | None = None) -> bool:
+                     device: torch.device | str | int | None = None, bits: int = 16) -> bool:
     """Whether the planned schedule is the faster decode for this shape: it is
     plannable, and either the batch has a unit (sequence x KV head x group of
     <= 16 query heads) per CU or its block tables can hold 16 tiles (256 keys)
@@ -371,7 +371,14 @@ def decode_plan_pays(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_blo
     per call): 64 sequences 57.2 (fixed) vs 49.7 us; 8 of 2k..32k keys 72.0 vs
     55.0 us; 16 skewed long ones 33.4 vs 31.8 us; 16 of 16..1024 keys 16.3 vs
     11.6 us; but 8 fp32 sequences of <= 512 keys 7.1 vs 10.5 us and 16 of <= 300
-    keys in tables of that width 7.9 vs 11.0 us."""
+    keys in tables of that width 7.9 vs 11.0 us.
+
+    ``bits=4``: the pool's, whose keys are so few bytes that tables of up to 1,024 keys
+    are never planned (64 sequences of 1..512 keys 7.0 vs 12.2 us, of 1..1024 10.3 vs
+    15.3; 512 of them 40.5 vs 42.0; of 1..2048 keys 64 sequences 16.2 vs 17.2, 128 27.5
+    vs 24.0)."""
+    if bits == 4 and max_blocks * block_size <= 1024:
+        return False
     if decode_plan_bytes(num_seqs, num_q_heads, num_kv_heads, max_blocks, block_size) <= 0:
         return False
     idx = torch.device(device if device is not None else "cuda").index

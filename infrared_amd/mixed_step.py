@@ -175,7 +175,8 @@ class MixedStep:
         self.out_pre = torch.empty_like(inputs.q_pre)
         hq, d = inputs.q_dec.shape[2], inputs.q_dec.shape[3]
         nd, max_blocks = batch.dec_tables.shape
-        self.planned = kernels.decode_plan_pays(nd, hq, pool.num_kv_heads, max_blocks, pool.block_size, dev)
+        self.planned = kernels.decode_plan_pays(nd, hq, pool.num_kv_heads, max_blocks, pool.block_size, dev,
+                                                getattr(pool, "bits", 16))
         if self.planned:
             need = kernels.planned_workspace_bytes(nd, hq, pool.num_kv_heads, d)
             self.plan_buf = torch.empty(

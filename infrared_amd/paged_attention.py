@@ -418,7 +418,8 @@ def _decode(q, pool, layer_idx: int, block_tables, context_lens, holder, scale: 
     h_kv = pool.k.shape[-2]
     k_layer, v_layer, scales = _layer(pool, layer_idx)
     max_blocks = block_tables.shape[1]
-    if hasattr(pool, "plan_buffer") and kernels.decode_plan_pays(b, hq, h_kv, max_blocks, pool.block_size, q.device):
+    if hasattr(pool, "plan_buffer") and kernels.decode_plan_pays(b, hq, h_kv, max_blocks, pool.block_size, q.device,
+                                                                 getattr(pool, "bits", 16)):
         # balanced schedule: built by the step's first layer, reused by the
         # rest -- unless another context's plan has since taken the pool's
         # plan buffer (two decode contexts run interleaved), then rebuilt.

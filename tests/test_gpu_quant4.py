@@ -741,7 +741,7 @@ def test_seam_writes_then_attends_as_its_parts_do():
     """``paged_attention`` over decode metadata: the write, then the kernels' decode."""
     hq, h, d, bs = 28, 4, 128, 16
     g = gen(17)
-    lens = [100, 1, 33, 700] * 20  # (enough sequences for the balanced schedule)
+    lens = [100, 1, 33, 1100] * 20  # (enough sequences, and keys of a table, for the balanced schedule)
     one, tables, _ = filled(40, torch.bfloat16, lens, h, d, bs)
     two, _, _ = filled(40, torch.bfloat16, lens, h, d, bs)
     paged, mask = metadata.decode_context(one, tables, lens)
@@ -755,6 +755,14 @@ def test_seam_writes_then_attends_as_its_parts_do():
     few.write_slots = torch.full((3,), -1, device=DEV)  # (already written)
     out = paged_attention(q[:3], k[:3], v[:3], few, None, 0, d**-0.5, hq // h)
     want = run_decode(two, q[:3, 0], few.block_tables, few.context_lens, False)
+    assert torch.equal(out[:, 0], want)
+    at = [i for i, n in enumerate(lens) if n < 1000] * 2  # tables of few keys are not planned
+    short = metadata.decode_context(two, [tables[i] for i in at], [lens[i] for i in at])[0]
+    short.write_slots = torch.full((len(at),), -1, device=DEV)
+    assert len(at) * h >= 256 and not kernels.decode_plan_pays(len(at), hq, h, short.block_tables.shape[1], bs, bits=4)
+    out = paged_attention(q[at], k[at], v[at], short, None, 0, d**-0.5, hq // h)
+    assert short.decode_plan is None
+    want = run_decode(two, q[at, 0], short.block_tables, short.context_lens, False)
     assert torch.equal(out[:, 0], want)
 
 

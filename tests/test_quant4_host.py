@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from infrared_amd import Quant4PagedKVPool, RotaryAxes, _lib, rotary
+from infrared_amd import _lib, kernels, Quant4PagedKVPool, rotary, RotaryAxes
 from oracle import quant4
 
 P = 256  # an aligned address that is never used
@@ -213,6 +213,10 @@ def test_attention_refusals(fn, kw, text):
 def test_attention_refuses_a_scale_that_is_no_number(fn, scale):
     assert _attend(fn, scale=scale) < 0
     assert b"scale" in _lib.lib().ir_last_error()
+
+
+def test_tables_of_few_keys_are_not_planned():
+    assert not kernels.decode_plan_pays(512, 28, 4, 64, 16, bits=4)
 
 
 def test_decode_plan_takes_the_4_bit_layers_strides():
