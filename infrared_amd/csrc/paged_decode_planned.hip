@@ -1054,6 +1054,8 @@ void launch_planned_dt_d(const DecodeArgs& a, const uint8_t* plan, const PlanLay
 // keys, 64 slices a unit, 35.0 us so against 26.4; three of 31,424, 21 slices, 28.8
 // against 26.4). With eight of 11,776, eight slices a unit, it is 25.1 either way, and
 // where the units are many it only adds a launch.
+// (Over a 4-bit cache, 32 / 4 heads: 30.2 and 20.8, three of 60,000 keys 31.3 and 27.7; eight of 16,000
+// 22.4 either way.)
 constexpr int kMergeSlices = 12;  // slices a unit has, on average, from which on
 constexpr int kMergeThreads = 256;
 
