@@ -639,6 +639,86 @@ def test_fp32_queries_of_a_16_bit_pool(path, dtype, hq, h, d, bs):
     assert off < 0.25 * rounded, (off, rounded)
 
 
+# (bf16 products of three pieces each: the pieces add up to the number, a product of 32 terms is off by
+# 2^-22 of their size at most, and a score has d / 32 * 3 of them: within the 4 (d + 8) 2^-24 of fp32_tolerance)
+@pytest.mark.parametrize("path", ["decode", "planned", "prefill"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_fp32_pools_keep_queries_of_unlike_elements(path, d):
+    """Elements of a row from 2^-14 to 2^14 times the others, rows of any size."""
+    bs, hq, h = 16, 6, 2
+    lens = [1, 40, 300, 1500]
+    pool, tables, values = filled(45, torch.float32, lens, h, d, bs)
+    g = gen(46)
+    q = torch.randn(len(lens), hq, d, generator=g, device=DEV)
+    q = q * torch.exp2(torch.randint(-14, 15, q.shape, generator=g, device=DEV).float())
+    q = q * torch.tensor([1.0, 2.0**-20, 2.0**-10, 2.0**-13], device=DEV)[:, None, None]
+    bt, ctx = device_tables(tables), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    if path == "prefill":
+        cu = torch.arange(len(lens) + 1, dtype=torch.int32, device=DEV)
+        out = kernels.paged_prefill(q, pool.k[0], pool.v[0], bt, cu, ctx - 1, 1, bs, d**-0.5,
+                                    kv_scales=pool.kv_scales[0])
+    else:
+        out = run_decode(pool, q, bt, ctx, path == "planned")
+    check_decode(out, q, values, tables, lens, bs, torch.float32)
+
+
+def test_prefill_writes_rows_of_a_wider_output_alone():
+    bs, hq, h, d = 48, 21, 3, 64
+    cached, new = [0, 5, 1111, 48], [1, 49, 300, 48]
+    lens = [c + n for c, n in zip(cached, new)]
+    for dtype in DTYPES:
+        pool, tables, values = filled(47, dtype, lens, h, d, bs)
+        total = sum(new)
+        q = torch.randn(total, 2 * hq, d + 8, generator=gen(48), device=DEV).to(dtype)[:, ::2, :d]
+        wide = torch.full((total, hq + 1, d + 8), 7.0, dtype=dtype, device=DEV)
+        cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+        start = torch.tensor(cached, dtype=torch.int32, device=DEV)
+        kernels.paged_prefill(q, pool.k[0], pool.v[0], device_tables(tables), cu, start, max(new), bs, d**-0.5,
+                              out=wide[:, :hq, :d], kv_scales=pool.kv_scales[0])
+        assert (wide[:, hq:] == 7).all() and (wide[:, :, d:] == 7).all()
+        row = 0
+        for t, c, n in zip(tables, cached, new):
+            o, a, reach = quant.attend(q[row : row + n], values, t, bs, c, d**-0.5)
+            tol = fp32_tolerance(o, a, reach, d) + small_probabilities(values, t, c + n, bs, hq, dtype)
+            if dtype != torch.float32:
+                tol = tol + prefill_tolerance(o, a, reach, dtype)
+            assert ((wide[row : row + n, :hq, :d].double().cpu() - o).abs() <= tol).all(), (dtype, c, n)
+            row += n
+
+
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.float32, 128), (torch.float16, 128)])
+def test_graphs_of_both_decodes_share_a_workspace(dtype, d):
+    """Replayed in turn, with eager calls between, the counters zero after each."""
+    hq, h, bs = 14, 2, 16
+    lens = [(i * 331) % 1300 + 1 for i in range(40)]
+    pool, tables, _ = filled(49, dtype, lens, h, d, bs)
+    bt, ctx = device_tables(tables), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    qs = torch.randn(2, len(lens), hq, d, generator=gen(50), device=DEV).to(dtype)
+    plan = kernels.decode_plan(bt, ctx, hq, pool.k[0], bs)
+    need = max(kernels.planned_workspace_bytes(len(lens), hq, h, d),
+               kernels.decode_workspace_bytes(len(lens), hq, h, d, bt.shape[1], bs))
+    kw = {"workspace": torch.empty(need, dtype=torch.uint8, device=DEV),
+          "counters": torch.zeros(kernels.decode_num_counters(len(lens), hq, h), dtype=torch.int32, device=DEV),
+          "kv_scales": pool.kv_scales[0]}
+    calls = [lambda q: kernels.paged_decode_planned(q, pool.k[0], pool.v[0], plan, 0.1, **kw),
+             lambda q: kernels.paged_decode(q, pool.k[0], pool.v[0], bt, ctx, bs, 0.1, **kw)]
+    want = [f(q).clone() for f, q in zip(calls, qs)]
+    graphs = []
+    for f, q in zip(calls, qs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f(q)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for (graph, out), w in zip(graphs, want):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w) and not kw["counters"].any()
+        for f, q in zip(calls, qs.flip(0)):
+            f(q)
+
+
 # ---- rotation into the pool
 
 
