@@ -467,7 +467,12 @@ struct Pair4 {
 //
 // valid_a, valid_b: the tiles' usable keys; col_a, col_b: whether the lane's column attends the tile;
 // whole: it is all of them. An absent key's scales become 0, what it holds finite.
-template <int DT, int D, bool QF, typename NextK, typename NextV>
+//
+// PAIRS: a unit can hold two sequences' columns, and a column's probability of 0 is no answer to a V
+// that is NaN. Where a tile that some column does not attend has such a group (its scale byte says so:
+// a branch that finite values never take), the group's channels become NaN in the columns that attend it,
+// which one product of zeros and ones finds for all of a lane's channels, and the group becomes 0.
+template <int DT, int D, bool QF, bool PAIRS, typename NextK, typename NextV>
 __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D, QF>& q, bool whole, int valid_a,
                                               int valid_b, bool col_a, bool col_b, float scale_log2, int lane,
                                               State<D>& st, NextK next_k, NextV next_v) {
@@ -488,6 +493,27 @@ __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D
     };
     ta.vs &= rows(valid_a);
     tb.vs &= rows(valid_b);
+    if (PAIRS && !__all(col_a && col_b)) {
+      auto nan_of = [](uint32_t w) {  // bit 7 of the bytes that are 255
+        return w & ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+      };
+      const uint32_t na = nan_of(ta.vs), nb = nan_of(tb.vs);
+      if (__any((na | nb) != 0)) {
+        const uint32_t one = Elem<KT>::pack2(1.f, 0.f), ones = one | one << 16;
+        auto flags = [&](uint32_t n, int r) {  // of the lane's rows r, r + 1
+          return (n >> (8 * r + 7) & 1u ? one : 0u) | (n >> (8 * r + 15) & 1u ? one << 16 : 0u);
+        };
+        const uint32_t pa = col_a ? ones : 0u, pb = col_b ? ones : 0u;
+        const f32x4 hit = mfma_k32<KT>(u32x4{flags(na, 0), flags(na, 2), flags(nb, 0), flags(nb, 2)},
+                                       u32x4{pa, pa, pb, pb}, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.acc[n][i] = hit[i] > 0.f ? __builtin_nanf("") : st.acc[n][i];
+        ta.vs &= ~((na >> 7) * 255u);
+        tb.vs &= ~((nb >> 7) * 255u);
+      }
+    }
   }
   auto scores = [&](const Code4Tile<D>& t) {
     uint32_t kop[Sh::KDW];
@@ -687,7 +713,6 @@ __device__ __forceinline__ void attend_tiles4(const DecodeArgs& a, const int32_t
                                               QueryRegs<DT, D, QF>& qr, int tile_lo, int tile_hi, int t_end,
                                               int lane, int w, State<D>& st, bool& bad) {
   constexpr int RUN = NW * kMaxWaveTiles;
-  const int g = lane >> 4;
   for (int r0 = tile_lo; r0 < tile_hi; r0 += RUN) {
     const int ntiles = min(tile_hi - r0, RUN);
     const int pairs = (ntiles + 1) / 2, my_pairs = pairs > w ? (pairs - w + NW - 1) / NW : 0;
@@ -733,7 +758,8 @@ __device__ __forceinline__ void attend_tiles4(const DecodeArgs& a, const int32_t
           issue_v4<DT, D>(vc, scales, sb.at, lo, x.b);
         }
       };
-      compute_pair4<DT, D, QF>(x, qr, va == 16 && vb == 16, va, vb, true, true, a.scale_log2, lane, st, next_k, next_v);
+      compute_pair4<DT, D, QF, false>(x, qr, va == 16 && vb == 16, va, vb, true, true, a.scale_log2, lane, st, next_k,
+                                      next_v);
     };
     for (int i = 0; i + 1 < my_pairs; ++i) step(i, std::true_type{});
     step(my_pairs - 1, std::false_type{});  // (nothing is issued past the end)

@@ -768,8 +768,8 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
         constexpr uint32_t kAll = 3u << 5 | 16u;  // every key, every column
         const bool whole = (na & 127u) == kAll && (nb & 127u) == kAll;
         const int half = PAIRS && c >= a.n_rep ? 6 : 5;
-        compute_pair4<DT, D, QF>(r.x, qr, whole, na & 31u, nb & 31u, (na >> half) & 1u, (nb >> half) & 1u, a.scale_log2,
-                                 lane, st, next_k, next_v);
+        compute_pair4<DT, D, QF, PAIRS>(r.x, qr, whole, na & 31u, nb & 31u, (na >> half) & 1u, (nb >> half) & 1u,
+                                        a.scale_log2, lane, st, next_k, next_v);
       };
       int held = 0;  // pairs in the ring
 #pragma unroll

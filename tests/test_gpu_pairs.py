@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from infrared_amd import kernels
+from infrared_amd import PagedKVPool, Quant4PagedKVPool, QuantPagedKVPool, kernels
 from infrared_amd._lib import ERR_BLOCK_RANGE, ERR_PLAN
 from infrared_amd.workloads import make_decode_case
 from oracle import naive as O
@@ -224,3 +224,61 @@ def test_pairs_through_the_seam():
         assert (out.float().cpu() - ref).abs().max().item() <= 2e-2
     expect = sum(1 for i in range(0, b - 1, 2) if min(num_cached[i], num_cached[i + 1]) // 2 // bs > 0)
     assert _pairs_in(paged.decode_plan) == expect > 0
+
+
+def _spoilt_pair(kind, dtype, d, hq, h, fp32_queries=False):
+    """A pool of ``kind`` bits whose sequences 0 and 1 begin with the same three blocks (an odd number, of
+    tiles of 16 keys, as each one's own are): ``run(spoil)`` attends it with, of ``spoil`` = (sequence,
+    position, K or V, number), that number in one channel of the last KV head."""
+    bs, lens = 16, [135, 121, 50]
+    pool_type = {4: Quant4PagedKVPool, 8: QuantPagedKVPool, 16: PagedKVPool}[kind]
+    own = [[3, 14, 7, 1, 20, 9, 12, 5, 0], [3, 14, 7, 2, 19, 11, 4, 21], [6, 16, 10, 8]]
+    bt = torch.tensor([t + [0] * (9 - len(t)) for t in own], dtype=torch.int32, device=DEV)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(d + hq)
+    k, v = torch.randn(2, 24 * bs, h, d, generator=gen, device=DEV).to(dtype)
+    q = torch.randn(3, hq, d, generator=gen, device=DEV).to(torch.float32 if fp32_queries else dtype)
+
+    def run(spoil=None):
+        pool = pool_type(1, 24, bs, h, d, dtype)
+        rows = [k.clone(), v.clone()]
+        if spoil is not None:
+            seq, pos, which, number = spoil
+            rows[which][own[seq][pos // bs] * bs + pos % bs, h - 1, 3] = number
+        pool.write(0, *rows, torch.arange(24 * bs, device=DEV))
+        scales = None if kind == 16 else pool.kv_scales[0]
+        plan = kernels.decode_plan(bt, ctx, hq, pool.k[0], bs, share_groups=True)
+        assert _pairs_in(plan) & 0xFFFF == 1
+        out = torch.empty(3, hq, d, dtype=dtype, device=DEV)
+        return kernels.paged_decode_planned(q, pool.k[0], pool.v[0], plan, d**-0.5, out=out, kv_scales=scales)
+
+    return run
+
+
+def _check_spoilt_pair(run, hq, h, numbers):
+    clean = run()
+    assert clean.isfinite().all()
+    last = hq // h * (h - 1)  # first query head of the last KV head
+    for seq, places in ((0, (48, 64, 134)), (1, (48, 70, 120))):
+        for pos in places:
+            for which in (0, 1):
+                for number in numbers:
+                    out = run((seq, pos, which, number))
+                    case = (seq, pos, which, number)
+                    assert torch.equal(out[1 - seq], clean[1 - seq]) and torch.equal(out[2], clean[2]), case
+                    assert torch.equal(out[seq, :last], clean[seq, :last]), case
+                    if which == 0:
+                        assert number != number or (out[seq, last:] != clean[seq, last:]).any(), case
+                        assert number == number or out[seq, last:].isnan().all(), case
+                    else:
+                        assert not out[seq, last:, 3].isfinite().any(), case
+                        assert out[seq, last:, 32:].equal(clean[seq, last:, 32:]), case
+
+
+@pytest.mark.parametrize("dtype, fp32_queries", [(torch.bfloat16, False), (torch.float16, False),
+                                                 (torch.float32, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("hq, h, d", [(28, 4, 128), (14, 2, 64), (2, 2, 128)])
+def test_pairs_over_4_bits_keep_a_number_that_is_none_to_its_own_sequence(dtype, fp32_queries, hq, h, d):
+    """NaN or an infinity behind the shared prefix spoils the sequence that attends it, as alone: the
+    other's output is the same bits as without it."""
+    _check_spoilt_pair(_spoilt_pair(4, dtype, d, hq, h, fp32_queries), hq, h, [float("nan"), float("inf")])
