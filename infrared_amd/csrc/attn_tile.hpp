@@ -13,6 +13,8 @@
 //               of column c, i.e. one lane owns 4*head_dim/16 consecutive d.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace ir {
@@ -262,9 +264,12 @@ constexpr float kProbUp = DT == IR_DTYPE_F16 ? 7.f : 0.f;
 // of LDS, and the probabilities of a 16-bit dtype in two pieces of it (off by 2^-18, fp16
 // 2^-24), so that the output's rounding is all that shows. A product of 32 k-slots holds both
 // pieces, the V rows twice, and takes as long as one of 16.
-template <int DT, int D, bool FULL, bool Q8 = false>
+// PAIRS: columns that are not `on` attend none of the tile's keys (their scores are -inf). A probability
+// of 0 is no answer to a V that is NaN or infinite, so where there is one, such numbers are multiplied apart
+// and added to the columns that attend them, and are 0 in the products of all.
+template <int DT, int D, bool FULL, bool Q8 = false, bool PAIRS = false>
 __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t (&vin)[4][TileShape<DT, D>::VDW],
-                                           const bool (&vok)[4], State<D>& st) {
+                                           const bool (&vok)[4], State<D>& st, bool on = true) {
   typedef TileShape<DT, D> Sh;
   constexpr int TILES = Sh::TILES;
   float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
@@ -287,25 +292,54 @@ __device__ __forceinline__ void softmax_pv(const float (&sv)[4], const uint32_t 
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int i = 0; i < Sh::VDW; ++i) v[r][i] = (FULL || vok[r]) ? vin[r][i] : 0u;
+  // element n of rows 4g..4g+3 -> the 4 k-slots of this lane (transpose)
+  auto operand = [&](int n) {
+    const int wdw = n >> 1;
+    if ((n & 1) == 0)
+      return u32x2{(v[0][wdw] & 0xffffu) | (v[1][wdw] << 16), (v[2][wdw] & 0xffffu) | (v[3][wdw] << 16)};
+    return u32x2{(v[0][wdw] >> 16) | (v[1][wdw] & 0xffff0000u), (v[2][wdw] >> 16) | (v[3][wdw] & 0xffff0000u)};
+  };
+  if constexpr (PAIRS) {
+    if (!__all(on)) {
+      float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < Sh::VDW; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = times_zero<DT>(v[r][i], z[r]);
+      z[0] = (z[0] + z[1]) + (z[2] + z[3]);
+      if (__any(z[0] != z[0])) {  // their products first, alone, for the columns that attend them
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+          f32x4 o = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (Sh::k16) {
+            const u32x2 x = operand(n);
+            o = mfma_k16<DT>(u32x2{x[0] & not_finite<DT>(x[0]), x[1] & not_finite<DT>(x[1])},
+                             u32x2{Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3])}, o);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              o = mfma_f32_k4(__uint_as_float(v[r][n] & not_finite<DT>(v[r][n])), p[r], o);
+          }
+          st.acc[n] += on ? o : f32x4{0.f, 0.f, 0.f, 0.f};
+          __builtin_amdgcn_sched_barrier(0);  // (one product at a time: registers)
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < Sh::VDW; ++i) v[r][i] &= ~not_finite<DT>(v[r][i]);
+      }
+    }
+  }
   if constexpr (Sh::k16) {
     // P rounded to the input dtype, as softmax(...).to(q.dtype) does (Q8: p0.hi, p1.hi).
     const Pieces p0 = split2<DT>(p[0], p[1]), p1 = split2<DT>(p[2], p[3]);
 #pragma unroll
     for (int n = 0; n < TILES; ++n) {
-      // element n of rows 4g..4g+3 -> the 4 k-slots of this lane (transpose)
-      const int wdw = n >> 1;
-      uint32_t lo, hi;
-      if ((n & 1) == 0) {
-        lo = (v[0][wdw] & 0xffffu) | (v[1][wdw] << 16);
-        hi = (v[2][wdw] & 0xffffu) | (v[3][wdw] << 16);
-      } else {
-        lo = (v[0][wdw] >> 16) | (v[1][wdw] & 0xffff0000u);
-        hi = (v[2][wdw] >> 16) | (v[3][wdw] & 0xffff0000u);
-      }
+      const u32x2 x = operand(n);
       if constexpr (Q8)
-        st.acc[n] = mfma_k32<DT>(u32x4{lo, hi, lo, hi}, u32x4{p0.hi, p1.hi, p0.lo, p1.lo}, st.acc[n]);
+        st.acc[n] = mfma_k32<DT>(u32x4{x[0], x[1], x[0], x[1]}, u32x4{p0.hi, p1.hi, p0.lo, p1.lo}, st.acc[n]);
       else
-        st.acc[n] = mfma_k16<DT>(u32x2{lo, hi}, u32x2{p0.hi, p1.hi}, st.acc[n]);
+        st.acc[n] = mfma_k16<DT>(x, u32x2{p0.hi, p1.hi}, st.acc[n]);
     }
   } else {
     // fp32: one 16x16x4 product per key row; k-slot = lane group.

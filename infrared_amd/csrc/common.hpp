@@ -151,6 +151,25 @@ __device__ __forceinline__ Pieces split2(float a, float b) {
   return {hi, Elem<DT>::pack2(a - Elem<DT>::lo(hi), b - Elem<DT>::hi(hi))};
 }
 
+// acc plus the elements of a dword times 0: NaN if one of them is no finite number.
+template <int DT>
+__device__ __forceinline__ float times_zero(uint32_t w, float acc) {
+  if constexpr (DT == IR_DTYPE_F32)
+    return __builtin_fmaf(__uint_as_float(w), 0.f, acc);
+  else if constexpr (DT == IR_DTYPE_BF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0u), acc, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0u), acc, false);
+}
+
+// The bits of a dword's elements that are no finite numbers.
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (DT == IR_DTYPE_F32) return (w & 0x7f800000u) == 0x7f800000u ? ~0u : 0u;
+  const uint32_t t = (w & 0x7fff7fffu) + (DT == IR_DTYPE_BF16 ? 0x00800080u : 0x04000400u);
+  return (t >> 15 & 0x00010001u) * 0xffffu;
+}
+
 // (a, b) as three pieces of bf16 that add up to them exactly: eight bits of the 24 each, by
 // truncation, so that the largest numbers do not become infinite.
 struct Pieces3 {

@@ -327,10 +327,10 @@ __device__ __forceinline__ uint32_t load_tile(const DecodeArgs& a, const int32_t
 // kmask: which of this lane's keys 4r+g are usable; a tile whose keys are
 // all usable in every lane takes the unmasked path. col_on: whether this
 // lane's query column attends the tile at all (a unit shared by two sequences
-// runs each one's private tiles with the other's columns off). An off column
-// gets -inf scores, so zero probabilities; the V rows stay, since a lane's V
-// operand serves every column of the PV product.
-template <int DT, int D>
+// runs each one's private tiles with the other's columns off; PAIRS: there are
+// such units). An off column gets -inf scores, so zero probabilities; the V rows
+// stay, since a lane's V operand serves every column of the PV product.
+template <int DT, int D, bool PAIRS = false>
 __device__ __forceinline__ void compute_tile(const Tile<DT, D>& tl, const uint32_t (&qr)[TileShape<DT, D>::KDW],
                                              uint32_t kmask, float scale_log2, uint8_t* kst, int lane, State<D>& st,
                                              bool col_on = true) {
@@ -345,14 +345,14 @@ __device__ __forceinline__ void compute_tile(const Tile<DT, D>& tl, const uint32
       vok[r] = true;
       sv[r] = col_on ? s[r] * scale_log2 : kNegInf;
     }
-    softmax_pv<DT, D, true>(sv, tl.v, vok, st);
+    softmax_pv<DT, D, true, false, PAIRS>(sv, tl.v, vok, st, col_on);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       vok[r] = (kmask >> r) & 1u;
       sv[r] = vok[r] && col_on ? s[r] * scale_log2 : kNegInf;
     }
-    softmax_pv<DT, D, false>(sv, tl.v, vok, st);
+    softmax_pv<DT, D, false, false, PAIRS>(sv, tl.v, vok, st, col_on);
   }
 }
 
@@ -365,8 +365,12 @@ __device__ __forceinline__ void compute_tile(const Tile<DT, D>& tl, const uint32
 // QF: a 16-bit pool's query is fp32 and held in two pieces of the dtype, its rounded value and
 // that of what it leaves, off by 2^-18 of an element (f16: 2^-24, or 2^-39 of the row's
 // largest where the pieces are subnormal) instead of 2^-9 (2^-12).
-template <int DT, int D, bool QF>
-__device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const QueryRegs<DT, D, QF>& q, uint32_t kmask,
+//
+// PAIRS: a V code of NaN in a tile that some column does not attend (whose probability of 0 is no answer
+// to it) becomes 0, and its channel NaN in the columns that attend it, which a product of zeros and ones
+// finds. Codes have no infinities, and a scale makes none.
+template <int DT, int D, bool QF, bool PAIRS = false>
+__device__ __forceinline__ void compute_codes(CodeTile<D>& tl, const QueryRegs<DT, D, QF>& q, uint32_t kmask,
                                               float scale_log2, float k_scale, float v_scale, uint8_t* kst, int lane,
                                               State<D>& st, bool col_on = true) {
   typedef TileShape<DT, D> Sh;
@@ -405,6 +409,35 @@ __device__ __forceinline__ void compute_codes(const CodeTile<D>& tl, const Query
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   f32x4 s = qk_tile<DT, D>(kop, q.x);
   if constexpr (QF) s += qk_tile<DT, D>(kop, q.rest);
+  if constexpr (PAIRS) {
+    if (!__all(col_on)) {
+      // bit 7 of the bytes that are NaN (of rows that may not be used too: softmax_pv masks those)
+      auto nan_of = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
+      uint32_t any = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < CodeTile<D>::NI; ++i) any |= nan_of(tl.v[r][i]);
+      if (__any(any != 0)) {
+        constexpr int KT = Sh::k16 ? DT : IR_DTYPE_BF16;
+        const uint32_t one = Elem<KT>::pack2(1.f, 0.f), p = col_on ? one | one << 16 : 0u;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          auto flag = [&](int r) {
+            return (kmask >> r) & (nan_of(tl.v[r][n / 4]) >> (8 * (n % 4) + 7)) & 1u ? one : 0u;
+          };
+          const f32x4 hit = mfma_k16<KT>(u32x2{flag(0) | flag(1) << 16, flag(2) | flag(3) << 16}, u32x2{p, p},
+                                         f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.acc[n][i] = hit[i] > 0.f ? __builtin_nanf("") : st.acc[n][i];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < CodeTile<D>::NI; ++i) tl.v[r][i] &= ~((nan_of(tl.v[r][i]) >> 7) * 255u);
+      }
+    }
+  }
   uint32_t v[4][Sh::VDW];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -662,7 +695,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeArgs& a, const int32_t*
     const int last = my_tiles - 1;
     Raw ring[DEPTH];
     uint32_t mk[DEPTH];
-    auto compute = [&](const Raw& tl, int i, uint32_t mask) {
+    auto compute = [&](Raw& tl, int i, uint32_t mask) {
       if constexpr (FMT == kCodes8) {
         const int ii = min(i, last);
         const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[0]), ii));

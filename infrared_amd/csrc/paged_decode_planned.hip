@@ -435,7 +435,7 @@ __global__ __launch_bounds__(plan_waves(FMT) * 64) void paged_decode_plan_kernel
       const int kvh = p.n_hg == 1 ? j : fdiv(j, p.n_hg);
       // which sequence's keys the tile holds, and which column halves see it
       int sq = b, tok0 = ti * 16;
-      uint32_t cm = FMT == kCodes4 ? 3u : 1u;  // (4 bits: a unit of one sequence has no other half)
+      uint32_t cm = 3u;  // (a unit of one sequence has no other half)
       if (s_lead[b] > 0) {
         const int S = s_share[b], ta = tiles0(b);
         cm = ti < S ? 3u : 1u;
@@ -838,9 +838,9 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
         if constexpr (FMT == kCodes8) {
           const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[0]), i));
           const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sc[1]), i));
-          compute_codes<DT, D, QF>(ring[r], qr, mk[r], a.scale_log2, ks, vs, kstage[w], lane, st, con[r]);
+          compute_codes<DT, D, QF, PAIRS>(ring[r], qr, mk[r], a.scale_log2, ks, vs, kstage[w], lane, st, con[r]);
         } else {
-          compute_tile<DT, D>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
+          compute_tile<DT, D, PAIRS>(ring[r], qr.x, mk[r], a.scale_log2, kstage[w], lane, st, con[r]);
         }
       };
 #pragma unroll

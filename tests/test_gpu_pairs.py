@@ -282,3 +282,13 @@ def test_pairs_over_4_bits_keep_a_number_that_is_none_to_its_own_sequence(dtype,
     """NaN or an infinity behind the shared prefix spoils the sequence that attends it, as alone: the
     other's output is the same bits as without it."""
     _check_spoilt_pair(_spoilt_pair(4, dtype, d, hq, h, fp32_queries), hq, h, [float("nan"), float("inf")])
+
+
+@pytest.mark.parametrize("kind, dtype, fp32_queries", [
+    (8, torch.bfloat16, False), (8, torch.float16, True), (8, torch.float32, False),
+    (16, torch.bfloat16, False), (16, torch.float16, False), (16, torch.float32, False),
+])
+@pytest.mark.parametrize("hq, h, d", [(28, 4, 128), (14, 2, 64), (2, 2, 128)])
+def test_pairs_keep_a_number_that_is_none_to_its_own_sequence(kind, dtype, fp32_queries, hq, h, d):
+    """The same over elements of the dtype and over 8-bit codes, where it spoils its own channel alone."""
+    _check_spoilt_pair(_spoilt_pair(kind, dtype, d, hq, h, fp32_queries), hq, h, [float("nan"), float("inf")])
