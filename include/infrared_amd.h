@@ -716,8 +716,7 @@ int ir_paged_prefill_q8(const void* q, int64_t q_tok_stride, int64_t q_head_stri
  * pool above; every value the pool holds is exactly a number of it.
  *
  * ir_kv_scatter_q4: ir_kv_scatter into such a layer (slots alike; of rows given the same
- * slot the last is written in calls of up to 1,024 tokens, in longer ones they must be
- * identical). A group's scale is the least 2^k with
+ * slot the last is written). A group's scale is the least 2^k with
  * amax <= 7 * 2^k, k in [-100, 125] (f16: [-23, 13]): 7 is where the largest magnitude would
  * round past 6, so that each value is off by half a step of the codes at most. Codes are
  * rounded to nearest even; magnitudes past 6 * 2^125 (f16: 49152) saturate; a group that

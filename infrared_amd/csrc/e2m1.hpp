@@ -52,9 +52,9 @@ struct Tile4 {
 
 // A line of a tile holds 8 tokens' K or all of its V's channels, some lanes of each, and workgroup i
 // runs on XCD i % 8: the order of workgroups in which four that follow one another (of a few tokens
-// each) meet in one XCD's L2, of a grid rounded up to whole runs of 32. (65,536 tokens of 4 heads of
-// 128, bf16: the write 46.5 -> 27.0 us, 6.4 TB/s, reading them 40.7 -> 26.1; 8,192: 6.7 -> 5.2 and
-// 4.8 -> 4.4. Slots in no order: the same either way.)
+// each) meet in one XCD's L2, of a grid rounded up to whole runs of 32. (Reading 65,536 tokens of 4 heads
+// of 128, bf16: 40.7 -> 26.1 us; 8,192: 4.8 -> 4.4; a write of 1,024: 4.1 -> 3.9. Slots in no order: the
+// same either way.)
 __device__ __forceinline__ uint32_t near_block(uint32_t i) { return (i & ~31u) | (i & 7) << 2 | (i >> 3 & 3); }
 inline int64_t near_blocks(int64_t blocks) { return (blocks + 31) & ~(int64_t)31; }
 

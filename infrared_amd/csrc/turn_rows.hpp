@@ -9,6 +9,8 @@
 // the launch and two trips).
 #pragma once
 
+#include <algorithm>
+
 #include "e2m1.hpp"
 #include "norm_rope.hpp"
 
@@ -18,10 +20,14 @@ enum { kAnglesNone = 0, kAnglesTables = 1, kAnglesPositions = 2 };
 enum { kToRows = 0, kToCache = 1, kToCodes4 = 2 };  // where keys go; values go with them, or nowhere
 
 constexpr int kMaxPairs = 128;  // of a head
-// Tokens of a call up to which a slot may be given twice: a decode step's, whose padding
-// repeats a row (all slots are read by each token's wavefronts, with its own).
-constexpr int kLastWins = 1024;
-constexpr int kTurnWaves = 4;
+constexpr int kTurnWaves = 4;  // of a workgroup, a token each
+// Of rows given the same slot of a 4-bit pool the last is written (a mixture of two would have one's codes
+// at the other's scales). In a launch of up to kWaveScan tokens each wavefront reads the slots behind its
+// own (1,024 tokens of 4 heads of 128: 0.7 us of 3.7); in a longer one a workgroup, of kScanWaves, reads those
+// behind all its tokens' (find_later; 4,096 tokens: 0.9 us of 5.1, 8,192: 1.6 of 7.3). That is n^2 / 4 bytes in
+// all, so a call of more than kScanTokens is several launches, in order (65,536 tokens in bf16: 60 us, 66 in
+// launches of 8,192 and 67 of 32,768).
+constexpr int kWaveScan = 1024, kScanWaves = 16, kScanTokens = 16384;
 
 struct TurnArgs {
   RowArgs r;
@@ -41,7 +47,8 @@ struct TurnArgs {
   int64_t c_slot, c_head;
   uint8_t* scales;
   int64_t num_slots;
-  int chunk_rows;  // rows of a wavefront
+  int64_t tok0, tok_end;  // the launch's tokens
+  int chunk_rows;         // rows of a wavefront
   int32_t* err;
 };
 
@@ -64,39 +71,87 @@ __device__ __forceinline__ void angles_of(const TurnArgs& a, int64_t tok, int la
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// D 0: a.head_dim (rows without norms only).
-template <int DT, int D, int MODE, int ANG, int DST>
-__global__ __launch_bounds__(kTurnWaves * 64) void turn_rows_kernel(TurnArgs a) {
+// Which of the first kScanWaves of n slots, the workgroup's tokens', come again later, a bit each (every thread
+// of the workgroup calls). A map of the slots' low bits tells most of the others apart.
+__device__ __forceinline__ uint32_t find_later(const int64_t* slots, int n) {
+  constexpr int NW = kScanWaves, NT = NW * 64, AHEAD = 4, BITS = 8192;
+  static_assert(NW * NW <= NT && BITS / 32 <= NT, "a thread for each pair of tokens and each word of the map");
+  __shared__ uint32_t s_map[BITS / 32], s_own[NW], s_later;
+  const int tid = threadIdx.x;
+  auto key = [](int64_t slot) { return (uint64_t)slot >> 32 ? ~0u : (uint32_t)slot; };  // (a pool's are below 2^31)
+  int64_t x[AHEAD];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = slots[min(j0 + tid + NT * i, n - 1)];
+  };
+  const uint32_t own = key(slots[min(tid, n - 1)]);
+  load(NW);
+  if (tid < BITS / 32) s_map[tid] = 0;
+  if (tid == 0) s_later = 0;
+  __syncthreads();
+  if (tid < NW) {
+    s_own[tid] = own;
+    atomicOr(&s_map[own % BITS / 32], 1u << (own % 32));
+  }
+  __syncthreads();
+  if (tid < NW * NW) {
+    const int k = tid % NW, m = tid / NW;
+    if (k < m && m < n && s_own[k] == s_own[m]) atomicOr(&s_later, 1u << k);
+  }
+  for (int j0 = NW; j0 < n; j0 += NT * AHEAD) {
+    if (j0 > NW) load(j0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (j0 + NT * i >= n) break;
+      const uint32_t y = key(x[i]);
+      if (s_map[y % BITS / 32] >> (y % 32) & 1u) {
+        uint32_t later = 0;
+        for (int k = 0; k < NW; ++k) later |= s_own[k] == y ? 1u << k : 0u;
+        if (later) atomicOr(&s_later, later);
+      }
+    }
+  }
+  __syncthreads();
+  return s_later;
+}
+
+// D 0: a.head_dim (rows without norms only). NW wavefronts, a token each.
+template <int DT, int D, int MODE, int ANG, int DST, int NW>
+__global__ __launch_bounds__(NW * 64) void turn_rows_kernel(TurnArgs a) {
   typedef Chunk8<DT> C;
   static_assert(D != 0 || (MODE == kRowsTurn && DST == kToRows), "the head's width is known for norms and pools");
-  __shared__ __attribute__((aligned(16))) float s_cs[ANG == kAnglesPositions ? kTurnWaves : 1][2 * kMaxPairs];
+  __shared__ __attribute__((aligned(16))) float s_cs[ANG == kAnglesPositions ? NW : 1][2 * kMaxPairs];
   const int hd = D ? D : a.head_dim, lpr = hd / 16, half = hd / 2 * C::EB;
   const int G = 64 / lpr;  // rows of a wavefront at a time
   const int lane = threadIdx.x & 63, grp = lane / lpr, ci = lane - grp * lpr;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t block = DST == kToCodes4 && gridDim.y == 1 ? near_block(blockIdx.x) : blockIdx.x;
-  const int64_t tok = (int64_t)block * kTurnWaves + w;
-  if (tok >= a.r.n_tokens) return;
+  constexpr bool SCAN = NW == kScanWaves;
+  static_assert(!SCAN || DST == kToCodes4, "only a 4-bit pool's writes need it");
+  const uint32_t block = DST == kToCodes4 && !SCAN && gridDim.y == 1 ? near_block(blockIdx.x) : blockIdx.x;
+  const int64_t tok = a.tok0 + (int64_t)block * NW + w;
   const int nq = MODE == kRowsPlain ? 0 : a.r.num_q_heads, nkv = a.r.num_kv_heads;
   const int rows = nq + (DST == kToRows ? nkv : 2 * nkv);
   const int row0 = blockIdx.y * a.chunk_rows;
   const int row_end = min(rows, row0 + a.chunk_rows);
-  int64_t slot = 0;
   bool kv_ok = true;
+  if constexpr (SCAN) {
+    if (row_end > nq) kv_ok = !(find_later(a.r.slots + tok - w, (int)(a.tok_end - tok) + w) >> w & 1u);
+  }
+  if (tok >= a.tok_end) return;
+  int64_t slot = 0;
   if constexpr (DST != kToRows) {
     slot = a.r.slots[tok];
-    kv_ok = slot >= 0 && slot < a.num_slots;
+    kv_ok = kv_ok && slot >= 0 && slot < a.num_slots;
     if (slot >= a.num_slots && lane == 0 && row0 == 0) flag_error(a.err, IR_ERR_SLOT_RANGE);
   }
-  if constexpr (DST == kToCodes4) {
-    // of rows given the same slot the last is written: a mixture of two would have one's
-    // codes at the other's scales (1,024 tokens of 4 heads of 128: 0.7 us of 3.7)
-    if (a.r.n_tokens <= kLastWins && row_end > nq) {
-      const int n = (int)a.r.n_tokens;
+  if constexpr (DST == kToCodes4 && !SCAN) {
+    if (row_end > nq) {
+      const int64_t* slots = a.r.slots + a.tok0;
+      const int n = (int)(a.tok_end - a.tok0);
       bool later = false;
-      for (int j = (int)tok + 1 + lane; j < n; j += 256) {
+      for (int j = (int)(tok - a.tok0) + 1 + lane; j < n; j += 256) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) later |= a.r.slots[min(j + 64 * i, n - 1)] == slot;
+        for (int i = 0; i < 4; ++i) later |= slots[min(j + 64 * i, n - 1)] == slot;
       }
       if (__any(later)) kv_ok = false;
     }
@@ -196,6 +251,14 @@ __global__ __launch_bounds__(kTurnWaves * 64) void turn_rows_kernel(TurnArgs a) 
 // decode step's few tokens are a single pass (qk_norm_rope.hip has both measured).
 constexpr int64_t kTurnTokensForDevice = 2048;
 
+template <int DT, int D, int MODE, int ANG, int DST, int NW>
+void launch_tokens(const TurnArgs& a, int runs, hipStream_t s) {
+  int64_t blocks = (a.tok_end - a.tok0 + NW - 1) / NW;
+  if (DST == kToCodes4 && NW == kTurnWaves && runs == 1) blocks = near_blocks(blocks);
+  hipLaunchKernelGGL((turn_rows_kernel<DT, D, MODE, ANG, DST, NW>), dim3((unsigned)blocks, runs), dim3(NW * 64), 0, s,
+                     a);
+}
+
 template <int DT, int D, int MODE, int ANG, int DST>
 int launch_turn(const char* name, TurnArgs a, hipStream_t s) {
   const int rows = a.r.num_q_heads + (DST == kToRows ? 1 : 2) * a.r.num_kv_heads;
@@ -205,10 +268,14 @@ int launch_turn(const char* name, TurnArgs a, hipStream_t s) {
   a.chunk_rows = runs == 1 ? rows : g;
   IR_REQUIRE(a.r.n_tokens <= 0x7fffffff, "%s: too many tokens", name);
   IR_REQUIRE(runs <= 65535, "%s: too many heads", name);
-  int64_t blocks = (a.r.n_tokens + kTurnWaves - 1) / kTurnWaves;
-  if (DST == kToCodes4 && runs == 1) blocks = near_blocks(blocks);
-  const dim3 grid((unsigned)blocks, runs);
-  hipLaunchKernelGGL((turn_rows_kernel<DT, D, MODE, ANG, DST>), grid, dim3(kTurnWaves * 64), 0, s, a);
+  const int64_t step = DST == kToCodes4 ? kScanTokens : a.r.n_tokens;
+  for (a.tok0 = 0; a.tok0 < a.r.n_tokens; a.tok0 = a.tok_end) {
+    a.tok_end = std::min(a.tok0 + step, a.r.n_tokens);
+    if (DST == kToCodes4 && a.tok_end - a.tok0 > kWaveScan)
+      launch_tokens<DT, D, MODE, ANG, DST, DST == kToCodes4 ? kScanWaves : kTurnWaves>(a, runs, s);
+    else
+      launch_tokens<DT, D, MODE, ANG, DST, kTurnWaves>(a, runs, s);
+  }
   return check_launch(name);
 }
 

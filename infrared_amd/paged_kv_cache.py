@@ -444,7 +444,7 @@ class Quant4PagedKVPool(QuantPagedKVPool):
     magnitude is at most 7, every value is rounded to the nearest code, the largest to 6, and
     a group with a NaN or an infinity becomes NaN. A token's scales are its own, so a
     write changes nothing but its slots, whatever else is in their blocks. Of equal slots the
-    last is written in calls of up to 1,024 tokens; in longer ones their rows must be equal.
+    last is written.
     """
 
     bits = 4

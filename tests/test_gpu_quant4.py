@@ -12,6 +12,7 @@ from infrared_amd import (
     PagedKVPool,
     Quant4PagedKVPool,
     QuantPagedKVPool,
+    RotaryAxes,
     kernels,
     metadata,
     paged_attention,
@@ -1110,3 +1111,47 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="kv_scales"):
         kernels.paged_gather_q4(pool.k[0], pool.v[0], scales[:, :2], *args[:2], bs, 4, torch.bfloat16)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n, spread", [(1025, 300), (1025, 1025), (2048, 1), (5000, 4000), (8193, 8000), (20001, 9000)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_last_of_equal_slots_is_written_in_calls_of_any_length(n, spread, d):
+    """Rows that differ, their slots up to a whole call apart; skipped ones and one out of range between
+    them. Plain, rotated, normed and turned by axes."""
+    h, bs, dtype = 2, 16, torch.bfloat16
+    g = gen(n + d)
+    q, k, v = rows(g, n, 2 * h, d, dtype), rows(g, n, h, d, dtype, 3.0), rows(g, n, h, d, dtype, 3.0)
+    slots = torch.randint(0, spread, (n,), generator=g, device=DEV)
+    slots[n // 3], slots[n // 2] = -1, 2**31 + int(slots[5])
+    slots[n - 1] = slots[0]
+    blocks = spread // bs + 2
+    valid = slots.clone()
+    valid[valid >= blocks * bs] = -1
+    last = {s: i for i, s in enumerate(valid.tolist()) if s >= 0}
+    at = torch.tensor(sorted(last.values()), device=DEV)
+    pool, want = (Quant4PagedKVPool(1, blocks, bs, h, d, dtype) for _ in range(2))
+    held_values = quant4.Quant4Cache(blocks * bs, h, d, dtype)
+    pool.write(0, k, v, slots)
+    with pytest.raises(IndexError, match="write slot"):
+        pool.check_errors()
+    held_values.write(k[at], v[at], slots[at])
+    assert same(held(pool), held_values.values)
+    cos, sin = rotation(g, n, d)
+    w = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+    rotary = RotaryAxes.sections(d, (d // 4, d // 4))
+    pos = torch.randint(0, 9999, (2, n), generator=g, device=DEV)
+    for norms in ((), (w[0], w[1], 1e-6)):
+        for axes in (False, True):
+            out = []
+            for p, i in ((pool, slice(None)), (want, at)):
+                p.k.zero_(), p.v.zero_(), p.kv_scales.fill_(27)
+                layer = (p.k[0], p.v[0])
+                if axes:
+                    out.append(kernels.rope_axes_kv_scatter(q[i], k[i], v[i], pos[:, i], rotary, *layer, slots[i], *norms,
+                                                            kv_scales=p.kv_scales[0], block_size=bs))
+                else:
+                    out.append(kernels.rope_kv_scatter_q4(q[i], k[i], v[i], cos[i], sin[i], *layer, p.kv_scales[0],
+                                                          slots[i], bs, *norms))
+            case = (bool(norms), axes)
+            assert torch.equal(pool.k, want.k) and torch.equal(pool.v, want.v), case
+            assert torch.equal(pool.kv_scales, want.kv_scales) and torch.equal(out[0][at], out[1]), case
