@@ -51,8 +51,8 @@ int dtype_code(const Tensor& t) {
   }
 }
 
-void unit_last(const char* name, const Tensor& t) {
-  require(t.dim() > 0 && t.stride(-1) == 1, name, ": the last (head_dim) dimension must be contiguous");
+void unit_last(const char* name, const Tensor& t, const char* which = "") {
+  require(t.dim() > 0 && t.stride(-1) == 1, name, which, ": the last (head_dim) dimension must be contiguous");
 }
 
 void cache_layer(const char* name, const Tensor& c) {
@@ -397,8 +397,8 @@ void kv_scatter_codes(const char* name, bool four, const Tensor& kc, const Tenso
   const int64_t n = k.size(0);
   require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name,
           ": slots must be int64 [", n, "], got ", slots.scalar_type(), " ", slots.sizes());
-  unit_last(name, k);
-  unit_last(name, v);
+  unit_last(name, k, " k");
+  unit_last(name, v, " v");
   const Tensor s = slots.contiguous();
   if (four) {
     check(ir_kv_scatter_q4(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
@@ -518,9 +518,9 @@ Tensor norm_rope_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
   require(cos.stride(0) == sin.stride(0), name, ": cos and sin must share strides");
   require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name,
           ": slots must be int64 [N]");
-  unit_last(name, q);
-  unit_last(name, k);
-  unit_last(name, v);
+  unit_last(name, q, " q");
+  unit_last(name, k, " k");
+  unit_last(name, v, " v");
   if (q_out_) {
     given_out(name, *q_out_, q, Wide::kOut);
     require(scales || q_out_->scalar_type() == q.scalar_type(), name, ": q_out must be of ", q.scalar_type());
@@ -581,8 +581,8 @@ Tensor check_axes(const char* name, const Tensor& q, const Tensor& k, const OptT
       require(t->dim() == 1 && t->size(0) == d && t->is_contiguous() && t->scalar_type() == q.scalar_type(), name, ": ",
               which, " must be contiguous [", d, "] of ", q.scalar_type());
   }
-  unit_last(name, q);
-  unit_last(name, k);
+  unit_last(name, q, " q");
+  unit_last(name, k, " k");
   return positions.size(1) <= 1 || positions.stride(1) == 1 ? positions : positions.contiguous();
 }
 
@@ -631,7 +631,7 @@ Tensor rope_axes_kv_scatter(const Tensor& q, const Tensor& k, const Tensor& v, c
           ": k_cache and v_cache must share shape, strides and dtype");
   require(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == n, name,
           ": slots must be int64 [", n, "], got ", slots.scalar_type(), " ", slots.sizes());
-  unit_last(name, v);
+  unit_last(name, v, " v");
   if (q_out_) given_out(name, *q_out_, q, Wide::kOut);
   const Tensor qo = q_out_ ? *q_out_ : at::empty(q.sizes(), q.options());
   const Tensor s = slots.contiguous();

@@ -1155,3 +1155,30 @@ def test_the_last_of_equal_slots_is_written_in_calls_of_any_length(n, spread, d)
             case = (bool(norms), axes)
             assert torch.equal(pool.k, want.k) and torch.equal(pool.v, want.v), case
             assert torch.equal(pool.kv_scales, want.kv_scales) and torch.equal(out[0][at], out[1]), case
+
+
+def test_refusals_name_the_rows_that_are_not_contiguous():
+    n, h, d, bs = 3, 2, 64, 16
+    even = torch.zeros(n, h, d, dtype=torch.bfloat16, device=DEV)
+    odd = torch.zeros(n, h, 2 * d, dtype=torch.bfloat16, device=DEV)[:, :, ::2]
+    slots, cs = torch.arange(n, device=DEV), torch.zeros(n, d, device=DEV)
+    rotary, pos = RotaryAxes.sections(d, (d // 2,)), torch.arange(n, device=DEV)
+    four, eight = (p(1, 2, bs, h, d, torch.bfloat16) for p in (Quant4PagedKVPool, QuantPagedKVPool))
+    layers = [(p.k[0], p.v[0], p.kv_scales[0]) for p in (four, eight)]
+    for which in range(3):
+        q, k, v = (odd if i == which else even for i in range(3))
+        bad = f" {'qkv'[which]}: the last"
+        for layer, write, rope in zip(layers, (kernels.kv_scatter_q4, kernels.kv_scatter_q8),
+                                      (kernels.rope_kv_scatter_q4, kernels.rope_kv_scatter_q8)):
+            if which:
+                with pytest.raises(RuntimeError, match=write.__name__ + bad):
+                    write(*layer, k, v, slots, bs)
+            with pytest.raises(RuntimeError, match=rope.__name__ + bad):
+                rope(q, k, v, cs, cs, *layer, slots, bs)
+        with pytest.raises(RuntimeError, match="rope_axes_kv_scatter" + bad):
+            kernels.rope_axes_kv_scatter(q, k, v, pos, rotary, *layers[0][:2], slots, kv_scales=layers[0][2],
+                                         block_size=bs)
+        if which < 2:
+            with pytest.raises(RuntimeError, match="rope_axes" + bad):
+                kernels.rope_axes(q, k, pos, rotary)
+    assert not four.k.any() and not eight.k.view(torch.uint8).any()
