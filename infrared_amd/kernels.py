@@ -373,8 +373,8 @@ def decode_plan_pays(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_blo
     11.6 us; but 8 fp32 sequences of <= 512 keys 7.1 vs 10.5 us and 16 of <= 300
     keys in tables of that width 7.9 vs 11.0 us.
 
-    ``bits=4``: the pool's, whose keys are so few bytes that tables of up to 1,024 keys
-    are never planned (64 sequences of 1..512 keys 7.0 vs 12.2 us, of 1..1024 10.3 vs
+    ``bits``: the pool's (``pool.bits``). The keys of a 4-bit one are so few bytes that
+    tables of up to 1,024 keys are never planned (64 sequences of 1..512 keys 7.0 vs 12.2 us, of 1..1024 10.3 vs
     15.3; 512 of them 40.5 vs 42.0; of 1..2048 keys 64 sequences 16.2 vs 17.2, 128 27.5
     vs 24.0)."""
     if bits == 4 and max_blocks * block_size <= 1024:

@@ -132,6 +132,11 @@ class PagedKVPool:
         self._verdict_np = None
         self._verdict_tag = 0
 
+    @property
+    def bits(self) -> int:
+        """Width of what the pool holds (``kernels.decode_plan_pays`` goes by it)."""
+        return 8 * self.dtype.itemsize
+
     # --- reference surface ------------------------------------------------
 
     def write(

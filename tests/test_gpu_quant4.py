@@ -1182,3 +1182,20 @@ def test_refusals_name_the_rows_that_are_not_contiguous():
             with pytest.raises(RuntimeError, match="rope_axes" + bad):
                 kernels.rope_axes(q, k, pos, rotary)
     assert not four.k.any() and not eight.k.view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("pool_type, dtype, bits", [
+    (PagedKVPool, torch.bfloat16, 16), (PagedKVPool, torch.float32, 32),
+    (QuantPagedKVPool, torch.bfloat16, 8), (Quant4PagedKVPool, torch.bfloat16, 4),
+])
+@pytest.mark.parametrize("seqs, keys", [(64, 304), (64, 1024), (64, 1040), (8, 1024), (3, 9008)])
+def test_the_seam_plans_what_pays_over_a_pool_of_its_bits(pool_type, dtype, bits, seqs, keys):
+    hq, h, d, bs = 14, 2, 64, 16
+    width = keys // bs
+    pool = pool_type(1, width, bs, h, d, dtype)
+    assert pool.bits == bits
+    paged, mask = metadata.decode_context(pool, [list(range(width))] * seqs, [keys - 1] * seqs)
+    q, k, v, _, _ = step_inputs(gen(seqs), seqs, 1, hq, h, d, dtype)
+    paged_attention(q, k, v, paged, mask, 0, d**-0.5, hq // h)
+    assert paged.block_tables.shape[1] == width
+    assert (paged.decode_plan is not None) == kernels.decode_plan_pays(seqs, hq, h, width, bs, DEV, pool.bits)
