@@ -281,7 +281,7 @@ def prepare(case, seed):
         # what a step shares over its layers: the work plan, the workspace
         if kind == "decode":
             s["counters"] = pool.decode_counters(kernels.decode_num_counters(nseq, hq, hkv))
-            if kernels.decode_plan_pays(nseq, hq, hkv, width, bs, "cuda"):
+            if kernels.decode_plan_pays(nseq, hq, hkv, width, bs, "cuda", pool.bits):
                 s["plan"] = kernels.decode_plan(s["bt"], s["ctx"], hq, pool.k[0], bs)
                 s["work"] = pool.workspace(kernels.planned_workspace_bytes(nseq, hq, hkv, d))
             else:
