@@ -16,6 +16,7 @@ from infrared_amd import (
     kernels,
     metadata,
     paged_attention,
+    rope_axes_paged_attention,
     rope_paged_attention,
 )
 from infrared_amd.hip_graph import HipGraphDecoder, build_decode_static_inputs
@@ -34,6 +35,8 @@ from test_gpu_quant import (
     same,
     step_inputs,
 )
+from test_gpu_rope_axes import positions
+from test_gpu_rope_axes import tolerance as turn_tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -1199,3 +1202,48 @@ def test_the_seam_plans_what_pays_over_a_pool_of_its_bits(pool_type, dtype, bits
     paged_attention(q, k, v, paged, mask, 0, d**-0.5, hq // h)
     assert paged.block_tables.shape[1] == width
     assert (paged.decode_plan is not None) == kernels.decode_plan_pays(seqs, hq, h, width, bs, DEV, pool.bits)
+
+
+# The queries that a step attends with are fp32 ones, off by turn_tolerance from the 64-bit rotation's: a
+# score by delta = scale sum |that| |k|, an output by (e^(2 delta) - 1) a, delta < 0.01: 2.1 delta a. Their two
+# pieces of the dtype leave 2^-18 of an element at most, which comes in the same way.
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_step_turned_by_axes_over_the_4_bit_pool_is_attention_in_64_bits(dtype, normed):
+    """Prompt chunks, then single tokens, of sequences two of which begin alike, through the seam."""
+    hq, h, d, bs, scale = 14, 2, 64, 16, 0.125
+    g = gen(50)
+    rotary = RotaryAxes.sections(d, (8, 12, 12), scaling=0.9)
+    pool = Quant4PagedKVPool(1, 40, bs, h, d, dtype)
+    tables = [[20, 3, 7, 30, 31, 32], [20, 3, 8, 33, 34, 35], [1, 2, 36], [9, 10, 11]]
+    w = (1 + 0.3 * torch.randn(2, d, generator=g, device=DEV)).to(dtype)
+    norms = {"q_norm": w[0], "k_norm": w[1], "eps": 1e-5} if normed else {}
+    cached = [0, 32, 0, 0]
+    for new in ([70, 41, 1, 20], [1, 1, 30, 9], [1, 1, 1, 1], [1, 1, 1, 1]):
+        total, decode = sum(new), max(new) == 1
+        b, sq = (total, 1) if decode else (1, total)
+        q, k, v = rows(g, total, hq + 2 * h, d, dtype, 0.7).view(b, sq, -1, d).split([hq, h, h], 2)
+        pos = positions(g, 3, total).view(3, b, sq)
+        paged, mask = (metadata.decode_context(pool, tables, cached) if decode
+                       else metadata.prefill_context(pool, tables, cached, new))
+        out = rope_axes_paged_attention(q, k, v, pos, rotary, paged, mask, 0, scale, hq // h, **norms)
+        assert out.dtype == dtype
+        pool.check_errors()
+        values = held(pool)
+        flat, weight, eps = q.reshape(-1, hq, d), (w[0] if normed else None), (1e-5 if normed else 0.0)
+        turned = quant4.turn(flat, pos.view(3, -1), rotary.inv_freq, rotary.axis_of, weight, eps, rotary.scaling)
+        off = turn_tolerance(flat, turned, torch.float32, weight, eps, rotary.scaling)
+        row = 0
+        for table, c, n in zip(tables, cached, new):
+            at = slice(row, row + n)
+            o, a, reach = quant.attend(turned[at], values, table, bs, c, scale)
+            delta = quant.attend(off[at], values, table, bs, c, scale)[2] + 2.0**-18 * reach
+            assert delta.max() < 0.01
+            tol = fp32_tolerance(o, a, reach, d) + 2.1 * delta[..., None] * a
+            tol = tol + small_probabilities(values, table, c + n, bs, hq, dtype)
+            if dtype != torch.float32:
+                tol = tol + (decode_tolerance(o, a, dtype) if decode else prefill_tolerance(o, a, reach, dtype))
+            err = (out.reshape(-1, hq, d)[at].double().cpu() - o).abs()
+            assert (err <= tol).all(), (new, c, (err / tol).max())
+            row += n
+        cached = [c + n for c, n in zip(cached, new)]
