@@ -24,10 +24,10 @@ constexpr int kTurnWaves = 4;  // of a workgroup, a token each
 // Of rows given the same slot of a 4-bit pool the last is written (a mixture of two would have one's codes
 // at the other's scales). In a launch of up to kWaveScan tokens each wavefront reads the slots behind its
 // own (1,024 tokens of 4 heads of 128: 0.7 us of 3.7); in a longer one a workgroup, of kScanWaves, reads those
-// behind all its tokens' (find_later; 4,096 tokens: 0.9 us of 5.1, 8,192: 1.6 of 7.3). That is n^2 / 4 bytes in
-// all, so a call of more than kScanTokens is several launches, in order (65,536 tokens in bf16: 60 us, 66 in
-// launches of 8,192 and 67 of 32,768).
-constexpr int kWaveScan = 1024, kScanWaves = 16, kScanTokens = 16384;
+// behind all its tokens' (find_later; 4,096 tokens: 0.9 us of 5.1, 8,192: 1.7 of 7.4; 2,048 take 4.7 us either
+// way, 1,216 4.1 and 4.5, 3,000 6.3 and 4.8). That is n^2 / 4 bytes in all, so a call of more than kScanTokens
+// is several launches, in order (65,536 tokens in bf16: 60 us, 66 in launches of 8,192 and 67 of 32,768).
+constexpr int kWaveScan = 2048, kScanWaves = 16, kScanTokens = 16384;
 
 struct TurnArgs {
   RowArgs r;
@@ -54,7 +54,8 @@ struct TurnArgs {
 
 // cos and sin of a token's pairs, one pair a lane, to the wavefront's LDS. position *
 // step modulo 2^64 is the angle as a fraction of a turn: the wrap-around is the reduction,
-// exact however far the position, and the signed upper half of it is half a turn at most.
+// exact however far the position, and the signed upper half of it (rounded: 2^-33 turns) is half
+// a turn at most, as an fp32 number off by 2^-24 of itself.
 __device__ __forceinline__ void angles_of(const TurnArgs& a, int64_t tok, int lane, int pairs, float* cs) {
   for (int j = lane; j < pairs; j += 64) {
     const u32x4 p = *(const u32x4*)(a.pairs + j);

@@ -1116,7 +1116,7 @@ def test_refusals():
     torch.cuda.synchronize()
 
 
-@pytest.mark.parametrize("n, spread", [(1025, 300), (1025, 1025), (2048, 1), (5000, 4000), (8193, 8000), (20001, 9000)])
+@pytest.mark.parametrize("n, spread", [(1025, 300), (1025, 1025), (2048, 1), (2049, 700), (5000, 4000), (8193, 8000), (20001, 9000)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_the_last_of_equal_slots_is_written_in_calls_of_any_length(n, spread, d):
     """Rows that differ, their slots up to a whole call apart; skipped ones and one out of range between
