@@ -798,7 +798,8 @@ int ir_paged_prefill_q4(const void* q, int64_t q_tok_stride, int64_t q_head_stri
  *              frequency in turns (radians / 2 pi) times 2^64, modulo 2^64; axis in
  *              [0, num_axes) (another is taken for the nearest of them). position * step
  *              modulo 2^64 is the angle as a fraction of a turn, off by at most
- *              |position| * 2^-65 turns however far the position.
+ *              |position| * 2^-65 turns however far the position; its upper 32 bits,
+ *              rounded, become the fp32 number that sine and cosine are taken of.
  *   num_axes:  1..IR_ROTARY_MAX_AXES.
  *   q_out_dtype: dtype, or IR_DTYPE_F32.
  *

@@ -13,8 +13,6 @@
 //               of column c, i.e. one lane owns 4*head_dim/16 consecutive d.
 #pragma once
 
-#include <type_traits>
-
 #include "common.hpp"
 
 namespace ir {

@@ -177,7 +177,9 @@ struct Pieces3 {
 };
 __device__ __forceinline__ Pieces3 split3(float a, float b) {
   auto top = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); };
-  auto pair = [](float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); };
+  auto pair = [](float x, float y) {
+    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+  };
   const float ra = a - top(a), rb = b - top(b);
   return {pair(a, b), pair(ra, rb), pair(ra - top(ra), rb - top(rb))};
 }

@@ -618,8 +618,9 @@ __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D
     typedef std::integral_constant<int, 1> R1;
     typedef std::integral_constant<int, 2> R2;
     typedef std::integral_constant<int, 3> R3;
-    const uint32_t v0 = value(ta, R0{}, dw), v1 = value(ta, R1{}, dw), v2 = value(ta, R2{}, dw), v3 = value(ta, R3{}, dw);
-    const uint32_t v4 = value(tb, R0{}, dw), v5 = value(tb, R1{}, dw), v6 = value(tb, R2{}, dw), v7 = value(tb, R3{}, dw);
+    const uint32_t v0 = value(ta, R0{}, dw), v1 = value(ta, R1{}, dw), v2 = value(ta, R2{}, dw);
+    const uint32_t v3 = value(ta, R3{}, dw), v4 = value(tb, R0{}, dw), v5 = value(tb, R1{}, dw);
+    const uint32_t v6 = value(tb, R2{}, dw), v7 = value(tb, R3{}, dw);
 #pragma unroll
     for (int odd = 0; odd < 2; ++odd) {
       const uint32_t sel = odd ? 0x07060302u : 0x05040100u;

@@ -194,14 +194,15 @@ constexpr int kLockstep = 0, kRing2 = 2;
 // kCodes8: the caches are codes with block scales (e4m3.hpp). A thread loads 16 codes of a
 // key's K and of its V with the key's scales, which turn into the dtype's elements,
 // exactly, where they are stored to LDS. kCodes4 (e2m1.hpp): 16 codes of a key's K and, as they
-// lie in a tile, 8 of two keys' V (4 of four at head_dim 64), likewise. CODES, either: The queries are used as they are given, in QP
-// pieces of the dtype: one for queries of it, so that a score is the sum of exact products in
-// fp32, two for fp32 queries (below), three for an fp32 pool of 4-bit codes, whose numbers are
-// bf16 ones all the same, exactly: DT is bf16 then, queries and probabilities are three pieces each,
-// exactly, and the output is fp32; three bf16 products take 3 / 16 of the time of the fp32 ones they
-// stand for (8 chunks of 512 tokens after up to 8192 cached, 28 / 4 heads of 128: 684 us, 2516 in fp32
-// products). scale * log2 e is multiplied with a score less the running maximum, in fp32, where its
-// exponential is taken.
+// lie in a tile, 8 of two keys' V (4 of four at head_dim 64), likewise.
+// CODES (either): the queries are used as they are given, in QP pieces of the dtype: one for queries
+// of it, so that a score is the sum of exact products in fp32, two for fp32 queries (below; 8 chunks of
+// 512 tokens after up to 8192 cached, 28 / 4 heads of 128, over 4 bits: 398 us, 314 with one), three for
+// an fp32 pool of 4-bit codes. Its numbers are bf16 ones all the same, exactly, so DT is bf16 there,
+// queries and probabilities are three pieces each, exactly, and the output is fp32: three bf16 products
+// take 3 / 16 of the time of the fp32 ones they stand for (the same chunks 684 us, 2516 in fp32 products).
+// scale * log2 e is multiplied with a score less the running maximum, in fp32, where its exponential is
+// taken.
 template <int DT, int D, bool FAST, int NW, int CTW, int SCHED, bool FUSED = false, int FMT = kElements, int QP = 1>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 8 || SCHED == kRing2 ? 2 : 1)))
 void paged_prefill_kernel(PrefillArgs a) {
@@ -415,7 +416,9 @@ void paged_prefill_kernel(PrefillArgs a) {
   struct Place {
     int gg, cc, half;
   };
-  auto k_place = [](int q) { return D == 128 ? Place{(q >> 1) & 3, (q % D) >> 3, q & 1} : Place{q & 3, (q % D) >> 2, 0}; };
+  auto k_place = [](int q) {
+    return D == 128 ? Place{(q >> 1) & 3, (q % D) >> 3, q & 1} : Place{q & 3, (q % D) >> 2, 0};
+  };
   auto v_place = [](int q) {
     return D == 128 ? Place{(q % D) >> 5, q & 15, (q >> 4) & 1} : Place{(q % D) >> 4, q & 15, 0};
   };
@@ -496,7 +499,8 @@ void paged_prefill_kernel(PrefillArgs a) {
         if constexpr (!C4) {
           kr[i] = *(const u32x4*)(kc + sl + part * PE);
           vr[i] = *(const u32x4*)(vc + sl + part * PE);
-          if constexpr (FMT == kCodes8) sc[i] = scales[block];  // (block 0's for an unusable key, whose codes become 0)
+          // (block 0's for an unusable key, whose codes become 0)
+          if constexpr (FMT == kCodes8) sc[i] = scales[block];
         }
         ku[i] = use;
       }

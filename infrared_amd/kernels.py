@@ -804,8 +804,8 @@ def paged_prefill(
                                + ("fp32" if plan.f32 else "16-bit") + f" calls, q is {q.dtype}")
     if kv_scales is not None:
         if new_kv is not None:
-            raise RuntimeError(f"paged_prefill: new_kv cannot be written to {'a 4' if kv_scales.dtype == CODES4 else 'an 8'}"
-                               "-bit cache by the same launch")
+            which = "a 4" if kv_scales.dtype == CODES4 else "an 8"
+            raise RuntimeError(f"paged_prefill: new_kv cannot be written to {which}-bit cache by the same launch")
         return seam().paged_prefill_q8(q, k_cache, v_cache, kv_scales, block_tables, cu_seqlens_q, q_start,
                                        int(max_q_len), block_size, scale, out, err_flags,
                                        None if plan is None else plan.buf, stream)

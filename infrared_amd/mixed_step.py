@@ -168,7 +168,8 @@ class MixedStep:
             for name in ("q_dec", "q_pre", "k_new", "v_new"):
                 dtype = getattr(inputs, name).dtype
                 if dtype != pool.dtype:
-                    raise RuntimeError(f"MixedStep: {name} is {dtype}, the {pool.bits}-bit pool's dtype is {pool.dtype}")
+                    raise RuntimeError(f"MixedStep: {name} is {dtype}, "
+                                       f"the {pool.bits}-bit pool's dtype is {pool.dtype}")
         self.fused = fused and not overlap and not self.quant
         dev = pool.device
         self.out_dec = torch.empty_like(inputs.q_dec)

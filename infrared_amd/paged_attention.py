@@ -212,7 +212,8 @@ def _check_quant(pool: QuantPagedKVPool, q: torch.Tensor, paged) -> None:
     if not tables or not (packed or (getattr(paged, "context_lens", None) is not None and q.shape[1] == 1)):
         raise RuntimeError(
             f"paged_attention: {'an 8' if pool.bits == 8 else 'a 4'}-bit pool is attended through block_tables, with "
-            "context_lens for a single-token decode or cu_seqlens_q and q_start for packed chunks (metadata.decode_context, prefill_context)"
+            "context_lens for a single-token decode or cu_seqlens_q and q_start for packed chunks "
+            "(metadata.decode_context, prefill_context)"
         )
 
 

@@ -385,7 +385,8 @@ class QuantPagedKVPool(PagedKVPool):
         dtype_code(dtype)
         a = "an" if cls.bits == 8 else "a"
         if block_size <= 0 or block_size % 16 or block_size > 1024:
-            raise ValueError(f"{a} {cls.bits}-bit pool's block size is a multiple of 16, at most 1024; got {block_size}")
+            raise ValueError(
+                f"{a} {cls.bits}-bit pool's block size is a multiple of 16, at most 1024; got {block_size}")
         if head_dim not in (64, 128):
             raise ValueError(f"{a} {cls.bits}-bit pool's head_dim is 64 or 128; got {head_dim}")
         if num_blocks * block_size >= 2**31:
@@ -473,8 +474,9 @@ class Quant4PagedKVPool(QuantPagedKVPool):
         self.dtype = dtype
         self._layers = None
         # (what was never written is 0 at the least scale)
-        self.kv_scales = torch.full((num_layers, num_kv_heads, self.num_slots // 16, head_dim),
-                                    127 - (23 if dtype == torch.float16 else 100), dtype=torch.uint8, device=self.device)
+        least = 127 - (23 if dtype == torch.float16 else 100)
+        self.kv_scales = torch.full((num_layers, num_kv_heads, self.num_slots // 16, head_dim), least,
+                                    dtype=torch.uint8, device=self.device)
 
     def write(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantises this step's K/V (``[N, num_kv_heads, head_dim]`` of ``dtype``) into ``slots``

@@ -53,7 +53,8 @@ class RotaryAxes:
         self.scaling = float(scaling)
         self.head_dim = 2 * len(self.inv_freq)
         if not self.inv_freq or len(self.axis_of) != len(self.inv_freq):
-            raise ValueError(f"{len(self.inv_freq)} frequencies and {len(self.axis_of)} axes: one of each a pair expected")
+            raise ValueError(
+                f"{len(self.inv_freq)} frequencies and {len(self.axis_of)} axes: one of each a pair expected")
         if self.head_dim % 16 or self.head_dim > 256:
             raise ValueError(f"heads of {self.head_dim}: a multiple of 16 up to 256 expected")
         if not all(math.isfinite(f) for f in (*self.inv_freq, self.scaling)):
