@@ -473,6 +473,8 @@ __device__ __forceinline__ void compute_codes(CodeTile<D>& tl, const QueryRegs<D
   }
 }
 
+constexpr float kFarScore = 0x1p20f;  // (half a step of it: 2^-4)
+
 // A pair of 4-bit tiles in registers.
 template <int D>
 struct Pair4 {
@@ -498,6 +500,11 @@ struct Pair4 {
 // The codes are dead once they are numbers, so the next pair's loads go into the same
 // registers: its K's as soon as the scores are there (next_k), its V's behind the products (next_v).
 //
+// far: whether a maximum has been past kFarScore, for the wavefront's next pairs too (false at first). The
+// multiply-add makes an exponent that is off from the rounded maximum by half a step of it, the same for
+// all keys: nothing where it cancels, but past 2^31 a power that overflows. Such scores are rounded
+// first, as the maximum is.
+//
 // valid_a, valid_b: the tiles' usable keys; col_a, col_b: whether the lane's column attends the tile;
 // whole: it is all of them. An absent key's scales become 0, what it holds finite.
 //
@@ -508,7 +515,7 @@ struct Pair4 {
 template <int DT, int D, bool QF, bool PAIRS, typename NextK, typename NextV>
 __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D, QF>& q, bool whole, int valid_a,
                                               int valid_b, bool col_a, bool col_b, float scale_log2, int lane,
-                                              State<D>& st, NextK next_k, NextV next_v) {
+                                              State<D>& st, bool& far, NextK next_k, NextV next_v) {
   constexpr bool WIDE = DT == IR_DTYPE_F32;
   static_assert(!WIDE || QF, "an fp32 pool's queries are fp32 ones in pieces");
   constexpr int KT = WIDE ? IR_DTYPE_BF16 : DT;  // the operands'
@@ -581,16 +588,25 @@ __device__ __forceinline__ void compute_pair4(Pair4<D>& x, const QueryRegs<DT, D
   }
   float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
   if (__any(mx * c > st.m + (kRescaleSlack + UP))) {
+#pragma clang fp contract(off)
     mx = wave_max_groups_swap(mx) * c;
-    const float m_new = mx > st.m + (kRescaleSlack + UP) ? mx - UP : st.m;
+    const bool grow = mx > st.m + (kRescaleSlack + UP);
+    const float m_new = grow ? mx - UP : st.m;
+    far = far || __any(grow && fabsf(mx) > kFarScore);
     const float alpha = fast_exp2(st.m - m_new);  // 1 if unchanged, 0 from the start value
     st.l *= alpha;
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) st.acc[n] *= alpha;
     st.m = m_new;
   }
+  if (far) {
+#pragma clang fp contract(off)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) p[i] = fast_exp2(__builtin_fmaf(p[i], c, -st.m));
+    for (int i = 0; i < 8; ++i) p[i] = fast_exp2(p[i] * c - st.m);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = fast_exp2(__builtin_fmaf(p[i], c, -st.m));
+  }
   st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
   // dword I of a row of V: elements 2 I, 2 I + 1 of the lane's key R of tile t
   auto value = [&](const Code4Tile<D>& t, auto row, auto dw) {
@@ -747,6 +763,7 @@ __device__ __forceinline__ void attend_tiles4(const DecodeArgs& a, const int32_t
                                               QueryRegs<DT, D, QF>& qr, int tile_lo, int tile_hi, int t_end,
                                               int lane, int w, State<D>& st, bool& bad) {
   constexpr int RUN = NW * kMaxWaveTiles;
+  bool far = false;
   for (int r0 = tile_lo; r0 < tile_hi; r0 += RUN) {
     const int ntiles = min(tile_hi - r0, RUN);
     const int pairs = (ntiles + 1) / 2, my_pairs = pairs > w ? (pairs - w + NW - 1) / NW : 0;
@@ -792,8 +809,8 @@ __device__ __forceinline__ void attend_tiles4(const DecodeArgs& a, const int32_t
           issue_v4<DT, D>(vc, scales, sb.at, lo, x.b);
         }
       };
-      compute_pair4<DT, D, QF, false>(x, qr, va == 16 && vb == 16, va, vb, true, true, a.scale_log2, lane, st, next_k,
-                                      next_v);
+      compute_pair4<DT, D, QF, false>(x, qr, va == 16 && vb == 16, va, vb, true, true, a.scale_log2, lane, st, far,
+                                      next_k, next_v);
     };
     for (int i = 0; i + 1 < my_pairs; ++i) step(i, std::true_type{});
     step(my_pairs - 1, std::false_type{});  // (nothing is issued past the end)

@@ -643,6 +643,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
   // pend: a unit finished at the loop's end whose output is written last, so
   // that no barrier of the end phase waits for its stores
   int cur = -1, keep = -1, pend = -1;
+  bool far = false;  // (kCodes4: of the current unit, compute_pair4)
 
   // Columns of unit x that are outputs, and column col's (sequence, head).
   auto n_cols = [&](const Lbl& x) {
@@ -710,6 +711,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
       if (to == cur) return;
       if (cur >= 0) wave_finish(cur, false);
       cur = to;
+      far = false;
       if (q_lbl != cur) {
         if (qn_lbl == cur) qr = qn;
         else q_of(cur, qr);
@@ -769,7 +771,7 @@ void paged_decode_planned_kernel(const uint8_t* plan, uint32_t o_seq_pre, uint32
         const bool whole = (na & 127u) == kAll && (nb & 127u) == kAll;
         const int half = PAIRS && c >= a.n_rep ? 6 : 5;
         compute_pair4<DT, D, QF, PAIRS>(r.x, qr, whole, na & 31u, nb & 31u, (na >> half) & 1u, (nb >> half) & 1u,
-                                        a.scale_log2, lane, st, next_k, next_v);
+                                        a.scale_log2, lane, st, far, next_k, next_v);
       };
       int held = 0;  // pairs in the ring
 #pragma unroll

@@ -1247,3 +1247,45 @@ def test_a_step_turned_by_axes_over_the_4_bit_pool_is_attention_in_64_bits(dtype
             assert (err <= tol).all(), (new, c, (err / tol).max())
             row += n
         cached = [c + n for c, n in zip(cached, new)]
+
+
+# Whole numbers of queries and keys, times powers of two, so that scores are exact in fp32 and the largest is
+# ahead of the next by more than any exponential holds: the answer is the mean of the V of the keys that have it,
+# rounded (V's sums of a few codes are exact too).
+@pytest.mark.parametrize("path, sign", [("decode", 1), ("decode", -1), ("planned", 1), ("planned", -1), ("prefill", 1)])
+@pytest.mark.parametrize("dtype, q_dtype, q_exp, scale_exp", [
+    (dtype, q_dtype, q_exp, scale_exp)
+    for dtype in DTYPES
+    for q_dtype in sorted({dtype, torch.float32}, key=str)
+    for q_exp, scale_exp in ((0, 100), (0, 12), (100, -3), (40, 0))
+    if q_exp == 0 or q_dtype != torch.float16
+])
+def test_scores_of_any_size(path, sign, dtype, q_dtype, q_exp, scale_exp):
+    bs, hq, h, d, lens = 16, 6, 2, 64, [700, 33, 1]
+    g = gen(60)
+    codes = torch.tensor(quant4.CODES, device=DEV)
+    pool = Quant4PagedKVPool(1, 50, bs, h, d, dtype)
+    tables = [list(range(44)), [44, 45, 46], [47]]
+    k, v = ((codes[torch.randint(0, 8, (2, 800, h, d), generator=g, device=DEV)]
+             * (2 * torch.randint(0, 2, (2, 800, h, d), generator=g, device=DEV) - 1)).to(dtype))
+    k[:, :, ::32] = v[:, :, ::32] = 6.0  # (every group's scale is 1)
+    pool.write(0, k, v, torch.arange(800, device=DEV))
+    whole = torch.randint(-3, 4, (len(lens), hq, d), generator=g, device=DEV).double()
+    q, scale = (whole * 2.0**q_exp).to(q_dtype), sign * 2.0**scale_exp
+    bt, ctx = device_tables(tables), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    kw = {"out": torch.empty(len(lens), hq, d, dtype=dtype, device=DEV), "kv_scales": pool.kv_scales[0]}
+    layer = (pool.k[0], pool.v[0])
+    if path == "decode":
+        out = kernels.paged_decode(q, *layer, bt, ctx, bs, scale, **kw)
+    elif path == "planned":
+        out = kernels.paged_decode_planned(q, *layer, kernels.decode_plan(bt, ctx, hq, pool.k[0], bs), scale, **kw)
+    else:
+        cu = torch.arange(len(lens) + 1, dtype=torch.int32, device=DEV)
+        out = kernels.paged_prefill(q, *layer, bt, cu, ctx - 1, 1, bs, scale, **kw)
+    for i, (table, n) in enumerate(zip(tables, lens)):
+        for head in range(hq):
+            at = slice(table[0] * bs, table[0] * bs + n)
+            s = sign * (k[at, head // 3].double() @ whole[i, head])
+            want = v[at, head // 3][s == s.max()].double().mean(0)
+            err = (out[i, head].double() - want).abs()
+            assert (err <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0**-20).all(), (i, head, err.max())
