@@ -1289,3 +1289,26 @@ def test_scores_of_any_size(path, sign, dtype, q_dtype, q_exp, scale_exp):
             want = v[at, head // 3][s == s.max()].double().mean(0)
             err = (out[i, head].double() - want).abs()
             assert (err <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0**-20).all(), (i, head, err.max())
+
+
+def test_a_graph_of_a_long_write_replays():
+    """A call of several launches, its slots repeated across them and changed between replays."""
+    n, h, d, bs, dtype = 17000, 2, 64, 16, torch.bfloat16
+    g = gen(70)
+    mine, other = (Quant4PagedKVPool(1, 600, bs, h, d, dtype) for _ in range(2))
+    k, v, slots = rows(g, n, h, d, dtype), rows(g, n, h, d, dtype), torch.arange(n, device=DEV) % mine.num_slots
+    mine.write(0, k, v, slots)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mine.write(0, k, v, slots)
+    for i in range(4):
+        k.copy_(rows(g, n, h, d, dtype)), v.copy_(rows(g, n, h, d, dtype))
+        slots.copy_(torch.randint(-1, mine.num_slots, (n,), generator=g, device=DEV))
+        other.k.copy_(mine.k), other.v.copy_(mine.v), other.kv_scales.copy_(mine.kv_scales)
+        other.write(0, k, v, slots)
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(mine.k, other.k) and torch.equal(mine.v, other.v)
+        assert torch.equal(mine.kv_scales, other.kv_scales), i
